@@ -18,8 +18,8 @@ import torch
 
 own = False
 
-# softmax constants of an integer artifact: ln 2, b and c / a of exp(x) ~ a ((x + b)^2 + c / a), Q30
-LN2_Q, B_Q, CA_Q = 744261118, 1453016424, 1030289154
+# the i-exp's constants in Q30: ln 2, and b and c / a of exp(x) ~ a ((x + b)^2 + c / a) on (-ln 2, 0]
+LN2_Q, B_Q, CA_Q = (int(x * 2 ** 30) for x in (0.6931471805599453, 1.353, 0.344 / 0.3585))
 SITE = (1518500250, -45)
 
 
