@@ -284,6 +284,120 @@ sslm_status sslm_hip_gemm_requant_noalloc(const int8_t* a, const int8_t* w, cons
                                           int32_t k, int64_t in_m, int64_t in_e, int64_t site_m, int64_t site_e,
                                           int8_t* out_codes, int64_t* out_me, int32_t* out_status, void* stream);
 
+/* ---- operators of a decode step whose rows are different requests (no reference counterpart) ----
+ *
+ * All three take device buffers and run asynchronously on `stream` (a hipStream_t of the current
+ * device; null = the default stream), allocate nothing and may be captured into a HIP graph.  The
+ * scratch is the caller's: `workspace` of at least the bytes that the entry's ..._workspace()
+ * names for the call's sizes (0: sizes outside its domain), 256-byte aligned; it carries nothing
+ * from call to call, and calls or graphs that may overlap need one each.  `struct_size` is
+ * sizeof the struct.  Sizes, null pointers, alignment and a short workspace are refused before
+ * anything is launched (SSLM_INVALID_ARGUMENT, SSLM_MISALIGNED_BUFFER, SSLM_BUFFER_TOO_SMALL, a stream
+ * of another device SSLM_INVALID_ARGUMENT); a launch that fails returns SSLM_HIP_LAUNCH_FAILED.  What
+ * stands in device memory (lengths, block and adapter indexes, rules) is checked by the kernels, row
+ * by row: a refused row gets a status (or token) that says so, and its outputs are left as they were. */
+
+/* Decode attention of rows that share prompts (reference src/forward/forward_sites.cpp:1791-1905 and
+ * checked_chain_funnel.cpp:257-364, one row's result the same as if it held its whole context).
+ * Row r attends to positions [0, row_width[r]) of its context.  Those below its prefix's length lie in
+ * the prefix's KV block, the others in the row's own block, each at its own position; a prefix's K/V are
+ * read once for all of its rows.  Blocks are the KV pool's: `blocks` of block_bytes bytes from kv_pool, K
+ * (V) of (KV head, position) at block + k_offset (v_offset) + (KV head * cap + position) * head_dim.
+ * Rows [prefix_rows[p], prefix_rows[p + 1]) have prefix p in block prefix_block[p]; rows outside every
+ * run have none.  heads / kv_heads query heads share a KV head; head_dim 32, 64, 128 or 256, heads *
+ * head_dim <= 8192.  ln2_q, b_q, ca_q: the i-exp's Q30 constants; khead: the carried scale of one K code
+ * over sqrt(head_dim) per KV head.  Writes per row the codes [heads * head_dim] and scale (m, e) of the
+ * context after the per-head ctx_fold [heads, 3] and the funnel at (site_m, site_e), and its status: 0,
+ * or the reference's SslmForwardStatus value (7: no position to attend to; 9: a length or block index
+ * outside what the call declares -- max_prefix and max_own, at least every prefix's length and every
+ * row's positions past its prefix's, size the launch). */
+#define SSLM_HIP_ATTENTION_MAX_WIDTH ((int64_t)1 << 24)
+typedef struct sslm_hip_shared_attention_args {
+	uint32_t struct_size;
+	int32_t rows, heads, kv_heads, head_dim, prefixes, blocks, reserved;
+	int64_t max_prefix, max_own;
+	const int8_t* kv_pool;
+	int64_t block_bytes, k_offset, v_offset, cap;
+	const int8_t* q;        /* [rows, heads * head_dim] rotated codes */
+	const int64_t* q_scale; /* [rows, 2] */
+	const int64_t* khead_m; /* [kv_heads] */
+	const int64_t* khead_e;
+	int64_t ln2_q, b_q, ca_q;
+	const int32_t* ctx_fold;
+	int64_t site_m, site_e;
+	const int32_t* row_block;    /* [rows] */
+	const int64_t* row_width;    /* [rows] */
+	const int32_t* prefix_rows;  /* [prefixes + 1] */
+	const int32_t* prefix_block; /* [prefixes] */
+	const int64_t* prefix_len;   /* [prefixes] */
+	int8_t* codes;
+	int64_t* scales; /* [rows, 2] */
+	int32_t* status; /* [rows] */
+} sslm_hip_shared_attention_args;
+size_t sslm_hip_shared_attention_workspace(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                           int32_t prefixes, int64_t max_prefix, int64_t max_own);
+sslm_status sslm_hip_shared_attention(const sslm_hip_shared_attention_args* args, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
+/* sslm_hip_gemm_requant for a batch whose rows each carry a low-rank adapter of their own (reference
+ * forward_sites.cpp:1051-1154: fold, adapter delta, funnel): row t has adapters[row_adapter[t]], a
+ * negative index none, and the incoming scale in_scale[t].  adapters is a device array; rank in
+ * [1, 64], ranks may differ.  out status -1: an index or rank outside those.  1 <= m <= 512, n a multiple
+ * of 16 up to 8192, k a multiple of 16 up to 65536. */
+#define SSLM_HIP_GEMM_LORA_MAX_M 512
+#define SSLM_HIP_GEMM_LORA_MAX_K 65536
+typedef struct sslm_hip_lora {
+	const int8_t* a;      /* [rank, k], 16-byte aligned */
+	const int32_t* ufold; /* [rank, 3] (identity, mult, exponent) */
+	const int8_t* b;      /* [n, rank] */
+	const int32_t* dfold; /* [n, 3] (identity, mult, exponent) */
+	int32_t rank, reserved;
+} sslm_hip_lora;
+typedef struct sslm_hip_gemm_lora_args {
+	uint32_t struct_size;
+	int32_t m, n, k, adapter_count, reserved;
+	const int8_t* a;         /* [m, k], 16-byte aligned */
+	const int8_t* w;         /* [n, k], 16-byte aligned */
+	const int32_t* fold;     /* [n, 3] (identity, mult, shift) */
+	const int64_t* in_scale; /* [m, 2] */
+	int64_t site_m, site_e;
+	const sslm_hip_lora* adapters;
+	const int32_t* row_adapter; /* [m] */
+	int8_t* codes;              /* [m, n] */
+	int64_t* scales;            /* [m, 2] */
+	int32_t* status;            /* [m] */
+} sslm_hip_gemm_lora_args;
+size_t sslm_hip_gemm_lora_workspace(int32_t m, int32_t n, int32_t k);
+sslm_status sslm_hip_gemm_lora_requant(const sslm_hip_gemm_lora_args* args, void* workspace, size_t workspace_bytes,
+                                       void* stream);
+
+/* The next token of rows of int32 logits under each row's own rules.  With c the count of token j among
+ * history [history_len] (ids outside the vocabulary count nowhere):
+ *   c > 0: x = x > 0 ? floor(x 2^16 / repetition_q16) : floor(x repetition_q16 / 2^16)
+ *   x += every bias_values[i] with bias_ids[i] = j;  c > 0: x -= presence + frequency c
+ *   saturated to int32;  INT32_MIN where the mask page's bit j is clear (null: every token is legal)
+ * tokens[r] is the lowest index of the row's largest legal x, -1 when no token is legal, -2 when the rule is
+ * outside its domain (a negative count, repetition_q16 < 1, a count with a null array).  `adjusted`
+ * (optional; may be `logits` itself with the same stride) receives the x.  rules is a device array. */
+typedef struct sslm_hip_logit_rule {
+	const int32_t* history;
+	const int32_t* bias_ids;
+	const int32_t* bias_values;
+	const uint8_t* mask; /* (vocab + 7) / 8 bytes, or null */
+	int32_t history_len, bias_count, repetition_q16, presence, frequency, reserved;
+} sslm_hip_logit_rule;
+typedef struct sslm_hip_pick_args {
+	uint32_t struct_size;
+	int32_t rows, vocab, reserved;
+	const int32_t* logits;
+	int64_t logits_ld, adjusted_ld; /* row strides in elements, at least vocab */
+	const sslm_hip_logit_rule* rules;
+	int32_t* adjusted;
+	int32_t* tokens; /* [rows] */
+} sslm_hip_pick_args;
+size_t sslm_hip_pick_workspace(int32_t rows, int32_t vocab);
+sslm_status sslm_hip_pick_tokens(const sslm_hip_pick_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
