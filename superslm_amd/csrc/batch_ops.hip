@@ -2,6 +2,9 @@
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "../../include/sslm_hip.h"
 #include "batch_ops.h"
 #include "device_util.h"
@@ -89,106 +92,509 @@ __device__ __forceinline__ RowConst row_const(const sslm_launch::SharedAttnArgs&
 	return c;
 }
 
-// One block per (row, query head): scores, i-exp values and Q15 probabilities recomputed from K in
-// three passes over the positions, as the reference's definition has them
-// (forward_sites.cpp:1791-1905).
-template <int D>
-__global__ __launch_bounds__(256) void k_shared_attn_row(sslm_launch::SharedAttnArgs a, int32_t* f, int32_t* hst) {
-	constexpr int BS = 256;
-	__shared__ __attribute__((aligned(16))) int8_t s_q[D];
-	__shared__ int32_t s_p[BS], s_acc[D];
-	__shared__ uint32_t s_mx[BS / 64], s_bad[BS / 64];
-	__shared__ int64_t s_sum[BS / 64];
-	const int h = blockIdx.x, r = blockIdx.y, i = threadIdx.x, kvh = h / (a.NH / a.NKV);
-	const RowSpan sp = row_span(a, r);
-	if (sp.st != kOk) {
-		if (i == 0) hst[(size_t)r * a.NH + h] = sp.st;
-		return;
+// The layout of one call's launches.  The unit of work is a wave with a tile of 16 query rows and a
+// range of positions, a "plane": shared planes cut a prefix into sb positions each and their tiles hold
+// the query heads of one KV head of 16 / G neighbouring rows (G heads share a KV head), so a K or V row
+// is read once for all of them; own planes cut a row's own positions, their tiles hold the row's G heads.
+// The softmax's maximum and sum run over the whole row and every probability is rounded by itself, so no
+// rescaling of partial results is exact: three launches -- maxima, sums, P.V -- recompute the scores,
+// which cost 8 MFMAs a step of 64 positions at D = 128 where the i-exp of the step's scores costs some
+// hundreds of vector instructions, and integer sums join the planes exactly in any order.
+struct SaPlan {
+	int tiles;       // tiles of shared rows: at least those of every prefix together
+	int shared, sb;  // shared planes and the positions of one (a multiple of 64)
+	int owned, ob;   // own planes and the positions of one
+	int ht;          // tiles of a row's own heads
+	int shared_blocks;
+};
+
+// (row, KV head): the softmax constants and whether the row is computed at all
+struct SaConst {
+	int64_t q_ln2, q_b, q_c, ceil;
+	int32_t st, pad;
+};
+
+struct SaWork {
+	SaConst* cst;   // [rows, NKV]
+	int32_t* pmax;  // [planes][rows NH]
+	int64_t* psum;  // [planes][rows NH]; negative: an i-exp value was refused
+	int32_t* part;  // [planes][rows][NH D]
+	int32_t* hst;   // [rows, NH] refusals of the softmax
+};
+
+constexpr int kSaWaves = 4;
+
+// What a wave works on; the fields that differ by lane belong to query row ri = lane & 15 of its tile.
+struct SaJob {
+	const int8_t *k, *v;  // the KV head's position 0
+	int64_t p0, p1;       // positions of the plane (p1: also the end of what may be read)
+	int plane, kvh;
+	int r, h;             // by lane: row and query head (r < 0: none)
+	int64_t start, width; // by lane: where the row's own positions begin, and its width
+	bool owned, first;    // an own plane; the row's first
+};
+
+__device__ __forceinline__ int64_t i64min(int64_t a, int64_t b) { return a < b ? a : b; }
+__device__ __forceinline__ int64_t i64max(int64_t a, int64_t b) { return a > b ? a : b; }
+
+// The prefixes' rows, as far as they are a division of the call's: ascending from at least 0 to at most `rows`.
+__device__ __forceinline__ bool prefix_rows_ok(const sslm_launch::SharedAttnArgs& a) {
+	bool bad = false;
+	for (int i = threadIdx.x & 63; i <= a.prefixes && a.prefixes > 0; i += 64) {
+		const int x = a.prefix_rows[i];
+		bad |= x < 0 || x > a.rows || (i > 0 && x < a.prefix_rows[i - 1]);
 	}
-	for (int d = i; d < D; d += BS) {
-		s_q[d] = a.q[((size_t)r * a.NH + h) * D + d];
-		s_acc[d] = 0;
-	}
-	__syncthreads();
-	const int64_t head = (int64_t)kvh * a.cap * D;
-	auto score = [&](int64_t p) {
-		const int8_t* k = (p < sp.start ? sp.pre : sp.own) + a.k_off + head + p * D;
-		int32_t s = 0;
-		for (int c = 0; c < D; c += 16) {
-			const v4i x = load16(k + c), q = *(const v4i*)(s_q + c);
-#pragma unroll
-			for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_sdot4(x[j], q[j], s, false);
-		}
-		return s;
-	};
-	uint32_t mx = 0;
-	for (int64_t p = i; p < sp.width; p += BS) mx = max(mx, (uint32_t)score(p) ^ 0x80000000u);
-	const int32_t top = (int32_t)(block_max_u32<BS>(mx, s_mx) ^ 0x80000000u);
-	const RowConst c = row_const(a, r, kvh, sp.width);
-	if (c.st != kOk) {
-		if (i == 0) hst[(size_t)r * a.NH + h] = c.st;
-		return;
-	}
-	const double inv_ln2 = 1.0 / (double)c.q_ln2;
-	int64_t sum = 0;
-	uint32_t bad = 0;
-	for (int64_t p = i; p < sp.width; p += BS) {
-		const int64_t e = iexp_fast((int64_t)score(p) - top, c.q_ln2, inv_ln2, c.q_b, c.q_c, c.ceil);
-		if (e < 0) bad = 1;
-		else sum += e;
-	}
-	sum = block_sum_i64<BS>(sum, s_sum);
-	if (block_max_u32<BS>(bad, s_bad)) {
-		if (i == 0) hst[(size_t)r * a.NH + h] = kSoftmaxKernelRefusedAfterGateAccepted;
-		return;
-	}
-	const int64_t den = sum > 1 ? sum : 1;
-	const double inv = 1.0 / (double)den;
-	int32_t acc = 0;
-	const int d = i % D, part = i / D;
-	for (int64_t b = 0; b < sp.width; b += BS) {
-		const int64_t p = b + i;
-		int64_t e = 0;
-		if (p < sp.width) e = iexp_fast((int64_t)score(p) - top, c.q_ln2, inv_ln2, c.q_b, c.q_c, c.ceil);
-		s_p[i] = e > 0 ? (int32_t)div_rcp(e << 15, den, inv, 32768) : 0;
-		__syncthreads();
-		const int n = (int)(sp.width - b < BS ? sp.width - b : BS);
-		for (int j = part; j < n; j += BS / D) {
-			const int64_t pj = b + j;
-			acc += s_p[j] * (int32_t)((pj < sp.start ? sp.pre : sp.own) + a.v_off + head + pj * D)[d];
-		}
-		__syncthreads();
-	}
-	atomicAdd(&s_acc[d], acc);
-	__syncthreads();
-	const int32_t* cf = a.ctx_fold + 3 * h;
-	if (i < D) f[((size_t)r * a.NH + h) * D + i] = sat_i32(apply_fold(s_acc[i], cf[0], cf[1], cf[2]));
-	if (i == 0) hst[(size_t)r * a.NH + h] = kOk;
+	return !__any(bad);
 }
 
-// The context funnel of one row (checked_chain_funnel.cpp:257-364), after the first refusing head.
-template <int BS, int EPT>
-__global__ __launch_bounds__(BS) void k_ctx_funnel(sslm_launch::SharedAttnArgs a, const int32_t* f, const int32_t* hst) {
-	__shared__ uint32_t s_m[BS / 64];
-	__shared__ int32_t s_st;
-	const int r = blockIdx.x, N = a.NH * a.D;
-	if (threadIdx.x == 0) {
-		int32_t st = kOk;
-		for (int h = a.NH - 1; h >= 0; --h) st = hst[(size_t)r * a.NH + h] != kOk ? hst[(size_t)r * a.NH + h] : st;
-		s_st = st;
+// A wave of the shared planes (block `blk` of them): false when there is nothing for it to do.
+__device__ __forceinline__ bool sa_shared_job(const sslm_launch::SharedAttnArgs& a, const SaPlan& pl, int blk, SaJob* j) {
+	// blocks go to the XCDs in turn: a (KV head, plane)'s tiles stay on one, whose L2 then holds its K/V
+	const int tb = (pl.tiles + kSaWaves - 1) / kSaWaves, grp = (blk / 8 / tb) * 8 + blk % 8;
+	int tile = (blk / 8) % tb * kSaWaves + ((int)threadIdx.x >> 6);
+	if (grp >= a.NKV * pl.shared || tile >= pl.tiles) return false;
+	j->plane = grp / a.NKV;
+	j->kvh = grp % a.NKV;
+	const int G = a.NH / a.NKV;
+	int p = 0, r0 = 0, r1 = 0;
+	for (;; ++p) {  // the tile's prefix
+		if (p >= a.prefixes) return false;
+		r0 = max(0, min(a.prefix_rows[p], a.rows));
+		r1 = max(r0, min(a.prefix_rows[p + 1], a.rows));
+		const int n = ((r1 - r0) * G + 15) / 16;
+		if (tile < n) break;
+		tile -= n;
 	}
-	__syncthreads();
-	if (s_st != kOk) {
-		if (threadIdx.x == 0) a.status[r] = s_st;
+	const int pb = a.prefix_block[p];
+	const int64_t len = a.prefix_len[p];
+	j->p0 = (int64_t)j->plane * pl.sb;
+	if (pb < 0 || pb >= a.blocks || len < 0 || len > a.cap || len > a.max_prefix || j->p0 >= len) return false;
+	j->p1 = i64min(len, j->p0 + pl.sb);
+	const int8_t* head = a.pool + (int64_t)pb * a.block_bytes + (int64_t)j->kvh * a.cap * a.D;
+	j->k = head + a.k_off;
+	j->v = head + a.v_off;
+	const int i = tile * 16 + (threadIdx.x & 15);
+	const bool live = i < (r1 - r0) * G;
+	j->r = live ? r0 + i / G : -1;
+	j->h = j->kvh * G + (live ? i % G : 0);
+	j->width = live ? a.row_width[j->r] : 0;
+	j->start = i64min(len, j->width);
+	j->owned = j->first = false;
+	return true;
+}
+
+// A wave of the own planes (number `w` of them), whose row lies at `sp`.
+__device__ __forceinline__ bool sa_own_job(const sslm_launch::SharedAttnArgs& a, const SaPlan& pl, int w, SaJob* j, RowSpan* sp) {
+	if (w >= a.rows * a.NKV * pl.ht * pl.owned) return false;
+	const int G = a.NH / a.NKV, plane = w % pl.owned, t = w / pl.owned % pl.ht;
+	j->kvh = w / pl.owned / pl.ht % a.NKV;
+	const int r = w / pl.owned / pl.ht / a.NKV, i = t * 16 + (threadIdx.x & 15);
+	*sp = row_span(a, r);
+	j->owned = true;
+	j->first = plane == 0;
+	j->plane = pl.shared + plane;
+	j->start = sp->start;
+	j->width = sp->width;
+	j->p0 = sp->start + (int64_t)plane * pl.ob;
+	j->p1 = i64min(sp->width, j->p0 + pl.ob);
+	const int8_t* head = sp->own + (int64_t)j->kvh * a.cap * a.D;
+	j->k = head + a.k_off;
+	j->v = head + a.v_off;
+	j->r = i < G ? r : -1;
+	j->h = j->kvh * G + (i < G ? i : 0);
+	return true;
+}
+
+// the wave's query rows as an MFMA operand: lane (ri, g) holds bytes 64 c + 16 g .. + 16 of row ri
+template <int D, int NC>
+__device__ __forceinline__ void sa_load_q(const sslm_launch::SharedAttnArgs& a, const SaJob& j, v4i (&q)[NC]) {
+	const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+	for (int c = 0; c < NC; ++c) {
+		const int off = c * 64 + g * 16;
+		q[c] = j.r >= 0 && off < D ? load16(a.q + ((size_t)j.r * a.NH + j.h) * D + off) : v4i{0, 0, 0, 0};
+	}
+}
+
+// K rows of the 64 positions from p (rows past `last` repeat it), the other operand
+template <int D, int NC>
+__device__ __forceinline__ void sa_load_k(const int8_t* k, int64_t p, int64_t last, v4i (&kf)[4][NC]) {
+	const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4;
+#pragma unroll
+	for (int t = 0; t < 4; ++t) {
+		const int8_t* row = k + i64min(p + t * 16 + ri, last) * D;
+#pragma unroll
+		for (int c = 0; c < NC; ++c) {
+			const int off = c * 64 + g * 16;
+			kf[t][c] = off < D ? load16(row + off) : v4i{0, 0, 0, 0};
+		}
+	}
+}
+
+// Scores of 64 positions: lane (ri, g) gets those of query row ri at positions 16 t + 4 g + v.
+template <int NC>
+__device__ __forceinline__ void sa_scores(const v4i (&q)[NC], const v4i (&kf)[4][NC], v4i (&s)[4]) {
+#pragma unroll
+	for (int t = 0; t < 4; ++t) {
+		s[t] = v4i{0, 0, 0, 0};
+#pragma unroll
+		for (int c = 0; c < NC; ++c) s[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][c], q[c], s[t], 0, 0, 0);
+	}
+}
+
+// The i-exp of one query row in doubles, each value exact: with y = q_b - x for a score x below the
+// maximum (x <= 30 q_ln2 by the clip), z = floor(x / q_ln2) = floor((x + 1/2) / q_ln2), whose argument is at
+// least 1 / (2 q_ln2) from an integer and estimated within (q_b + 30 q_ln2) 2^-51 / q_ln2 of its value;
+// base = y + z q_ln2, and base^2 + q_c <= q_b^2 + q_c <= 2^47 by the softmax gate.  `fast` rows have
+// 0 <= q_b, q_ln2 <= 2 q_b + 1 (then base^2 <= q_b^2, so no value leaves the domain) and a sum
+// below 2^53, exact in doubles.  Eleven instructions a value; the integer form takes some forty.
+struct SaExp {
+	double ninv, c0, l, qc;
+	int32_t add, ymin;
+};
+__device__ __forceinline__ bool sa_fast(const SaConst& c, int64_t width) {
+	return c.q_b >= 0 && c.q_ln2 >= 1 && c.ceil >= 1 && c.q_ln2 <= 2 * c.q_b + 1 && (double)c.ceil * (double)width < 0x1p53;
+}
+__device__ __forceinline__ SaExp sa_exp_of(const SaConst& c, int32_t top) {
+	SaExp e;
+	e.l = (double)c.q_ln2;
+	e.ninv = -1.0 / e.l;
+	e.c0 = -((double)c.q_b + 0.5) * e.ninv;
+	e.qc = (double)c.q_c;
+	e.add = (int32_t)c.q_b - top;
+	e.ymin = (int32_t)(c.q_b - 30 * c.q_ln2);
+	return e;
+}
+__device__ __forceinline__ double sa_exp(const SaExp& e, int32_t score) {
+	const double y = (double)max(score + e.add, e.ymin);
+	const double z = floor(fma(y, e.ninv, e.c0));
+	const double base = fma(z, e.l, y);
+	return floor(ldexp(fma(base, base, e.qc), -(int)z));
+}
+
+// the wave's rows joined over their planes; a lane's row is read by the lanes ri, ri + 16, ri + 32, ri + 48
+__device__ __forceinline__ int sa_plane_count(const SaPlan& pl, const SaJob& j, int* shared) {
+	const int64_t own = j.width - j.start;
+	*shared = (int)((j.start + pl.sb - 1) / pl.sb);
+	return *shared + (int)((own + pl.ob - 1) / pl.ob);
+}
+__device__ __forceinline__ int32_t sa_row_max(const sslm_launch::SharedAttnArgs& a, const SaPlan& pl, const SaWork& w, const SaJob& j, bool live) {
+	int sh, m = INT32_MIN;
+	const int n = live ? sa_plane_count(pl, j, &sh) : 0;
+	const int32_t* at = w.pmax + (size_t)(live ? j.r : 0) * a.NH + j.h;
+	for (int i = (threadIdx.x & 63) >> 4; i < n; i += 4) m = max(m, at[(size_t)(i < sh ? i : pl.shared + i - sh) * a.rows * a.NH]);
+	m = max(m, __shfl_xor(m, 16, 64));
+	return max(m, __shfl_xor(m, 32, 64));
+}
+// negative: refused
+__device__ __forceinline__ int64_t sa_row_sum(const sslm_launch::SharedAttnArgs& a, const SaPlan& pl, const SaWork& w, const SaJob& j, bool live) {
+	int sh, bad = 0;
+	int64_t m = 0;
+	const int n = live ? sa_plane_count(pl, j, &sh) : 0;
+	const int64_t* at = w.psum + (size_t)(live ? j.r : 0) * a.NH + j.h;
+	for (int i = (threadIdx.x & 63) >> 4; i < n; i += 4) {
+		const int64_t x = at[(size_t)(i < sh ? i : pl.shared + i - sh) * a.rows * a.NH];
+		bad |= x < 0;
+		m += x < 0 ? 0 : x;
+	}
+	for (int o = 16; o < 64; o *= 2) {
+		m += __shfl_xor(m, o, 64);
+		bad |= __shfl_xor(bad, o, 64);
+	}
+	return bad ? -1 : m;
+}
+
+template <int D>
+__global__ __launch_bounds__(64 * kSaWaves) void k_sa_max(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
+	constexpr int NC = (D + 63) / 64;
+	const int lane = threadIdx.x & 63, g = lane >> 4;
+	SaJob j;
+	if ((int)blockIdx.x < pl.shared_blocks) {
+		if (!sa_shared_job(a, pl, blockIdx.x, &j)) return;
+	} else {
+		RowSpan sp;
+		if (!sa_own_job(a, pl, (blockIdx.x - pl.shared_blocks) * kSaWaves + (threadIdx.x >> 6), &j, &sp)) return;
+		if (j.first) {
+			SaConst c{0, 0, 0, 0, prefix_rows_ok(a) ? sp.st : kPositionOverCap, 0};
+			if (c.st == kOk) {
+				const RowConst rc = row_const(a, __builtin_amdgcn_readfirstlane(j.r), j.kvh, sp.width);
+				c = SaConst{rc.q_ln2, rc.q_b, rc.q_c, rc.ceil, rc.st, 0};
+			}
+			if (lane == 0) w.cst[(size_t)j.r * a.NKV + j.kvh] = c;
+		}
+		if (sp.st != kOk) return;
+	}
+	v4i q[NC];
+	sa_load_q<D>(a, j, q);
+	const int64_t end = j.owned ? j.p1 : i64min(j.p1, j.start);  // by lane
+	int32_t m = INT32_MIN;
+	v4i kf[4][NC], s[4];
+	for (int64_t p = j.p0; p < j.p1; p += 64) {
+		sa_load_k<D>(j.k, p, j.p1 - 1, kf);
+		sa_scores(q, kf, s);
+#pragma unroll
+		for (int t = 0; t < 4; ++t)
+#pragma unroll
+			for (int v = 0; v < 4; ++v) m = max(m, p + t * 16 + g * 4 + v < end ? s[t][v] : INT32_MIN);
+	}
+	m = max(m, __shfl_xor(m, 16, 64));
+	m = max(m, __shfl_xor(m, 32, 64));
+	if (g == 0 && j.r >= 0) w.pmax[(size_t)j.plane * a.rows * a.NH + (size_t)j.r * a.NH + j.h] = m;
+}
+
+// A wave's job in the launches after k_sa_max, and its rows' constants: live (by lane) rows are computed.
+__device__ __forceinline__ bool sa_job(const sslm_launch::SharedAttnArgs& a, const SaPlan& pl, const SaWork& w, SaJob* j, SaConst* c, bool* live) {
+	if ((int)blockIdx.x < pl.shared_blocks) {
+		if (!sa_shared_job(a, pl, blockIdx.x, j)) return false;
+	} else {
+		RowSpan sp;
+		if (!sa_own_job(a, pl, (blockIdx.x - pl.shared_blocks) * kSaWaves + (threadIdx.x >> 6), j, &sp)) return false;
+		if (sp.st != kOk) return false;
+	}
+	*c = w.cst[(size_t)max(j->r, 0) * a.NKV + j->kvh];
+	*live = j->r >= 0 && c->st == kOk;
+	return __any(*live);
+}
+
+template <int D>
+__global__ __launch_bounds__(64 * kSaWaves) void k_sa_sum(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
+	constexpr int NC = (D + 63) / 64;
+	const int g = (threadIdx.x & 63) >> 4;
+	SaJob j;
+	SaConst c;
+	bool live;
+	if (!sa_job(a, pl, w, &j, &c, &live) || j.p0 >= j.p1) return;
+	v4i q[NC];
+	sa_load_q<D>(a, j, q);
+	const int32_t top = sa_row_max(a, pl, w, j, live);
+	const int64_t end = !live ? 0 : (j.owned ? j.p1 : i64min(j.p1, j.start));
+	int64_t sum = 0;
+	int bad = 0;
+	v4i kf[4][NC], s[4];
+	if (!__any(live && !sa_fast(c, j.width))) {
+		const SaExp e = sa_exp_of(live ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
+		double acc = 0.0;
+		for (int64_t p = j.p0; p < j.p1; p += 64) {
+			sa_load_k<D>(j.k, p, j.p1 - 1, kf);
+			sa_scores(q, kf, s);
+#pragma unroll
+			for (int t = 0; t < 4; ++t)
+#pragma unroll
+				for (int v = 0; v < 4; ++v) {
+					const double x = sa_exp(e, s[t][v]);
+					acc += p + t * 16 + g * 4 + v < end ? x : 0.0;
+				}
+		}
+		sum = (int64_t)acc;
+	} else {
+		const double inv = 1.0 / (double)c.q_ln2;
+		for (int64_t p = j.p0; p < j.p1; p += 64) {
+			sa_load_k<D>(j.k, p, j.p1 - 1, kf);
+			sa_scores(q, kf, s);
+			for (int i = 0; i < 16; ++i) {
+				if (p + (i >> 2) * 16 + g * 4 + (i & 3) >= end) continue;
+				const int64_t x = iexp_fast_cold((int64_t)s[i >> 2][i & 3] - top, c.q_ln2, inv, c.q_b, c.q_c, c.ceil);
+				bad |= x < 0;
+				sum += x < 0 ? 0 : x;
+			}
+		}
+	}
+	for (int o = 16; o < 64; o *= 2) {
+		sum += __shfl_xor(sum, o, 64);
+		bad |= __shfl_xor(bad, o, 64);
+	}
+	if (g == 0 && live) w.psum[(size_t)j.plane * a.rows * a.NH + (size_t)j.r * a.NH + j.h] = bad ? -1 : sum;
+}
+
+// The Q15 probability floor(2^15 e / d) in doubles, d the row's sum: for d < 2^36 the truncation of
+// (2^15 e + 1/2) / d, which is at least 2^-37 from an integer and estimated within 2^-37; else an estimate
+// from below, off by less than one, and the exact remainder (a multiple of 2^-15 below 2^38).
+struct SaProb {
+	double c1, c2, d;  // small sums: 2^15 / d, 1 / (2 d); else the estimate's factor, unused, d / 2^15
+};
+__device__ __forceinline__ SaProb sa_prob_of(double d, bool small) {
+	SaProb p;
+	p.d = d * 0x1p-15;
+	p.c1 = small ? 32768.0 / d : (1.0 - 0x1p-50) / p.d;
+	p.c2 = 0.5 / d;
+	return p;
+}
+template <bool SMALL>
+__device__ __forceinline__ int32_t sa_prob(const SaProb& p, double e) {
+	if constexpr (SMALL) return (int32_t)fma(e, p.c1, p.c2);
+	const double q = floor(e * p.c1);
+	return (int32_t)q + (fma(-q, p.d, e) >= p.d ? 1 : 0);
+}
+
+// Probabilities p of 64 positions as two int8 MFMA operands with p = 256 hi + lo: lo is p's low byte taken
+// as signed, -hi = floor((127 - p) / 256) in [-128, 0] (hi itself reaches 128).  Byte 4 t + v of lane
+// (ri, g) is position 16 t + 4 g + v: the products sum over positions, so the scores' own order serves.
+__device__ __forceinline__ void sa_pack(const int32_t (&p)[16], v4i* lo, v4i* nhi) {
+#pragma unroll
+	for (int t = 0; t < 4; ++t) {
+		const uint32_t a = __builtin_amdgcn_perm(p[4 * t + 1], p[4 * t], 0x0c0c0400), b = __builtin_amdgcn_perm(p[4 * t + 3], p[4 * t + 2], 0x0c0c0400);
+		(*lo)[t] = (int)(a | b << 16);
+		const uint32_t c = __builtin_amdgcn_perm(127 - p[4 * t + 1], 127 - p[4 * t], 0x0c0c0501),
+		               d = __builtin_amdgcn_perm(127 - p[4 * t + 3], 127 - p[4 * t + 2], 0x0c0c0501);
+		(*nhi)[t] = (int)(c | d << 16);
+	}
+}
+
+// V rows of 64 positions through LDS (one wave's own rows of it) into MFMA operands: lane (ri, g) of dim
+// tile dt gets dim 16 dt + ri of the positions in sa_pack's order, by the byte-transposing LDS read.
+template <int D>
+struct SaV {
+	static constexpr int PER = D / 16;
+	v4i r[PER];
+	// where 16-byte chunk `ch` of row `row` lies: chunks change places by row, so that one chunk of
+	// neighbouring rows covers all banks
+	static __device__ __forceinline__ int at(int row, int ch) { return row * D + ((ch ^ (row & (PER - 1))) << 4); }
+	__device__ __forceinline__ void load(const int8_t* v, int64_t p, int64_t last) {
+		const int lane = threadIdx.x & 63;
+#pragma unroll
+		for (int u = 0; u < PER; ++u) {
+			const int i = lane + 64 * u;
+			r[u] = load16(v + i64min(p + i / PER, last) * D + i % PER * 16);
+		}
+	}
+	__device__ __forceinline__ void stage(int8_t* lds) const {
+		const int lane = threadIdx.x & 63;
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+		for (int u = 0; u < PER; ++u) {
+			const int i = lane + 64 * u;
+			*(v4i*)(lds + at(i / PER, i % PER)) = r[u];
+		}
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		__builtin_amdgcn_wave_barrier();
+	}
+	// context += P V: lane (ri, g) of acc[dt][part] holds dims 16 dt + 4 g .. + 3 of query row ri
+	static __device__ __forceinline__ void multiply(const int8_t* lds, const v4i& lo, const v4i& nhi, v4i (&acc)[D / 16][2]) {
+		const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4, i = ri >> 1;
+		const int row = (i >> 2) * 16 + g * 4 + (i & 3);
+#pragma unroll
+		for (int dt = 0; dt < D / 16; ++dt) {
+			const int8_t* from = lds + at(row, dt) + 8 * (ri & 1);  // rows `row` and row + 32 agree in row % 16
+			const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)from);
+			const v2i y = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(from + 32 * D));
+			const v4i b = v4i{x.x, x.y, y.x, y.y};
+			acc[dt][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, lo, acc[dt][0], 0, 0, 0);
+			acc[dt][1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, nhi, acc[dt][1], 0, 0, 0);
+		}
+	}
+};
+
+template <int D>
+__global__ __launch_bounds__(64 * kSaWaves) void k_sa_pv(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
+	constexpr int NC = (D + 63) / 64, DT = D / 16;
+	__shared__ __attribute__((aligned(16))) int8_t s_v[kSaWaves][64 * D];
+	int8_t* lds = s_v[threadIdx.x >> 6];
+	const int g = (threadIdx.x & 63) >> 4;
+	SaJob j;
+	SaConst c;
+	bool live;
+	if (!sa_job(a, pl, w, &j, &c, &live)) return;
+	const int32_t top = sa_row_max(a, pl, w, j, live);
+	const int64_t sum = sa_row_sum(a, pl, w, j, live);
+	if (j.first && g == 0 && live) w.hst[(size_t)j.r * a.NH + j.h] = sum < 0 ? kSoftmaxKernelRefusedAfterGateAccepted : kOk;
+	if (j.p0 >= j.p1) return;
+	live = live && sum >= 0;
+	const int64_t den = live && sum > 1 ? sum : 1;
+	const int64_t end = !live ? 0 : (j.owned ? j.p1 : i64min(j.p1, j.start));
+	v4i q[NC], kf[4][NC], s[4], acc[DT][2], lo, nhi;
+	sa_load_q<D>(a, j, q);
+#pragma unroll
+	for (int d = 0; d < DT; ++d) acc[d][0] = acc[d][1] = v4i{0, 0, 0, 0};
+	SaV<D> vr;
+	int32_t pr[16];
+	if (!__any(live && !sa_fast(c, j.width))) {
+		const SaExp e = sa_exp_of(live ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
+		auto run = [&](auto small) {
+			constexpr bool SMALL = decltype(small)::value;
+			const SaProb pb = sa_prob_of((double)den, SMALL);
+			for (int64_t p = j.p0; p < j.p1; p += 64) {
+				sa_load_k<D>(j.k, p, j.p1 - 1, kf);
+				vr.load(j.v, p, j.p1 - 1);
+				sa_scores(q, kf, s);
+#pragma unroll
+				for (int i = 0; i < 16; ++i) {
+					const int32_t x = sa_prob<SMALL>(pb, sa_exp(e, s[i >> 2][i & 3]));
+					pr[i] = p + (i >> 2) * 16 + g * 4 + (i & 3) < end ? x : 0;
+				}
+				sa_pack(pr, &lo, &nhi);
+				vr.stage(lds);
+				SaV<D>::multiply(lds, lo, nhi, acc);
+			}
+		};
+		if (!__any(den >= ((int64_t)1 << 36))) run(std::true_type{});
+		else run(std::false_type{});
+	} else {
+		const double inv = 1.0 / (double)c.q_ln2, dinv = 1.0 / (double)den;
+		for (int64_t p = j.p0; p < j.p1; p += 64) {
+			sa_load_k<D>(j.k, p, j.p1 - 1, kf);
+			vr.load(j.v, p, j.p1 - 1);
+			sa_scores(q, kf, s);
+#pragma unroll
+			for (int i = 0; i < 16; ++i) {
+				pr[i] = 0;
+				if (p + (i >> 2) * 16 + g * 4 + (i & 3) >= end) continue;
+				const int64_t x = iexp_fast_cold((int64_t)s[i >> 2][i & 3] - top, c.q_ln2, inv, c.q_b, c.q_c, c.ceil);
+				pr[i] = (int32_t)div_rcp_cold(x << 15, den, dinv, 32768);
+			}
+			sa_pack(pr, &lo, &nhi);
+			vr.stage(lds);
+			SaV<D>::multiply(lds, lo, nhi, acc);
+		}
+	}
+	if (j.r < 0) return;
+	int32_t* out = w.part + ((size_t)j.plane * a.rows + j.r) * a.NH * D + (size_t)j.h * D + 4 * g;
+#pragma unroll
+	for (int d = 0; d < DT; ++d) {
+		v4i o;
+#pragma unroll
+		for (int v = 0; v < 4; ++v) o[v] = acc[d][0][v] - 256 * acc[d][1][v];
+		*(v4i*)(out + 16 * d) = o;
+	}
+}
+
+// The planes' contexts joined, the per-head fold and the funnel of one row (checked_chain_funnel.cpp:257-364),
+// after the first refusing head.  U units of four dims per thread.
+template <int BS, int U>
+__global__ __launch_bounds__(BS) void k_sa_out(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
+	__shared__ uint32_t s_m[BS / 64], s_bad[BS / 64];
+	const int r = blockIdx.x, N = a.NH * a.D, G = a.NH / a.NKV;
+	// the first refusing head, heads of one KV head sharing its constants' status: (head << 8) | status
+	uint32_t first = 0xffffffffu;
+	for (int h = threadIdx.x; h < a.NH; h += BS) {
+		const int32_t st = w.cst[(size_t)r * a.NKV + h / G].st;
+		const int32_t x = st != kOk ? st : w.hst[(size_t)r * a.NH + h];
+		if (x != kOk) first = min(first, (uint32_t)h << 8 | (uint32_t)x);
+	}
+	first = ~block_max_u32<BS>(~first, s_bad);
+	if (first != 0xffffffffu) {
+		if (threadIdx.x == 0) a.status[r] = (int32_t)(first & 0xff);
 		return;
 	}
-	int32_t v[EPT];
+	const RowSpan sp = row_span(a, r);
+	const int sh = (int)((sp.start + pl.sb - 1) / pl.sb), n = sh + (int)((sp.width - sp.start + pl.ob - 1) / pl.ob);
+	v4i v[U];
 	uint32_t mx = 0;
 #pragma unroll
-	for (int k = 0; k < EPT; ++k) {
-		const int j = (int)threadIdx.x + k * BS;
-		v[k] = j < N ? f[(size_t)r * N + j] : 0;
-		mx = max(mx, sat_abs_u32(v[k]));
+	for (int u = 0; u < U; ++u) {
+		const int i = (int)threadIdx.x + u * BS;
+		v[u] = v4i{0, 0, 0, 0};
+		if (4 * i < N) {
+			const int32_t* at = w.part + (size_t)r * N + 4 * i;
+#pragma unroll 4
+			for (int k = 0; k < n; ++k) v[u] += *(const v4i*)(at + (size_t)(k < sh ? k : pl.shared + k - sh) * a.rows * N);
+			const int32_t* cf = a.ctx_fold + 3 * (4 * i / a.D);
+#pragma unroll
+			for (int x = 0; x < 4; ++x) {
+				const int64_t f = apply_fold(v[u][x], cf[0], cf[1], cf[2]);
+				mx = max(mx, sat_abs_u32(f));
+				v[u][x] = sat_i32(f);
+			}
+		}
 	}
 	mx = block_max_u32<BS>(mx, s_m);
 	FunnelPlan plan;
@@ -199,9 +605,14 @@ __global__ __launch_bounds__(BS) void k_ctx_funnel(sslm_launch::SharedAttnArgs a
 	}
 	if (st != kOk) return;
 #pragma unroll
-	for (int k = 0; k < EPT; ++k) {
-		const int j = (int)threadIdx.x + k * BS;
-		if (j < N) a.codes[(size_t)r * N + j] = requant_code_f(v[k], plan.f);
+	for (int u = 0; u < U; ++u) {
+		const int i = (int)threadIdx.x + u * BS;
+		if (4 * i < N) {
+			uint32_t o = 0;
+#pragma unroll
+			for (int x = 0; x < 4; ++x) o |= (uint32_t)(uint8_t)requant_code_f(v[u][x], plan.f) << 8 * x;
+			*(uint32_t*)(a.codes + (size_t)r * N + 4 * i) = o;
+		}
 	}
 }
 
@@ -380,6 +791,8 @@ __global__ __launch_bounds__(64) void k_pick_final(sslm_launch::PickArgs a, cons
 // ------------------------------------------------------------------------------------------
 namespace sslm_launch {
 
+constexpr int kSaTargetWaves = 1024;
+
 static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 bool shared_attn_ok(int rows, int NH, int NKV, int D) {
@@ -387,21 +800,72 @@ bool shared_attn_ok(int rows, int NH, int NKV, int D) {
 	       (int64_t)NH * D <= kFunnelMaxN;
 }
 
+// Planes: enough waves for the chip's 1024 SIMDs, a plane at least one step of 64 positions.
+static SaPlan sa_plan(int rows, int NH, int NKV, int prefixes, int64_t max_prefix, int64_t max_own) {
+	SaPlan p{};
+	const int G = NH / NKV;
+	p.tiles = prefixes > 0 && max_prefix > 0 ? rows * G / 16 + prefixes : 0;
+	const int64_t steps = (max_prefix + 63) / 64, jobs = (int64_t)p.tiles * NKV;
+	if (jobs > 0) {
+		const int64_t want = std::min<int64_t>(steps, std::max<int64_t>(1, (kSaTargetWaves + jobs - 1) / jobs));
+		p.sb = (int)((steps + want - 1) / want) * 64;
+		p.shared = (int)((max_prefix + p.sb - 1) / p.sb);
+	} else {
+		p.sb = 64;
+	}
+	p.ht = (G + 15) / 16;
+	const int64_t osteps = std::max<int64_t>(1, (max_own + 63) / 64), ojobs = (int64_t)rows * NKV * p.ht;
+	const int64_t owant = std::min<int64_t>(osteps, std::max<int64_t>(1, (kSaTargetWaves + ojobs - 1) / ojobs));
+	p.ob = (int)((osteps + owant - 1) / owant) * 64;
+	p.owned = (int)std::max<int64_t>(1, (max_own + p.ob - 1) / p.ob);
+	const int tb = (p.tiles + kSaWaves - 1) / kSaWaves;
+	p.shared_blocks = (NKV * p.shared + 7) / 8 * 8 * tb;
+	return p;
+}
+
+static size_t sa_work(const SaPlan& p, int rows, int NH, int NKV, int D, char* base, SaWork* w) {
+	size_t at = 0;
+	auto take = [&](size_t n) {
+		char* x = base + at;
+		at += up256(n);
+		return x;
+	};
+	const size_t planes = p.shared + p.owned, r = (size_t)rows * NH;
+	w->cst = (SaConst*)take((size_t)rows * NKV * sizeof(SaConst));
+	w->pmax = (int32_t*)take(planes * r * 4);
+	w->psum = (int64_t*)take(planes * r * 8);
+	w->hst = (int32_t*)take(r * 4);
+	w->part = (int32_t*)take(planes * r * D * 4);
+	return at;
+}
+
 size_t shared_attn_workspace(int rows, int NH, int NKV, int D, int prefixes, int64_t max_prefix, int64_t max_own) {
-	return up256((size_t)rows * NH * D * 4) + up256((size_t)rows * NH * 4);
+	SaWork w;
+	return sa_work(sa_plan(rows, NH, NKV, prefixes, max_prefix, max_own), rows, NH, NKV, D, nullptr, &w);
+}
+
+template <int D>
+static void sa_launch(const SharedAttnArgs& a, const SaPlan& p, const SaWork& w, hipStream_t s) {
+	const dim3 grid(p.shared_blocks + (a.rows * a.NKV * p.ht * p.owned + kSaWaves - 1) / kSaWaves), block(64 * kSaWaves);
+	hipLaunchKernelGGL(k_sa_max<D>, grid, block, 0, s, a, p, w);
+	hipLaunchKernelGGL(k_sa_sum<D>, grid, block, 0, s, a, p, w);
+	hipLaunchKernelGGL(k_sa_pv<D>, grid, block, 0, s, a, p, w);
 }
 
 void shared_attn(const SharedAttnArgs& a, hipStream_t s) {
-	int32_t* f = (int32_t*)a.ws;
-	int32_t* hst = (int32_t*)((char*)a.ws + up256((size_t)a.rows * a.NH * a.D * 4));
-	const dim3 grid(a.NH, a.rows);
+	const SaPlan p = sa_plan(a.rows, a.NH, a.NKV, a.prefixes, a.max_prefix, a.max_own);
+	SaWork w;
+	sa_work(p, a.rows, a.NH, a.NKV, a.D, (char*)a.ws, &w);
 	switch (a.D) {
-		case 32: hipLaunchKernelGGL(k_shared_attn_row<32>, grid, dim3(256), 0, s, a, f, hst); break;
-		case 64: hipLaunchKernelGGL(k_shared_attn_row<64>, grid, dim3(256), 0, s, a, f, hst); break;
-		case 128: hipLaunchKernelGGL(k_shared_attn_row<128>, grid, dim3(256), 0, s, a, f, hst); break;
-		default: hipLaunchKernelGGL(k_shared_attn_row<256>, grid, dim3(256), 0, s, a, f, hst); break;
+		case 32: sa_launch<32>(a, p, w, s); break;
+		case 64: sa_launch<64>(a, p, w, s); break;
+		case 128: sa_launch<128>(a, p, w, s); break;
+		default: sa_launch<256>(a, p, w, s); break;
 	}
-	hipLaunchKernelGGL((k_ctx_funnel<1024, 8>), dim3(a.rows), dim3(1024), 0, s, a, f, hst);
+	const int units = a.NH * a.D / 4;
+	if (units <= 512) hipLaunchKernelGGL((k_sa_out<512, 1>), dim3(a.rows), dim3(512), 0, s, a, p, w);
+	else if (units <= 1024) hipLaunchKernelGGL((k_sa_out<512, 2>), dim3(a.rows), dim3(512), 0, s, a, p, w);
+	else hipLaunchKernelGGL((k_sa_out<512, 4>), dim3(a.rows), dim3(512), 0, s, a, p, w);
 }
 
 size_t lora_gemm_workspace(int m, int n, int k) { return up256((size_t)m * n * 4) + up256((size_t)m * kMaxRank); }
