@@ -631,14 +631,25 @@ __device__ __forceinline__ bool row_adapter(const sslm_launch::LoraGemmArgs& g, 
 	return true;
 }
 
-// u = clamp(amp_fold(A x)) of a row (forward_sites.cpp:1066-1086), one wave per rank.
-__global__ __launch_bounds__(256) void k_rows_u(sslm_launch::LoraGemmArgs g, int8_t* u) {
-	const int t = blockIdx.x, rk = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+// u = clamp(amp_fold(A x)) of a row (forward_sites.cpp:1066-1086), one wave per rank: waves `wave` of row t.
+__device__ __forceinline__ void rows_u(const sslm_launch::LoraGemmArgs& g, int t, int rk, int8_t* u) {
+	const int lane = threadIdx.x & 63;
 	const LoraRef* ad;
 	if (!row_adapter(g, t, &ad) || !ad || rk >= ad->rank) return;
 	const int8_t *x = g.a + (size_t)t * g.k, *w = ad->a + (size_t)rk * g.k;
-	int32_t acc = 0;  // |A.x| <= 127^2 k < 2^31
-	for (int c = lane * 16; c < g.k; c += 1024) {
+	int32_t acc = 0;  // |A.x| <= 128^2 k <= 2^29
+	int c = lane * 16;
+	for (; c + 3072 < g.k; c += 4096) {  // four loads of each in flight
+		v4i p[4], q[4];
+#pragma unroll
+		for (int i = 0; i < 4; ++i) {
+			p[i] = load16(x + c + 1024 * i);
+			q[i] = load16(w + c + 1024 * i);
+		}
+#pragma unroll
+		for (int i = 0; i < 16; ++i) acc = __builtin_amdgcn_sdot4(p[i >> 2][i & 3], q[i >> 2][i & 3], acc, false);
+	}
+	for (; c < g.k; c += 1024) {
 		const v4i p = load16(x + c), q = load16(w + c);
 #pragma unroll
 		for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_sdot4(p[j], q[j], acc, false);
@@ -650,51 +661,177 @@ __global__ __launch_bounds__(256) void k_rows_u(sslm_launch::LoraGemmArgs g, int
 	}
 }
 
-// Fold, adapter delta and funnel of a row of accumulators.
-template <int BS, int EPT>
-__global__ __launch_bounds__(BS) void k_lora_funnel(sslm_launch::LoraGemmArgs g, const int32_t* acc, const int8_t* u) {
-	__shared__ uint32_t s_m[BS / 64];
-	const int t = blockIdx.x;
-	const LoraRef* ad;
-	if (!row_adapter(g, t, &ad)) {
-		if (threadIdx.x == 0) g.status[t] = kBadAdapter;
+__global__ __launch_bounds__(256) void k_rows_u(sslm_launch::LoraGemmArgs g, int8_t* u) {
+	rows_u(g, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 6), u);
+}
+
+// The products of up to 64 rows and their adapters' u in one launch, neither waiting for the other.
+// A block holds 16 columns and one plane's share of K, cut over its four waves; each lane streams 16
+// bytes of its column's weights per 64-byte chunk (kLoraChunks loads in flight, the weights being what
+// has to be read) against MB MFMA tiles of 16 rows, whose codes come from L2.  The waves' int32 sums are
+// joined in LDS and stored as plane blockIdx / tiles of [planes][m][n].  Blocks past the products' do
+// rows_u: 16 of them per row, four ranks each.
+constexpr int kLoraChunks = 4;
+template <int MB>
+__global__ __launch_bounds__(256) void k_lora_proj(sslm_launch::LoraGemmArgs g, int planes, int32_t* part, int8_t* u) {
+	__shared__ v4i s_acc[3][MB][64];
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ri = lane & 15, gr = lane >> 4, tiles = g.n / 16;
+	if ((int)blockIdx.x >= tiles * planes) {
+		const int b = blockIdx.x - tiles * planes;
+		rows_u(g, b >> 4, (b & 15) * 4 + wave, u);
 		return;
 	}
-	const int rank = ad ? ad->rank : 0;
-	const int8_t* ur = u + (size_t)t * kMaxRank;
-	int32_t v[EPT];
-	uint32_t mx = 0;
+	const int tile = blockIdx.x % tiles, plane = blockIdx.x / tiles, chunks = (g.k + 63) / 64;
+	const int per = (chunks + planes * 4 - 1) / (planes * 4), c0 = (plane * 4 + wave) * per, c1 = min(chunks, c0 + per);
+	const int8_t* w = g.w + (size_t)(tile * 16 + ri) * g.k + gr * 16;
+	const int8_t* x[MB];
 #pragma unroll
-	for (int k = 0; k < EPT; ++k) {
-		const int j = (int)threadIdx.x + k * BS;
-		v[k] = 0;
-		if (j < g.n) {
-			const int32_t* fd = g.fold + 3 * j;
-			int64_t x = apply_fold((int64_t)acc[(size_t)t * g.n + j], fd[0], fd[1], fd[2]);
-			if (ad) {
-				const int8_t* b = ad->b + (size_t)j * rank;
-				int32_t d = 0;  // |B.u| <= 127^2 64 < 2^31
-				for (int i = 0; i < rank; ++i) d += (int32_t)b[i] * (int32_t)ur[i];
-				const int32_t* df = ad->dfold + 3 * j;
-				x += apply_amp_fold((int64_t)d, df[0], df[1], df[2]);
-			}
-			mx = max(mx, sat_abs_u32(x));
-			v[k] = sat_i32(x);
+	for (int i = 0; i < MB; ++i) x[i] = g.a + (size_t)min(i * 16 + ri, g.m - 1) * g.k + gr * 16;
+	v4i acc[MB];
+#pragma unroll
+	for (int i = 0; i < MB; ++i) acc[i] = v4i{0, 0, 0, 0};
+	for (int c = c0; c < c1; c += kLoraChunks) {
+		v4i wf[kLoraChunks], xf[MB][kLoraChunks];
+#pragma unroll
+		for (int e = 0; e < kLoraChunks; ++e) {
+			// past the range or K: row 0's bytes, taken as zero on the weights' side
+			const bool in = c + e < c1 && (c + e) * 64 + gr * 16 < g.k;
+			const int off = in ? (c + e) * 64 : -gr * 16;
+			wf[e] = load16(w + off);
+#pragma unroll
+			for (int i = 0; i < MB; ++i) xf[i][e] = load16(x[i] + off);
+			if (!in) wf[e] = v4i{0, 0, 0, 0};
+		}
+#pragma unroll
+		for (int e = 0; e < kLoraChunks; ++e)
+#pragma unroll
+			for (int i = 0; i < MB; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[e], xf[i][e], acc[i], 0, 0, 0);
+	}
+	if (wave) {
+#pragma unroll
+		for (int i = 0; i < MB; ++i) s_acc[wave - 1][i][lane] = acc[i];
+	}
+	__syncthreads();
+	if (wave) return;
+	// lane (ri, gr): columns 16 tile + 4 gr .. + 3 of row 16 i + ri
+#pragma unroll
+	for (int i = 0; i < MB; ++i) {
+		const v4i o = acc[i] + s_acc[0][i][lane] + s_acc[1][i][lane] + s_acc[2][i][lane];
+		const int t = i * 16 + ri;
+		if (t < g.m) *(v4i*)(part + ((size_t)plane * g.m + t) * g.n + tile * 16 + gr * 4) = o;
+	}
+}
+
+// A row's u as dot operands of a B row: pieces of 16 bytes (4 where the rank is below 16) at byte
+// min(16 q, rank - 16); the last piece's bytes that an earlier one holds are zero.
+__device__ __forceinline__ int lora_piece(int q, int rank, int w) { return min(w * q, rank - w); }
+
+struct __attribute__((packed)) unaligned16 {
+	v4i v;
+};
+struct __attribute__((packed)) unaligned4 {
+	int32_t v;
+};
+
+__device__ __forceinline__ int32_t lora_dot(const int8_t* b, const int8_t* su, int rank) {
+	int32_t d = 0;  // |B.u| <= 128 127 64 < 2^31
+	if (rank >= 16) {
+		for (int q = 0; 16 * q < rank; ++q) {
+			const v4i x = ((const unaligned16*)(b + lora_piece(q, rank, 16)))->v, y = *(const v4i*)(su + 16 * q);
+#pragma unroll
+			for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_sdot4(x[i], y[i], d, false);
+		}
+	} else if (rank >= 4) {
+		for (int q = 0; 4 * q < rank; ++q)
+			d = __builtin_amdgcn_sdot4(((const unaligned4*)(b + lora_piece(q, rank, 4)))->v, *(const int32_t*)(su + 4 * q), d, false);
+	} else {
+		for (int i = 0; i < rank; ++i) d += (int32_t)b[i] * (int32_t)su[i];
+	}
+	return d;
+}
+
+// Fold, adapter delta and funnel (forward_sites.cpp:1114-1154) of R rows of accumulators (the sum of
+// `planes` planes): the folds are read once for them, and an adapter that a row shares with the one
+// before it too.
+template <int BS, int EPT, int R>
+__global__ __launch_bounds__(BS) void k_lora_funnel(sslm_launch::LoraGemmArgs g, int planes, const int32_t* part, const int8_t* u) {
+	__shared__ __attribute__((aligned(16))) int8_t s_u[R][kMaxRank];
+	__shared__ uint32_t s_m[R][BS / 64];
+	const int t0 = blockIdx.x * R;
+	const LoraRef* ad[R];
+	bool ok[R];
+	LoraRef ref[R];
+#pragma unroll
+	for (int r = 0; r < R; ++r) {
+		ok[r] = t0 + r < g.m && row_adapter(g, t0 + r, &ad[r]);
+		if (!ok[r]) ad[r] = nullptr;
+		ref[r] = ad[r] ? *ad[r] : LoraRef{};
+		const int rank = ref[r].rank, w = rank >= 16 ? 16 : (rank >= 4 ? 4 : 1), i = threadIdx.x;
+		if (i < kMaxRank) {
+			const int q = i / w, at = w == 1 ? i : lora_piece(q, rank, w) + i % w;
+			s_u[r][i] = w * q < rank && at >= w * q ? u[(size_t)(t0 + r) * kMaxRank + at] : (int8_t)0;
 		}
 	}
-	mx = block_max_u32<BS>(mx, s_m);
-	FunnelPlan plan;
-	const Scale in = g.in_scale[t];
-	const int32_t st = funnel_plan(mx, &in, 1, g.site, &plan);
-	if (threadIdx.x == 0) {
-		g.status[t] = st;
-		if (st == kOk) g.scales[t] = plan.out;
-	}
-	if (st != kOk) return;
+	__syncthreads();
+	int32_t v[R][EPT];
+	uint32_t mx[R] = {};
 #pragma unroll
 	for (int k = 0; k < EPT; ++k) {
 		const int j = (int)threadIdx.x + k * BS;
-		if (j < g.n) g.codes[(size_t)t * g.n + j] = requant_code_f(v[k], plan.f);
+#pragma unroll
+		for (int r = 0; r < R; ++r) v[r][k] = 0;
+		if (j < g.n) {
+			const int32_t* fd = g.fold + 3 * j;
+			const FoldConsts fc = fold_consts(fd[0], fd[1], fd[2]);  // |acc| <= 128^2 k <= 2^29
+			int32_t df[3];
+#pragma unroll
+			for (int r = 0; r < R; ++r) {
+				if (R > 1 && !ok[r]) continue;
+				int32_t acc = 0;
+				for (int p = 0; p < planes; ++p) acc += part[((size_t)p * g.m + t0 + r) * g.n + j];
+				int64_t x = fold_bounded(acc, fc);
+				if (ad[r]) {
+					if (r == 0 || ad[r] != ad[r - 1]) {
+#pragma unroll
+						for (int i = 0; i < 3; ++i) df[i] = ref[r].dfold[3 * j + i];
+					}
+					x += apply_amp_fold((int64_t)lora_dot(ref[r].b + (size_t)j * ref[r].rank, s_u[r], ref[r].rank), df[0], df[1], df[2]);
+				}
+				mx[r] = max(mx[r], sat_abs_u32(x));
+				v[r][k] = sat_i32(x);
+			}
+		}
+	}
+#pragma unroll
+	for (int r = 0; r < R; ++r) {
+		mx[r] = wave_max32(mx[r]);
+		if ((threadIdx.x & 63) == 0) s_m[r][threadIdx.x >> 6] = mx[r];
+	}
+	__syncthreads();
+#pragma unroll
+	for (int r = 0; r < R; ++r) {
+		const int t = t0 + r;
+		if (t >= g.m) return;
+		if (!ok[r]) {
+			if (threadIdx.x == 0) g.status[t] = kBadAdapter;
+			continue;
+		}
+		uint32_t m = s_m[r][0];
+#pragma unroll
+		for (int i = 1; i < BS / 64; ++i) m = max(m, s_m[r][i]);
+		FunnelPlan plan;
+		const Scale in = g.in_scale[t];
+		const int32_t st = funnel_plan(__builtin_amdgcn_readfirstlane(m), &in, 1, g.site, &plan);
+		if (threadIdx.x == 0) {
+			g.status[t] = st;
+			if (st == kOk) g.scales[t] = plan.out;
+		}
+		if (st != kOk) continue;
+#pragma unroll
+		for (int k = 0; k < EPT; ++k) {
+			const int j = (int)threadIdx.x + k * BS;
+			if (j < g.n) g.codes[(size_t)t * g.n + j] = requant_code_f(v[r][k], plan.f);
+		}
 	}
 }
 
@@ -868,22 +1005,46 @@ void shared_attn(const SharedAttnArgs& a, hipStream_t s) {
 	else hipLaunchKernelGGL((k_sa_out<512, 4>), dim3(a.rows), dim3(512), 0, s, a, p, w);
 }
 
-size_t lora_gemm_workspace(int m, int n, int k) { return up256((size_t)m * n * 4) + up256((size_t)m * kMaxRank); }
+// Planes of k_lora_proj: a wave's share of K at most some ten chunks of 64 bytes, where that takes more
+// than one plane (their sums are read back by the funnel).
+static int lora_planes(int k) { return std::min(8, ((k + 63) / 64 + 39) / 40); }
+constexpr int kLoraProjRows = 64;  // rows k_lora_proj takes; past them the prefill GEMM and k_rows_u
+
+size_t lora_gemm_workspace(int m, int n, int k) {
+	const int planes = m <= kLoraProjRows ? lora_planes(k) : 1;
+	return up256((size_t)planes * m * n * 4) + up256((size_t)m * kMaxRank);
+}
+
+template <int EPT, int R>
+static void lora_funnel(const LoraGemmArgs& g, int planes, const int32_t* part, const int8_t* u, hipStream_t s) {
+	hipLaunchKernelGGL((k_lora_funnel<512, EPT, R>), dim3((g.m + R - 1) / R), dim3(512), 0, s, g, planes, part, u);
+}
 
 void lora_gemm(const LoraGemmArgs& g, hipStream_t s) {
-	int32_t* acc = (int32_t*)g.ws;
-	int8_t* u = (int8_t*)g.ws + up256((size_t)g.m * g.n * 4);
-	GemmArgs ga{};
-	ga.a = g.a;
-	ga.w = g.w;
-	ga.M = g.m;
-	ga.N = g.n;
-	ga.K = g.k;
-	ga.lda = g.k;
-	ga.epi.raw_out = acc;
-	gemm(ga, s);
-	hipLaunchKernelGGL(k_rows_u, dim3(g.m, kMaxRank / 4), dim3(256), 0, s, g, u);
-	hipLaunchKernelGGL((k_lora_funnel<1024, 8>), dim3(g.m), dim3(1024), 0, s, g, acc, u);
+	const int planes = g.m <= kLoraProjRows ? lora_planes(g.k) : 1;
+	int32_t* part = (int32_t*)g.ws;
+	int8_t* u = (int8_t*)g.ws + up256((size_t)planes * g.m * g.n * 4);
+	if (g.m <= kLoraProjRows) {
+		const dim3 grid(g.n / 16 * planes + (g.count > 0 ? g.m * (kMaxRank / 4) : 0));
+		if (g.m <= 16) hipLaunchKernelGGL(k_lora_proj<1>, grid, dim3(256), 0, s, g, planes, part, u);
+		else if (g.m <= 32) hipLaunchKernelGGL(k_lora_proj<2>, grid, dim3(256), 0, s, g, planes, part, u);
+		else hipLaunchKernelGGL(k_lora_proj<4>, grid, dim3(256), 0, s, g, planes, part, u);
+	} else {
+		GemmArgs ga{};
+		ga.a = g.a;
+		ga.w = g.w;
+		ga.M = g.m;
+		ga.N = g.n;
+		ga.K = g.k;
+		ga.lda = g.k;
+		ga.epi.raw_out = part;
+		gemm(ga, s);
+		if (g.count > 0) hipLaunchKernelGGL(k_rows_u, dim3(g.m, kMaxRank / 4), dim3(256), 0, s, g, u);
+	}
+	const bool many = g.m > kLoraProjRows;
+	if (g.n <= 2048) many ? lora_funnel<4, 2>(g, planes, part, u, s) : lora_funnel<4, 1>(g, planes, part, u, s);
+	else if (g.n <= 5120) many ? lora_funnel<10, 2>(g, planes, part, u, s) : lora_funnel<10, 1>(g, planes, part, u, s);
+	else many ? lora_funnel<16, 2>(g, planes, part, u, s) : lora_funnel<16, 1>(g, planes, part, u, s);
 }
 
 static int pick_slices(int vocab) { return (vocab + kPickSlice - 1) / kPickSlice; }

@@ -53,7 +53,7 @@ def lora(ops, **change):
 
 @pytest.mark.parametrize("change,status", [
     ({"m": 0}, INVALID), ({"m": 513}, INVALID), ({"n": 0}, INVALID), ({"n": 24}, INVALID), ({"n": 8208}, INVALID),
-    ({"k": 0}, INVALID), ({"k": 24}, INVALID), ({"k": 65552}, INVALID), ({"adapter_count": -1}, INVALID),
+    ({"k": 0}, INVALID), ({"k": 24}, INVALID), ({"k": 32784}, INVALID), ({"adapter_count": -1}, INVALID),
     ({"a": ANY + 8}, INVALID), ({"w": ANY + 1}, INVALID),
     *[({k: None}, INVALID) for k in ("a", "w", "fold", "in_scale", "adapters", "row_adapter", "codes", "scales", "status",
                                      "workspace")],
