@@ -631,6 +631,8 @@ __device__ __forceinline__ bool row_adapter(const sslm_launch::LoraGemmArgs& g, 
 	return true;
 }
 
+constexpr int kUChunks = 5;
+
 // u = clamp(amp_fold(A x)) of a row (forward_sites.cpp:1066-1086), one wave per rank: waves `wave` of row t.
 __device__ __forceinline__ void rows_u(const sslm_launch::LoraGemmArgs& g, int t, int rk, int8_t* u) {
 	const int lane = threadIdx.x & 63;
@@ -638,21 +640,21 @@ __device__ __forceinline__ void rows_u(const sslm_launch::LoraGemmArgs& g, int t
 	if (!row_adapter(g, t, &ad) || !ad || rk >= ad->rank) return;
 	const int8_t *x = g.a + (size_t)t * g.k, *w = ad->a + (size_t)rk * g.k;
 	int32_t acc = 0;  // |A.x| <= 128^2 k <= 2^29
-	int c = lane * 16;
-	for (; c + 3072 < g.k; c += 4096) {  // four loads of each in flight
-		v4i p[4], q[4];
+	for (int c0 = lane * 16; c0 < g.k; c0 += 1024 * kUChunks) {  // kUChunks loads of each in flight
+		v4i p[kUChunks], q[kUChunks];
 #pragma unroll
-		for (int i = 0; i < 4; ++i) {
-			p[i] = load16(x + c + 1024 * i);
-			q[i] = load16(w + c + 1024 * i);
+		for (int i = 0; i < kUChunks; ++i) {
+			const int c = min(c0 + 1024 * i, g.k - 16);
+			p[i] = load16(x + c);
+			q[i] = load16(w + c);
 		}
+		__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-		for (int i = 0; i < 16; ++i) acc = __builtin_amdgcn_sdot4(p[i >> 2][i & 3], q[i >> 2][i & 3], acc, false);
-	}
-	for (; c < g.k; c += 1024) {
-		const v4i p = load16(x + c), q = load16(w + c);
+		for (int i = 0; i < kUChunks; ++i) {
+			if (c0 + 1024 * i >= g.k) p[i] = v4i{0, 0, 0, 0};
 #pragma unroll
-		for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_sdot4(p[j], q[j], acc, false);
+			for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_sdot4(p[i][j], q[i][j], acc, false);
+		}
 	}
 	acc = wave_sum32(acc);
 	if (lane == 0) {
@@ -667,12 +669,11 @@ __global__ __launch_bounds__(256) void k_rows_u(sslm_launch::LoraGemmArgs g, int
 
 // The products of up to 64 rows and their adapters' u in one launch, neither waiting for the other.
 // A block holds 16 columns and one plane's share of K, cut over its four waves; each lane streams 16
-// bytes of its column's weights per 64-byte chunk (kLoraChunks loads in flight, the weights being what
-// has to be read) against MB MFMA tiles of 16 rows, whose codes come from L2.  The waves' int32 sums are
+// bytes of its column's weights per 64-byte chunk (KC loads in flight, the weights being what has to be
+// read) against MB MFMA tiles of 16 rows, whose codes come from L2.  The waves' int32 sums are
 // joined in LDS and stored as plane blockIdx / tiles of [planes][m][n].  Blocks past the products' do
 // rows_u: 16 of them per row, four ranks each.
-constexpr int kLoraChunks = 4;
-template <int MB>
+template <int MB, int KC>
 __global__ __launch_bounds__(256) void k_lora_proj(sslm_launch::LoraGemmArgs g, int planes, int32_t* part, int8_t* u) {
 	__shared__ v4i s_acc[3][MB][64];
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ri = lane & 15, gr = lane >> 4, tiles = g.n / 16;
@@ -690,20 +691,23 @@ __global__ __launch_bounds__(256) void k_lora_proj(sslm_launch::LoraGemmArgs g, 
 	v4i acc[MB];
 #pragma unroll
 	for (int i = 0; i < MB; ++i) acc[i] = v4i{0, 0, 0, 0};
-	for (int c = c0; c < c1; c += kLoraChunks) {
-		v4i wf[kLoraChunks], xf[MB][kLoraChunks];
+	for (int c = c0; c < c1; c += KC) {
+		v4i wf[KC], xf[MB][KC];
 #pragma unroll
-		for (int e = 0; e < kLoraChunks; ++e) {
+		for (int e = 0; e < KC; ++e) {
 			// past the range or K: row 0's bytes, taken as zero on the weights' side
 			const bool in = c + e < c1 && (c + e) * 64 + gr * 16 < g.k;
 			const int off = in ? (c + e) * 64 : -gr * 16;
 			wf[e] = load16(w + off);
 #pragma unroll
 			for (int i = 0; i < MB; ++i) xf[i][e] = load16(x[i] + off);
-			if (!in) wf[e] = v4i{0, 0, 0, 0};
 		}
+		__builtin_amdgcn_sched_barrier(0);  // every load issued before the first is waited for
 #pragma unroll
-		for (int e = 0; e < kLoraChunks; ++e)
+		for (int e = 0; e < KC; ++e)
+			if (c + e >= c1 || (c + e) * 64 + gr * 16 >= g.k) wf[e] = v4i{0, 0, 0, 0};
+#pragma unroll
+		for (int e = 0; e < KC; ++e)
 #pragma unroll
 			for (int i = 0; i < MB; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[e], xf[i][e], acc[i], 0, 0, 0);
 	}
@@ -733,79 +737,109 @@ struct __attribute__((packed)) unaligned4 {
 	int32_t v;
 };
 
-__device__ __forceinline__ int32_t lora_dot(const int8_t* b, const int8_t* su, int rank) {
-	int32_t d = 0;  // |B.u| <= 128 127 64 < 2^31
-	if (rank >= 16) {
-		for (int q = 0; 16 * q < rank; ++q) {
-			const v4i x = ((const unaligned16*)(b + lora_piece(q, rank, 16)))->v, y = *(const v4i*)(su + 16 * q);
-#pragma unroll
-			for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_sdot4(x[i], y[i], d, false);
-		}
-	} else if (rank >= 4) {
-		for (int q = 0; 4 * q < rank; ++q)
-			d = __builtin_amdgcn_sdot4(((const unaligned4*)(b + lora_piece(q, rank, 4)))->v, *(const int32_t*)(su + 4 * q), d, false);
-	} else {
-		for (int i = 0; i < rank; ++i) d += (int32_t)b[i] * (int32_t)su[i];
-	}
-	return d;
-}
-
 // Fold, adapter delta and funnel (forward_sites.cpp:1114-1154) of R rows of accumulators (the sum of
-// `planes` planes): the folds are read once for them, and an adapter that a row shares with the one
-// before it too.
-template <int BS, int EPT, int R>
-__global__ __launch_bounds__(BS) void k_lora_funnel(sslm_launch::LoraGemmArgs g, int planes, const int32_t* part, const int8_t* u) {
+// PL planes), whose folds are read once for them.  Every load of a thread's EPT columns is issued
+// from a clamped index before the first is used: taken column by column they cost a round trip each.
+template <int BS, int EPT, int R, int PL>
+__global__ __launch_bounds__(BS) void k_lora_funnel(sslm_launch::LoraGemmArgs g, const int32_t* part, const int8_t* u) {
 	__shared__ __attribute__((aligned(16))) int8_t s_u[R][kMaxRank];
 	__shared__ uint32_t s_m[R][BS / 64];
 	const int t0 = blockIdx.x * R;
+	int32_t v[R][EPT];
+	int col[EPT];
+#pragma unroll
+	for (int k = 0; k < EPT; ++k) col[k] = min((int)threadIdx.x + k * BS, g.n - 1);
+	int32_t fd[EPT][3];
+#pragma unroll
+	for (int k = 0; k < EPT; ++k)
+#pragma unroll
+		for (int i = 0; i < 3; ++i) fd[k][i] = g.fold[3 * col[k] + i];
 	const LoraRef* ad[R];
 	bool ok[R];
 	LoraRef ref[R];
 #pragma unroll
 	for (int r = 0; r < R; ++r) {
-		ok[r] = t0 + r < g.m && row_adapter(g, t0 + r, &ad[r]);
-		if (!ok[r]) ad[r] = nullptr;
-		ref[r] = ad[r] ? *ad[r] : LoraRef{};
+		const int t = min(t0 + r, g.m - 1);
+		const int32_t* at = part + (size_t)t * g.n;
+		int32_t pv[PL][EPT];
+#pragma unroll
+		for (int p = 0; p < PL; ++p)
+#pragma unroll
+			for (int k = 0; k < EPT; ++k) pv[p][k] = at[(size_t)p * g.m * g.n + col[k]];
+#pragma unroll
+		for (int k = 0; k < EPT; ++k) {
+			v[r][k] = pv[0][k];
+#pragma unroll
+			for (int p = 1; p < PL; ++p) v[r][k] += pv[p][k];
+		}
+		ok[r] = row_adapter(g, t, &ad[r]);
+		ref[r] = ok[r] && ad[r] ? *ad[r] : LoraRef{};
 		const int rank = ref[r].rank, w = rank >= 16 ? 16 : (rank >= 4 ? 4 : 1), i = threadIdx.x;
 		if (i < kMaxRank) {
-			const int q = i / w, at = w == 1 ? i : lora_piece(q, rank, w) + i % w;
-			s_u[r][i] = w * q < rank && at >= w * q ? u[(size_t)(t0 + r) * kMaxRank + at] : (int8_t)0;
+			const int q = i / w, from = w == 1 ? i : lora_piece(q, rank, w) + i % w;
+			s_u[r][i] = w * q < rank && from >= w * q ? u[(size_t)t * kMaxRank + from] : (int8_t)0;
 		}
 	}
 	__syncthreads();
-	int32_t v[R][EPT];
-	uint32_t mx[R] = {};
-#pragma unroll
-	for (int k = 0; k < EPT; ++k) {
-		const int j = (int)threadIdx.x + k * BS;
-#pragma unroll
-		for (int r = 0; r < R; ++r) v[r][k] = 0;
-		if (j < g.n) {
-			const int32_t* fd = g.fold + 3 * j;
-			const FoldConsts fc = fold_consts(fd[0], fd[1], fd[2]);  // |acc| <= 128^2 k <= 2^29
-			int32_t df[3];
-#pragma unroll
-			for (int r = 0; r < R; ++r) {
-				if (R > 1 && !ok[r]) continue;
-				int32_t acc = 0;
-				for (int p = 0; p < planes; ++p) acc += part[((size_t)p * g.m + t0 + r) * g.n + j];
-				int64_t x = fold_bounded(acc, fc);
-				if (ad[r]) {
-					if (r == 0 || ad[r] != ad[r - 1]) {
-#pragma unroll
-						for (int i = 0; i < 3; ++i) df[i] = ref[r].dfold[3 * j + i];
-					}
-					x += apply_amp_fold((int64_t)lora_dot(ref[r].b + (size_t)j * ref[r].rank, s_u[r], ref[r].rank), df[0], df[1], df[2]);
-				}
-				mx[r] = max(mx[r], sat_abs_u32(x));
-				v[r][k] = sat_i32(x);
-			}
-		}
-	}
 #pragma unroll
 	for (int r = 0; r < R; ++r) {
-		mx[r] = wave_max32(mx[r]);
-		if ((threadIdx.x & 63) == 0) s_m[r][threadIdx.x >> 6] = mx[r];
+		const int rank = ref[r].rank;
+		uint32_t mx = 0;
+		if (rank > 0) {
+			int32_t d[EPT] = {}, df[EPT][3];  // |B.u| <= 128 127 64 < 2^31
+#pragma unroll
+			for (int k = 0; k < EPT; ++k)
+#pragma unroll
+				for (int i = 0; i < 3; ++i) df[k][i] = ref[r].dfold[3 * col[k] + i];
+			if (rank >= 16) {
+				constexpr int PQ = EPT <= 5 ? 2 : 1;  // pieces in flight; past the rank u is zero
+				for (int q = 0; 16 * q < rank; q += PQ) {
+					v4i x[PQ][EPT];
+#pragma unroll
+					for (int e = 0; e < PQ; ++e)
+#pragma unroll
+						for (int k = 0; k < EPT; ++k)
+							x[e][k] = ((const unaligned16*)(ref[r].b + (size_t)col[k] * rank + lora_piece(q + e, rank, 16)))->v;
+#pragma unroll
+					for (int e = 0; e < PQ; ++e) {
+						const v4i y = *(const v4i*)(s_u[r] + 16 * (q + e));
+#pragma unroll
+						for (int k = 0; k < EPT; ++k)
+#pragma unroll
+							for (int i = 0; i < 4; ++i) d[k] = __builtin_amdgcn_sdot4(x[e][k][i], y[i], d[k], false);
+					}
+				}
+			} else if (rank >= 4) {
+				for (int q = 0; 4 * q < rank; ++q) {
+					const int8_t* b = ref[r].b + lora_piece(q, rank, 4);
+					const int32_t y = *(const int32_t*)(s_u[r] + 4 * q);
+					int32_t x[EPT];
+#pragma unroll
+					for (int k = 0; k < EPT; ++k) x[k] = ((const unaligned4*)(b + (size_t)col[k] * rank))->v;
+#pragma unroll
+					for (int k = 0; k < EPT; ++k) d[k] = __builtin_amdgcn_sdot4(x[k], y, d[k], false);
+				}
+			} else {
+				for (int i = 0; i < rank; ++i)
+#pragma unroll
+					for (int k = 0; k < EPT; ++k) d[k] += (int32_t)ref[r].b[(size_t)col[k] * rank + i] * (int32_t)s_u[r][i];
+			}
+#pragma unroll
+			for (int k = 0; k < EPT; ++k) {
+				const int64_t x = (int64_t)fold_bounded(v[r][k], fold_consts(fd[k][0], fd[k][1], fd[k][2])) +
+				                  apply_amp_fold((int64_t)d[k], df[k][0], df[k][1], df[k][2]);
+				mx = max(mx, sat_abs_u32(x));  // a clamped column repeats the last one
+				v[r][k] = sat_i32(x);
+			}
+		} else {
+#pragma unroll
+			for (int k = 0; k < EPT; ++k) {
+				v[r][k] = fold_bounded(v[r][k], fold_consts(fd[k][0], fd[k][1], fd[k][2]));  // |acc| <= 128^2 k <= 2^29
+				mx = max(mx, sat_abs_u32(v[r][k]));
+			}
+		}
+		mx = wave_max32(mx);
+		if ((threadIdx.x & 63) == 0) s_m[r][threadIdx.x >> 6] = mx;
 	}
 	__syncthreads();
 #pragma unroll
@@ -1005,9 +1039,13 @@ void shared_attn(const SharedAttnArgs& a, hipStream_t s) {
 	else hipLaunchKernelGGL((k_sa_out<512, 4>), dim3(a.rows), dim3(512), 0, s, a, p, w);
 }
 
-// Planes of k_lora_proj: a wave's share of K at most some ten chunks of 64 bytes, where that takes more
-// than one plane (their sums are read back by the funnel).
-static int lora_planes(int k) { return std::min(8, ((k + 63) / 64 + 39) / 40); }
+// Planes of k_lora_proj (a power of two): a wave's share of K at most ten chunks of 64 bytes, where that
+// takes more than one plane (their sums are read back by the funnel).
+static int lora_planes(int k) {
+	int p = 1;
+	while (p < 8 && (k + 63) / 64 > 40 * p) p *= 2;
+	return p;
+}
 constexpr int kLoraProjRows = 64;  // rows k_lora_proj takes; past them the prefill GEMM and k_rows_u
 
 size_t lora_gemm_workspace(int m, int n, int k) {
@@ -1015,9 +1053,15 @@ size_t lora_gemm_workspace(int m, int n, int k) {
 	return up256((size_t)planes * m * n * 4) + up256((size_t)m * kMaxRank);
 }
 
-template <int EPT, int R>
+template <int BS, int EPT, int R>
 static void lora_funnel(const LoraGemmArgs& g, int planes, const int32_t* part, const int8_t* u, hipStream_t s) {
-	hipLaunchKernelGGL((k_lora_funnel<512, EPT, R>), dim3((g.m + R - 1) / R), dim3(512), 0, s, g, planes, part, u);
+	const dim3 grid((g.m + R - 1) / R), block(BS);
+	switch (planes) {
+		case 1: hipLaunchKernelGGL((k_lora_funnel<BS, EPT, R, 1>), grid, block, 0, s, g, part, u); break;
+		case 2: hipLaunchKernelGGL((k_lora_funnel<BS, EPT, R, 2>), grid, block, 0, s, g, part, u); break;
+		case 4: hipLaunchKernelGGL((k_lora_funnel<BS, EPT, R, 4>), grid, block, 0, s, g, part, u); break;
+		default: hipLaunchKernelGGL((k_lora_funnel<BS, EPT, R, 8>), grid, block, 0, s, g, part, u); break;
+	}
 }
 
 void lora_gemm(const LoraGemmArgs& g, hipStream_t s) {
@@ -1026,9 +1070,15 @@ void lora_gemm(const LoraGemmArgs& g, hipStream_t s) {
 	int8_t* u = (int8_t*)g.ws + up256((size_t)planes * g.m * g.n * 4);
 	if (g.m <= kLoraProjRows) {
 		const dim3 grid(g.n / 16 * planes + (g.count > 0 ? g.m * (kMaxRank / 4) : 0));
-		if (g.m <= 16) hipLaunchKernelGGL(k_lora_proj<1>, grid, dim3(256), 0, s, g, planes, part, u);
-		else if (g.m <= 32) hipLaunchKernelGGL(k_lora_proj<2>, grid, dim3(256), 0, s, g, planes, part, u);
-		else hipLaunchKernelGGL(k_lora_proj<4>, grid, dim3(256), 0, s, g, planes, part, u);
+		auto proj = [&](auto mb) {
+			// loads in flight against waves per SIMD: 3 chunks of 64 rows' codes take as many registers as
+			// let u's waves in (64 x 1536 x 8960 with 64 adapters: 15.0 us, 17.8 at 10 chunks)
+			constexpr int MB = decltype(mb)::value, KC = MB == 4 ? 3 : 4;
+			hipLaunchKernelGGL((k_lora_proj<MB, KC>), grid, dim3(256), 0, s, g, planes, part, u);
+		};
+		if (g.m <= 16) proj(std::integral_constant<int, 1>{});
+		else if (g.m <= 32) proj(std::integral_constant<int, 2>{});
+		else proj(std::integral_constant<int, 4>{});
 	} else {
 		GemmArgs ga{};
 		ga.a = g.a;
@@ -1041,10 +1091,9 @@ void lora_gemm(const LoraGemmArgs& g, hipStream_t s) {
 		gemm(ga, s);
 		if (g.count > 0) hipLaunchKernelGGL(k_rows_u, dim3(g.m, kMaxRank / 4), dim3(256), 0, s, g, u);
 	}
-	const bool many = g.m > kLoraProjRows;
-	if (g.n <= 2048) many ? lora_funnel<4, 2>(g, planes, part, u, s) : lora_funnel<4, 1>(g, planes, part, u, s);
-	else if (g.n <= 5120) many ? lora_funnel<10, 2>(g, planes, part, u, s) : lora_funnel<10, 1>(g, planes, part, u, s);
-	else many ? lora_funnel<16, 2>(g, planes, part, u, s) : lora_funnel<16, 1>(g, planes, part, u, s);
+	if (g.n <= 2048) lora_funnel<512, 4, 1>(g, planes, part, u, s);
+	else if (g.n <= 5120) lora_funnel<1024, 5, 1>(g, planes, part, u, s);
+	else lora_funnel<1024, 8, 1>(g, planes, part, u, s);
 }
 
 static int pick_slices(int vocab) { return (vocab + kPickSlice - 1) / kPickSlice; }
