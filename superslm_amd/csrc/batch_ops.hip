@@ -44,26 +44,38 @@ __device__ __forceinline__ uint32_t block_max_u32(uint32_t v, uint32_t* slots) {
 struct RowSpan {
 	int64_t width, start;
 	const int8_t *own, *pre;
-	int32_t st;
+	int32_t st, pad;
 };
 
+// All lanes of the wave call it for one row.  The tables are read a lane to a prefix, so that the row's
+// span costs two round trips whatever the number of prefixes; prefix_rows has to be a division of the
+// rows, ascending from at least 0 to at most `rows`.
 __device__ __forceinline__ RowSpan row_span(const sslm_launch::SharedAttnArgs& a, int r) {
-	RowSpan s{a.row_width[r], 0, a.pool, a.pool, kOk};
-	int p = -1;
-	for (int i = 0; i < a.prefixes; ++i)
-		if (a.prefix_rows[i] <= r && r < a.prefix_rows[i + 1]) p = i;
-	const int blk = a.row_block[r];
-	if (blk < 0 || blk >= a.blocks || s.width < 0 || s.width > a.cap) s.st = kPositionOverCap;
-	else s.own += (int64_t)blk * a.block_bytes;
-	if (p >= 0) {
-		const int pb = a.prefix_block[p];
-		const int64_t len = a.prefix_len[p];
-		if (pb < 0 || pb >= a.blocks || len < 0 || len > a.cap || len > a.max_prefix) s.st = kPositionOverCap;
-		else {
-			s.pre += (int64_t)pb * a.block_bytes;
-			s.start = len < s.width ? len : s.width;
+	RowSpan s{a.row_width[r], 0, a.pool, a.pool, kOk, 0};
+	const int blk = a.row_block[r], lane = threadIdx.x & 63;
+	bool bad = false;
+	int pb = 0;
+	int64_t len = -1;
+	for (int i0 = 0; i0 < a.prefixes; i0 += 64) {
+		const int i = min(i0 + lane, a.prefixes - 1);
+		const int x = a.prefix_rows[i], y = a.prefix_rows[i + 1], b = a.prefix_block[i];
+		const int64_t l = a.prefix_len[i];
+		bad |= x < 0 || y < x || y > a.rows;
+		const uint64_t hit = __ballot(x <= r && r < y && i0 + lane < a.prefixes);
+		if (hit) {
+			const int at = __builtin_ctzll(hit);
+			pb = __builtin_amdgcn_readlane(b, at);
+			len = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)l >> 32), at) << 32 |
+			                (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)l, at));
+			if (pb < 0 || pb >= a.blocks || len < 0 || len > a.cap || len > a.max_prefix) s.st = kPositionOverCap;
+			else {
+				s.pre = a.pool + (int64_t)pb * a.block_bytes;
+				s.start = len < s.width ? len : s.width;
+			}
 		}
 	}
+	if (__any(bad) || blk < 0 || blk >= a.blocks || s.width < 0 || s.width > a.cap) s.st = kPositionOverCap;
+	else s.own += (int64_t)blk * a.block_bytes;
 	if (s.st == kOk && s.width - s.start > a.max_own) s.st = kPositionOverCap;
 	if (s.st == kOk && s.width == 0) s.st = kSoftmaxRowWidthOutOfDomain;
 	return s;
@@ -74,22 +86,59 @@ struct RowConst {
 	int32_t st;
 };
 
-// The softmax constants of (row, KV head) (forward_sites.cpp:1805-1830).
-__device__ __forceinline__ RowConst row_const(const sslm_launch::SharedAttnArgs& a, int r, int kvh, int64_t width) {
+// The softmax constants of (row, KV head) (forward_sites.cpp:1805-1830): the general form.
+__device__ __forceinline__ RowConst row_const_general(Scale sm, int64_t ln2_q, int64_t b_q, int64_t ca_q, int64_t width) {
 	RowConst c{0, 0, 0, 0, kOk};
-	const Scale qs = a.q_scale[r];
-	const int64_t km = a.khead_m[kvh], ke = a.khead_e[kvh];
+	if (iexp_scale_constants(sm.m, sm.e, ln2_q, b_q, ca_q, &c.q_ln2, &c.q_b, &c.q_c) != 0) c.st = kIExpScaleDerivationOutOfDomain;
+	else c.st = check_softmax_width(c.q_b, c.q_c, width);
+	if (c.st == kOk) c.ceil = softmax_ceiling(c.q_b, c.q_c);
+	return c;
+}
+
+// The same in 64 bits where it fits (iexp_scale_constants' products below 2^63 and 2^126, its shifts in
+// [1, 63], check_softmax_width's q_b below 2^24): some forty scalar instructions in the row's chain of
+// latencies instead of several hundred.
+struct RowScales {
+	Scale q;
+	int64_t km, ke;
+};
+__device__ __forceinline__ RowScales row_scales(const sslm_launch::SharedAttnArgs& a, int r, int kvh) {
+	return RowScales{a.q_scale[r], a.khead_m[kvh], a.khead_e[kvh]};
+}
+__device__ __forceinline__ RowConst row_const(const sslm_launch::SharedAttnArgs& a, const RowScales& rs, int64_t width) {
+	RowConst c{0, 0, 0, 0, kOk};
+	const Scale qs = rs.q;
+	const int64_t km = rs.km, ke = rs.ke;
 	if (!fits_i32(qs.m) || !fits_i32(km)) {
 		c.st = kCarriedScaleMantissaOutOfDomain;
 		return c;
 	}
 	const Scale sm = combine_scale(qs, Scale{km, ke});
-	if (!fits_i32(sm.m)) c.st = kCarriedScaleMantissaOutOfDomain;
-	else if (iexp_scale_constants(sm.m, sm.e, a.ln2_q, a.b_q, a.ca_q, &c.q_ln2, &c.q_b, &c.q_c) != 0)
-		c.st = kIExpScaleDerivationOutOfDomain;
-	else c.st = check_softmax_width(c.q_b, c.q_c, width);
-	if (c.st == kOk) c.ceil = softmax_ceiling(c.q_b, c.q_c);
-	return c;
+	if (!fits_i32(sm.m)) {
+		c.st = kCarriedScaleMantissaOutOfDomain;
+		return c;
+	}
+	const int64_t lim = (int64_t)1 << 30;
+	// 92 + e and 154 + 2 e in [1, 63] (e <= -46 already gives the latter's bound, e >= -76 its least)
+	if (sm.m >= lim && a.ln2_q > 0 && a.ln2_q < lim && a.b_q > 0 && a.b_q < 2 * lim && a.ca_q > 0 && a.ca_q < lim && sm.e >= -76 && sm.e <= -46) {
+		const uint64_t rc = (uint64_t)reciprocal_norm(sm.m);  // in (2^31, 2^32]
+		const uint64_t ca = (uint64_t)a.ca_q * rc, lo = ca * rc, hi = __umul64hi(ca, rc);
+		const int sh = (int)(92 + sm.e), sc = (int)(154 + 2 * sm.e);  // sc even, in [2, 62]
+		const uint64_t b = (uint64_t)a.b_q * rc >> sh;
+		if ((hi >> sc) == 0 && b < ((uint64_t)1 << 24)) {
+			const uint64_t qc = hi << (64 - sc) | lo >> sc, m = b * b + qc;
+			if (qc < ((uint64_t)1 << 62) && m >= 1) {
+				c.q_ln2 = (int64_t)((uint64_t)a.ln2_q * rc >> sh);
+				c.q_b = (int64_t)b;
+				c.q_c = (int64_t)qc;
+				const bool wide = m > (uint64_t)kSoftmaxMaxSafe || width <= 0 || __umul64hi(m, (uint64_t)width) != 0 || (int64_t)(m * (uint64_t)width) < 0;
+				c.st = wide ? kSoftmaxRowWidthOutOfDomain : kOk;
+				c.ceil = wide ? 0 : (int64_t)m;
+				return c;
+			}
+		}
+	}
+	return row_const_general(sm, a.ln2_q, a.b_q, a.ca_q, width);
 }
 
 // The layout of one call's launches.  The unit of work is a wave with a tile of 16 query rows and a
@@ -115,6 +164,7 @@ struct SaConst {
 };
 
 struct SaWork {
+	RowSpan* span;  // [rows], written with cst by k_sa_max
 	SaConst* cst;   // [rows, NKV]
 	int32_t* pmax;  // [planes][rows NH]
 	int64_t* psum;  // [planes][rows NH]; negative: an i-exp value was refused
@@ -130,6 +180,7 @@ struct SaJob {
 	int64_t p0, p1;       // positions of the plane (p1: also the end of what may be read)
 	int plane, kvh;
 	int r, h;             // by lane: row and query head (r < 0: none)
+	int row;              // an own plane's row
 	int64_t start, width; // by lane: where the row's own positions begin, and its width
 	bool owned, first;    // an own plane; the row's first
 };
@@ -137,21 +188,12 @@ struct SaJob {
 __device__ __forceinline__ int64_t i64min(int64_t a, int64_t b) { return a < b ? a : b; }
 __device__ __forceinline__ int64_t i64max(int64_t a, int64_t b) { return a > b ? a : b; }
 
-// The prefixes' rows, as far as they are a division of the call's: ascending from at least 0 to at most `rows`.
-__device__ __forceinline__ bool prefix_rows_ok(const sslm_launch::SharedAttnArgs& a) {
-	bool bad = false;
-	for (int i = threadIdx.x & 63; i <= a.prefixes && a.prefixes > 0; i += 64) {
-		const int x = a.prefix_rows[i];
-		bad |= x < 0 || x > a.rows || (i > 0 && x < a.prefix_rows[i - 1]);
-	}
-	return !__any(bad);
-}
-
 // A wave of the shared planes (block `blk` of them): false when there is nothing for it to do.
-__device__ __forceinline__ bool sa_shared_job(const sslm_launch::SharedAttnArgs& a, const SaPlan& pl, int blk, SaJob* j) {
+__device__ __forceinline__ bool sa_shared_job(const sslm_launch::SharedAttnArgs& a, const SaPlan& pl, SaJob* j) {
+	const int blk = blockIdx.x;
 	// blocks go to the XCDs in turn: a (KV head, plane)'s tiles stay on one, whose L2 then holds its K/V
 	const int tb = (pl.tiles + kSaWaves - 1) / kSaWaves, grp = (blk / 8 / tb) * 8 + blk % 8;
-	int tile = (blk / 8) % tb * kSaWaves + ((int)threadIdx.x >> 6);
+	int tile = (blk / 8) % tb * kSaWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	if (grp >= a.NKV * pl.shared || tile >= pl.tiles) return false;
 	j->plane = grp / a.NKV;
 	j->kvh = grp % a.NKV;
@@ -183,26 +225,29 @@ __device__ __forceinline__ bool sa_shared_job(const sslm_launch::SharedAttnArgs&
 	return true;
 }
 
-// A wave of the own planes (number `w` of them), whose row lies at `sp`.
-__device__ __forceinline__ bool sa_own_job(const sslm_launch::SharedAttnArgs& a, const SaPlan& pl, int w, SaJob* j, RowSpan* sp) {
+// A wave of the own planes (number `w` of them): its row, and the rest once the row's span is known.
+__device__ __forceinline__ bool sa_own_row(const sslm_launch::SharedAttnArgs& a, const SaPlan& pl, SaJob* j) {
+	const int w = ((int)blockIdx.x - pl.shared_blocks) * kSaWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	if (w >= a.rows * a.NKV * pl.ht * pl.owned) return false;
 	const int G = a.NH / a.NKV, plane = w % pl.owned, t = w / pl.owned % pl.ht;
 	j->kvh = w / pl.owned / pl.ht % a.NKV;
 	const int r = w / pl.owned / pl.ht / a.NKV, i = t * 16 + (threadIdx.x & 15);
-	*sp = row_span(a, r);
 	j->owned = true;
 	j->first = plane == 0;
 	j->plane = pl.shared + plane;
-	j->start = sp->start;
-	j->width = sp->width;
-	j->p0 = sp->start + (int64_t)plane * pl.ob;
-	j->p1 = i64min(sp->width, j->p0 + pl.ob);
-	const int8_t* head = sp->own + (int64_t)j->kvh * a.cap * a.D;
-	j->k = head + a.k_off;
-	j->v = head + a.v_off;
+	j->row = r;
 	j->r = i < G ? r : -1;
 	j->h = j->kvh * G + (i < G ? i : 0);
 	return true;
+}
+__device__ __forceinline__ void sa_own_span(const sslm_launch::SharedAttnArgs& a, const SaPlan& pl, const RowSpan& sp, SaJob* j) {
+	j->start = sp.start;
+	j->width = sp.width;
+	j->p0 = sp.start + (int64_t)(j->plane - pl.shared) * pl.ob;
+	j->p1 = i64min(sp.width, j->p0 + pl.ob);
+	const int8_t* head = sp.own + (int64_t)j->kvh * a.cap * a.D;
+	j->k = head + a.k_off;
+	j->v = head + a.v_off;
 }
 
 // the wave's query rows as an MFMA operand: lane (ri, g) holds bytes 64 c + 16 g .. + 16 of row ri
@@ -216,31 +261,79 @@ __device__ __forceinline__ void sa_load_q(const sslm_launch::SharedAttnArgs& a, 
 	}
 }
 
-// K rows of the 64 positions from p (rows past `last` repeat it), the other operand
-template <int D, int NC>
-__device__ __forceinline__ void sa_load_k(const int8_t* k, int64_t p, int64_t last, v4i (&kf)[4][NC]) {
-	const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4;
+// K or V rows of 64 positions on their way through LDS (32 D bytes of the wave's own, half the rows at a
+// time).  An MFMA operand has a row per lane, which as a global load touches 64 lines an instruction; loaded
+// D / 16 lanes to a row and turned in LDS it touches D / 2 (the maxima of 96 rows over 4096 positions: 20 us
+// with direct loads, whatever the waves and the loads in flight).  LDS operations of one wave take effect in
+// order, so no barrier but the compiler's stands between them.
+template <int D>
+struct SaRows {
+	static constexpr int PER = D / 16;
+	v4i r[PER];
+	// where 16-byte chunk `ch` of row `row` lies: chunks change places by row, so that one chunk of
+	// neighbouring rows covers all banks
+	static __device__ __forceinline__ int at(int row, int ch) { return row * D + ((ch ^ (row & (PER - 1))) << 4); }
+	// row(p): position p's row; positions past `last` repeat it
+	template <typename F>
+	__device__ __forceinline__ void load(int64_t p, int64_t last, F&& row) {
+		const int lane = threadIdx.x & 63;
 #pragma unroll
-	for (int t = 0; t < 4; ++t) {
-		const int8_t* row = k + i64min(p + t * 16 + ri, last) * D;
-#pragma unroll
-		for (int c = 0; c < NC; ++c) {
-			const int off = c * 64 + g * 16;
-			kf[t][c] = off < D ? load16(row + off) : v4i{0, 0, 0, 0};
+		for (int u = 0; u < PER; ++u) {
+			const int i = lane + 64 * u;
+			r[u] = load16(row(i64min(p + i / PER, last)) + i % PER * 16);
 		}
 	}
-}
-
-// Scores of 64 positions: lane (ri, g) gets those of query row ri at positions 16 t + 4 g + v.
-template <int NC>
-__device__ __forceinline__ void sa_scores(const v4i (&q)[NC], const v4i (&kf)[4][NC], v4i (&s)[4]) {
+	// rows 32 h .. 32 h + 31 into LDS
+	__device__ __forceinline__ void stage(int8_t* lds, int h) const {
+		const int lane = threadIdx.x & 63;
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-	for (int t = 0; t < 4; ++t) {
-		s[t] = v4i{0, 0, 0, 0};
-#pragma unroll
-		for (int c = 0; c < NC; ++c) s[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][c], q[c], s[t], 0, 0, 0);
+		for (int u = 0; u < PER / 2; ++u) {
+			const int c = lane + 64 * u;
+			*(v4i*)(lds + at(c / PER, c % PER)) = r[h * (PER / 2) + u];
+		}
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		__builtin_amdgcn_wave_barrier();
 	}
-}
+	// As K: the scores of query operand q, added to s.  Lane (ri, g) gets those of query row ri at positions
+	// 16 t + 4 g + v.
+	template <int NC>
+	__device__ __forceinline__ void scores(int8_t* lds, const v4i (&q)[NC], v4i (&s)[4]) const {
+		const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4;
+#pragma unroll
+		for (int h = 0; h < 2; ++h) {
+			stage(lds, h);
+#pragma unroll
+			for (int t = 2 * h; t < 2 * h + 2; ++t) {
+#pragma unroll
+				for (int c = 0; c < NC; ++c) {
+					const int ch = c * 4 + g;  // q is zero past D
+					const v4i k = *(const v4i*)(lds + at((t & 1) * 16 + ri, D < 64 ? ch & (PER - 1) : ch));
+					s[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, q[c], s[t], 0, 0, 0);
+				}
+			}
+		}
+	}
+	// As V: context += P V by the byte-transposing LDS read, which gives lane (ri, g) dim 16 dt + ri of the
+	// positions in sa_pack's order.  Lane (ri, g) of acc[dt][part] holds dims 16 dt + 4 g .. + 3 of query row ri.
+	__device__ __forceinline__ void multiply(int8_t* lds, const v4i& lo, const v4i& nhi, v4i (&acc)[D / 16][2]) const {
+		const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4, i = ri >> 1, row = (i >> 2) * 16 + g * 4 + (i & 3);
+		v2i half[2][D / 16];
+#pragma unroll
+		for (int h = 0; h < 2; ++h) {
+			stage(lds, h);
+#pragma unroll
+			for (int dt = 0; dt < D / 16; ++dt)
+				half[h][dt] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(lds + at(row, dt) + 8 * (ri & 1)));
+		}
+#pragma unroll
+		for (int dt = 0; dt < D / 16; ++dt) {
+			const v4i b = v4i{half[0][dt].x, half[0][dt].y, half[1][dt].x, half[1][dt].y};
+			acc[dt][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, lo, acc[dt][0], 0, 0, 0);
+			acc[dt][1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, nhi, acc[dt][1], 0, 0, 0);
+		}
+	}
+};
 
 // The i-exp of one query row in doubles, each value exact: with y = q_b - x for a score x below the
 // maximum (x <= 30 q_ln2 by the clip), z = floor(x / q_ln2) = floor((x + 1/2) / q_ln2), whose argument is at
@@ -304,79 +397,103 @@ __device__ __forceinline__ int64_t sa_row_sum(const sslm_launch::SharedAttnArgs&
 	return bad ? -1 : m;
 }
 
+// Steps of 64 positions over a plane's K: `step(p, scores)`, the rows of the next one (AHEAD = 2: two) steps in
+// flight meanwhile.
+template <int D, int AHEAD, int NC, typename F>
+__device__ __forceinline__ void sa_steps(const SaJob& j, int8_t* lds, const v4i (&q)[NC], F&& step) {
+	SaRows<D> k[AHEAD];
+	v4i s[4];
+	const int64_t last = j.p1 - 1;
+	auto row = [&](int64_t p) { return j.k + p * D; };
+#pragma unroll
+	for (int i = 0; i < AHEAD; ++i) k[i].load(j.p0 + 64 * i, last, row);
+	for (int64_t p = j.p0; p < j.p1; p += 64 * AHEAD) {
+#pragma unroll
+		for (int i = 0; i < AHEAD; ++i) {
+			if (i && p + 64 * i >= j.p1) break;
+			s[0] = s[1] = s[2] = s[3] = v4i{0, 0, 0, 0};
+			k[i].scores(lds, q, s);
+			k[i].load(p + 64 * (i + AHEAD), last, row);
+			__builtin_amdgcn_sched_barrier(0);
+			step(p + 64 * i, s);
+		}
+	}
+}
+
 template <int D>
 __global__ __launch_bounds__(64 * kSaWaves) void k_sa_max(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
-	constexpr int NC = (D + 63) / 64;
+	constexpr int NC = (D + 63) / 64, AHEAD = D <= 128 ? 2 : 1;
+	__shared__ __attribute__((aligned(16))) int8_t s_kv[kSaWaves][32 * D];
+	int8_t* lds = s_kv[threadIdx.x >> 6];
 	const int lane = threadIdx.x & 63, g = lane >> 4;
 	SaJob j;
+	RowSpan sp;
+	RowScales rs;
 	if ((int)blockIdx.x < pl.shared_blocks) {
-		if (!sa_shared_job(a, pl, blockIdx.x, &j)) return;
+		if (!sa_shared_job(a, pl, &j)) return;
 	} else {
-		RowSpan sp;
-		if (!sa_own_job(a, pl, (blockIdx.x - pl.shared_blocks) * kSaWaves + (threadIdx.x >> 6), &j, &sp)) return;
-		if (j.first) {
-			SaConst c{0, 0, 0, 0, prefix_rows_ok(a) ? sp.st : kPositionOverCap, 0};
-			if (c.st == kOk) {
-				const RowConst rc = row_const(a, __builtin_amdgcn_readfirstlane(j.r), j.kvh, sp.width);
-				c = SaConst{rc.q_ln2, rc.q_b, rc.q_c, rc.ceil, rc.st, 0};
-			}
-			if (lane == 0) w.cst[(size_t)j.r * a.NKV + j.kvh] = c;
-		}
-		if (sp.st != kOk) return;
+		if (!sa_own_row(a, pl, &j)) return;
+		rs = row_scales(a, j.row, j.kvh);
+		sp = row_span(a, j.row);
+		sa_own_span(a, pl, sp, &j);
 	}
-	v4i q[NC];
-	sa_load_q<D>(a, j, q);
 	const int64_t end = j.owned ? j.p1 : i64min(j.p1, j.start);  // by lane
-	int32_t m = INT32_MIN;
-	v4i kf[4][NC], s[4];
-	for (int64_t p = j.p0; p < j.p1; p += 64) {
-		sa_load_k<D>(j.k, p, j.p1 - 1, kf);
-		sa_scores(q, kf, s);
+	if (j.p0 < j.p1 && (!j.owned || sp.st == kOk)) {
+		v4i q[NC];
+		sa_load_q<D>(a, j, q);
+		int32_t m = INT32_MIN;
+		sa_steps<D, AHEAD>(j, lds, q, [&](int64_t p, v4i (&s)[4]) {
 #pragma unroll
-		for (int t = 0; t < 4; ++t)
+			for (int t = 0; t < 4; ++t)
 #pragma unroll
-			for (int v = 0; v < 4; ++v) m = max(m, p + t * 16 + g * 4 + v < end ? s[t][v] : INT32_MIN);
+				for (int v = 0; v < 4; ++v) m = max(m, p + t * 16 + g * 4 + v < end ? s[t][v] : INT32_MIN);
+		});
+		m = max(m, __shfl_xor(m, 16, 64));
+		m = max(m, __shfl_xor(m, 32, 64));
+		if (g == 0 && j.r >= 0) w.pmax[(size_t)j.plane * a.rows * a.NH + (size_t)j.r * a.NH + j.h] = m;
 	}
-	m = max(m, __shfl_xor(m, 16, 64));
-	m = max(m, __shfl_xor(m, 32, 64));
-	if (g == 0 && j.r >= 0) w.pmax[(size_t)j.plane * a.rows * a.NH + (size_t)j.r * a.NH + j.h] = m;
+	if (!j.owned || !j.first) return;
+	SaConst c{0, 0, 0, 0, sp.st, 0};
+	if (c.st == kOk) {
+		const RowConst rc = row_const(a, rs, sp.width);
+		c = SaConst{rc.q_ln2, rc.q_b, rc.q_c, rc.ceil, rc.st, 0};
+	}
+	if (lane == 0) {
+		w.cst[(size_t)j.row * a.NKV + j.kvh] = c;
+		w.span[j.row] = sp;
+	}
 }
 
-// A wave's job in the launches after k_sa_max, and its rows' constants: live (by lane) rows are computed.
-__device__ __forceinline__ bool sa_job(const sslm_launch::SharedAttnArgs& a, const SaPlan& pl, const SaWork& w, SaJob* j, SaConst* c, bool* live) {
-	if ((int)blockIdx.x < pl.shared_blocks) {
-		if (!sa_shared_job(a, pl, blockIdx.x, j)) return false;
-	} else {
-		RowSpan sp;
-		if (!sa_own_job(a, pl, (blockIdx.x - pl.shared_blocks) * kSaWaves + (threadIdx.x >> 6), j, &sp)) return false;
-		if (sp.st != kOk) return false;
-	}
-	*c = w.cst[(size_t)max(j->r, 0) * a.NKV + j->kvh];
-	*live = j->r >= 0 && c->st == kOk;
-	return __any(*live);
+// A wave's job in the launches after k_sa_max.
+__device__ __forceinline__ bool sa_job(const sslm_launch::SharedAttnArgs& a, const SaPlan& pl, const SaWork& w, SaJob* j) {
+	if ((int)blockIdx.x < pl.shared_blocks) return sa_shared_job(a, pl, j);
+	if (!sa_own_row(a, pl, j)) return false;
+	const RowSpan sp = w.span[j->row];
+	if (sp.st != kOk) return false;
+	sa_own_span(a, pl, sp, j);
+	return true;
 }
 
 template <int D>
-__global__ __launch_bounds__(64 * kSaWaves) void k_sa_sum(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
-	constexpr int NC = (D + 63) / 64;
+__global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 4 : 2) void k_sa_sum(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
+	constexpr int NC = (D + 63) / 64, AHEAD = 1;
+	__shared__ __attribute__((aligned(16))) int8_t s_kv[kSaWaves][32 * D];
+	int8_t* lds = s_kv[threadIdx.x >> 6];
 	const int g = (threadIdx.x & 63) >> 4;
 	SaJob j;
-	SaConst c;
-	bool live;
-	if (!sa_job(a, pl, w, &j, &c, &live) || j.p0 >= j.p1) return;
+	if (!sa_job(a, pl, w, &j) || j.p0 >= j.p1) return;
 	v4i q[NC];
 	sa_load_q<D>(a, j, q);
+	const SaConst c = w.cst[(size_t)max(j.r, 0) * a.NKV + j.kvh];
+	const bool live = j.r >= 0 && c.st == kOk;  // by lane
 	const int32_t top = sa_row_max(a, pl, w, j, live);
 	const int64_t end = !live ? 0 : (j.owned ? j.p1 : i64min(j.p1, j.start));
 	int64_t sum = 0;
 	int bad = 0;
-	v4i kf[4][NC], s[4];
 	if (!__any(live && !sa_fast(c, j.width))) {
 		const SaExp e = sa_exp_of(live ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
 		double acc = 0.0;
-		for (int64_t p = j.p0; p < j.p1; p += 64) {
-			sa_load_k<D>(j.k, p, j.p1 - 1, kf);
-			sa_scores(q, kf, s);
+		sa_steps<D, AHEAD>(j, lds, q, [&](int64_t p, v4i (&s)[4]) {
 #pragma unroll
 			for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -384,20 +501,19 @@ __global__ __launch_bounds__(64 * kSaWaves) void k_sa_sum(sslm_launch::SharedAtt
 					const double x = sa_exp(e, s[t][v]);
 					acc += p + t * 16 + g * 4 + v < end ? x : 0.0;
 				}
-		}
+		});
 		sum = (int64_t)acc;
 	} else {
 		const double inv = 1.0 / (double)c.q_ln2;
-		for (int64_t p = j.p0; p < j.p1; p += 64) {
-			sa_load_k<D>(j.k, p, j.p1 - 1, kf);
-			sa_scores(q, kf, s);
+		sa_steps<D, AHEAD>(j, lds, q, [&](int64_t p, v4i (&s)[4]) {
+#pragma unroll
 			for (int i = 0; i < 16; ++i) {
 				if (p + (i >> 2) * 16 + g * 4 + (i & 3) >= end) continue;
 				const int64_t x = iexp_fast_cold((int64_t)s[i >> 2][i & 3] - top, c.q_ln2, inv, c.q_b, c.q_c, c.ceil);
 				bad |= x < 0;
 				sum += x < 0 ? 0 : x;
 			}
-		}
+		});
 	}
 	for (int o = 16; o < 64; o *= 2) {
 		sum += __shfl_xor(sum, o, 64);
@@ -440,100 +556,53 @@ __device__ __forceinline__ void sa_pack(const int32_t (&p)[16], v4i* lo, v4i* nh
 	}
 }
 
-// V rows of 64 positions through LDS (one wave's own rows of it) into MFMA operands: lane (ri, g) of dim
-// tile dt gets dim 16 dt + ri of the positions in sa_pack's order, by the byte-transposing LDS read.
 template <int D>
-struct SaV {
-	static constexpr int PER = D / 16;
-	v4i r[PER];
-	// where 16-byte chunk `ch` of row `row` lies: chunks change places by row, so that one chunk of
-	// neighbouring rows covers all banks
-	static __device__ __forceinline__ int at(int row, int ch) { return row * D + ((ch ^ (row & (PER - 1))) << 4); }
-	__device__ __forceinline__ void load(const int8_t* v, int64_t p, int64_t last) {
-		const int lane = threadIdx.x & 63;
-#pragma unroll
-		for (int u = 0; u < PER; ++u) {
-			const int i = lane + 64 * u;
-			r[u] = load16(v + i64min(p + i / PER, last) * D + i % PER * 16);
-		}
-	}
-	__device__ __forceinline__ void stage(int8_t* lds) const {
-		const int lane = threadIdx.x & 63;
-		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-		for (int u = 0; u < PER; ++u) {
-			const int i = lane + 64 * u;
-			*(v4i*)(lds + at(i / PER, i % PER)) = r[u];
-		}
-		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-		__builtin_amdgcn_wave_barrier();
-	}
-	// context += P V: lane (ri, g) of acc[dt][part] holds dims 16 dt + 4 g .. + 3 of query row ri
-	static __device__ __forceinline__ void multiply(const int8_t* lds, const v4i& lo, const v4i& nhi, v4i (&acc)[D / 16][2]) {
-		const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4, i = ri >> 1;
-		const int row = (i >> 2) * 16 + g * 4 + (i & 3);
-#pragma unroll
-		for (int dt = 0; dt < D / 16; ++dt) {
-			const int8_t* from = lds + at(row, dt) + 8 * (ri & 1);  // rows `row` and row + 32 agree in row % 16
-			const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)from);
-			const v2i y = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(from + 32 * D));
-			const v4i b = v4i{x.x, x.y, y.x, y.y};
-			acc[dt][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, lo, acc[dt][0], 0, 0, 0);
-			acc[dt][1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, nhi, acc[dt][1], 0, 0, 0);
-		}
-	}
-};
-
-template <int D>
-__global__ __launch_bounds__(64 * kSaWaves) void k_sa_pv(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
-	constexpr int NC = (D + 63) / 64, DT = D / 16;
-	__shared__ __attribute__((aligned(16))) int8_t s_v[kSaWaves][64 * D];
-	int8_t* lds = s_v[threadIdx.x >> 6];
+__global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 2 : 1) void k_sa_pv(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
+	constexpr int NC = (D + 63) / 64, DT = D / 16, AHEAD = 1;
+	__shared__ __attribute__((aligned(16))) int8_t s_kv[kSaWaves][32 * D];
+	int8_t* lds = s_kv[threadIdx.x >> 6];
 	const int g = (threadIdx.x & 63) >> 4;
 	SaJob j;
-	SaConst c;
-	bool live;
-	if (!sa_job(a, pl, w, &j, &c, &live)) return;
+	if (!sa_job(a, pl, w, &j)) return;
+	const SaConst c = w.cst[(size_t)max(j.r, 0) * a.NKV + j.kvh];
+	bool live = j.r >= 0 && c.st == kOk;  // by lane
 	const int32_t top = sa_row_max(a, pl, w, j, live);
 	const int64_t sum = sa_row_sum(a, pl, w, j, live);
 	if (j.first && g == 0 && live) w.hst[(size_t)j.r * a.NH + j.h] = sum < 0 ? kSoftmaxKernelRefusedAfterGateAccepted : kOk;
 	if (j.p0 >= j.p1) return;
 	live = live && sum >= 0;
 	const int64_t den = live && sum > 1 ? sum : 1;
-	const int64_t end = !live ? 0 : (j.owned ? j.p1 : i64min(j.p1, j.start));
-	v4i q[NC], kf[4][NC], s[4], acc[DT][2], lo, nhi;
+	const int64_t end = !live ? 0 : (j.owned ? j.p1 : i64min(j.p1, j.start)), last = j.p1 - 1;
+	v4i q[NC], acc[DT][2], lo, nhi;
 	sa_load_q<D>(a, j, q);
 #pragma unroll
 	for (int d = 0; d < DT; ++d) acc[d][0] = acc[d][1] = v4i{0, 0, 0, 0};
-	SaV<D> vr;
+	SaRows<D> vr;
 	int32_t pr[16];
+	auto vrow = [&](int64_t p) { return j.v + p * D; };
 	if (!__any(live && !sa_fast(c, j.width))) {
 		const SaExp e = sa_exp_of(live ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
 		auto run = [&](auto small) {
 			constexpr bool SMALL = decltype(small)::value;
 			const SaProb pb = sa_prob_of((double)den, SMALL);
-			for (int64_t p = j.p0; p < j.p1; p += 64) {
-				sa_load_k<D>(j.k, p, j.p1 - 1, kf);
-				vr.load(j.v, p, j.p1 - 1);
-				sa_scores(q, kf, s);
+			sa_steps<D, AHEAD>(j, lds, q, [&](int64_t p, v4i (&s)[4]) {
+				vr.load(p, last, vrow);
+				__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
 				for (int i = 0; i < 16; ++i) {
 					const int32_t x = sa_prob<SMALL>(pb, sa_exp(e, s[i >> 2][i & 3]));
 					pr[i] = p + (i >> 2) * 16 + g * 4 + (i & 3) < end ? x : 0;
 				}
 				sa_pack(pr, &lo, &nhi);
-				vr.stage(lds);
-				SaV<D>::multiply(lds, lo, nhi, acc);
-			}
+				vr.multiply(lds, lo, nhi, acc);
+			});
 		};
 		if (!__any(den >= ((int64_t)1 << 36))) run(std::true_type{});
 		else run(std::false_type{});
 	} else {
 		const double inv = 1.0 / (double)c.q_ln2, dinv = 1.0 / (double)den;
-		for (int64_t p = j.p0; p < j.p1; p += 64) {
-			sa_load_k<D>(j.k, p, j.p1 - 1, kf);
-			vr.load(j.v, p, j.p1 - 1);
-			sa_scores(q, kf, s);
+		sa_steps<D, AHEAD>(j, lds, q, [&](int64_t p, v4i (&s)[4]) {
+			vr.load(p, last, vrow);
 #pragma unroll
 			for (int i = 0; i < 16; ++i) {
 				pr[i] = 0;
@@ -542,63 +611,58 @@ __global__ __launch_bounds__(64 * kSaWaves) void k_sa_pv(sslm_launch::SharedAttn
 				pr[i] = (int32_t)div_rcp_cold(x << 15, den, dinv, 32768);
 			}
 			sa_pack(pr, &lo, &nhi);
-			vr.stage(lds);
-			SaV<D>::multiply(lds, lo, nhi, acc);
-		}
+			vr.multiply(lds, lo, nhi, acc);
+		});
 	}
 	if (j.r < 0) return;
 	int32_t* out = w.part + ((size_t)j.plane * a.rows + j.r) * a.NH * D + (size_t)j.h * D + 4 * g;
 #pragma unroll
-	for (int d = 0; d < DT; ++d) {
-		v4i o;
+	for (int d = 0; d < DT; ++d) *(v4i*)(out + 16 * d) = acc[d][0] - 256 * acc[d][1];
+}
+
+// The fold of this thread's units of four dims, read ahead: unit u's head is the same for all four.
+template <int BS, int U>
+__device__ __forceinline__ void sa_folds(const sslm_launch::SharedAttnArgs& a, FoldConsts (&fc)[U]) {
 #pragma unroll
-		for (int v = 0; v < 4; ++v) o[v] = acc[d][0][v] - 256 * acc[d][1][v];
-		*(v4i*)(out + 16 * d) = o;
+	for (int u = 0; u < U; ++u) {
+		const int32_t* cf = a.ctx_fold + 3 * (4 * min((int)threadIdx.x + u * BS, a.NH * a.D / 4 - 1) / a.D);
+		fc[u] = fold_consts(cf[0], cf[1], cf[2]);
 	}
 }
 
-// The planes' contexts joined, the per-head fold and the funnel of one row (checked_chain_funnel.cpp:257-364),
-// after the first refusing head.  U units of four dims per thread.
+// The fold and funnel of one row's context (checked_chain_funnel.cpp:257-364), U units of four dims per
+// thread, unless `first`, the smallest (head << 8) | status of a refusing head, is there.
 template <int BS, int U>
-__global__ __launch_bounds__(BS) void k_sa_out(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
-	__shared__ uint32_t s_m[BS / 64], s_bad[BS / 64];
-	const int r = blockIdx.x, N = a.NH * a.D, G = a.NH / a.NKV;
-	// the first refusing head, heads of one KV head sharing its constants' status: (head << 8) | status
-	uint32_t first = 0xffffffffu;
-	for (int h = threadIdx.x; h < a.NH; h += BS) {
-		const int32_t st = w.cst[(size_t)r * a.NKV + h / G].st;
-		const int32_t x = st != kOk ? st : w.hst[(size_t)r * a.NH + h];
-		if (x != kOk) first = min(first, (uint32_t)h << 8 | (uint32_t)x);
+__device__ __forceinline__ void sa_finish(const sslm_launch::SharedAttnArgs& a, int r, v4i (&v)[U], const FoldConsts (&fc)[U],
+                                          uint32_t first, uint32_t* s_red) {
+	const int N = a.NH * a.D;
+	uint32_t mx = 0;
+#pragma unroll
+	for (int u = 0; u < U; ++u) {  // a clamped unit repeats the last one
+#pragma unroll
+		for (int x = 0; x < 4; ++x) {
+			v[u][x] = fold_bounded(v[u][x], fc[u]);  // |context| <= 2^15 128
+			mx = max(mx, (uint32_t)(v[u][x] < 0 ? -v[u][x] : v[u][x]));
+		}
 	}
-	first = ~block_max_u32<BS>(~first, s_bad);
+	mx = wave_max32(mx);
+	first = ~wave_max32(~first);
+	if ((threadIdx.x & 63) == 0) {
+		s_red[threadIdx.x >> 6] = mx;
+		s_red[BS / 64 + (threadIdx.x >> 6)] = first;
+	}
+	__syncthreads();
+#pragma unroll
+	for (int i = 0; i < BS / 64; ++i) {
+		mx = max(mx, s_red[i]);
+		first = min(first, s_red[BS / 64 + i]);
+	}
 	if (first != 0xffffffffu) {
 		if (threadIdx.x == 0) a.status[r] = (int32_t)(first & 0xff);
 		return;
 	}
-	const RowSpan sp = row_span(a, r);
-	const int sh = (int)((sp.start + pl.sb - 1) / pl.sb), n = sh + (int)((sp.width - sp.start + pl.ob - 1) / pl.ob);
-	v4i v[U];
-	uint32_t mx = 0;
-#pragma unroll
-	for (int u = 0; u < U; ++u) {
-		const int i = (int)threadIdx.x + u * BS;
-		v[u] = v4i{0, 0, 0, 0};
-		if (4 * i < N) {
-			const int32_t* at = w.part + (size_t)r * N + 4 * i;
-#pragma unroll 4
-			for (int k = 0; k < n; ++k) v[u] += *(const v4i*)(at + (size_t)(k < sh ? k : pl.shared + k - sh) * a.rows * N);
-			const int32_t* cf = a.ctx_fold + 3 * (4 * i / a.D);
-#pragma unroll
-			for (int x = 0; x < 4; ++x) {
-				const int64_t f = apply_fold(v[u][x], cf[0], cf[1], cf[2]);
-				mx = max(mx, sat_abs_u32(f));
-				v[u][x] = sat_i32(f);
-			}
-		}
-	}
-	mx = block_max_u32<BS>(mx, s_m);
 	FunnelPlan plan;
-	const int32_t st = funnel_plan(mx, nullptr, 0, a.site, &plan);
+	const int32_t st = funnel_plan(__builtin_amdgcn_readfirstlane(mx), nullptr, 0, a.site, &plan);
 	if (threadIdx.x == 0) {
 		a.status[r] = st;
 		if (st == kOk) a.scales[r] = plan.out;
@@ -614,6 +678,221 @@ __global__ __launch_bounds__(BS) void k_sa_out(sslm_launch::SharedAttnArgs a, Sa
 			*(uint32_t*)(a.codes + (size_t)r * N + 4 * i) = o;
 		}
 	}
+}
+
+// The planes' contexts joined and finished, a block per row.
+template <int BS, int U>
+__global__ __launch_bounds__(BS) void k_sa_out(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
+	__shared__ uint32_t s_red[2 * BS / 64];
+	const int r = blockIdx.x, N = a.NH * a.D, G = a.NH / a.NKV;
+	const RowSpan sp = w.span[r];
+	// the first refusing head, heads of one KV head sharing its constants' status
+	uint32_t first = 0xffffffffu;
+	for (int h = threadIdx.x; h < a.NH; h += BS) {
+		const int32_t st = w.cst[(size_t)r * a.NKV + h / G].st;
+		const int32_t x = st != kOk ? st : w.hst[(size_t)r * a.NH + h];
+		if (x != kOk) first = min(first, (uint32_t)h << 8 | (uint32_t)x);
+	}
+	const int sh = (int)((sp.start + pl.sb - 1) / pl.sb);
+	const int n = sp.st != kOk ? 0 : sh + (int)((sp.width - sp.start + pl.ob - 1) / pl.ob);
+	FoldConsts fc[U];
+	sa_folds<BS>(a, fc);
+	v4i v[U];
+	const int32_t* at[U];
+#pragma unroll
+	for (int u = 0; u < U; ++u) {
+		v[u] = v4i{0, 0, 0, 0};
+		at[u] = w.part + (size_t)r * N + 4 * min((int)threadIdx.x + u * BS, N / 4 - 1);
+	}
+	constexpr int PK = 8 / U;  // planes in flight
+	for (int k = 0; k < n; k += PK) {
+		v4i x[PK][U];
+#pragma unroll
+		for (int e = 0; e < PK; ++e) {
+			const int p = min(k + e, n - 1);
+			const size_t off = (size_t)(p < sh ? p : pl.shared + p - sh) * a.rows * N;
+#pragma unroll
+			for (int u = 0; u < U; ++u) x[e][u] = *(const v4i*)(at[u] + off);
+		}
+#pragma unroll
+		for (int e = 0; e < PK; ++e)
+#pragma unroll
+			for (int u = 0; u < U; ++u) v[u] += k + e < n ? x[e][u] : v4i{0, 0, 0, 0};
+	}
+	sa_finish<BS>(a, r, v, fc, first, s_red);
+}
+
+// The whole of a short row in one launch: a block per row, its eight waves cut over the KV heads and
+// then over the positions, NS steps to a wave whose scores stay in registers; maxima, sums and contexts are
+// joined in LDS.  A step is F times 64 positions: where G <= 8 heads would leave half of a tile's columns
+// empty, columns 8 .. 15 hold the same heads at the next 64 positions (F = 2), by adding the products of
+// the second 64 with a query operand that is zero in the other half; the i-exp, which bounds the
+// kernel, then works on full waves.  K and V are read once per row here, from L2 for the prefix's.
+constexpr int kSaRowWaves = 8, kSaRowSteps = 2, kSaRowN = 4096;
+template <int D, int F, int NS>
+__global__ __launch_bounds__(64 * kSaRowWaves, 2) void k_sa_row(sslm_launch::SharedAttnArgs a) {
+	constexpr int NC = (D + 63) / 64, DT = D / 16, NW = kSaRowWaves, BS = 64 * NW, U = kSaRowN / 4 / BS, GP = 16 / F;
+	constexpr bool KEEP = NS == 1;  // the i-exp values kept in registers between the sums and the probabilities
+	__shared__ __attribute__((aligned(16))) int8_t s_kv[NW][32 * D];
+	__shared__ __attribute__((aligned(16))) int32_t s_ctx[kSaRowN];
+	__shared__ int32_t s_max[NW][16];
+	__shared__ int64_t s_sum[NW][16];
+	__shared__ uint32_t s_first, s_red[2 * NW];
+	const int r = blockIdx.x, lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4, col = ri % GP, part = ri / GP;
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = NW / a.NKV, kvh = wave / per, sub = wave % per;
+	const int G = a.NH / a.NKV;
+	int8_t* lds = s_kv[wave];
+	const RowScales rs = row_scales(a, r, kvh);
+	const RowSpan sp = row_span(a, r);
+	if (sp.st != kOk) {
+		if (threadIdx.x == 0) a.status[r] = sp.st;
+		return;
+	}
+	const int64_t head = (int64_t)kvh * a.cap * D, last = sp.width - 1;
+	auto krow = [&](int64_t p) { return (p < sp.start ? sp.pre : sp.own) + a.k_off + head + p * D; };
+	auto vrow = [&](int64_t p) { return (p < sp.start ? sp.pre : sp.own) + a.v_off + head + p * D; };
+	auto base = [&](int n) { return (int64_t)(sub + n * per) * (64 * F); };  // step n's first position
+	auto at = [&](int n, int i) { return base(n) + part * 64 + (i >> 2) * 16 + g * 4 + (i & 3); };  // score i's, by lane
+	SaJob j{};
+	j.r = col < G ? r : -1;
+	j.h = kvh * G + (col < G ? col : 0);
+	// 64-position blocks of K (V) in flight: a wave alone waits a memory round trip for each that is not
+	constexpr int NB = NS * F, AK = NB < 2 ? NB : 2, AV = 1;
+	auto block = [&](int b) { return base(b / F) + b % F * 64; };
+	SaRows<D> kr[AK], vr[AV];
+#pragma unroll
+	for (int b = 0; b < AK; ++b) kr[b].load(block(b), last, krow);
+	v4i q[F][NC], s[NS][4];
+	sa_load_q<D>(a, j, q[0]);
+	if constexpr (F == 2) {
+#pragma unroll
+		for (int c = 0; c < NC; ++c) {
+			q[1][c] = part == 1 ? q[0][c] : v4i{0, 0, 0, 0};
+			q[0][c] = part == 0 ? q[0][c] : v4i{0, 0, 0, 0};
+		}
+	}
+	FoldConsts fc[U];
+	sa_folds<BS>(a, fc);
+	if (threadIdx.x == 0) s_first = 0xffffffffu;
+	for (int i = threadIdx.x; i < a.NH * D / 4; i += BS) ((v4i*)s_ctx)[i] = v4i{0, 0, 0, 0};
+	const RowConst rc = row_const(a, rs, sp.width);
+	const SaConst c{rc.q_ln2, rc.q_b, rc.q_c, rc.ceil, rc.st, 0};
+	int32_t m = INT32_MIN;
+#pragma unroll
+	for (int n = 0; n < NS; ++n) {
+		if (base(n) > last) break;
+		s[n][0] = s[n][1] = s[n][2] = s[n][3] = v4i{0, 0, 0, 0};
+#pragma unroll
+		for (int f = 0; f < F; ++f) {
+			const int b = n * F + f;
+			kr[b % AK].scores(lds, q[f], s[n]);
+			if (b + AK < NB) kr[b % AK].load(block(b + AK), last, krow);
+		}
+#pragma unroll
+		for (int i = 0; i < 16; ++i) m = max(m, at(n, i) <= last ? s[n][i >> 2][i & 3] : INT32_MIN);
+	}
+#pragma unroll
+	for (int b = 0; b < AV; ++b) vr[b].load(block(b), last, vrow);  // in flight through the softmax
+	if (F == 2) m = max(m, __shfl_xor(m, 8, 64));
+	m = max(m, __shfl_xor(m, 16, 64));
+	m = max(m, __shfl_xor(m, 32, 64));
+	if (lane < GP) s_max[wave][lane] = m;
+	__syncthreads();
+	int32_t top = INT32_MIN;
+	for (int i = 0; i < per; ++i) top = max(top, s_max[kvh * per + i][col]);
+	const bool ok = c.st == kOk, fast = ok && sa_fast(c, sp.width);
+	if (!ok && sub == 0 && lane == 0) atomicMin(&s_first, (uint32_t)(kvh * G) << 8 | (uint32_t)c.st);
+	const SaExp e = sa_exp_of(fast ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
+	const double inv = fast ? 0.0 : 1.0 / (double)c.q_ln2;
+	int64_t sum = 0;
+	int bad = 0;
+	double ev[KEEP ? NS : 1][16];
+	if (fast) {
+		double acc = 0.0;
+#pragma unroll
+		for (int n = 0; n < NS; ++n) {
+			if (base(n) > last) break;
+#pragma unroll
+			for (int i = 0; i < 16; ++i) {
+				const double x = at(n, i) <= last ? sa_exp(e, s[n][i >> 2][i & 3]) : 0.0;
+				acc += x;
+				if (KEEP) ev[n][i] = x;
+			}
+		}
+		sum = (int64_t)acc;
+	} else if (ok) {
+#pragma unroll
+		for (int n = 0; n < NS; ++n) {
+#pragma unroll
+			for (int i = 0; i < 16; ++i) {
+				if (at(n, i) > last) continue;
+				const int64_t x = iexp_fast_cold((int64_t)s[n][i >> 2][i & 3] - top, c.q_ln2, inv, c.q_b, c.q_c, c.ceil);
+				bad |= x < 0;
+				sum += x < 0 ? 0 : x;
+			}
+		}
+	}
+	for (int o = GP; o < 64; o *= 2) {
+		sum += __shfl_xor(sum, o, 64);
+		bad |= __shfl_xor(bad, o, 64);
+	}
+	if (lane < GP) s_sum[wave][lane] = sum;
+	if (lane < G && bad) atomicMin(&s_first, (uint32_t)(kvh * G + lane) << 8 | (uint32_t)kSoftmaxKernelRefusedAfterGateAccepted);
+	__syncthreads();
+	sum = 0;
+	for (int i = 0; i < per; ++i) sum += s_sum[kvh * per + i][col];
+	const int64_t den = sum > 1 ? sum : 1;
+	v4i acc[DT][2], lo, nhi;
+#pragma unroll
+	for (int d = 0; d < DT; ++d) acc[d][0] = acc[d][1] = v4i{0, 0, 0, 0};
+	const bool small = fast && !__any(den >= ((int64_t)1 << 36));
+	const SaProb pb = sa_prob_of((double)den, small);
+	const double dinv = 1.0 / (double)den;
+#pragma unroll
+	for (int n = 0; n < NS; ++n) {
+		if (base(n) > last || s_first != 0xffffffffu) break;
+		int32_t pr[16];
+		auto value = [&](int i) { return KEEP ? ev[KEEP ? n : 0][i] : (at(n, i) <= last ? sa_exp(e, s[n][i >> 2][i & 3]) : 0.0); };
+		if (small) {
+#pragma unroll
+			for (int i = 0; i < 16; ++i) pr[i] = sa_prob<true>(pb, value(i));
+		} else if (fast) {
+#pragma unroll
+			for (int i = 0; i < 16; ++i) pr[i] = sa_prob<false>(pb, value(i));
+		} else {
+#pragma unroll
+			for (int i = 0; i < 16; ++i) {
+				pr[i] = 0;
+				if (at(n, i) > last) continue;
+				const int64_t x = iexp_fast_cold((int64_t)s[n][i >> 2][i & 3] - top, c.q_ln2, inv, c.q_b, c.q_c, c.ceil);
+				pr[i] = (int32_t)div_rcp_cold(x << 15, den, dinv, 32768);
+			}
+		}
+		sa_pack(pr, &lo, &nhi);
+#pragma unroll
+		for (int f = 0; f < F; ++f) {
+			const v4i z{0, 0, 0, 0};
+			const int b = n * F + f;
+			vr[b % AV].multiply(lds, F == 1 || part == f ? lo : z, F == 1 || part == f ? nhi : z, acc);
+			if (b + AV < NB) vr[b % AV].load(block(b + AV), last, vrow);
+		}
+	}
+	// dims change places within a head by its row, so that a tile's additions meet different banks
+	if (col < G) {
+		int32_t* ctx = s_ctx + j.h * D;
+#pragma unroll
+		for (int d = 0; d < DT; ++d)
+#pragma unroll
+			for (int x = 0; x < 4; ++x) atomicAdd(ctx + (((16 * d + 4 * g) ^ (col * 4 & (D - 1))) + x), acc[d][0][x] - 256 * acc[d][1][x]);
+	}
+	__syncthreads();
+	v4i v[U];
+#pragma unroll
+	for (int u = 0; u < U; ++u) {
+		const int i = min((int)threadIdx.x + u * BS, a.NH * D / 4 - 1), h = 4 * i / D;
+		v[u] = *(const v4i*)(s_ctx + h * D + ((4 * i % D) ^ (h % G * 4 & (D - 1))));
+	}
+	sa_finish<BS>(a, r, v, fc, s_first, s_red);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -962,7 +1241,10 @@ __global__ __launch_bounds__(64) void k_pick_final(sslm_launch::PickArgs a, cons
 // ------------------------------------------------------------------------------------------
 namespace sslm_launch {
 
-constexpr int kSaTargetWaves = 1024;
+#ifndef TW
+#define TW 1536
+#endif
+constexpr int kSaTargetWaves = TW;
 
 static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -1002,6 +1284,7 @@ static size_t sa_work(const SaPlan& p, int rows, int NH, int NKV, int D, char* b
 		return x;
 	};
 	const size_t planes = p.shared + p.owned, r = (size_t)rows * NH;
+	w->span = (RowSpan*)take((size_t)rows * sizeof(RowSpan));
 	w->cst = (SaConst*)take((size_t)rows * NKV * sizeof(SaConst));
 	w->pmax = (int32_t*)take(planes * r * 4);
 	w->psum = (int64_t*)take(planes * r * 8);
@@ -1010,9 +1293,25 @@ static size_t sa_work(const SaPlan& p, int rows, int NH, int NKV, int D, char* b
 	return at;
 }
 
+// Steps of a wave of k_sa_row, 0 where it does not take the call.
+static int sa_row_steps(int NH, int NKV, int D, int prefixes, int64_t max_prefix, int64_t max_own) {
+	const int G = NH / NKV;
+	if (NKV > kSaRowWaves || kSaRowWaves % NKV || G > 16 || NH * D > kSaRowN || D > 128) return 0;
+	const int64_t step = G <= 8 ? 128 : 64, steps = ((prefixes > 0 ? max_prefix : 0) + max_own + step - 1) / step;
+	const int64_t per = kSaRowWaves / NKV, n = std::max<int64_t>(1, (steps + per - 1) / per);
+	return n > kSaRowSteps ? 0 : (int)n;
+}
+
 size_t shared_attn_workspace(int rows, int NH, int NKV, int D, int prefixes, int64_t max_prefix, int64_t max_own) {
 	SaWork w;
 	return sa_work(sa_plan(rows, NH, NKV, prefixes, max_prefix, max_own), rows, NH, NKV, D, nullptr, &w);
+}
+
+template <int D, int F>
+static void sa_row_launch(const SharedAttnArgs& a, int steps, hipStream_t s) {
+	const dim3 grid(a.rows), block(64 * kSaRowWaves);
+	if (steps == 1) hipLaunchKernelGGL((k_sa_row<D, F, 1>), grid, block, 0, s, a);
+	else hipLaunchKernelGGL((k_sa_row<D, F, kSaRowSteps>), grid, block, 0, s, a);
 }
 
 template <int D>
@@ -1024,6 +1323,13 @@ static void sa_launch(const SharedAttnArgs& a, const SaPlan& p, const SaWork& w,
 }
 
 void shared_attn(const SharedAttnArgs& a, hipStream_t s) {
+	if (const int n = sa_row_steps(a.NH, a.NKV, a.D, a.prefixes, a.max_prefix, a.max_own)) {
+		const bool two = a.NH / a.NKV <= 8;
+		if (a.D == 32) two ? sa_row_launch<32, 2>(a, n, s) : sa_row_launch<32, 1>(a, n, s);
+		else if (a.D == 64) two ? sa_row_launch<64, 2>(a, n, s) : sa_row_launch<64, 1>(a, n, s);
+		else two ? sa_row_launch<128, 2>(a, n, s) : sa_row_launch<128, 1>(a, n, s);
+		return;
+	}
 	const SaPlan p = sa_plan(a.rows, a.NH, a.NKV, a.prefixes, a.max_prefix, a.max_own);
 	SaWork w;
 	sa_work(p, a.rows, a.NH, a.NKV, a.D, (char*)a.ws, &w);
