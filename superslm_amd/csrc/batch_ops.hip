@@ -1151,61 +1151,118 @@ __global__ __launch_bounds__(BS) void k_lora_funnel(sslm_launch::LoraGemmArgs g,
 // ------------------------------------------------------------------------------------------
 // the next token under each row's rules
 // ------------------------------------------------------------------------------------------
-constexpr int kPickSlice = 4096;  // tokens per block: counts and biases of a slice take 48 KB of LDS
-constexpr int kPickBlock = 256;
+constexpr int kPickSlice = 4096;  // tokens per block: a slice's counts and half its biases take 32 KB of LDS
+constexpr int kPickBlock = 512;
 
 __device__ __forceinline__ bool rule_ok(const LogitRule& r) {
 	return r.history_len >= 0 && r.bias_count >= 0 && r.repetition_q16 >= 1 && (r.history_len == 0 || r.history) &&
 	       (r.bias_count == 0 || (r.bias_ids && r.bias_values));
 }
 
-// One block per (slice of the vocabulary, row): the slice's token counts and bias sums in LDS, then
-// one pass over its logits.  Keys order by logit, then by the lower index; 0 marks no legal token.
+// A row's token from its best (logit, index) keys: they order by logit, then by the lower index, and 0 marks
+// no legal token.
+__device__ __forceinline__ int32_t pick_of(uint64_t key) { return key ? (int32_t)(0xffffffffu - (uint32_t)key) : -1; }
+
+// One block per (slice of the vocabulary, row): the slice's token counts and (a half at a time) bias sums in
+// LDS while its logits are in flight, then one pass over them in registers.  Bound by the logits' traffic: a thread's
+// 16 are four 16-byte loads and stores (VEC: rows 16-byte aligned), the row's history (read by every slice
+// of it, from L2) four loads at a time.  With one slice to a row the block writes the token itself.
+template <bool VEC>
 __global__ __launch_bounds__(kPickBlock) void k_pick_slice(sslm_launch::PickArgs a, unsigned long long* keys) {
-	__shared__ int32_t s_cnt[kPickSlice];
-	__shared__ unsigned long long s_bias[kPickSlice];
+	__shared__ __attribute__((aligned(16))) int32_t s_cnt[kPickSlice];
+	__shared__ __attribute__((aligned(16))) unsigned long long s_bias[kPickSlice / 2];
 	__shared__ uint64_t s_key[kPickBlock / 64];
+	constexpr int U = kPickSlice / kPickBlock / 4;
 	const int r = blockIdx.y, v0 = blockIdx.x * kPickSlice, n = min(kPickSlice, a.vocab - v0);
-	const LogitRule ru = a.rules[r];
-	if (!rule_ok(ru)) return;
-	const bool any = ru.history_len > 0 || ru.bias_count > 0;
-	if (any) {
-		for (int j = threadIdx.x; j < kPickSlice; j += kPickBlock) {
-			s_cnt[j] = 0;
-			s_bias[j] = 0;
-		}
-		__syncthreads();
-		for (int i = threadIdx.x; i < ru.history_len; i += kPickBlock) {
-			const int64_t j = (int64_t)ru.history[i] - v0;
-			if (j >= 0 && j < n) atomicAdd(&s_cnt[j], 1);
-		}
-		for (int i = threadIdx.x; i < ru.bias_count; i += kPickBlock) {
-			const int64_t j = (int64_t)ru.bias_ids[i] - v0;
-			if (j >= 0 && j < n) atomicAdd(&s_bias[j], (unsigned long long)(int64_t)ru.bias_values[i]);
-		}
-		__syncthreads();
-	}
 	const int32_t* row = a.logits + (int64_t)r * a.ld + v0;
-	uint64_t key = 0;
-	for (int j = threadIdx.x; j < n; j += kPickBlock) {
-		int64_t x = row[j];
-		if (any) {
-			const int32_t c = s_cnt[j];
-			if (c > 0) {
-				// (x << 16) / rho: below 2^47, so the double quotient's truncation is the integer one
-				x = x > 0 ? (int64_t)((double)(x << 16) / (double)ru.repetition_q16) : (x * ru.repetition_q16) >> 16;
-				x -= (int64_t)ru.presence + (int64_t)ru.frequency * c;
-			}
-			x += (int64_t)s_bias[j];
+	v4i x[U];
+#pragma unroll
+	for (int u = 0; u < U; ++u) {
+		const int j = 4 * ((int)threadIdx.x + u * kPickBlock);
+		if (VEC && j + 4 <= n) x[u] = *(const v4i*)(row + j);
+		else {
+#pragma unroll
+			for (int i = 0; i < 4; ++i) x[u][i] = row[min(j + i, n - 1)];
 		}
-		int32_t y = sat_i32(x);
-		const int id = v0 + j;
-		const bool legal = !ru.mask || ((ru.mask[id >> 3] >> (id & 7)) & 1u);
-		y = legal ? y : kI32Min;
-		if (a.adjusted) a.adjusted[(int64_t)r * a.adjusted_ld + id] = y;
-		const uint64_t k = legal ? ((uint64_t)((uint32_t)y ^ 0x80000000u) << 32) | (0xffffffffu - (uint32_t)id) : 0;
-		key = k > key ? k : key;
 	}
+	const LogitRule ru = a.rules[r];
+	if (!rule_ok(ru)) {
+		if (gridDim.x == 1 && threadIdx.x == 0) a.tokens[r] = -2;
+		return;
+	}
+	const bool seen = ru.history_len > 0, biased = ru.bias_count > 0;
+	uint32_t legal[U];  // bit i: token 4 i of the group
+#pragma unroll
+	for (int u = 0; u < U; ++u) {
+		const int id = v0 + 4 * ((int)threadIdx.x + u * kPickBlock);
+		legal[u] = ru.mask ? ru.mask[min(id, a.vocab - 1) >> 3] >> (id & 4) : 15u;
+	}
+	if (seen) {
+#pragma unroll
+		for (int u = 0; u < U; ++u) *(v4i*)(s_cnt + 4 * ((int)threadIdx.x + u * kPickBlock)) = v4i{0, 0, 0, 0};
+		__syncthreads();
+		for (int i = threadIdx.x; i < ru.history_len; i += 4 * kPickBlock) {
+			int32_t h[4];
+#pragma unroll
+			for (int e = 0; e < 4; ++e) h[e] = ru.history[min(i + e * kPickBlock, ru.history_len - 1)];
+#pragma unroll
+			for (int e = 0; e < 4; ++e) {
+				const int64_t j = (int64_t)h[e] - v0;
+				if (i + e * kPickBlock < ru.history_len && j >= 0 && j < n) atomicAdd(&s_cnt[j], 1);
+			}
+		}
+		__syncthreads();
+	}
+	int32_t best = 0;
+	int at = -1;
+#pragma unroll
+	for (int u = 0; u < U; ++u) {
+		const int j = 4 * ((int)threadIdx.x + u * kPickBlock);
+		if (biased && u % (U / 2) == 0) {  // the next half of the slice's biases
+			const int h0 = u * 4 * kPickBlock;
+			if (u) __syncthreads();
+			for (int i = threadIdx.x; i < kPickSlice / 4; i += kPickBlock) ((v4i*)s_bias)[i] = v4i{0, 0, 0, 0};
+			__syncthreads();
+			for (int i = threadIdx.x; i < ru.bias_count; i += kPickBlock) {
+				const int64_t t = (int64_t)ru.bias_ids[i] - v0;
+				if (t >= h0 && t < h0 + kPickSlice / 2 && t < n) atomicAdd(&s_bias[t - h0], (unsigned long long)(int64_t)ru.bias_values[i]);
+			}
+			__syncthreads();
+		}
+		v4i c{0, 0, 0, 0};
+		if (seen) c = *(const v4i*)(s_cnt + j);
+#pragma unroll
+		for (int i = 0; i < 4; ++i) {
+			int32_t y = x[u][i];
+			if (biased || c[i] > 0) {
+				int64_t w = y;
+				if (c[i] > 0) {
+					// (w << 16) / rho: below 2^47, so the double quotient's truncation is the integer one
+					w = w > 0 ? (int64_t)((double)(w << 16) / (double)ru.repetition_q16) : (w * ru.repetition_q16) >> 16;
+					w -= (int64_t)ru.presence + (int64_t)ru.frequency * c[i];
+				}
+				if (biased) w += (int64_t)s_bias[j + i - u / (U / 2) * (kPickSlice / 2)];
+				y = sat_i32(w);
+			}
+			const bool ok = (legal[u] >> i & 1) != 0;
+			y = ok ? y : kI32Min;
+			x[u][i] = y;
+			if (ok && j + i < n && (at < 0 || y > best)) {
+				best = y;
+				at = v0 + j + i;
+			}
+		}
+		if (a.adjusted) {
+			int32_t* out = a.adjusted + (int64_t)r * a.adjusted_ld + v0;
+			if (VEC && j + 4 <= n) *(v4i*)(out + j) = x[u];
+			else {
+#pragma unroll
+				for (int i = 0; i < 4; ++i)
+					if (j + i < n) out[j + i] = x[u][i];
+			}
+		}
+	}
+	uint64_t key = at < 0 ? 0 : ((uint64_t)((uint32_t)best ^ 0x80000000u) << 32) | (0xffffffffu - (uint32_t)at);
 	for (int o = 32; o > 0; o >>= 1) {
 		const uint64_t w = __shfl_xor(key, o, 64);
 		key = w > key ? w : key;
@@ -1214,7 +1271,8 @@ __global__ __launch_bounds__(kPickBlock) void k_pick_slice(sslm_launch::PickArgs
 	__syncthreads();
 	if (threadIdx.x == 0) {
 		for (int w = 1; w < kPickBlock / 64; ++w) key = s_key[w] > key ? s_key[w] : key;
-		keys[(size_t)r * gridDim.x + blockIdx.x] = key;
+		if (gridDim.x == 1) a.tokens[r] = pick_of(key);
+		else keys[(size_t)r * gridDim.x + blockIdx.x] = key;
 	}
 }
 
@@ -1231,7 +1289,7 @@ __global__ __launch_bounds__(64) void k_pick_final(sslm_launch::PickArgs a, cons
 		const uint64_t w = __shfl_xor(key, o, 64);
 		key = w > key ? w : key;
 	}
-	if (threadIdx.x == 0) a.tokens[r] = key ? (int32_t)(0xffffffffu - (uint32_t)key) : -1;
+	if (threadIdx.x == 0) a.tokens[r] = pick_of(key);
 }
 
 }  // namespace sslm
@@ -1241,10 +1299,7 @@ __global__ __launch_bounds__(64) void k_pick_final(sslm_launch::PickArgs a, cons
 // ------------------------------------------------------------------------------------------
 namespace sslm_launch {
 
-#ifndef TW
-#define TW 1536
-#endif
-constexpr int kSaTargetWaves = TW;
+constexpr int kSaTargetWaves = 1536;
 
 static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -1409,8 +1464,10 @@ size_t pick_workspace(int rows, int vocab) { return up256((size_t)rows * pick_sl
 void pick_tokens(const PickArgs& a, hipStream_t s) {
 	const int slices = pick_slices(a.vocab);
 	unsigned long long* keys = (unsigned long long*)a.ws;
-	hipLaunchKernelGGL(k_pick_slice, dim3(slices, a.rows), dim3(kPickBlock), 0, s, a, keys);
-	hipLaunchKernelGGL(k_pick_final, dim3(a.rows), dim3(64), 0, s, a, keys, slices);
+	const bool vec = a.ld % 4 == 0 && (uintptr_t)a.logits % 16 == 0 && (!a.adjusted || (a.adjusted_ld % 4 == 0 && (uintptr_t)a.adjusted % 16 == 0));
+	if (vec) hipLaunchKernelGGL(k_pick_slice<true>, dim3(slices, a.rows), dim3(kPickBlock), 0, s, a, keys);
+	else hipLaunchKernelGGL(k_pick_slice<false>, dim3(slices, a.rows), dim3(kPickBlock), 0, s, a, keys);
+	if (slices > 1) hipLaunchKernelGGL(k_pick_final, dim3(a.rows), dim3(64), 0, s, a, keys, slices);
 }
 
 }  // namespace sslm_launch
