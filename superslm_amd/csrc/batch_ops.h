@@ -34,15 +34,6 @@ size_t shared_attn_workspace(int rows, int NH, int NKV, int D, int prefixes, int
 bool shared_attn_ok(int rows, int NH, int NKV, int D);
 void shared_attn(const SharedAttnArgs& a, hipStream_t s);
 
-// One adapter of a batch: A [rank, k], its fold [rank, 3], B [n, rank], its fold [n, 3].
-struct LoraRef {
-	const int8_t* a;
-	const int32_t* ufold;
-	const int8_t* b;
-	const int32_t* dfold;
-	int32_t rank, reserved;
-};
-
 // A projection of m rows, row t with adapter row_adapter[t] (negative: none) and incoming scale in_scale[t].
 struct LoraGemmArgs {
 	int m, n, k, count;
@@ -59,6 +50,19 @@ struct LoraGemmArgs {
 };
 size_t lora_gemm_workspace(int m, int n, int k);
 void lora_gemm(const LoraGemmArgs& g, hipStream_t s);
+
+// The rows' adapters of a launch sequence: out[(l 7 + p) ld + t] = rows[t][l 7 + p], nothing where rows[t] is null,
+// for layers l in [l0, l1), the 7 projections p and rows t < M.
+void lora_table(const LoraRef* const* rows, int M, int l0, int l1, LoraRef* out, int ld, hipStream_t s);
+
+// u = clamp(amp_fold(A x)) of the rows' own adapters for up to 3 projections sharing one input
+struct RowsUArgs {
+	int M, K, nproj;
+	const int8_t* x;          // [M, K]
+	const LoraRef* refs[3];   // [M]
+	int8_t* u[3];             // [M, kMaxRank]
+};
+void rows_u(const RowsUArgs& a, hipStream_t s);
 
 // The rules of one row of logits.
 struct LogitRule {

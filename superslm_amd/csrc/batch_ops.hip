@@ -12,7 +12,6 @@
 namespace sslm {
 
 using sslm_launch::LogitRule;
-using sslm_launch::LoraRef;
 
 template <int BS>
 __device__ __forceinline__ int64_t block_sum_i64(int64_t v, int64_t* slots) {
@@ -912,38 +911,54 @@ __device__ __forceinline__ bool row_adapter(const sslm_launch::LoraGemmArgs& g, 
 
 constexpr int kUChunks = 5;
 
-// u = clamp(amp_fold(A x)) of a row (forward_sites.cpp:1066-1086), one wave per rank: waves `wave` of row t.
-__device__ __forceinline__ void rows_u(const sslm_launch::LoraGemmArgs& g, int t, int rk, int8_t* u) {
+// u = clamp(amp_fold(A x)) of a row (forward_sites.cpp:1066-1086), one wave per rank `rk`.
+__device__ __forceinline__ void row_u(const LoraRef& ad, const int8_t* x, int k, int rk, int8_t* u) {
+	if (rk >= ad.rank) return;
 	const int lane = threadIdx.x & 63;
-	const LoraRef* ad;
-	if (!row_adapter(g, t, &ad) || !ad || rk >= ad->rank) return;
-	const int8_t *x = g.a + (size_t)t * g.k, *w = ad->a + (size_t)rk * g.k;
+	const int8_t* w = ad.a + (size_t)rk * k;
 	int32_t acc = 0;  // |A.x| <= 128^2 k <= 2^29
-	for (int c0 = lane * 16; c0 < g.k; c0 += 1024 * kUChunks) {  // kUChunks loads of each in flight
+	for (int c0 = lane * 16; c0 < k; c0 += 1024 * kUChunks) {  // kUChunks loads of each in flight
 		v4i p[kUChunks], q[kUChunks];
 #pragma unroll
 		for (int i = 0; i < kUChunks; ++i) {
-			const int c = min(c0 + 1024 * i, g.k - 16);
+			const int c = min(c0 + 1024 * i, k - 16);
 			p[i] = load16(x + c);
 			q[i] = load16(w + c);
 		}
 		__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
 		for (int i = 0; i < kUChunks; ++i) {
-			if (c0 + 1024 * i >= g.k) p[i] = v4i{0, 0, 0, 0};
+			if (c0 + 1024 * i >= k) p[i] = v4i{0, 0, 0, 0};
 #pragma unroll
 			for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_sdot4(p[i][j], q[i][j], acc, false);
 		}
 	}
 	acc = wave_sum32(acc);
 	if (lane == 0) {
-		const int32_t* fd = ad->ufold + 3 * rk;
-		u[(size_t)t * kMaxRank + rk] = (int8_t)clamp_code(apply_amp_fold((int64_t)acc, fd[0], fd[1], fd[2]));
+		const int32_t* fd = ad.ufold + 3 * rk;
+		u[rk] = (int8_t)clamp_code(apply_amp_fold((int64_t)acc, fd[0], fd[1], fd[2]));
 	}
+}
+
+__device__ __forceinline__ void rows_u(const sslm_launch::LoraGemmArgs& g, int t, int rk, int8_t* u) {
+	const LoraRef* ad;
+	if (!row_adapter(g, t, &ad) || !ad) return;
+	row_u(*ad, g.a + (size_t)t * g.k, g.k, rk, u + (size_t)t * kMaxRank);
 }
 
 __global__ __launch_bounds__(256) void k_rows_u(sslm_launch::LoraGemmArgs g, int8_t* u) {
 	rows_u(g, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 6), u);
+}
+
+__global__ __launch_bounds__(256) void k_refs_u(sslm_launch::RowsUArgs a) {
+	const int t = blockIdx.x, p = blockIdx.z;
+	const LoraRef ad = a.refs[p][t];
+	if (ad.a) row_u(ad, a.x + (size_t)t * a.K, a.K, blockIdx.y * 4 + (threadIdx.x >> 6), a.u[p] + (size_t)t * kMaxRank);
+}
+
+__global__ __launch_bounds__(64) void k_lora_table(const LoraRef* const* rows, int M, int i0, LoraRef* out, int ld) {
+	const int t = blockIdx.y * 64 + threadIdx.x, i = i0 + blockIdx.x;
+	if (t < M) out[(size_t)i * ld + t] = rows[t] ? rows[t][i] : LoraRef{};
 }
 
 // The products of up to 64 rows and their adapters' u in one launch, neither waiting for the other.
@@ -1455,6 +1470,14 @@ void lora_gemm(const LoraGemmArgs& g, hipStream_t s) {
 	if (g.n <= 2048) lora_funnel<512, 4, 1>(g, planes, part, u, s);
 	else if (g.n <= 5120) lora_funnel<1024, 5, 1>(g, planes, part, u, s);
 	else lora_funnel<1024, 8, 1>(g, planes, part, u, s);
+}
+
+void lora_table(const LoraRef* const* rows, int M, int l0, int l1, LoraRef* out, int ld, hipStream_t s) {
+	hipLaunchKernelGGL(k_lora_table, dim3((l1 - l0) * 7, (M + 63) / 64), dim3(64), 0, s, rows, M, l0 * 7, out, ld);
+}
+
+void rows_u(const RowsUArgs& a, hipStream_t s) {
+	hipLaunchKernelGGL(k_refs_u, dim3(a.M, kMaxRank / 4, a.nproj), dim3(256), 0, s, a);
 }
 
 static int pick_slices(int vocab) { return (vocab + kPickSlice - 1) / kPickSlice; }

@@ -28,12 +28,23 @@ struct Segment {
 	                            // maxpart[(col / 16) * kPartLd + t]; the consumer reduces the tiles
 	const int32_t* fold;        // [n, 3] (identity, mult, shift)
 	const int64_t* bias;        // [n] BIA1 codes, or null
-	const int8_t* lora_b;       // [n, rank] or null
+	const int8_t* lora_b;       // [n, rank] or null; with Epilogue::rank = kRankPerRow the rows' adapters, LoraRef [M]
 	const int32_t* lora_dfold;  // [n, 3] (identity, mult, exponent)
 	const int8_t* lora_u;       // [M, kMaxRank] adapter intermediate codes of this projection
 };
 
 constexpr int kMaxRank = 64;
+constexpr int kRankPerRow = -1;  // Epilogue::rank of a launch whose rows have adapters of their own
+
+// One adapter's tensors of one projection: A [rank, K], its fold [rank, 3], B [N, rank], its fold [N, 3].
+// b null: the adapter does not adapt it.
+struct LoraRef {
+	const int8_t* a;
+	const int32_t* ufold;
+	const int8_t* b;
+	const int32_t* dfold;
+	int32_t rank, reserved;
+};
 constexpr int kPartLd = 8192;  // token stride of the per-tile partial maxima (>= tokens per launch)
 constexpr int kMaxSeg = 3;
 constexpr int kFunnelMaxN = 8192;  // widest row the standalone funnel kernel covers

@@ -106,8 +106,16 @@ __device__ __forceinline__ int64_t lora_delta_v(const int8_t* lora_b, const int8
 // A leaf function (its byte loop inline, no further call): a non-leaf callee saves its return
 // address in scratch memory, and any private segment on a kernel costs every dispatch of it
 // about 0.5 us of launch time on MI355X, taken or not.
+// With rank = kRankPerRow the adapter is row t's own.
 __device__ __attribute__((noinline)) int64_t lora_delta_cold(const int8_t* lora_b, const int8_t* lora_u,
                                                              const int32_t* dfold, int rank, int t, int jj) {
+	if (rank == kRankPerRow) {
+		const LoraRef ref = ((const LoraRef*)lora_b)[t];
+		if (!ref.b) return 0;
+		lora_b = ref.b;
+		dfold = ref.dfold;
+		rank = ref.rank;
+	}
 	const int8_t* br = lora_b + (size_t)jj * rank;
 	const int8_t* ur = lora_u + (size_t)t * kMaxRank;
 	int32_t d = 0;

@@ -24,6 +24,7 @@
 
 #include "../../include/sslm_hip.h"
 #include "artifact.h"
+#include "batch_ops.h"
 #include "kernels.h"
 
 using namespace sslm;
@@ -175,6 +176,7 @@ struct sslm_adapter_s {
 	sslm_model model = nullptr;
 	uint32_t rank = 0;
 	std::vector<AdapterProj> proj;  // [layer * 7 + p], order q k v o gate up down
+	LoraRef* refs = nullptr;        // the same on the device, for launches whose rows have adapters of their own
 	std::vector<void*> owned;
 	size_t bytes = 0;
 	std::atomic<int> live_refs{0};
@@ -202,6 +204,8 @@ struct Track {
 	int8_t* kv_stage;    // prefill tracks: landed K/V rows awaiting kv_commit [T][2 * KVH]
 	uint32_t* sat_stage;  // prefill tracks: their clamp counts [T]
 	int8_t* lora_u[3];
+	const LoraRef** row_refs = nullptr;  // decode: per row its adapter's refs, or null [T]
+	LoraRef* lora_rows = nullptr;        // decode: (layer, projection, row) of them [L * 7][T]
 	TokenInfo* lg_tok;    // head tracks: tokens of the joined final norm + head
 	int32_t* lg_slot;
 	const uint8_t** lg_mask;  // head tracks: per token its schema mask page in HBM, or null
@@ -621,16 +625,50 @@ RawIn split_raw(sslm_model m, Track& w, GemmArgs& g, bool allow_multi, bool allo
 	return r;
 }
 
-void attach_lora(sslm_model m, Track& w, sslm_adapter ad, int layer, int proj, Segment* seg, int slot_u) {
-	if (!ad) return;
-	const AdapterProj& p = ad->proj[(size_t)layer * 7 + proj];
+// The adapters of a launch sequence: none, one for all of its rows, or one per row.
+struct UnitAdapters {
+	sslm_adapter one = nullptr;
+	std::vector<char> any;  // one per row: which (layer, projection)s some row's adapter has; else empty
+	UnitAdapters(sslm_adapter a = nullptr) : one(a) {}
+	bool none() const { return !one && any.empty(); }
+	int rank() const { return one ? (int)one->rank : (any.empty() ? 0 : kRankPerRow); }
+};
+
+void attach_lora(sslm_model m, Track& w, const UnitAdapters& ad, int layer, int proj, Segment* seg, int slot_u) {
+	const size_t at = (size_t)layer * 7 + proj;
+	if (!ad.any.empty()) {
+		if (!ad.any[at]) return;
+		seg->lora_b = (const int8_t*)(w.lora_rows + at * w.capacity);
+		seg->lora_u = w.lora_u[slot_u];
+		return;
+	}
+	if (!ad.one) return;
+	const AdapterProj& p = ad.one->proj[at];
 	if (!p.a) return;
 	seg->lora_b = p.b;
 	seg->lora_dfold = p.dfold;
 	seg->lora_u = w.lora_u[slot_u];
 }
 
-void run_lora_u(sslm_model m, Track& w, sslm_adapter ad, int layer, const int* projs, int n, const int8_t* x, int M, int K) {
+void run_lora_u(sslm_model m, Track& w, const UnitAdapters& use, int layer, const int* projs, int n, const int8_t* x, int M, int K) {
+	if (!use.any.empty()) {
+		sslm_launch::RowsUArgs a{};
+		a.M = M;
+		a.K = K;
+		a.x = x;
+		for (int i = 0; i < n; ++i) {
+			const size_t at = (size_t)layer * 7 + projs[i];
+			if (!use.any[at]) continue;
+			a.refs[a.nproj] = w.lora_rows + at * w.capacity;
+			a.u[a.nproj++] = w.lora_u[i];
+		}
+		if (!a.nproj) return;
+		ProfScope ps(w.stream, kProfLora, (int64_t)M * K, 0);
+		sslm_launch::rows_u(a, w.stream);
+		ck(hipGetLastError());
+		return;
+	}
+	const sslm_adapter ad = use.one;
 	if (!ad) return;
 	sslm_launch::LoraUArgs a{};
 	a.M = M;
@@ -661,14 +699,14 @@ struct ProjArgs {
 	RawIn raw;
 };
 
-ProjArgs qkv_args(sslm_model m, Track& w, int l, int M, sslm_adapter ad, bool fused) {
+ProjArgs qkv_args(sslm_model m, Track& w, int l, int M, const UnitAdapters& ad, bool fused) {
 	const DevLayer& lw = m->layers[l];
 	const int H = m->H, KVH = m->KVH;
 	GemmArgs g = gemm_args(m, w, w.normed, M, H, lw.w_qkv, H + 2 * KVH, H, lw.p_qkv);
 	g.epi.layer = l;
 	g.epi.in_recip = w.normed_recip;
 	g.epi.in_scale = w.normed_scale;
-	g.epi.rank = ad ? (int)ad->rank : 0;
+	g.epi.rank = ad.rank();
 	g.epi.nseg = 3;
 	g.epi.seg[0] = funnel_seg(0, H, w.q_f, H, w.mx_q, lw.f_qkv, lw.b_q);
 	Segment sk{};
@@ -696,12 +734,12 @@ ProjArgs qkv_args(sslm_model m, Track& w, int l, int M, sslm_adapter ad, bool fu
 	return pa;
 }
 
-ProjArgs o_args(sslm_model m, Track& w, int l, int M, sslm_adapter ad) {
+ProjArgs o_args(sslm_model m, Track& w, int l, int M, const UnitAdapters& ad) {
 	const DevLayer& lw = m->layers[l];
 	const int H = m->H;
 	GemmArgs g = gemm_args(m, w, w.ctx, M, H, lw.w_o, H, H, lw.p_o);
 	g.epi.layer = l;
-	g.epi.rank = ad ? (int)ad->rank : 0;
+	g.epi.rank = ad.rank();
 	g.epi.nseg = 1;
 	g.epi.seg[0] = funnel_seg(0, H, w.o_f, H, w.mx_o, lw.f_o, nullptr);
 	attach_lora(m, w, ad, l, 3, &g.epi.seg[0], 0);
@@ -710,12 +748,12 @@ ProjArgs o_args(sslm_model m, Track& w, int l, int M, sslm_adapter ad) {
 	return pa;
 }
 
-ProjArgs gu_args(sslm_model m, Track& w, int l, int M, sslm_adapter ad) {
+ProjArgs gu_args(sslm_model m, Track& w, int l, int M, const UnitAdapters& ad) {
 	const DevLayer& lw = m->layers[l];
 	const int H = m->H, I = m->I;
 	GemmArgs g = gemm_args(m, w, w.mlp_normed, M, H, lw.w_gu, 2 * I, H, lw.p_gu);
 	g.epi.layer = l;
-	g.epi.rank = ad ? (int)ad->rank : 0;
+	g.epi.rank = ad.rank();
 	g.epi.nseg = 2;
 	g.epi.seg[0] = funnel_seg(0, I, w.gu_f, 2 * I, w.mx_gu, lw.f_gu, nullptr);
 	g.epi.seg[1] = funnel_seg(I, 2 * I, w.gu_f + I, 2 * I, w.mx_gu, lw.f_gu + 3 * I, nullptr);
@@ -726,12 +764,12 @@ ProjArgs gu_args(sslm_model m, Track& w, int l, int M, sslm_adapter ad) {
 	return pa;
 }
 
-ProjArgs down_args(sslm_model m, Track& w, int l, int M, sslm_adapter ad) {
+ProjArgs down_args(sslm_model m, Track& w, int l, int M, const UnitAdapters& ad) {
 	const DevLayer& lw = m->layers[l];
 	const int H = m->H, I = m->I;
 	GemmArgs g = gemm_args(m, w, w.act, M, I, lw.w_down, H, I, lw.p_down);
 	g.epi.layer = l;
-	g.epi.rank = ad ? (int)ad->rank : 0;
+	g.epi.rank = ad.rank();
 	g.epi.nseg = 1;
 	g.epi.seg[0] = funnel_seg(0, H, w.down_f, H, w.mx_down, lw.f_down, nullptr);
 	attach_lora(m, w, ad, l, 6, &g.epi.seg[0], 0);
@@ -820,7 +858,7 @@ struct StreamRef {
 // Layers [l0, l1) for M tokens whose TokenInfo is already on the device.
 // `decode`: every token belongs to a different sequence (a decode step), so attention may take
 // the fused path.
-void run_layers(sslm_model m, Track& w, int M, StreamRef st, int l0, int l1, sslm_adapter ad, bool decode) {
+void run_layers(sslm_model m, Track& w, int M, StreamRef st, int l0, int l1, const UnitAdapters& ad, bool decode) {
 	const int H = m->H, I = m->I, KVH = m->KVH;
 	hipStream_t s = w.stream;
 	{
@@ -837,7 +875,7 @@ void run_layers(sslm_model m, Track& w, int M, StreamRef st, int l0, int l1, ssl
 	// a few sequences: the context and activation funnels run inside the GEMVs that read their codes, for
 	// one sequence the residual rows too (the q|k|v projection of layers past the first in the one before)
 	const DevLayer& lp = m->layers[l0];
-	const bool chain = fused && !ad && !dbg && w.raw_part && lp.p_qkv && lp.p_o && lp.p_gu && lp.p_down && w.act_prod &&
+	const bool chain = fused && ad.none() && !dbg && w.raw_part && lp.p_qkv && lp.p_o && lp.p_gu && lp.p_down && w.act_prod &&
 	                   sslm_launch::decode_chain_ok(M, H, m->NH, KVH, I);
 	const bool chain_rows = chain && M == 1;
 	for (int l = l0; l < l1; ++l) {
@@ -1324,6 +1362,8 @@ void alloc_track(sslm_model m, Track& w, int T, bool head) {
 		w.raw_part = elems ? dalloc<int32_t>(elems, &own) : nullptr;
 	}
 	for (int i = 0; i < 3; ++i) w.lora_u[i] = dalloc<int8_t>((size_t)T * kMaxRank, &own);
+	w.row_refs = w.prefill ? nullptr : (const LoraRef**)dalloc<uintptr_t>(T, &own);
+	w.lora_rows = w.prefill ? nullptr : dalloc<LoraRef>((size_t)T * m->L * 7, &own);
 	w.act_prod = dalloc<int32_t>((size_t)sslm_launch::kMaxSlicedActRows * I, &own);
 	w.act_maxpart = dalloc<uint32_t>((size_t)sslm_launch::kMaxActSlices * kPartLd, &own);
 	w.gu_scale = dalloc<Scale>((size_t)sslm_launch::kMaxSlicedActRows * 2, &own);
@@ -2173,10 +2213,11 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 	need_logits.erase(std::remove_if(need_logits.begin(), need_logits.end(), [&](int i) { return i >= n; }),
 	                  need_logits.end());
 
-	// launch units: (layer range, adapter, tokens), at most kTrackTokens tokens each
+	// launch units: (layer range, adapters, tokens), at most kTrackTokens tokens each.  Sequences with
+	// different adapters share a unit: a unit of its own for each reads every weight again.
 	struct Unit {
 		uint32_t l0, l1;
-		sslm_adapter ad;
+		UnitAdapters ad;
 		std::vector<int> idx;
 	};
 	std::vector<Unit> units;
@@ -2184,20 +2225,23 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 	for (auto& g : groups) {
 		const uint32_t l0 = g.first;
 		const uint32_t l1 = std::min<uint32_t>(m->L, l0 + budget);
-		std::vector<sslm_adapter> ads;
-		for (int i : g.second)
-			if (std::find(ads.begin(), ads.end(), seqs[i]->adapter) == ads.end()) ads.push_back(seqs[i]->adapter);
-		for (sslm_adapter ad : ads) {
-			std::vector<int> members;
-			for (int i : g.second)
-				if (seqs[i]->adapter == ad) members.push_back(i);
-			const int total = (int)members.size();
-			int parts = std::max(1, std::min(track_limit(), total / track_min()));
-			parts = std::max(parts, (total + kTrackTokens - 1) / kTrackTokens);
-			for (int p = 0; p < parts; ++p) {
-				const int b = (int)((int64_t)total * p / parts), e = (int)((int64_t)total * (p + 1) / parts);
-				if (e > b) units.push_back(Unit{l0, l1, ad, std::vector<int>(members.begin() + b, members.begin() + e)});
+		const std::vector<int>& members = g.second;
+		const int total = (int)members.size();
+		int parts = std::max(1, std::min(track_limit(), total / track_min()));
+		parts = std::max(parts, (total + kTrackTokens - 1) / kTrackTokens);
+		for (int p = 0; p < parts; ++p) {
+			const int b = (int)((int64_t)total * p / parts), e = (int)((int64_t)total * (p + 1) / parts);
+			if (e <= b) continue;
+			Unit un{l0, l1, UnitAdapters(seqs[members[b]]->adapter), std::vector<int>(members.begin() + b, members.begin() + e)};
+			std::set<sslm_adapter> ads;
+			for (int i : un.idx) ads.insert(seqs[i]->adapter);
+			if (ads.size() > 1) {
+				un.ad = UnitAdapters();
+				un.ad.any.assign((size_t)m->L * 7, 0);
+				for (sslm_adapter ad : ads)
+					for (size_t k = 0; ad && k < ad->proj.size(); ++k) un.ad.any[k] |= ad->proj[k].a != nullptr;
 			}
+			units.push_back(std::move(un));
 		}
 		if (l1 == (uint32_t)m->L)
 			for (int i : g.second) finished.push_back(i);
@@ -2226,6 +2270,7 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 	std::deque<std::vector<TokenInfo>> h_tok;  // deque: references to earlier entries stay valid
 	std::deque<std::vector<int32_t>> h_i32;
 	std::deque<std::vector<const uint8_t*>> h_ptr;
+	std::deque<std::vector<const LoraRef*>> h_ref;
 	// the grouped decode attention's score rows for a unit: from its widest row (pos + 1)
 	auto unit_wcap = [&](const Unit& un) {
 		int64_t mw = 1;
@@ -2252,6 +2297,23 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 		ck(hipMemcpyAsync(w.tok, ti.data(), M * sizeof(TokenInfo), hipMemcpyHostToDevice, s));
 		ck(hipMemcpyAsync(w.slot_idx, slots.data(), M * 4, hipMemcpyHostToDevice, s));
 		if (un.l0 == 0) ck(hipMemcpyAsync(w.tok_ids, ids.data(), M * 4, hipMemcpyHostToDevice, s));
+		if (!un.ad.any.empty()) {
+			h_ref.emplace_back(M);
+			std::vector<const LoraRef*>& refs = h_ref.back();
+			for (int t = 0; t < M; ++t) {
+				const sslm_adapter ad = seqs[un.idx[t]]->adapter;
+				refs[t] = ad ? ad->refs : nullptr;
+			}
+			ck(hipMemcpyAsync(w.row_refs, refs.data(), M * sizeof(void*), hipMemcpyHostToDevice, s));
+		}
+	};
+	// a graph holds one adapter's addresses, or which projections read the rows' own
+	auto adapters_key = [](const UnitAdapters& ad) {
+		std::string k = std::to_string((uintptr_t)ad.one);
+		for (size_t i = 0; i < ad.any.size(); i += 4)
+			k += "0123456789abcdef"[ad.any[i] | (i + 1 < ad.any.size() ? ad.any[i + 1] << 1 : 0) |
+			                        (i + 2 < ad.any.size() ? ad.any[i + 2] << 2 : 0) | (i + 3 < ad.any.size() ? ad.any[i + 3] << 3 : 0)];
+		return k;
 	};
 	// units whose snapshot was enqueued for execution (not merely recorded into a graph that a
 	// refused launch then discarded): what a refused launch must restore
@@ -2266,6 +2328,11 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 		sslm_launch::slot_state_copy(slot_copy_args(m, w.tok, (int)un.l0, (int)un.l1), M, false, w.stream);
 		ck(hipGetLastError());
 		if (!capturing) snapped[u] = 1;
+		if (!un.ad.any.empty()) {
+			ProfScope p(w.stream, kProfLora, 0, 0);
+			sslm_launch::lora_table(w.row_refs, M, (int)un.l0, (int)un.l1, w.lora_rows, w.capacity, w.stream);
+			ck(hipGetLastError());
+		}
 		if (un.l0 == 0) {  // embed the pending token (src/sslm_abi.cpp:2237-2249)
 			ProfScope p(w.stream, kProfRow, 0, 0);
 			sslm_launch::embed(w.tok_ids, M, m->embed, m->H, m->V, m->embed_site, m->stream_codes, w.slot_idx,
@@ -2333,7 +2400,7 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 					const Unit& un = units[u];
 					const std::string key = "u" + std::to_string(u % ntr) + "|" + std::to_string(un.idx.size()) + "|" +
 					                        std::to_string(un.l0) + "|" + std::to_string(un.l1) + "|" +
-					                        std::to_string((uintptr_t)un.ad) + "|" + std::to_string((uintptr_t)m->pool_dev) +
+					                        adapters_key(un.ad) + "|" + std::to_string((uintptr_t)m->pool_dev) +
 					                        (sslm_launch::grouped_attention_chosen((int)un.idx.size(), m->NKV, m->cap)
 					                             ? "|g" + std::to_string(unit_wcap(un)) + "h" +
 					                                   std::to_string(sslm_launch::group_row_halves(
@@ -2777,6 +2844,9 @@ sslm_status sslm_adapter_map(const void* data, size_t size, sslm_model base, ssl
 			p.ufold = dupload(uf, &h->owned);
 			p.dfold = dupload(df, &h->owned);
 		}
+		std::vector<LoraRef> refs;
+		for (const AdapterProj& p : h->proj) refs.push_back(LoraRef{p.a, p.ufold, p.b, p.dfold, p.a ? (int32_t)rank : 0, 0});
+		h->refs = dupload(refs, &h->owned);
 		return SSLM_OK;
 	});
 	if (st != SSLM_OK) {
