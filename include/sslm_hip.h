@@ -284,6 +284,22 @@ sslm_status sslm_hip_gemm_requant_noalloc(const int8_t* a, const int8_t* w, cons
                                           int32_t k, int64_t in_m, int64_t in_e, int64_t site_m, int64_t site_e,
                                           int8_t* out_codes, int64_t* out_me, int32_t* out_status, void* stream);
 
+/* ---- requests with rules of their own (no reference counterpart) ----
+ * Token rules of a sequence for the greedy verbs' picks, with the arithmetic of sslm_hip_pick_tokens: the
+ * context counted is every token the sequence has taken in by prefill and produced since it was created,
+ * reset or restored; a bound schema masks as before.  Batches may mix sequences with and without rules.  The
+ * arrays are copied.  Null removes the rules; they survive sslm_seq_reset and are not part of a saved blob.
+ * Damped-greedy calls refuse a sequence that has rules (SSLM_INVALID_ARGUMENT). */
+typedef struct sslm_hip_rules {
+	uint32_t struct_size;
+	int32_t repetition_q16; /* 65536: no penalty; at least 1 */
+	int32_t presence, frequency; /* logit units */
+	int32_t bias_count, reserved;
+	const int32_t* bias_ids; /* below the vocabulary, else SSLM_TOKEN_ID_OUT_OF_RANGE */
+	const int32_t* bias_values;
+} sslm_hip_rules;
+sslm_status sslm_hip_seq_set_rules(sslm_seq seq, const sslm_hip_rules* rules);
+
 /* ---- operators of a decode step whose rows are different requests (no reference counterpart) ----
  *
  * All three take device buffers and run asynchronously on `stream` (a hipStream_t of the current

@@ -81,6 +81,8 @@ struct PickArgs {
 	void* ws;  // pick_workspace() bytes
 };
 size_t pick_workspace(int rows, int vocab);
+// *at[i] = token[i] for every i < n with at[i]
+void append_tokens(int32_t* const* at, const int32_t* token, int n, hipStream_t s);
 void pick_tokens(const PickArgs& a, hipStream_t s);
 
 }  // namespace sslm_launch

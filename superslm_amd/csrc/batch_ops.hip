@@ -1291,6 +1291,11 @@ __global__ __launch_bounds__(kPickBlock) void k_pick_slice(sslm_launch::PickArgs
 	}
 }
 
+__global__ __launch_bounds__(64) void k_append_tokens(int32_t* const* at, const int32_t* token, int n) {
+	const int i = blockIdx.x * 64 + threadIdx.x;
+	if (i < n && at[i]) *at[i] = token[i];
+}
+
 __global__ __launch_bounds__(64) void k_pick_final(sslm_launch::PickArgs a, const unsigned long long* keys, int slices) {
 	const int r = blockIdx.x;
 	const LogitRule ru = a.rules[r];
@@ -1481,6 +1486,10 @@ void rows_u(const RowsUArgs& a, hipStream_t s) {
 }
 
 static int pick_slices(int vocab) { return (vocab + kPickSlice - 1) / kPickSlice; }
+
+void append_tokens(int32_t* const* at, const int32_t* token, int n, hipStream_t s) {
+	hipLaunchKernelGGL(k_append_tokens, dim3((n + 63) / 64), dim3(64), 0, s, at, token, n);
+}
 
 size_t pick_workspace(int rows, int vocab) { return up256((size_t)rows * pick_slices(vocab) * 8); }
 

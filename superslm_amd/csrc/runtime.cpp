@@ -332,6 +332,11 @@ struct sslm_model_s {
 	int64_t dg_q_ln2 = 0, dg_q_b = 0, dg_q_c = 0;
 	int32_t* logits = nullptr;  // [kMaxTokens, V] raw head rows, allocated on first use
 	int2* topk = nullptr;       // [kMaxTokens, kTopKMax] damped greedy's device candidates
+	// token rules: the rows' rules, what to append to their histories and pick_tokens' scratch, on first use
+	sslm_launch::LogitRule* rules = nullptr;  // [kMaxTokens]
+	int32_t** append_at = nullptr;            // [kMaxTokens]
+	int32_t* append_token = nullptr;          // [kMaxTokens]
+	void* pick_ws = nullptr;
 	std::vector<SchemaEntry> schemas;
 	std::vector<sslm_schema_s> schema_handles;
 	uint32_t page_bytes = 0;  // (V + 7) / 8
@@ -369,6 +374,18 @@ struct sslm_kv_pool_s {
 	std::mutex mu;
 };
 
+// A sequence's token rules (sslm_hip_seq_set_rules), its biases and the tokens of its context on the device.
+struct SeqRules {
+	sslm_launch::LogitRule rule{};  // but for the mask
+	int32_t* history = nullptr;     // [capacity]
+	size_t capacity = 0;
+	size_t uploaded = 0;            // tokens of the context that `history` holds
+	std::vector<void*> owned;
+	~SeqRules() {
+		for (void* p : owned) (void)hipFree(p);
+	}
+};
+
 struct sslm_seq_s {
 	sslm_model model = nullptr;
 	sslm_kv_pool pool = nullptr;
@@ -383,6 +400,8 @@ struct sslm_seq_s {
 	AntiLm anti_lm;  // damped-greedy n-gram state (order 0: none)
 	sslm_schema schema = nullptr;       // bound schema
 	uint32_t walk = 0xFFFFFFFFu;        // DFA walk state (0xFFFFFFFF: no schema bound)
+	std::vector<int32_t> context;       // the tokens taken in and produced, what token rules count
+	std::unique_ptr<SeqRules> rules;
 	std::mutex mu;
 };
 
@@ -1134,10 +1153,18 @@ void run_layers(sslm_model m, Track& w, int M, StreamRef st, int l0, int l1, con
 }
 
 
+// the rules of a row that has none
+sslm_launch::LogitRule neutral_rule() {
+	sslm_launch::LogitRule r{};
+	r.repetition_q16 = 1 << 16;
+	return r;
+}
+
 // final norm + LM head + lowest-index argmax for M tokens whose stream rows are st.idx
 // (src/sslm_abi.cpp:2280-2289, forward_sites.cpp:2412-2441)
+// `rules`: the head's raw logits to m->logits and each row's token under its rules instead.
 void run_logits(sslm_model m, Track& w, int M, StreamRef st, const TokenInfo* tok,
-                const uint8_t* const* mask = nullptr) {
+                const uint8_t* const* mask = nullptr, bool rules = false) {
 	hipStream_t s = w.stream;
 	{
 		ProfScope p(s, kProfRow, 0, 0);
@@ -1147,6 +1174,25 @@ void run_logits(sslm_model m, Track& w, int M, StreamRef st, const TokenInfo* to
 		ck(hipGetLastError());
 	}
 	GemmArgs g = head_args(m, w, M, tok);
+	if (rules) {
+		g.epi.argmax_key = nullptr;
+		g.epi.raw_out = m->logits;
+		run_gemm(m, w, g, kProfHead);
+		ProfScope p(s, kProfRow, 0, 0);
+		sslm_launch::append_tokens(m->append_at, m->append_token, M, s);
+		ck(hipGetLastError());
+		sslm_launch::PickArgs a{};
+		a.rows = M;
+		a.vocab = m->V;
+		a.logits = m->logits;
+		a.ld = m->V;
+		a.rules = m->rules;
+		a.tokens = w.out_tokens;
+		a.ws = m->pick_ws;
+		sslm_launch::pick_tokens(a, s);
+		ck(hipGetLastError());
+		return;
+	}
 	g.epi.mask_page = mask;
 	run_gemm(m, w, g, kProfHead);
 	sslm_launch::argmax_finalize(w.argmax_key, (m->V + 15) / 16, M, w.out_tokens, s);
@@ -2069,6 +2115,8 @@ sslm_status sslm_seq_reset(sslm_seq seq) {
 		seq->forced_token_count = 0;
 		seq->anti_lm.reset(0);
 		seq->walk = seq->schema ? 0u : kWalkUnused;
+		seq->context.clear();
+		if (seq->rules) seq->rules->uploaded = 0;
 		return SSLM_OK;
 	});
 }
@@ -2127,6 +2175,7 @@ sslm_status sslm_prefill(sslm_model model, sslm_seq seq, const int32_t* tokens, 
 				seq->forced_token_count += admit;
 			}
 			seq->current_token = tokens[admit - 1];
+			seq->context.insert(seq->context.end(), tokens, tokens + admit);
 			*consumed = admit;
 			seq->ready_for_logits = true;  // src/sslm_abi.cpp:1969-1972
 		}
@@ -2256,7 +2305,15 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 	const bool rows_needed = damped && !cands;
 	bool masked = false;
 	for (int i : lg) masked = masked || seqs[i]->schema;
-	if (damped && !m->logits) m->logits = dalloc<int32_t>((size_t)kMaxTokens * m->V, &m->owned);
+	bool ruled = false;
+	for (int i : lg) ruled = ruled || seqs[i]->rules;
+	if ((damped || ruled) && !m->logits) m->logits = dalloc<int32_t>((size_t)kMaxTokens * m->V, &m->owned);
+	if (ruled && !m->pick_ws) {
+		m->rules = dalloc<sslm_launch::LogitRule>(kMaxTokens, &m->owned);
+		m->append_at = (int32_t**)dalloc<uintptr_t>(kMaxTokens, &m->owned);
+		m->append_token = dalloc<int32_t>(kMaxTokens, &m->owned);
+		m->pick_ws = dalloc<uint8_t>(sslm_launch::pick_workspace(kMaxTokens, m->V), &m->owned);
+	}
 	if (cands && !m->topk) m->topk = dalloc<int2>((size_t)kMaxTokens * sslm_launch::kTopKMax, &m->owned);
 
 	// Host staging, uploaded before the kernels (kept alive until the sync below).  The common
@@ -2271,6 +2328,8 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 	std::deque<std::vector<int32_t>> h_i32;
 	std::deque<std::vector<const uint8_t*>> h_ptr;
 	std::deque<std::vector<const LoraRef*>> h_ref;
+	std::deque<std::vector<sslm_launch::LogitRule>> h_rule;
+	std::deque<std::vector<int32_t*>> h_at;
 	// the grouped decode attention's score rows for a unit: from its widest row (pos + 1)
 	auto unit_wcap = [&](const Unit& un) {
 		int64_t mw = 1;
@@ -2363,10 +2422,42 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 			}
 			ck(hipMemcpyAsync(t0.lg_mask, pg.data(), M * sizeof(void*), hipMemcpyHostToDevice, s));
 		}
+		if (ruled) {
+			h_rule.emplace_back(M);
+			h_at.emplace_back(M, nullptr);
+			h_i32.emplace_back(M, 0);
+			std::vector<int32_t>& token = h_i32.back();
+			for (int t = 0; t < M; ++t) {
+				sslm_seq q = seqs[lg[b + t]];
+				sslm_launch::LogitRule& ru = h_rule.back()[t];
+				ru = q->rules ? q->rules->rule : neutral_rule();
+				if (q->schema) ru.mask = m->d_pages + m->page_off[q->schema->index] + (size_t)q->walk * m->page_bytes;
+				if (!q->rules) continue;
+				// the context's tokens that the device lacks: one, the last one produced, in a running decode
+				SeqRules& sr = *q->rules;
+				const size_t n = q->context.size();
+				if (n > sr.capacity) {  // a produced token that a prefill passes over stays counted
+					sr.capacity = 2 * n;
+					sr.history = dalloc<int32_t>(sr.capacity, &sr.owned);
+					sr.uploaded = 0;
+				}
+				const size_t have = sr.uploaded;
+				if (n > have) {
+					if (n - have > 1) ck(hipMemcpyAsync(sr.history + have, q->context.data() + have, (n - 1 - have) * 4, hipMemcpyHostToDevice, s));
+					h_at.back()[t] = sr.history + n - 1;
+					token[t] = q->context[n - 1];
+				}
+				ru.history = sr.history;
+				ru.history_len = (int32_t)n;
+			}
+			ck(hipMemcpyAsync(m->rules, h_rule.back().data(), M * sizeof(sslm_launch::LogitRule), hipMemcpyHostToDevice, s));
+			ck(hipMemcpyAsync(m->append_at, h_at.back().data(), M * sizeof(void*), hipMemcpyHostToDevice, s));
+			ck(hipMemcpyAsync(m->append_token, token.data(), M * 4, hipMemcpyHostToDevice, s));
+		}
 	};
 	auto launch_logits = [&](int M) {
 		run_logits(m, t0, M, StreamRef{m->stream_codes, m->stream_scale, t0.lg_slot}, t0.lg_tok,
-		           masked ? t0.lg_mask : nullptr);
+		           masked ? t0.lg_mask : nullptr, ruled);
 		if (damped) {  // the whole logit rows as well: the head's raw int32 accumulators
 			GemmArgs g = head_args(m, t0, M, t0.lg_tok);
 			g.epi.argmax_key = nullptr;
@@ -2423,7 +2514,7 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 				const int M = (int)lg.size();
 				if (use_graph)
 					ck(hipGraphLaunch(graph_of(m, "lg|" + std::to_string(M) + (rows_needed ? "|r" : "") +
-					                                  (cands ? "|c" + std::to_string(params.top_k) : "") + (masked ? "|m" : ""),
+					                                  (cands ? "|c" + std::to_string(params.top_k) : "") + (masked ? "|m" : "") + (ruled ? "|t" : ""),
 					                           t0.stream,
 					                           [&] { launch_logits(M); }),
 					                  t0.stream));
@@ -2481,6 +2572,8 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 	std::vector<int32_t> words(kSlotCapacity);
 	ck(hipMemcpyAsync(words.data(), m->status, kSlotCapacity * 4, hipMemcpyDeviceToHost, t0.stream));
 	ck(hipStreamSynchronize(t0.stream));
+	for (int i : lg)
+		if (seqs[i]->rules) seqs[i]->rules->uploaded = seqs[i]->context.size();
 	prof_collect();
 
 	// Outcomes in call order.  The reference runs the sequences one after another and returns at
@@ -2554,6 +2647,7 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 		}
 		if (damped) s->anti_lm.update(tok);
 		s->current_token = tok;
+		s->context.push_back(tok);
 		s->layer_index = 0;
 		out_tokens[i] = tok;
 	}
@@ -2603,6 +2697,7 @@ static sslm_status decode_impl(sslm_model model, sslm_seq* seqs, int32_t n, cons
 		for (int i = 0; i < n; ++i) {
 			if (!live[i]) continue;
 			if (seqs[i]->model != model) return SSLM_INVALID_ARGUMENT;
+			if (seqs[i]->rules && params->mode == SSLM_DECODE_MODE_DAMPED_GREEDY) return SSLM_INVALID_ARGUMENT;
 			if (seqs[i]->layer_index == 0 && seqs[i]->current_token < 0 && !seqs[i]->ready_for_logits)
 				return SSLM_INVALID_ARGUMENT;
 		}
@@ -2887,6 +2982,36 @@ sslm_status sslm_seq_set_adapter(sslm_seq seq, sslm_adapter adapter) {
 	seq->adapter = adapter;
 	if (adapter) adapter->live_refs++;
 	return SSLM_OK;
+}
+
+sslm_status sslm_hip_seq_set_rules(sslm_seq seq, const sslm_hip_rules* rules) {
+	if (!seq) return SSLM_INVALID_ARGUMENT;
+	sslm_model m = seq->model;
+	if (rules) {
+		if (rules->struct_size != sizeof(*rules) || rules->repetition_q16 < 1 || rules->bias_count < 0 ||
+		    (rules->bias_count > 0 && (!rules->bias_ids || !rules->bias_values)))
+			return SSLM_INVALID_ARGUMENT;
+		for (int32_t i = 0; i < rules->bias_count; ++i)
+			if (rules->bias_ids[i] < 0 || rules->bias_ids[i] >= m->V) return SSLM_TOKEN_ID_OUT_OF_RANGE;
+	}
+	return guarded([&]() -> sslm_status {
+		std::lock_guard<std::mutex> lk(m->mu);  // no decode step reads the old rules meanwhile
+		std::unique_ptr<SeqRules> r;
+		if (rules) {
+			r.reset(new SeqRules());
+			r->capacity = (size_t)m->cap + 1;
+			r->history = dalloc<int32_t>(r->capacity, &r->owned);
+			const int n = rules->bias_count;
+			r->rule.bias_ids = dupload(std::vector<int32_t>(rules->bias_ids, rules->bias_ids + n), &r->owned);
+			r->rule.bias_values = dupload(std::vector<int32_t>(rules->bias_values, rules->bias_values + n), &r->owned);
+			r->rule.bias_count = n;
+			r->rule.repetition_q16 = rules->repetition_q16;
+			r->rule.presence = rules->presence;
+			r->rule.frequency = rules->frequency;
+		}
+		seq->rules = std::move(r);
+		return SSLM_OK;
+	});
 }
 
 // ---- outside the integer forward path ----

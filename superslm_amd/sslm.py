@@ -45,6 +45,13 @@ class DecodeParams(ctypes.Structure):
                 ("q_ln2", ctypes.c_int64), ("q_b", ctypes.c_int64), ("q_c", ctypes.c_int64)]
 
 
+class Rules(ctypes.Structure):
+    """sslm_hip_rules (include/sslm_hip.h): a backend extra."""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("repetition_q16", ctypes.c_int32), ("presence", ctypes.c_int32),
+                ("frequency", ctypes.c_int32), ("bias_count", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("bias_ids", ctypes.c_void_p), ("bias_values", ctypes.c_void_p)]
+
+
 class StatsOut(ctypes.Structure):
     """sslm_stats_out (sslm_abi.h:232-238)."""
     _fields_ = [("decode_step_ceiling", ctypes.c_int64), ("decode_step_actual", ctypes.c_int64),
@@ -108,6 +115,8 @@ class SslmLib:
         sig("sslm_schema_name", ctypes.c_int, vp, i32, vp, ctypes.POINTER(sz))
         sig("sslm_seq_set_schema", ctypes.c_int, vp, vp)
         sig("sslm_stats", ctypes.c_int, vp, vp, ctypes.POINTER(StatsOut))
+        if hasattr(L, "sslm_hip_seq_set_rules"):
+            sig("sslm_hip_seq_set_rules", ctypes.c_int, vp, ctypes.POINTER(Rules))
         self.has_peek = hasattr(L, "sslm_g5_test_only_peek_kv_block_bytes")
         if self.has_peek:
             sig("sslm_g5_test_only_peek_kv_block_bytes", ctypes.c_int, vp, u32, vp, sz)
@@ -288,6 +297,26 @@ class Seq:
         m = self.pool.model
         m.lib.check("sslm_seq_set_adapter",
                     m.lib.lib.sslm_seq_set_adapter(self.handle, adapter.handle if adapter else None))
+
+    def set_rules(self, repetition: float = 1.0, presence: int = 0, frequency: int = 0, bias=(), raw: bool = False):
+        """sslm_hip_seq_set_rules: a penalty factor for tokens the context holds (rounded to Q16), its
+        additive penalties in logit units, and (token, value) biases."""
+        pairs = list(bias.items()) if isinstance(bias, dict) else list(bias)
+        ids = np.array([t for t, _ in pairs], dtype=np.int32)
+        values = np.array([v for _, v in pairs], dtype=np.int32)
+        r = Rules(ctypes.sizeof(Rules), int(round(repetition * 65536)), presence, frequency, len(pairs), 0,
+                  ids.ctypes.data, values.ctypes.data)
+        return self._rules(ctypes.byref(r), raw)
+
+    def clear_rules(self, raw: bool = False):
+        return self._rules(None, raw)
+
+    def _rules(self, ref, raw):
+        m = self.pool.model
+        st = m.lib.lib.sslm_hip_seq_set_rules(self.handle, ref)
+        if raw:
+            return st
+        m.lib.check("sslm_hip_seq_set_rules", st)
 
     def save_size(self):
         """The two-call sizing form: (status, required size) of sslm_seq_save with no buffer."""
