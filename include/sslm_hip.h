@@ -10,7 +10,7 @@
  * The caller-owned KV-pool and workspace buffers are still required and validated exactly as the
  * reference validates them (size, 64-byte alignment) and hold only host bookkeeping.
  *
- * Verbs outside the integer forward path (tokenizer, prefixes, detokenize) are exported with
+ * Verbs outside the integer forward path (tokenizer, detokenize) are exported with
  * their reference signatures and return SSLM_INVALID_ARGUMENT.
  */
 #ifndef SSLM_HIP_H
@@ -166,15 +166,24 @@ sslm_status sslm_workspace_create(sslm_model model, const sslm_config* config, v
 sslm_status sslm_g5_test_only_peek_kv_block_bytes(sslm_kv_pool pool, uint32_t block_index, uint8_t* out_buf,
                                                   size_t n);
 
-/* ---- outside the integer forward path: exported, always SSLM_INVALID_ARGUMENT ---- */
+/* ---- shared prompts (the reference's prefix verbs) ----
+ * A prefix takes a block of its pool and is prefilled like a sequence without an adapter (in any number
+ * of calls) until it is frozen (then SSLM_PREFIX_FROZEN_REJECTED).  A fresh sequence of the same pool, with the
+ * same schema bound (else SSLM_PREFIX_SCHEMA_MISMATCH), adopts a frozen prefix: its tokens, KV block, blob
+ * and every later result are those of a sequence that took the prompt itself.  Decode steps then read the
+ * prompt's K/V once for all of the batch's adopters (sslm_hip_shared_attention) where that is the faster
+ * form.  Anything else -- a prefix not frozen, a sequence that holds context, another pool -- is refused
+ * (SSLM_INVALID_ARGUMENT).  A released prefix keeps its block until its last adopter is released or reset. */
 sslm_status sslm_prefix_begin(sslm_model model, sslm_kv_pool* pool, sslm_prefix* out);
 sslm_status sslm_prefix_prefill(sslm_model model, sslm_prefix prefix, const int32_t* tokens, int32_t count,
                                 int32_t chunk_budget, sslm_span_kind kind, sslm_workspace ws, int32_t* consumed);
 sslm_status sslm_prefix_freeze(sslm_prefix prefix);
 sslm_status sslm_prefix_release(sslm_prefix prefix);
 sslm_status sslm_seq_adopt_prefix(sslm_seq seq, sslm_prefix prefix);
-sslm_status sslm_tokenize(sslm_model model, const char* utf8, int32_t* tokens, int32_t* n);
 sslm_status sslm_prefix_set_schema(sslm_prefix prefix, sslm_schema schema);
+
+/* ---- outside the integer forward path: exported, always SSLM_INVALID_ARGUMENT ---- */
+sslm_status sslm_tokenize(sslm_model model, const char* utf8, int32_t* tokens, int32_t* n);
 sslm_status sslm_detokenize_stream(sslm_model model, sslm_detok_state* state, const int32_t* tokens, int32_t n,
                                    char* utf8, int32_t* out_n);
 

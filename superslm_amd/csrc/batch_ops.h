@@ -27,7 +27,11 @@ struct SharedAttnArgs {
 	const int64_t* prefix_len;
 	int8_t* codes;    // [rows, NH D]
 	Scale* scales;    // [rows]
-	int32_t* status;  // [rows]
+	int32_t* status;  // [rows]; with `tok` the slots' status words instead
+	// a model's decode step: a row whose slot holds a refusal is left alone, its own refusal is reported as
+	// `layer`'s (set_status).  Null: status[r] of every row is written.
+	const TokenInfo* tok;
+	int32_t layer;
 	void* ws;         // shared_attn_workspace() bytes
 };
 size_t shared_attn_workspace(int rows, int NH, int NKV, int D, int prefixes, int64_t max_prefix, int64_t max_own);

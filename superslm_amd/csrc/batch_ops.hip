@@ -619,6 +619,13 @@ __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 2 : 1) void k_sa_pv(sslm_
 	for (int d = 0; d < DT; ++d) *(v4i*)(out + 16 * d) = acc[d][0] - 256 * acc[d][1];
 }
 
+// The status of row r, from one thread.  In a model's step (a.tok) a slot's first refusal stays.
+__device__ __forceinline__ void sa_status(const sslm_launch::SharedAttnArgs& a, int r, int32_t st) {
+	if (!a.tok) a.status[r] = st;
+	else set_status(a.status, a.tok[r].slot, a.layer, st);
+}
+__device__ __forceinline__ bool sa_refused(const sslm_launch::SharedAttnArgs& a, int r) { return a.tok && a.status[a.tok[r].slot] != 0; }
+
 // The fold of this thread's units of four dims, read ahead: unit u's head is the same for all four.
 template <int BS, int U>
 __device__ __forceinline__ void sa_folds(const sslm_launch::SharedAttnArgs& a, FoldConsts (&fc)[U]) {
@@ -633,7 +640,7 @@ __device__ __forceinline__ void sa_folds(const sslm_launch::SharedAttnArgs& a, F
 // thread, unless `first`, the smallest (head << 8) | status of a refusing head, is there.
 template <int BS, int U>
 __device__ __forceinline__ void sa_finish(const sslm_launch::SharedAttnArgs& a, int r, v4i (&v)[U], const FoldConsts (&fc)[U],
-                                          uint32_t first, uint32_t* s_red) {
+                                          uint32_t first, bool refused, uint32_t* s_red) {
 	const int N = a.NH * a.D;
 	uint32_t mx = 0;
 #pragma unroll
@@ -656,14 +663,15 @@ __device__ __forceinline__ void sa_finish(const sslm_launch::SharedAttnArgs& a, 
 		mx = max(mx, s_red[i]);
 		first = min(first, s_red[BS / 64 + i]);
 	}
+	if (refused) return;
 	if (first != 0xffffffffu) {
-		if (threadIdx.x == 0) a.status[r] = (int32_t)(first & 0xff);
+		if (threadIdx.x == 0) sa_status(a, r, (int32_t)(first & 0xff));
 		return;
 	}
 	FunnelPlan plan;
 	const int32_t st = funnel_plan(__builtin_amdgcn_readfirstlane(mx), nullptr, 0, a.site, &plan);
 	if (threadIdx.x == 0) {
-		a.status[r] = st;
+		sa_status(a, r, st);
 		if (st == kOk) a.scales[r] = plan.out;
 	}
 	if (st != kOk) return;
@@ -685,6 +693,8 @@ __global__ __launch_bounds__(BS) void k_sa_out(sslm_launch::SharedAttnArgs a, Sa
 	__shared__ uint32_t s_red[2 * BS / 64];
 	const int r = blockIdx.x, N = a.NH * a.D, G = a.NH / a.NKV;
 	const RowSpan sp = w.span[r];
+	// read before this row's own status is written: by one thread, after the block's reduction
+	const bool refused = sa_refused(a, r);
 	// the first refusing head, heads of one KV head sharing its constants' status
 	uint32_t first = 0xffffffffu;
 	for (int h = threadIdx.x; h < a.NH; h += BS) {
@@ -718,7 +728,7 @@ __global__ __launch_bounds__(BS) void k_sa_out(sslm_launch::SharedAttnArgs a, Sa
 #pragma unroll
 			for (int u = 0; u < U; ++u) v[u] += k + e < n ? x[e][u] : v4i{0, 0, 0, 0};
 	}
-	sa_finish<BS>(a, r, v, fc, first, s_red);
+	sa_finish<BS>(a, r, v, fc, first, refused, s_red);
 }
 
 // The whole of a short row in one launch: a block per row, its eight waves cut over the KV heads and
@@ -742,9 +752,10 @@ __global__ __launch_bounds__(64 * kSaRowWaves, 2) void k_sa_row(sslm_launch::Sha
 	const int G = a.NH / a.NKV;
 	int8_t* lds = s_kv[wave];
 	const RowScales rs = row_scales(a, r, kvh);
+	const bool refused = sa_refused(a, r);  // before this row's own status is written
 	const RowSpan sp = row_span(a, r);
 	if (sp.st != kOk) {
-		if (threadIdx.x == 0) a.status[r] = sp.st;
+		if (threadIdx.x == 0) sa_status(a, r, sp.st);
 		return;
 	}
 	const int64_t head = (int64_t)kvh * a.cap * D, last = sp.width - 1;
@@ -891,7 +902,7 @@ __global__ __launch_bounds__(64 * kSaRowWaves, 2) void k_sa_row(sslm_launch::Sha
 		const int i = min((int)threadIdx.x + u * BS, a.NH * D / 4 - 1), h = 4 * i / D;
 		v[u] = *(const v4i*)(s_ctx + h * D + ((4 * i % D) ^ (h % G * 4 & (D - 1))));
 	}
-	sa_finish<BS>(a, r, v, fc, s_first, s_red);
+	sa_finish<BS>(a, r, v, fc, s_first, refused, s_red);
 }
 
 // ------------------------------------------------------------------------------------------

@@ -40,6 +40,12 @@ constexpr int kSlotCapacity = 1024;  // live sequences per model
 // (8 prompts 23.2 against 23.5 and 23.6 against 24.9 ms).
 constexpr int kSlicedActPrefillRows = 32;
 
+// The attention of one block per (row, KV head) passes over its row alone: its time is the longest row's
+// positions times the rounds that its blocks take over the CUs.  From this many on, a unit with adopted
+// prefixes reads them shared and cut over the whole chip (a step of the 7B shape's layer, shared against
+// not: 32 rows of 2080 positions 199 / 191 us, 16 of 4128 189 / 197 us, 64 of 4196 249 / 471 us).
+constexpr int64_t kSharedPositions = 3500;
+
 struct HipError {
 	hipError_t e;
 };
@@ -206,6 +212,15 @@ struct Track {
 	int8_t* lora_u[3];
 	const LoraRef** row_refs = nullptr;  // decode: per row its adapter's refs, or null [T]
 	LoraRef* lora_rows = nullptr;        // decode: (layer, projection, row) of them [L * 7][T]
+	// decode: a unit whose attention reads shared prompts (SharedAttnArgs); rows 0: it does not
+	struct Shared {
+		int rows = 0, prefixes = 0;
+		int64_t max_prefix = 0, max_own = 0;
+		int32_t *row_block = nullptr, *prefix_rows = nullptr, *prefix_block = nullptr;  // [T], [T + 1], [T]
+		int64_t *row_width = nullptr, *prefix_len = nullptr;                            // [T], [T]
+		void* ws = nullptr;
+		size_t ws_bytes = 0;
+	} shared;
 	TokenInfo* lg_tok;    // head tracks: tokens of the joined final norm + head
 	int32_t* lg_slot;
 	const uint8_t** lg_mask;  // head tracks: per token its schema mask page in HBM, or null
@@ -358,6 +373,7 @@ struct sslm_model_s {
 	std::map<std::string, hipGraphExec_t> graphs;  // captured submissions by shape
 	std::map<std::string, int> graph_seen;         // prefill shapes seen (captured on a repeat)
 	int8_t* pool_dev = nullptr;  // KV pool of the launch sequence being recorded
+	int pool_blocks = 0;
 	std::atomic<int> live_refs{0};
 	std::mutex mu;  // serializes GPU submission on this model
 };
@@ -402,7 +418,18 @@ struct sslm_seq_s {
 	uint32_t walk = 0xFFFFFFFFu;        // DFA walk state (0xFFFFFFFF: no schema bound)
 	std::vector<int32_t> context;       // the tokens taken in and produced, what token rules count
 	std::unique_ptr<SeqRules> rules;
+	sslm_prefix prefix = nullptr;       // the adopted prompt: positions below prefix->seq's context are its
 	std::mutex mu;
+};
+
+// A shared prompt: a sequence of its own, whose block holds the prompt's K/V.  Sequences that adopt it
+// copy its state and K/V rows (so each one's block, blob and every verb are as if it had taken the prompt
+// itself) and a decode step reads the shared positions from this block, once for all of them.
+struct sslm_prefix_s {
+	sslm_model model = nullptr;
+	sslm_seq seq = nullptr;
+	bool frozen = false, released = false;
+	int adopters = 0;  // under model->mu
 };
 
 struct sslm_workspace_s {
@@ -836,6 +863,48 @@ sslm_launch::AttnArgs attn_args(sslm_model m, Track& w, int l, int M) {
 	return a;
 }
 
+// The attention of a unit that reads shared prompts.
+sslm_launch::SharedAttnArgs shared_attn_args(sslm_model m, Track& w, int l) {
+	const DevLayer& lw = m->layers[l];
+	const Track::Shared& sh = w.shared;
+	const int64_t half = m->cap * m->KVH;
+	sslm_launch::SharedAttnArgs a{};
+	a.rows = sh.rows;
+	a.NH = m->NH;
+	a.NKV = m->NKV;
+	a.D = m->D;
+	a.prefixes = sh.prefixes;
+	a.blocks = m->pool_blocks;
+	a.max_prefix = sh.max_prefix;
+	a.max_own = sh.max_own;
+	a.pool = m->pool_dev;
+	a.block_bytes = (int64_t)m->block_bytes;
+	a.k_off = l * 2 * half;
+	a.v_off = a.k_off + half;
+	a.cap = m->cap;
+	a.q = w.q_rot;
+	a.q_scale = w.q_scale;
+	a.khead_m = lw.khead_m;
+	a.khead_e = lw.khead_e;
+	a.ln2_q = m->ln2_q;
+	a.b_q = m->b_q;
+	a.ca_q = m->ca_q;
+	a.ctx_fold = lw.ctx_fold;
+	a.site = lw.ctx;
+	a.row_block = sh.row_block;
+	a.row_width = sh.row_width;
+	a.prefix_rows = sh.prefix_rows;
+	a.prefix_block = sh.prefix_block;
+	a.prefix_len = sh.prefix_len;
+	a.codes = w.ctx;
+	a.scales = w.ctx_scale;
+	a.status = m->status;
+	a.tok = w.tok;
+	a.layer = l;
+	a.ws = sh.ws;
+	return a;
+}
+
 bool fused_attention_enabled() {
 	static const bool on = [] {
 		const char* e = getenv("SSLM_HIP_FUSED_ATTN");
@@ -887,7 +956,8 @@ void run_layers(sslm_model m, Track& w, int M, StreamRef st, int l0, int l1, con
 		sslm_launch::rmsnorm(a, M, H, w.tok, m->status, l0, s);
 		ck(hipGetLastError());
 	}
-	const bool fused = decode && fused_attention_enabled() &&
+	const bool shared = decode && w.shared.rows > 0;
+	const bool fused = decode && !shared && fused_attention_enabled() &&
 	                   sslm_launch::decode_fused_ok(M, H, m->NKV, KVH, m->cap, m->layers[l0].p_qkv != nullptr);
 	const bool staged_attn = !decode && w.kv_stage && sslm_launch::tiled_attention_staged(M, m->NKV, m->NH);
 	const bool dbg = dbg_on(m, M);
@@ -970,6 +1040,13 @@ void run_layers(sslm_model m, Track& w, int M, StreamRef st, int l0, int l1, con
 				}
 			}
 			if (dbg) dbg_gather(m, w, l, kDbgQRot, w.q_rot, w.q_scale, nullptr, H, M);
+		}
+		if (shared) {  // with the context funnel
+			ProfScope p(s, kProfAttn, 0, 0);
+			sslm_launch::shared_attn(shared_attn_args(m, w, l), s);
+			ck(hipGetLastError());
+			if (dbg) dbg_gather(m, w, l, kDbgCtx, w.ctx, w.ctx_scale, nullptr, H, M);
+		} else if (!fused) {
 			sslm_launch::AttnArgs aa = attn_args(m, w, l, M);
 			aa.q_rot = w.q_rot;
 			aa.q_scale = w.q_scale;
@@ -982,7 +1059,7 @@ void run_layers(sslm_model m, Track& w, int M, StreamRef st, int l0, int l1, con
 			sslm_launch::attention(aa, s, !decode);  // prefill chunks: one sequence, consecutive positions
 			ck(hipGetLastError());
 		}
-		{
+		if (!shared) {
 			sslm_launch::FunnelArgs a{};
 			a.M = M;
 			a.N = H;
@@ -1408,6 +1485,13 @@ void alloc_track(sslm_model m, Track& w, int T, bool head) {
 		w.raw_part = elems ? dalloc<int32_t>(elems, &own) : nullptr;
 	}
 	for (int i = 0; i < 3; ++i) w.lora_u[i] = dalloc<int8_t>((size_t)T * kMaxRank, &own);
+	if (!w.prefill) {
+		w.shared.row_block = dalloc<int32_t>(T, &own);
+		w.shared.prefix_rows = dalloc<int32_t>(T + 1, &own);
+		w.shared.prefix_block = dalloc<int32_t>(T, &own);
+		w.shared.row_width = dalloc<int64_t>(T, &own);
+		w.shared.prefix_len = dalloc<int64_t>(T, &own);
+	}
 	w.row_refs = w.prefill ? nullptr : (const LoraRef**)dalloc<uintptr_t>(T, &own);
 	w.lora_rows = w.prefill ? nullptr : dalloc<LoraRef>((size_t)T * m->L * 7, &own);
 	w.act_prod = dalloc<int32_t>((size_t)sslm_launch::kMaxSlicedActRows * I, &own);
@@ -2074,6 +2158,18 @@ sslm_status sslm_seq_create(sslm_model model, sslm_kv_pool* pool, sslm_seq* out)
 	});
 }
 
+// The sequence lets go of its prefix (model->mu held): the prefix to destroy once the lock is free, or null.
+static sslm_prefix unref_prefix(sslm_seq seq) {
+	const sslm_prefix p = seq->prefix;
+	seq->prefix = nullptr;
+	return p && --p->adopters == 0 && p->released ? p : nullptr;
+}
+static sslm_status destroy_prefix(sslm_prefix p) {
+	const sslm_status st = sslm_seq_release(p->seq);
+	delete p;
+	return st;
+}
+
 sslm_status sslm_seq_release(sslm_seq seq) {
 	if (!seq) return SSLM_INVALID_ARGUMENT;
 	{
@@ -2081,8 +2177,10 @@ sslm_status sslm_seq_release(sslm_seq seq) {
 		if (!g_live_seqs.erase(seq)) return SSLM_INVALID_ARGUMENT;
 	}
 	sslm_model m = seq->model;
+	sslm_prefix last = nullptr;
 	{
 		std::lock_guard<std::mutex> lk(m->mu);
+		last = unref_prefix(seq);
 		if (seq->adapter) seq->adapter->live_refs--;
 		{
 			std::lock_guard<std::mutex> pl(seq->pool->mu);
@@ -2093,6 +2191,7 @@ sslm_status sslm_seq_release(sslm_seq seq) {
 		m->live_refs--;
 	}
 	delete seq;
+	if (last) (void)destroy_prefix(last);
 	return SSLM_OK;
 }
 
@@ -2100,7 +2199,8 @@ sslm_status sslm_seq_reset(sslm_seq seq) {
 	if (!seq) return SSLM_INVALID_ARGUMENT;
 	if (seq->layer_index != 0) return SSLM_SEQ_RESET_MIDTOKEN_REJECTED;  // src/sslm_abi.cpp:1820-1846
 	sslm_model m = seq->model;
-	return guarded([&]() -> sslm_status {
+	sslm_prefix last = nullptr;
+	const sslm_status st = guarded([&]() -> sslm_status {
 		std::lock_guard<std::mutex> lk(m->mu);
 		ck(hipMemsetAsync(seq->pool->dev + (size_t)seq->block * seq->pool->block_size, 0, seq->pool->block_size,
 		                  m->tracks[0].stream));
@@ -2117,8 +2217,11 @@ sslm_status sslm_seq_reset(sslm_seq seq) {
 		seq->walk = seq->schema ? 0u : kWalkUnused;
 		seq->context.clear();
 		if (seq->rules) seq->rules->uploaded = 0;
+		last = unref_prefix(seq);
 		return SSLM_OK;
 	});
+	if (last) (void)destroy_prefix(last);
+	return st;
 }
 
 sslm_status sslm_prefill(sslm_model model, sslm_seq seq, const int32_t* tokens, int32_t count, int32_t chunk_budget,
@@ -2228,6 +2331,35 @@ int track_min() {
 	return v;
 }
 
+// Whether a decode unit's attention reads its shared prompts once for all of their sequences, and if so
+// the unit's order (the prefixes' sequences first, run by run) and the launch's sizes: own positions in
+// steps of 256, so that a graph is re-recorded once per 256 tokens.  Otherwise *prefixes stays empty.
+// SSLM_HIP_SHARED_ATTN=1 (0) takes it wherever a prefix is adopted (never); read per call.
+static void share_prompts(sslm_model m, sslm_seq* seqs, std::vector<int>* idx, std::vector<sslm_prefix>* prefixes,
+                          std::vector<int32_t>* rows, int64_t* max_prefix, int64_t* max_own) {
+	std::vector<sslm_prefix> ps;
+	for (int i : *idx)
+		if (seqs[i]->prefix && std::find(ps.begin(), ps.end(), seqs[i]->prefix) == ps.end()) ps.push_back(seqs[i]->prefix);
+	if (ps.empty() || !sslm_launch::shared_attn_ok((int)idx->size(), m->NH, m->NKV, m->D)) return;
+	auto where = [&](int i) { return std::find(ps.begin(), ps.end(), seqs[i]->prefix) - ps.begin(); };
+	const char* e = getenv("SSLM_HIP_SHARED_ATTN");
+	int64_t longest = 0, own = 0, width = 0;
+	for (sslm_prefix p : ps) longest = std::max(longest, p->seq->context_length);
+	for (int i : *idx) {
+		width = std::max(width, seqs[i]->context_length + 1);
+		own = std::max(own, seqs[i]->context_length + 1 - (seqs[i]->prefix ? seqs[i]->prefix->seq->context_length : 0));
+	}
+	const int64_t cus = sslm_launch::device_cus(), rounds = ((int64_t)idx->size() * m->NKV + cus - 1) / cus;
+	if (e && (e[0] == '0' || e[0] == '1') ? e[0] == '0' : width * rounds < kSharedPositions) return;
+	std::stable_sort(idx->begin(), idx->end(), [&](int x, int y) { return where(x) < where(y); });
+	rows->push_back(0);
+	for (size_t k = 0; k < ps.size(); ++k)
+		rows->push_back(rows->back() + (int32_t)std::count_if(idx->begin(), idx->end(), [&](int i) { return seqs[i]->prefix == ps[k]; }));
+	*prefixes = std::move(ps);
+	*max_prefix = longest;
+	*max_own = std::min(m->cap, (own + 255) / 256 * 256);
+}
+
 static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const sslm_decode_params& params,
                                 int32_t* out_tokens, sslm_status* stop) {
 	const uint32_t budget = (uint32_t)params.layer_budget;
@@ -2268,6 +2400,10 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 		uint32_t l0, l1;
 		UnitAdapters ad;
 		std::vector<int> idx;
+		// attention over shared prompts, when it pays: idx then begins with the prefixes' sequences, run by run
+		std::vector<sslm_prefix> prefixes;
+		std::vector<int32_t> prefix_rows;  // [prefixes + 1]
+		int64_t max_prefix = 0, max_own = 0;
 	};
 	std::vector<Unit> units;
 	std::vector<int> finished;
@@ -2290,6 +2426,7 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 				for (sslm_adapter ad : ads)
 					for (size_t k = 0; ad && k < ad->proj.size(); ++k) un.ad.any[k] |= ad->proj[k].a != nullptr;
 			}
+			share_prompts(m, seqs, &un.idx, &un.prefixes, &un.prefix_rows, &un.max_prefix, &un.max_own);
 			units.push_back(std::move(un));
 		}
 		if (l1 == (uint32_t)m->L)
@@ -2327,6 +2464,7 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 	std::deque<std::vector<TokenInfo>> h_tok;  // deque: references to earlier entries stay valid
 	std::deque<std::vector<int32_t>> h_i32;
 	std::deque<std::vector<const uint8_t*>> h_ptr;
+	std::deque<std::vector<int64_t>> h_i64;
 	std::deque<std::vector<const LoraRef*>> h_ref;
 	std::deque<std::vector<sslm_launch::LogitRule>> h_rule;
 	std::deque<std::vector<int32_t*>> h_at;
@@ -2336,11 +2474,46 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 		for (int i : un.idx) mw = std::max<int64_t>(mw, (int64_t)seqs[i]->context_length + 1);
 		return sslm_launch::group_width_cap(mw, m->cap);
 	};
+	auto set_shared = [](Track& w, const Unit& un) {
+		w.shared.rows = un.prefixes.empty() ? 0 : (int)un.idx.size();
+		w.shared.prefixes = (int)un.prefixes.size();
+		w.shared.max_prefix = un.max_prefix;
+		w.shared.max_own = un.max_own;
+	};
 	auto stage_unit = [&](size_t u, hipStream_t s) {
 		const Unit& un = units[u];
 		Track& w = m->tracks[u % ntr];
 		const int M = (int)un.idx.size();
 		w.attn_wcap = unit_wcap(un);
+		set_shared(w, un);
+		if (w.shared.rows) {
+			const size_t need = sslm_launch::shared_attn_workspace(M, m->NH, m->NKV, m->D, w.shared.prefixes, un.max_prefix, un.max_own);
+			if (need > w.shared.ws_bytes) {  // the old one stays: graphs recorded with it are sized for it
+				w.shared.ws = dalloc<uint8_t>(need, &w.own);
+				w.shared.ws_bytes = need;
+			}
+			h_i32.emplace_back(M);
+			std::vector<int32_t>& blocks = h_i32.back();
+			h_i64.emplace_back(M);
+			std::vector<int64_t>& widths = h_i64.back();
+			for (int t = 0; t < M; ++t) {
+				blocks[t] = (int32_t)seqs[un.idx[t]]->block;
+				widths[t] = seqs[un.idx[t]]->context_length + 1;
+			}
+			h_i32.emplace_back();
+			std::vector<int32_t>& pb = h_i32.back();
+			h_i64.emplace_back();
+			std::vector<int64_t>& pl = h_i64.back();
+			for (sslm_prefix p : un.prefixes) {
+				pb.push_back((int32_t)p->seq->block);
+				pl.push_back(p->seq->context_length);
+			}
+			ck(hipMemcpyAsync(w.shared.row_block, blocks.data(), M * 4, hipMemcpyHostToDevice, s));
+			ck(hipMemcpyAsync(w.shared.row_width, widths.data(), M * 8, hipMemcpyHostToDevice, s));
+			ck(hipMemcpyAsync(w.shared.prefix_rows, un.prefix_rows.data(), un.prefix_rows.size() * 4, hipMemcpyHostToDevice, s));
+			ck(hipMemcpyAsync(w.shared.prefix_block, pb.data(), pb.size() * 4, hipMemcpyHostToDevice, s));
+			ck(hipMemcpyAsync(w.shared.prefix_len, pl.data(), pl.size() * 8, hipMemcpyHostToDevice, s));
+		}
 		h_tok.emplace_back(M);
 		std::vector<TokenInfo>& ti = h_tok.back();
 		h_i32.emplace_back(M);
@@ -2383,6 +2556,7 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 		Track& w = m->tracks[u % ntr];
 		const int M = (int)un.idx.size();
 		w.attn_wcap = unit_wcap(un);
+		set_shared(w, un);
 		// snapshot of the rows this unit changes, restored if an earlier sequence of the call refuses
 		sslm_launch::slot_state_copy(slot_copy_args(m, w.tok, (int)un.l0, (int)un.l1), M, false, w.stream);
 		ck(hipGetLastError());
@@ -2474,6 +2648,7 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 	std::vector<int2> cand(cands ? lg.size() * (size_t)params.top_k : 0);
 	// every sequence of one call shares the pool of the first (checked by the caller)
 	m->pool_dev = seqs[0]->pool->dev;
+	m->pool_blocks = (int)seqs[0]->pool->block_count;
 	std::vector<int32_t> toks(lg.size());
 	try {
 		if (one_per_track) {
@@ -2496,7 +2671,9 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 					                             ? "|g" + std::to_string(unit_wcap(un)) + "h" +
 					                                   std::to_string(sslm_launch::group_row_halves(
 					                                       (int)un.idx.size(), m->NKV, m->NH / m->NKV))
-					                             : "");
+					                             : "") +
+					                        (un.prefixes.empty() ? "" : "|s" + std::to_string(un.prefixes.size()) + "," +
+					                                                        std::to_string(un.max_prefix) + "," + std::to_string(un.max_own));
 					capturing = true;
 					const hipGraphExec_t ge = graph_of(m, key, w.stream, [&] { launch_unit(u); });
 					capturing = false;
@@ -3014,19 +3191,76 @@ sslm_status sslm_hip_seq_set_rules(sslm_seq seq, const sslm_hip_rules* rules) {
 	});
 }
 
-// ---- outside the integer forward path ----
-sslm_status sslm_prefix_begin(sslm_model, sslm_kv_pool*, sslm_prefix* out) {
-	if (out) *out = nullptr;
-	return SSLM_INVALID_ARGUMENT;
+// ---- shared prompts ----
+sslm_status sslm_prefix_begin(sslm_model model, sslm_kv_pool* pool, sslm_prefix* out) {
+	if (!out) return SSLM_INVALID_ARGUMENT;
+	*out = nullptr;
+	std::unique_ptr<sslm_prefix_s> p(new (std::nothrow) sslm_prefix_s());
+	if (!p) return SSLM_ALLOCATION_FAILED;
+	const sslm_status st = sslm_seq_create(model, pool, &p->seq);
+	if (st != SSLM_OK) return st;
+	p->model = model;
+	*out = p.release();
+	return SSLM_OK;
 }
-sslm_status sslm_prefix_prefill(sslm_model, sslm_prefix, const int32_t*, int32_t, int32_t, sslm_span_kind,
-                                sslm_workspace, int32_t* consumed) {
+sslm_status sslm_prefix_prefill(sslm_model model, sslm_prefix prefix, const int32_t* tokens, int32_t count,
+                                int32_t chunk_budget, sslm_span_kind kind, sslm_workspace ws, int32_t* consumed) {
 	if (consumed) *consumed = 0;
-	return SSLM_INVALID_ARGUMENT;
+	if (!prefix || prefix->released) return SSLM_INVALID_ARGUMENT;
+	if (prefix->frozen) return SSLM_PREFIX_FROZEN_REJECTED;
+	return sslm_prefill(model, prefix->seq, tokens, count, chunk_budget, kind, ws, consumed);
 }
-sslm_status sslm_prefix_freeze(sslm_prefix) { return SSLM_INVALID_ARGUMENT; }
-sslm_status sslm_prefix_release(sslm_prefix) { return SSLM_INVALID_ARGUMENT; }
-sslm_status sslm_seq_adopt_prefix(sslm_seq, sslm_prefix) { return SSLM_INVALID_ARGUMENT; }
+sslm_status sslm_prefix_freeze(sslm_prefix prefix) {
+	if (!prefix || prefix->released) return SSLM_INVALID_ARGUMENT;
+	std::lock_guard<std::mutex> lk(prefix->model->mu);
+	prefix->frozen = true;
+	return SSLM_OK;
+}
+sslm_status sslm_prefix_release(sslm_prefix prefix) {
+	if (!prefix) return SSLM_INVALID_ARGUMENT;
+	{
+		std::lock_guard<std::mutex> lk(prefix->model->mu);
+		if (prefix->released) return SSLM_INVALID_ARGUMENT;
+		prefix->released = true;
+		if (prefix->adopters > 0) return SSLM_OK;  // the last adopter takes it down
+	}
+	return destroy_prefix(prefix);
+}
+// A fresh sequence of the prefix's pool takes over its state: context, stream row, clamp counter, schema
+// walk, and the K/V rows [0, context) of every layer and head.
+sslm_status sslm_seq_adopt_prefix(sslm_seq seq, sslm_prefix prefix) {
+	if (!seq || !prefix) return SSLM_INVALID_ARGUMENT;
+	sslm_model m = seq->model;
+	if (prefix->model != m) return SSLM_INVALID_ARGUMENT;
+	return guarded([&]() -> sslm_status {
+		std::lock_guard<std::mutex> lk(m->mu);
+		const sslm_seq from = prefix->seq;
+		if (!prefix->frozen || prefix->released || from->pool != seq->pool || seq->prefix || seq->context_length != 0 ||
+		    seq->layer_index != 0 || seq->current_token != -1 || seq->ready_for_logits)
+			return SSLM_INVALID_ARGUMENT;
+		if (seq->schema != from->schema) return SSLM_PREFIX_SCHEMA_MISMATCH;
+		if (from->context_length == 0) return SSLM_OK;
+		hipStream_t s = m->tracks[0].stream;
+		const size_t pitch = (size_t)m->cap * m->D, size = seq->pool->block_size;
+		int8_t* pool = seq->pool->dev;
+		ck(hipMemcpy2DAsync(pool + seq->block * size, pitch, pool + from->block * size, pitch, (size_t)from->context_length * m->D,
+		                    (size_t)m->L * 2 * m->NKV, hipMemcpyDeviceToDevice, s));
+		ck(hipMemcpyAsync(m->stream_codes + (size_t)seq->slot * m->H, m->stream_codes + (size_t)from->slot * m->H, m->H,
+		                  hipMemcpyDeviceToDevice, s));
+		ck(hipMemcpyAsync(m->stream_scale + seq->slot, m->stream_scale + from->slot, sizeof(Scale), hipMemcpyDeviceToDevice, s));
+		ck(hipMemcpyAsync(m->sat + seq->slot, m->sat + from->slot, 8, hipMemcpyDeviceToDevice, s));
+		ck(hipStreamSynchronize(s));
+		seq->context = from->context;
+		seq->context_length = from->context_length;
+		seq->current_token = from->current_token;
+		seq->ready_for_logits = from->ready_for_logits;
+		seq->forced_token_count = from->forced_token_count;
+		seq->walk = from->walk;
+		seq->prefix = prefix;
+		++prefix->adopters;
+		return SSLM_OK;
+	});
+}
 // src/sslm_abi.cpp:2722-2987: checks in the reference's order (magic SSB3 or SSB2, sizes, model
 // hash, kv precision, schema binding -- none can resolve here, as no schema is ever bound --
 // field domains, exact size, KV block count, pool identity), then a block is drawn, the KV
@@ -3171,7 +3405,10 @@ sslm_status sslm_seq_set_schema(sslm_seq seq, sslm_schema schema) {
 	seq->walk = schema ? 0u : kWalkUnused;
 	return SSLM_OK;
 }
-sslm_status sslm_prefix_set_schema(sslm_prefix, sslm_schema) { return SSLM_INVALID_ARGUMENT; }
+sslm_status sslm_prefix_set_schema(sslm_prefix prefix, sslm_schema schema) {
+	if (!prefix || prefix->released) return SSLM_INVALID_ARGUMENT;
+	return prefix->frozen ? SSLM_PREFIX_FROZEN_REJECTED : sslm_seq_set_schema(prefix->seq, schema);
+}
 sslm_status sslm_detokenize_stream(sslm_model, sslm_detok_state*, const int32_t*, int32_t, char*, int32_t* out_n) {
 	if (out_n) *out_n = 0;
 	return SSLM_INVALID_ARGUMENT;

@@ -108,6 +108,12 @@ class SslmLib:
         sig("sslm_seq_set_adapter", ctypes.c_int, vp, vp)
         sig("sslm_adapter_map", ctypes.c_int, vp, sz, vp, pvp)
         sig("sslm_adapter_release", ctypes.c_int, vp)
+        sig("sslm_prefix_begin", ctypes.c_int, vp, pvp, pvp)
+        sig("sslm_prefix_prefill", ctypes.c_int, vp, vp, pi32, i32, i32, ctypes.c_int, vp, pi32)
+        sig("sslm_prefix_freeze", ctypes.c_int, vp)
+        sig("sslm_prefix_release", ctypes.c_int, vp)
+        sig("sslm_prefix_set_schema", ctypes.c_int, vp, vp)
+        sig("sslm_seq_adopt_prefix", ctypes.c_int, vp, vp)
         sig("sslm_seq_save", ctypes.c_int, vp, vp, ctypes.POINTER(sz))
         sig("sslm_seq_restore", ctypes.c_int, vp, pvp, vp, sz, pvp)
         sig("sslm_schema_lookup", ctypes.c_int, vp, ctypes.c_char_p, pvp)
@@ -246,6 +252,9 @@ class KvPool:
     def seq(self) -> "Seq":
         return Seq(self)
 
+    def prefix(self) -> "Prefix":
+        return Prefix(self)
+
     def restore(self, blob: bytes, raw: bool = False):
         """sslm_seq_restore of a saved sequence blob into this pool: a Seq, or with `raw` the
         status and the Seq (None unless the status is SSLM_OK)."""
@@ -265,6 +274,44 @@ class KvPool:
             self.handle = None
 
 
+class Prefix:
+    """A shared prompt: prefilled, frozen, then adopted by any number of fresh sequences of its pool."""
+
+    def __init__(self, pool: KvPool):
+        m = pool.model
+        self.pool = pool
+        h = ctypes.c_void_p()
+        m.lib.check("sslm_prefix_begin", m.lib.lib.sslm_prefix_begin(m.handle, ctypes.byref(pool.handle), ctypes.byref(h)))
+        self.handle = h
+
+    def prefill(self, tokens, chunk_budget: int | None = None, raw: bool = False, kind: int = SPAN_PROMPT):
+        m = self.pool.model
+        arr = np.ascontiguousarray(np.asarray(tokens, dtype=np.int32))
+        consumed = ctypes.c_int32(0)
+        budget = chunk_budget if chunk_budget is not None else max(1, len(arr))
+        st = m.lib.lib.sslm_prefix_prefill(m.handle, self.handle, arr.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)),
+                                           len(arr), budget, kind, None, ctypes.byref(consumed))
+        if raw:
+            return st, consumed.value
+        m.lib.check("sslm_prefix_prefill", st)
+        return consumed.value
+
+    def freeze(self):
+        lib = self.pool.model.lib
+        lib.check("sslm_prefix_freeze", lib.lib.sslm_prefix_freeze(self.handle))
+
+    def set_schema(self, schema) -> int:
+        """sslm_prefix_set_schema; returns the status."""
+        return self.pool.model.lib.lib.sslm_prefix_set_schema(self.handle, schema)
+
+    def release(self):
+        """Its block lives on until the last sequence that adopted it is released or reset."""
+        if self.handle:
+            lib = self.pool.model.lib
+            lib.check("sslm_prefix_release", lib.lib.sslm_prefix_release(self.handle))
+            self.handle = None
+
+
 class Seq:
     def __init__(self, pool: KvPool, handle=None):
         lib = pool.model.lib
@@ -276,6 +323,14 @@ class Seq:
         lib.check("sslm_seq_create", lib.lib.sslm_seq_create(pool.model.handle, ctypes.byref(pool.handle),
                                                               ctypes.byref(h)))
         self.handle = h
+
+    def adopt(self, prefix: "Prefix", raw: bool = False):
+        """sslm_seq_adopt_prefix: this fresh sequence continues a frozen prefix."""
+        lib = self.pool.model.lib
+        st = lib.lib.sslm_seq_adopt_prefix(self.handle, prefix.handle)
+        if raw:
+            return st
+        lib.check("sslm_seq_adopt_prefix", st)
 
     def set_schema(self, schema) -> int:
         """sslm_seq_set_schema (None unbinds); returns the status."""

@@ -31,3 +31,18 @@ class AdapterView:
         self.b = {k[:-7]: v for k, v in w.items() if k.endswith(".lora_B")}
         self.d_fold = _manifest(blob, sections[SEC_DELTA_FOLD], np.int32)
         self.u_fold = _manifest(blob, sections[SEC_U_FOLD], np.int32)
+
+
+def with_delta_exponent(blob, exponent):
+    """The adapter with every delta fold row (identity 0, mult 2^30, `exponent`), its hash recomputed."""
+    from superslm_amd.sslm_artifact import with_flags
+    out = bytearray(blob)
+    for i in range(struct.unpack_from("<I", out, 12)[0]):
+        typ, _, off = struct.unpack_from("<IIQ", out, HEADER_BYTES + i * SECTION_DESC_BYTES)
+        if typ != SEC_DELTA_FOLD:
+            continue
+        for k in range(struct.unpack_from("<I", out, off + 8)[0]):
+            _, _, nd, *rest = struct.unpack_from("<III4IQQI", out, off + 16 + 48 * k)
+            rows = np.frombuffer(out, np.int32, int(np.prod(rest[:nd])), off + rest[4]).reshape(-1, 3)
+            rows[:] = (0, 1 << 30, exponent)
+    return with_flags(bytes(out), struct.unpack_from("<I", out, 16)[0])
