@@ -149,7 +149,7 @@ __device__ __forceinline__ RowConst row_const(const sslm_launch::SharedAttnArgs&
 // which cost 8 MFMAs a step of 64 positions at D = 128 where the i-exp of the step's scores costs some
 // hundreds of vector instructions, and integer sums join the planes exactly in any order.
 struct SaPlan {
-	int tiles;       // tiles of shared rows: at least those of every prefix together
+	int tb;          // blocks of kSaWaves tiles of shared rows: at least those of every prefix together
 	int shared, sb;  // shared planes and the positions of one (a multiple of 64)
 	int owned, ob;   // own planes and the positions of one
 	int ht;          // tiles of a row's own heads
@@ -187,25 +187,27 @@ struct SaJob {
 __device__ __forceinline__ int64_t i64min(int64_t a, int64_t b) { return a < b ? a : b; }
 __device__ __forceinline__ int64_t i64max(int64_t a, int64_t b) { return a > b ? a : b; }
 
-// A wave of the shared planes (block `blk` of them): false when there is nothing for it to do.
+// A wave of the shared planes: false, for its whole block, when there is nothing to do.  A block's waves have
+// neighbouring tiles of one prefix and the same positions; a wave past the last tile has no live lane.
 __device__ __forceinline__ bool sa_shared_job(const sslm_launch::SharedAttnArgs& a, const SaPlan& pl, SaJob* j) {
 	const int blk = blockIdx.x;
 	// blocks go to the XCDs in turn: a (KV head, plane)'s tiles stay on one, whose L2 then holds its K/V
-	const int tb = (pl.tiles + kSaWaves - 1) / kSaWaves, grp = (blk / 8 / tb) * 8 + blk % 8;
-	int tile = (blk / 8) % tb * kSaWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	if (grp >= a.NKV * pl.shared || tile >= pl.tiles) return false;
+	const int grp = (blk / 8 / pl.tb) * 8 + blk % 8;
+	int b = (blk / 8) % pl.tb;
+	if (grp >= a.NKV * pl.shared) return false;
 	j->plane = grp / a.NKV;
 	j->kvh = grp % a.NKV;
 	const int G = a.NH / a.NKV;
 	int p = 0, r0 = 0, r1 = 0;
-	for (;; ++p) {  // the tile's prefix
+	for (;; ++p) {  // the block's prefix
 		if (p >= a.prefixes) return false;
 		r0 = max(0, min(a.prefix_rows[p], a.rows));
 		r1 = max(r0, min(a.prefix_rows[p + 1], a.rows));
-		const int n = ((r1 - r0) * G + 15) / 16;
-		if (tile < n) break;
-		tile -= n;
+		const int n = ((r1 - r0) * G + 16 * kSaWaves - 1) / (16 * kSaWaves);
+		if (b < n) break;
+		b -= n;
 	}
+	const int tile = b * kSaWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int pb = a.prefix_block[p];
 	const int64_t len = a.prefix_len[p];
 	j->p0 = (int64_t)j->plane * pl.sb;
@@ -334,6 +336,35 @@ struct SaRows {
 	}
 };
 
+// The same from 64 rows that a whole block staged.
+template <int D, int NC>
+__device__ __forceinline__ void sa_block_scores(const int8_t* lds, const v4i (&q)[NC], v4i (&s)[4]) {
+	const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4;
+#pragma unroll
+	for (int t = 0; t < 4; ++t) {
+		s[t] = v4i{0, 0, 0, 0};
+#pragma unroll
+		for (int c = 0; c < NC; ++c) {
+			const int ch = c * 4 + g;
+			const v4i k = *(const v4i*)(lds + SaRows<D>::at(t * 16 + ri, D < 64 ? ch & (D / 16 - 1) : ch));
+			s[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, q[c], s[t], 0, 0, 0);
+		}
+	}
+}
+template <int D>
+__device__ __forceinline__ void sa_block_multiply(const int8_t* lds, const v4i& lo, const v4i& nhi, v4i (&acc)[D / 16][2]) {
+	const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4, i = ri >> 1, row = (i >> 2) * 16 + g * 4 + (i & 3);
+#pragma unroll
+	for (int dt = 0; dt < D / 16; ++dt) {
+		const int8_t* from = lds + SaRows<D>::at(row, dt) + 8 * (ri & 1);  // rows 32 apart change places alike
+		const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)from);
+		const v2i y = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(from + 32 * D));
+		const v4i b = v4i{x.x, x.y, y.x, y.y};
+		acc[dt][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, lo, acc[dt][0], 0, 0, 0);
+		acc[dt][1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, nhi, acc[dt][1], 0, 0, 0);
+	}
+}
+
 // The i-exp of one query row in doubles, each value exact: with y = q_b - x for a score x below the
 // maximum (x <= 30 q_ln2 by the clip), z = floor(x / q_ln2) = floor((x + 1/2) / q_ln2), whose argument is at
 // least 1 / (2 q_ln2) from an integer and estimated within (q_b + 30 q_ln2) 2^-51 / q_ln2 of its value;
@@ -396,34 +427,80 @@ __device__ __forceinline__ int64_t sa_row_sum(const sslm_launch::SharedAttnArgs&
 	return bad ? -1 : m;
 }
 
-// Steps of 64 positions over a plane's K: `step(p, scores)`, the rows of the next one (AHEAD = 2: two) steps in
-// flight meanwhile.
-template <int D, int AHEAD, int NC, typename F>
-__device__ __forceinline__ void sa_steps(const SaJob& j, int8_t* lds, const v4i (&q)[NC], F&& step) {
-	SaRows<D> k[AHEAD];
+// Steps of 64 positions over an own plane: `step(p, scores, multiply)`, where multiply(lo, nhi, acc) adds P V (WITH_V).
+// The next step's K rows are in flight meanwhile.  LDS: the wave's 32 D bytes.
+template <int D, bool WITH_V, int NC, typename F>
+__device__ __forceinline__ void sa_own_steps(const SaJob& j, int8_t* lds, const v4i (&q)[NC], F&& step) {
+	SaRows<D> k, v;
 	v4i s[4];
 	const int64_t last = j.p1 - 1;
-	auto row = [&](int64_t p) { return j.k + p * D; };
+	auto krow = [&](int64_t p) { return j.k + p * D; };
+	auto vrow = [&](int64_t p) { return j.v + p * D; };
+	k.load(j.p0, last, krow);
+	for (int64_t p = j.p0; p < j.p1; p += 64) {
+		s[0] = s[1] = s[2] = s[3] = v4i{0, 0, 0, 0};
+		if (WITH_V) v.load(p, last, vrow);
+		k.scores(lds, q, s);
+		k.load(p + 64, last, krow);
+		__builtin_amdgcn_sched_barrier(0);
+		step(p, s, [&](const v4i& lo, const v4i& nhi, v4i (&acc)[D / 16][2]) { v.multiply(lds, lo, nhi, acc); });
+	}
+}
+
+// The same over a shared plane, whose rows all waves of the block use: each thread loads its share of a step's
+// rows, AHEAD steps ahead, and stages it into one of two buffers, so a step costs one barrier (buffer b was
+// last read before the previous one).  LDS: 64 D bytes a buffer, K's two and then V's two.
+template <int D, bool WITH_V, int NC, typename F>
+__device__ __forceinline__ void sa_block_steps(const SaJob& j, int8_t* lds, const v4i (&q)[NC], F&& step) {
+	constexpr int BS = 64 * kSaWaves, CH = 4 * D, PT = (CH + BS - 1) / BS, PER = D / 16, AHEAD = D <= 128 ? 2 : 1;
+	const int64_t last = j.p1 - 1;
+	v4i kr[AHEAD][PT], vr[AHEAD][PT], s[4];
+	auto load = [&](int64_t p, v4i (&k)[PT], v4i (&v)[PT]) {
 #pragma unroll
-	for (int i = 0; i < AHEAD; ++i) k[i].load(j.p0 + 64 * i, last, row);
-	for (int64_t p = j.p0; p < j.p1; p += 64 * AHEAD) {
+		for (int u = 0; u < PT; ++u) {
+			const int c = min((int)threadIdx.x + u * BS, CH - 1);
+			const int64_t at = i64min(p + c / PER, last) * D + c % PER * 16;
+			k[u] = load16(j.k + at);
+			if (WITH_V) v[u] = load16(j.v + at);
+		}
+	};
+#pragma unroll
+	for (int i = 0; i < AHEAD; ++i) load(j.p0 + 64 * i, kr[i], vr[i]);
+	int b = 0;
+	for (int64_t p0 = j.p0; p0 < j.p1; p0 += 64 * AHEAD) {
 #pragma unroll
 		for (int i = 0; i < AHEAD; ++i) {
-			if (i && p + 64 * i >= j.p1) break;
-			s[0] = s[1] = s[2] = s[3] = v4i{0, 0, 0, 0};
-			k[i].scores(lds, q, s);
-			k[i].load(p + 64 * (i + AHEAD), last, row);
-			__builtin_amdgcn_sched_barrier(0);
-			step(p + 64 * i, s);
+			const int64_t p = p0 + 64 * i;
+			if (i && p >= j.p1) break;
+			int8_t *kb = lds + b * 64 * D, *vb = lds + (2 + b) * 64 * D;
+#pragma unroll
+			for (int u = 0; u < PT; ++u) {
+				const int c = (int)threadIdx.x + u * BS;
+				if (CH % BS == 0 || c < CH) {
+					*(v4i*)(kb + SaRows<D>::at(c / PER, c % PER)) = kr[i][u];
+					if (WITH_V) *(v4i*)(vb + SaRows<D>::at(c / PER, c % PER)) = vr[i][u];
+				}
+			}
+			load(p + 64 * AHEAD, kr[i], vr[i]);
+			__syncthreads();
+			sa_block_scores<D>(kb, q, s);
+			step(p, s, [&](const v4i& lo, const v4i& nhi, v4i (&acc)[D / 16][2]) { sa_block_multiply<D>(vb, lo, nhi, acc); });
+			b ^= 1;
 		}
 	}
 }
 
+// `step` over the wave's plane.
+template <int D, bool WITH_V, int NC, typename F>
+__device__ __forceinline__ void sa_steps(const SaJob& j, int8_t* lds, const v4i (&q)[NC], F&& step) {
+	if (j.owned) sa_own_steps<D, WITH_V>(j, lds + (threadIdx.x >> 6) * 32 * D, q, step);
+	else sa_block_steps<D, WITH_V>(j, lds, q, step);
+}
+
 template <int D>
 __global__ __launch_bounds__(64 * kSaWaves) void k_sa_max(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
-	constexpr int NC = (D + 63) / 64, AHEAD = D <= 128 ? 2 : 1;
-	__shared__ __attribute__((aligned(16))) int8_t s_kv[kSaWaves][32 * D];
-	int8_t* lds = s_kv[threadIdx.x >> 6];
+	constexpr int NC = (D + 63) / 64;
+	__shared__ __attribute__((aligned(16))) int8_t lds[2 * 64 * D];  // also kSaWaves 32 D
 	const int lane = threadIdx.x & 63, g = lane >> 4;
 	SaJob j;
 	RowSpan sp;
@@ -441,7 +518,7 @@ __global__ __launch_bounds__(64 * kSaWaves) void k_sa_max(sslm_launch::SharedAtt
 		v4i q[NC];
 		sa_load_q<D>(a, j, q);
 		int32_t m = INT32_MIN;
-		sa_steps<D, AHEAD>(j, lds, q, [&](int64_t p, v4i (&s)[4]) {
+		sa_steps<D, false>(j, lds, q, [&](int64_t p, v4i (&s)[4], auto&&) {
 #pragma unroll
 			for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -475,9 +552,8 @@ __device__ __forceinline__ bool sa_job(const sslm_launch::SharedAttnArgs& a, con
 
 template <int D>
 __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 4 : 2) void k_sa_sum(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
-	constexpr int NC = (D + 63) / 64, AHEAD = 1;
-	__shared__ __attribute__((aligned(16))) int8_t s_kv[kSaWaves][32 * D];
-	int8_t* lds = s_kv[threadIdx.x >> 6];
+	constexpr int NC = (D + 63) / 64;
+	__shared__ __attribute__((aligned(16))) int8_t lds[2 * 64 * D];  // also kSaWaves 32 D
 	const int g = (threadIdx.x & 63) >> 4;
 	SaJob j;
 	if (!sa_job(a, pl, w, &j) || j.p0 >= j.p1) return;
@@ -492,7 +568,7 @@ __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 4 : 2) void k_sa_sum(sslm
 	if (!__any(live && !sa_fast(c, j.width))) {
 		const SaExp e = sa_exp_of(live ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
 		double acc = 0.0;
-		sa_steps<D, AHEAD>(j, lds, q, [&](int64_t p, v4i (&s)[4]) {
+		sa_steps<D, false>(j, lds, q, [&](int64_t p, v4i (&s)[4], auto&&) {
 #pragma unroll
 			for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -504,7 +580,7 @@ __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 4 : 2) void k_sa_sum(sslm
 		sum = (int64_t)acc;
 	} else {
 		const double inv = 1.0 / (double)c.q_ln2;
-		sa_steps<D, AHEAD>(j, lds, q, [&](int64_t p, v4i (&s)[4]) {
+		sa_steps<D, false>(j, lds, q, [&](int64_t p, v4i (&s)[4], auto&&) {
 #pragma unroll
 			for (int i = 0; i < 16; ++i) {
 				if (p + (i >> 2) * 16 + g * 4 + (i & 3) >= end) continue;
@@ -557,9 +633,8 @@ __device__ __forceinline__ void sa_pack(const int32_t (&p)[16], v4i* lo, v4i* nh
 
 template <int D>
 __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 2 : 1) void k_sa_pv(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
-	constexpr int NC = (D + 63) / 64, DT = D / 16, AHEAD = 1;
-	__shared__ __attribute__((aligned(16))) int8_t s_kv[kSaWaves][32 * D];
-	int8_t* lds = s_kv[threadIdx.x >> 6];
+	constexpr int NC = (D + 63) / 64, DT = D / 16;
+	__shared__ __attribute__((aligned(16))) int8_t lds[4 * 64 * D];
 	const int g = (threadIdx.x & 63) >> 4;
 	SaJob j;
 	if (!sa_job(a, pl, w, &j)) return;
@@ -571,37 +646,32 @@ __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 2 : 1) void k_sa_pv(sslm_
 	if (j.p0 >= j.p1) return;
 	live = live && sum >= 0;
 	const int64_t den = live && sum > 1 ? sum : 1;
-	const int64_t end = !live ? 0 : (j.owned ? j.p1 : i64min(j.p1, j.start)), last = j.p1 - 1;
+	const int64_t end = !live ? 0 : (j.owned ? j.p1 : i64min(j.p1, j.start));
 	v4i q[NC], acc[DT][2], lo, nhi;
 	sa_load_q<D>(a, j, q);
 #pragma unroll
 	for (int d = 0; d < DT; ++d) acc[d][0] = acc[d][1] = v4i{0, 0, 0, 0};
-	SaRows<D> vr;
 	int32_t pr[16];
-	auto vrow = [&](int64_t p) { return j.v + p * D; };
 	if (!__any(live && !sa_fast(c, j.width))) {
 		const SaExp e = sa_exp_of(live ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
 		auto run = [&](auto small) {
 			constexpr bool SMALL = decltype(small)::value;
 			const SaProb pb = sa_prob_of((double)den, SMALL);
-			sa_steps<D, AHEAD>(j, lds, q, [&](int64_t p, v4i (&s)[4]) {
-				vr.load(p, last, vrow);
-				__builtin_amdgcn_sched_barrier(0);
+			sa_steps<D, true>(j, lds, q, [&](int64_t p, v4i (&s)[4], auto&& multiply) {
 #pragma unroll
 				for (int i = 0; i < 16; ++i) {
 					const int32_t x = sa_prob<SMALL>(pb, sa_exp(e, s[i >> 2][i & 3]));
 					pr[i] = p + (i >> 2) * 16 + g * 4 + (i & 3) < end ? x : 0;
 				}
 				sa_pack(pr, &lo, &nhi);
-				vr.multiply(lds, lo, nhi, acc);
+				multiply(lo, nhi, acc);
 			});
 		};
 		if (!__any(den >= ((int64_t)1 << 36))) run(std::true_type{});
 		else run(std::false_type{});
 	} else {
 		const double inv = 1.0 / (double)c.q_ln2, dinv = 1.0 / (double)den;
-		sa_steps<D, AHEAD>(j, lds, q, [&](int64_t p, v4i (&s)[4]) {
-			vr.load(p, last, vrow);
+		sa_steps<D, true>(j, lds, q, [&](int64_t p, v4i (&s)[4], auto&& multiply) {
 #pragma unroll
 			for (int i = 0; i < 16; ++i) {
 				pr[i] = 0;
@@ -610,7 +680,7 @@ __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 2 : 1) void k_sa_pv(sslm_
 				pr[i] = (int32_t)div_rcp_cold(x << 15, den, dinv, 32768);
 			}
 			sa_pack(pr, &lo, &nhi);
-			vr.multiply(lds, lo, nhi, acc);
+			multiply(lo, nhi, acc);
 		});
 	}
 	if (j.r < 0) return;
@@ -1343,8 +1413,8 @@ bool shared_attn_ok(int rows, int NH, int NKV, int D) {
 static SaPlan sa_plan(int rows, int NH, int NKV, int prefixes, int64_t max_prefix, int64_t max_own) {
 	SaPlan p{};
 	const int G = NH / NKV;
-	p.tiles = prefixes > 0 && max_prefix > 0 ? rows * G / 16 + prefixes : 0;
-	const int64_t steps = (max_prefix + 63) / 64, jobs = (int64_t)p.tiles * NKV;
+	p.tb = prefixes > 0 && max_prefix > 0 ? rows * G / (16 * kSaWaves) + prefixes : 0;
+	const int64_t steps = (max_prefix + 63) / 64, jobs = std::min<int64_t>((int64_t)p.tb * kSaWaves, (int64_t)rows * G / 16 + prefixes) * NKV;
 	if (jobs > 0) {
 		const int64_t want = std::min<int64_t>(steps, std::max<int64_t>(1, (kSaTargetWaves + jobs - 1) / jobs));
 		p.sb = (int)((steps + want - 1) / want) * 64;
@@ -1357,8 +1427,7 @@ static SaPlan sa_plan(int rows, int NH, int NKV, int prefixes, int64_t max_prefi
 	const int64_t owant = std::min<int64_t>(osteps, std::max<int64_t>(1, (kSaTargetWaves + ojobs - 1) / ojobs));
 	p.ob = (int)((osteps + owant - 1) / owant) * 64;
 	p.owned = (int)std::max<int64_t>(1, (max_own + p.ob - 1) / p.ob);
-	const int tb = (p.tiles + kSaWaves - 1) / kSaWaves;
-	p.shared_blocks = (NKV * p.shared + 7) / 8 * 8 * tb;
+	p.shared_blocks = (NKV * p.shared + 7) / 8 * 8 * p.tb;
 	return p;
 }
 
