@@ -40,10 +40,11 @@ constexpr int kSlotCapacity = 1024;  // live sequences per model
 // (8 prompts 23.2 against 23.5 and 23.6 against 24.9 ms).
 constexpr int kSlicedActPrefillRows = 32;
 
-// The attention of one block per (row, KV head) passes over its row alone: its time is the longest row's
-// positions times the rounds that its blocks take over the CUs.  From this many on, a unit with adopted
-// prefixes reads them shared and cut over the whole chip (a step of the 7B shape's layer, shared against
-// not: 32 rows of 2080 positions 199 / 191 us, 16 of 4128 189 / 197 us, 64 of 4196 249 / 471 us).
+// The attention of one block per (row, KV head) passes over its row alone, so its time is the longest row's
+// positions, once more where the blocks pass the CUs.  A unit with adopted prefixes reads them shared and cut
+// over the whole chip from this many positions on, and always with more blocks than CUs (a step of four layers
+// of the 7B shape, shared against not: 16 rows of 2080 positions 0.741 / 0.694 ms, 16 of 4128 0.749 / 0.786, 64
+// of 1632 0.934 / 0.910, 64 of 4196 0.97 / 1.88; 96 of 32 positions 0.945 / 0.984, 96 of 1056 1.05 / 1.26).
 constexpr int64_t kSharedPositions = 3500;
 
 struct HipError {
@@ -2349,8 +2350,8 @@ static void share_prompts(sslm_model m, sslm_seq* seqs, std::vector<int>* idx, s
 		width = std::max(width, seqs[i]->context_length + 1);
 		own = std::max(own, seqs[i]->context_length + 1 - (seqs[i]->prefix ? seqs[i]->prefix->seq->context_length : 0));
 	}
-	const int64_t cus = sslm_launch::device_cus(), rounds = ((int64_t)idx->size() * m->NKV + cus - 1) / cus;
-	if (e && (e[0] == '0' || e[0] == '1') ? e[0] == '0' : width * rounds < kSharedPositions) return;
+	const int64_t blocks = (int64_t)idx->size() * m->NKV;
+	if (e && (e[0] == '0' || e[0] == '1') ? e[0] == '0' : width < kSharedPositions && blocks <= sslm_launch::device_cus()) return;
 	std::stable_sort(idx->begin(), idx->end(), [&](int x, int y) { return where(x) < where(y); });
 	rows->push_back(0);
 	for (size_t k = 0; k < ps.size(); ++k)
