@@ -1101,9 +1101,14 @@ __global__ __launch_bounds__(256) void k_lora_proj(sslm_launch::LoraGemmArgs g, 
 	}
 }
 
-// A row's u as dot operands of a B row: pieces of 16 bytes (4 where the rank is below 16) at byte
-// min(16 q, rank - 16); the last piece's bytes that an earlier one holds are zero.
-__device__ __forceinline__ int lora_piece(int q, int rank, int w) { return min(w * q, rank - w); }
+// A row's u as dot operands of the rows of B, which are taken in pieces of w bytes (16, or 4 where the rank is
+// below 16) from the 4 bytes that hold a row's first one: a 16-byte load that is not 4-byte aligned takes
+// about twice as long.  A row whose first byte is the f-th of its four spans lora_span bytes from there,
+// piece q lies at byte lora_piece of them, and copy f of u has zeros where a piece holds other rows' bytes or
+// those of an earlier piece.  n rank is a multiple of 16, so nothing past B is read.
+__device__ __forceinline__ int lora_span(int rank, int f) { return (f + rank + 3) & ~3; }
+__device__ __forceinline__ int lora_piece(int q, int rank, int f, int w) { return min(w * q, lora_span(rank, f) - w); }
+constexpr int kLoraU = 80;  // bytes of a copy: a span of 68 in 16-byte pieces
 
 struct __attribute__((packed)) unaligned16 {
 	v4i v;
@@ -1112,135 +1117,134 @@ struct __attribute__((packed)) unaligned4 {
 	int32_t v;
 };
 
-// Fold, adapter delta and funnel (forward_sites.cpp:1114-1154) of R rows of accumulators (the sum of
-// PL planes), whose folds are read once for them.  Every load of a thread's EPT columns is issued
-// from a clamped index before the first is used: taken column by column they cost a round trip each.
-template <int BS, int EPT, int R, int PL>
+// A column's folded accumulator plus its adapter's apply_amp_fold(d), |d| <= 128 127 64 < 2^20.  There the
+// doubling high multiplication cannot saturate and keeps |x| < 2^20, so that for exponents in [-10, 31] the
+// rounding shift is fold_bounded's and a left shift stays below 2^30: with |folded| <= 2^29 the sum needs no
+// 64 bits and no saturation.  Other exponents take the general form.
+__device__ __forceinline__ int32_t lora_add(int32_t folded, int32_t d, const int32_t (&df)[3], uint32_t* mag) {
+	const int e = df[2];
+	if ((uint32_t)(e + 10) > 41u) {
+		const int64_t x = (int64_t)folded + apply_amp_fold((int64_t)d, df[0], df[1], e);
+		*mag = sat_abs_u32(x);
+		return sat_i32(x);
+	}
+	const int32_t hi = (int32_t)(((int64_t)d * df[1] + ((int64_t)1 << 30)) >> 31);
+	const int right = max(e, 0);
+	const int32_t half = (int32_t)((1u << right) >> 1), neg = e > 0 ? hi >> 31 : 0;
+	const int32_t amp = ((hi + half + neg) >> right) << max(-e, 0);
+	const int32_t x = folded + (df[0] != 0 ? d : amp);
+	*mag = (uint32_t)abs(x);
+	return x;
+}
+
+// Fold, adapter delta and funnel (forward_sites.cpp:1114-1154) of a row of accumulators (the sum of PL planes).
+// Every load of a thread's EPT columns is issued from a clamped index before the first is used (taken column
+// by column they cost a round trip each); two pieces of B in flight take more registers and are slower.
+// 512 rows of 8192: 10.9 us without adapters, 18.6 at rank 16, 24.8 at rank 32, bound by the B rows and
+// folds from L2, some 300 KB a row.
+template <int BS, int EPT, int PL>
 __global__ __launch_bounds__(BS) void k_lora_funnel(sslm_launch::LoraGemmArgs g, const int32_t* part, const int8_t* u) {
-	__shared__ __attribute__((aligned(16))) int8_t s_u[R][kMaxRank];
-	__shared__ uint32_t s_m[R][BS / 64];
-	const int t0 = blockIdx.x * R;
-	int32_t v[R][EPT];
-	int col[EPT];
-#pragma unroll
-	for (int k = 0; k < EPT; ++k) col[k] = min((int)threadIdx.x + k * BS, g.n - 1);
-	int32_t fd[EPT][3];
+	__shared__ __attribute__((aligned(16))) int8_t s_u[4][kLoraU];
+	__shared__ uint32_t s_m[BS / 64];
+	const int t = blockIdx.x;
+	auto col = [&](int k) { return min((int)threadIdx.x + k * BS, g.n - 1); };
+	int32_t v[EPT], fd[EPT][3], pv[PL][EPT];
 #pragma unroll
 	for (int k = 0; k < EPT; ++k)
 #pragma unroll
-		for (int i = 0; i < 3; ++i) fd[k][i] = g.fold[3 * col[k] + i];
-	const LoraRef* ad[R];
-	bool ok[R];
-	LoraRef ref[R];
+		for (int i = 0; i < 3; ++i) fd[k][i] = g.fold[3 * col(k) + i];
+	const int32_t* at = part + (size_t)t * g.n;
 #pragma unroll
-	for (int r = 0; r < R; ++r) {
-		const int t = min(t0 + r, g.m - 1);
-		const int32_t* at = part + (size_t)t * g.n;
-		int32_t pv[PL][EPT];
+	for (int p = 0; p < PL; ++p)
 #pragma unroll
-		for (int p = 0; p < PL; ++p)
-#pragma unroll
-			for (int k = 0; k < EPT; ++k) pv[p][k] = at[(size_t)p * g.m * g.n + col[k]];
-#pragma unroll
-		for (int k = 0; k < EPT; ++k) {
-			v[r][k] = pv[0][k];
-#pragma unroll
-			for (int p = 1; p < PL; ++p) v[r][k] += pv[p][k];
-		}
-		ok[r] = row_adapter(g, t, &ad[r]);
-		ref[r] = ok[r] && ad[r] ? *ad[r] : LoraRef{};
-		const int rank = ref[r].rank, w = rank >= 16 ? 16 : (rank >= 4 ? 4 : 1), i = threadIdx.x;
-		if (i < kMaxRank) {
-			const int q = i / w, from = w == 1 ? i : lora_piece(q, rank, w) + i % w;
-			s_u[r][i] = w * q < rank && from >= w * q ? u[(size_t)t * kMaxRank + from] : (int8_t)0;
+		for (int k = 0; k < EPT; ++k) pv[p][k] = at[(size_t)p * g.m * g.n + col(k)];
+	const LoraRef* ad;
+	const bool ok = row_adapter(g, t, &ad);
+	const LoraRef ref = ok && ad ? *ad : LoraRef{};
+	const int rank = ref.rank;
+	if (rank > 0) {
+		const int w = rank >= 16 ? 16 : 4, last = rank % 4 ? 4 : 1;
+		for (int x = threadIdx.x; x < last * kLoraU; x += BS) {
+			const int f = x / kLoraU, q = x % kLoraU / w, p = lora_piece(q, rank, f, w) + x % w, i = p - f;
+			s_u[f][x % kLoraU] = p >= w * q && i >= 0 && i < rank ? u[(size_t)t * kMaxRank + i] : (int8_t)0;
 		}
 	}
-	__syncthreads();
 #pragma unroll
-	for (int r = 0; r < R; ++r) {
-		const int rank = ref[r].rank;
-		uint32_t mx = 0;
-		if (rank > 0) {
-			int32_t d[EPT] = {}, df[EPT][3];  // |B.u| <= 128 127 64 < 2^31
+	for (int k = 0; k < EPT; ++k) {
+		v[k] = pv[0][k];
 #pragma unroll
-			for (int k = 0; k < EPT; ++k)
+		for (int p = 1; p < PL; ++p) v[k] += pv[p][k];
+		v[k] = fold_bounded(v[k], fold_consts(fd[k][0], fd[k][1], fd[k][2]));  // |acc| <= 128^2 k <= 2^29
+	}
+	__builtin_amdgcn_sched_barrier(0);  // the folds' registers are B's from here on
+	uint32_t mx = 0;
+	if (rank > 0) {
+		int32_t d[EPT] = {}, df[EPT][3];  // |B.u| <= 128 127 64 < 2^31
 #pragma unroll
-				for (int i = 0; i < 3; ++i) df[k][i] = ref[r].dfold[3 * col[k] + i];
-			if (rank >= 16) {
-				constexpr int PQ = EPT <= 5 ? 2 : 1;  // pieces in flight; past the rank u is zero
-				for (int q = 0; 16 * q < rank; q += PQ) {
-					v4i x[PQ][EPT];
+		for (int k = 0; k < EPT; ++k)
 #pragma unroll
-					for (int e = 0; e < PQ; ++e)
+			for (int i = 0; i < 3; ++i) df[k][i] = ref.dfold[3 * col(k) + i];
+		const int span = lora_span(rank, rank % 4 ? 3 : 0);
+		__syncthreads();
+		if (rank >= 16) {
+			for (int q = 0; 16 * q < span; ++q) {
+				v4i x[EPT];
 #pragma unroll
-						for (int k = 0; k < EPT; ++k)
-							x[e][k] = ((const unaligned16*)(ref[r].b + (size_t)col[k] * rank + lora_piece(q + e, rank, 16)))->v;
-#pragma unroll
-					for (int e = 0; e < PQ; ++e) {
-						const v4i y = *(const v4i*)(s_u[r] + 16 * (q + e));
-#pragma unroll
-						for (int k = 0; k < EPT; ++k)
-#pragma unroll
-							for (int i = 0; i < 4; ++i) d[k] = __builtin_amdgcn_sdot4(x[e][k][i], y[i], d[k], false);
-					}
+				for (int k = 0; k < EPT; ++k) {
+					const int off = col(k) * rank;
+					x[k] = ((const unaligned16*)(ref.b + (uint32_t)((off & ~3) + lora_piece(q, rank, off & 3, 16))))->v;
 				}
-			} else if (rank >= 4) {
-				for (int q = 0; 4 * q < rank; ++q) {
-					const int8_t* b = ref[r].b + lora_piece(q, rank, 4);
-					const int32_t y = *(const int32_t*)(s_u[r] + 4 * q);
-					int32_t x[EPT];
 #pragma unroll
-					for (int k = 0; k < EPT; ++k) x[k] = ((const unaligned4*)(b + (size_t)col[k] * rank))->v;
+				for (int k = 0; k < EPT; ++k) {
+					const v4i y = *(const v4i*)(s_u[col(k) * rank & 3] + 16 * q);
 #pragma unroll
-					for (int k = 0; k < EPT; ++k) d[k] = __builtin_amdgcn_sdot4(x[k], y, d[k], false);
+					for (int i = 0; i < 4; ++i) d[k] = __builtin_amdgcn_sdot4(x[k][i], y[i], d[k], false);
 				}
-			} else {
-				for (int i = 0; i < rank; ++i)
-#pragma unroll
-					for (int k = 0; k < EPT; ++k) d[k] += (int32_t)ref[r].b[(size_t)col[k] * rank + i] * (int32_t)s_u[r][i];
-			}
-#pragma unroll
-			for (int k = 0; k < EPT; ++k) {
-				const int64_t x = (int64_t)fold_bounded(v[r][k], fold_consts(fd[k][0], fd[k][1], fd[k][2])) +
-				                  apply_amp_fold((int64_t)d[k], df[k][0], df[k][1], df[k][2]);
-				mx = max(mx, sat_abs_u32(x));  // a clamped column repeats the last one
-				v[r][k] = sat_i32(x);
 			}
 		} else {
+			for (int q = 0; 4 * q < span; ++q) {
+				int32_t x[EPT];
 #pragma unroll
-			for (int k = 0; k < EPT; ++k) {
-				v[r][k] = fold_bounded(v[r][k], fold_consts(fd[k][0], fd[k][1], fd[k][2]));  // |acc| <= 128^2 k <= 2^29
-				mx = max(mx, sat_abs_u32(v[r][k]));
+				for (int k = 0; k < EPT; ++k) {
+					const int off = col(k) * rank;
+					x[k] = ((const unaligned4*)(ref.b + (uint32_t)((off & ~3) + lora_piece(q, rank, off & 3, 4))))->v;
+				}
+#pragma unroll
+				for (int k = 0; k < EPT; ++k) d[k] = __builtin_amdgcn_sdot4(x[k], *(const int32_t*)(s_u[col(k) * rank & 3] + 4 * q), d[k], false);
 			}
 		}
-		mx = wave_max32(mx);
-		if ((threadIdx.x & 63) == 0) s_m[r][threadIdx.x >> 6] = mx;
-	}
-	__syncthreads();
-#pragma unroll
-	for (int r = 0; r < R; ++r) {
-		const int t = t0 + r;
-		if (t >= g.m) return;
-		if (!ok[r]) {
-			if (threadIdx.x == 0) g.status[t] = kBadAdapter;
-			continue;
-		}
-		uint32_t m = s_m[r][0];
-#pragma unroll
-		for (int i = 1; i < BS / 64; ++i) m = max(m, s_m[r][i]);
-		FunnelPlan plan;
-		const Scale in = g.in_scale[t];
-		const int32_t st = funnel_plan(__builtin_amdgcn_readfirstlane(m), &in, 1, g.site, &plan);
-		if (threadIdx.x == 0) {
-			g.status[t] = st;
-			if (st == kOk) g.scales[t] = plan.out;
-		}
-		if (st != kOk) continue;
 #pragma unroll
 		for (int k = 0; k < EPT; ++k) {
-			const int j = (int)threadIdx.x + k * BS;
-			if (j < g.n) g.codes[(size_t)t * g.n + j] = requant_code_f(v[r][k], plan.f);
+			uint32_t mag;
+			v[k] = lora_add(v[k], d[k], df[k], &mag);
+			mx = max(mx, mag);  // a clamped column repeats the last one
 		}
+	} else {
+#pragma unroll
+		for (int k = 0; k < EPT; ++k) mx = max(mx, sat_abs_u32(v[k]));
+	}
+	mx = wave_max32(mx);
+	if ((threadIdx.x & 63) == 0) s_m[threadIdx.x >> 6] = mx;
+	__syncthreads();
+	if (!ok) {
+		if (threadIdx.x == 0) g.status[t] = kBadAdapter;
+		return;
+	}
+	uint32_t m = s_m[0];
+#pragma unroll
+	for (int i = 1; i < BS / 64; ++i) m = max(m, s_m[i]);
+	FunnelPlan plan;
+	const Scale in = g.in_scale[t];
+	const int32_t st = funnel_plan(__builtin_amdgcn_readfirstlane(m), &in, 1, g.site, &plan);
+	if (threadIdx.x == 0) {
+		g.status[t] = st;
+		if (st == kOk) g.scales[t] = plan.out;
+	}
+	if (st != kOk) return;
+#pragma unroll
+	for (int k = 0; k < EPT; ++k) {
+		const int j = (int)threadIdx.x + k * BS;
+		if (j < g.n) g.codes[(size_t)t * g.n + j] = requant_code_f(v[k], plan.f);
 	}
 }
 
@@ -1514,14 +1518,14 @@ size_t lora_gemm_workspace(int m, int n, int k) {
 	return up256((size_t)planes * m * n * 4) + up256((size_t)m * kMaxRank);
 }
 
-template <int BS, int EPT, int R>
+template <int BS, int EPT>
 static void lora_funnel(const LoraGemmArgs& g, int planes, const int32_t* part, const int8_t* u, hipStream_t s) {
-	const dim3 grid((g.m + R - 1) / R), block(BS);
+	const dim3 grid(g.m), block(BS);
 	switch (planes) {
-		case 1: hipLaunchKernelGGL((k_lora_funnel<BS, EPT, R, 1>), grid, block, 0, s, g, part, u); break;
-		case 2: hipLaunchKernelGGL((k_lora_funnel<BS, EPT, R, 2>), grid, block, 0, s, g, part, u); break;
-		case 4: hipLaunchKernelGGL((k_lora_funnel<BS, EPT, R, 4>), grid, block, 0, s, g, part, u); break;
-		default: hipLaunchKernelGGL((k_lora_funnel<BS, EPT, R, 8>), grid, block, 0, s, g, part, u); break;
+		case 1: hipLaunchKernelGGL((k_lora_funnel<BS, EPT, 1>), grid, block, 0, s, g, part, u); break;
+		case 2: hipLaunchKernelGGL((k_lora_funnel<BS, EPT, 2>), grid, block, 0, s, g, part, u); break;
+		case 4: hipLaunchKernelGGL((k_lora_funnel<BS, EPT, 4>), grid, block, 0, s, g, part, u); break;
+		default: hipLaunchKernelGGL((k_lora_funnel<BS, EPT, 8>), grid, block, 0, s, g, part, u); break;
 	}
 }
 
@@ -1552,9 +1556,9 @@ void lora_gemm(const LoraGemmArgs& g, hipStream_t s) {
 		gemm(ga, s);
 		if (g.count > 0) hipLaunchKernelGGL(k_rows_u, dim3(g.m, kMaxRank / 4), dim3(256), 0, s, g, u);
 	}
-	if (g.n <= 2048) lora_funnel<512, 4, 1>(g, planes, part, u, s);
-	else if (g.n <= 5120) lora_funnel<1024, 5, 1>(g, planes, part, u, s);
-	else lora_funnel<1024, 8, 1>(g, planes, part, u, s);
+	if (g.n <= 2048) lora_funnel<512, 4>(g, planes, part, u, s);
+	else if (g.n <= 5120) lora_funnel<1024, 5>(g, planes, part, u, s);
+	else lora_funnel<1024, 8>(g, planes, part, u, s);
 }
 
 void lora_table(const LoraRef* const* rows, int M, int l0, int l1, LoraRef* out, int ld, hipStream_t s) {

@@ -302,6 +302,23 @@ def test_lora_matches_the_oracle(m, n, k, ranks, rows, ops, dev, host):
     b.check(host, b.run(ops, dev))
 
 
+@pytest.mark.parametrize("n,lo,hi", [(32, -31, 32), (2064, -31, 32), (2064, -3, 5), (2064, 5, 32)])
+def test_lora_every_rank_and_exponent(n, lo, hi, ops, dev, host):
+    """One row per rank, its B rows beginning at every byte of their words; delta exponents over the whole
+    range, with deltas that saturate and that meet ties, and over parts of it, so that no delta hides the
+    others; folds with hardly a shift, so that sums are large."""
+    b = LoraBatch(n, 64, n, 256, list(range(1, 65)), list(range(64)))
+    rng = np.random.default_rng(n + 1)
+    for a, uf, lb, df in b.adapters:
+        uf[:, 2] = rng.integers(8, 20, len(uf))
+        df[:, 2] = rng.integers(lo, hi, n)
+        df[::7, 1] = -(1 << 31)
+        df[::5, 1] = 1 << 30
+    b.fold[:, 2] = rng.integers(0, 2, n)
+    b.check(host, b.run(ops, dev))
+
+
+
 def test_lora_without_adapters_is_the_shared_projection(ops, dev, host):
     b = LoraBatch(3, 6, 96, 128, [], [-1])
     print("case lora none", flush=True)
