@@ -39,6 +39,14 @@ __device__ __forceinline__ uint32_t block_max_u32(uint32_t v, uint32_t* slots) {
 // attention of rows that share prompts
 // ------------------------------------------------------------------------------------------
 
+// A pointer that was read from memory is generic to the compiler, whose flat loads count as LDS operations
+// too: each wait for LDS would then be one for every load in flight.  All of these point to global memory.
+template <typename T>
+__device__ __forceinline__ const __attribute__((address_space(1))) T* global_ptr(const T* p) {
+	return (const __attribute__((address_space(1))) T*)p;
+}
+__device__ __forceinline__ v4i global16(const int8_t* p) { return *global_ptr((const v4i*)p); }
+
 // Where a row's positions lie: [0, start) in its prefix's block, [start, width) in its own.
 struct RowSpan {
 	int64_t width, start;
@@ -281,7 +289,7 @@ struct SaRows {
 #pragma unroll
 		for (int u = 0; u < PER; ++u) {
 			const int i = lane + 64 * u;
-			r[u] = load16(row(i64min(p + i / PER, last)) + i % PER * 16);
+			r[u] = global16(row(i64min(p + i / PER, last)) + i % PER * 16);
 		}
 	}
 	// rows 32 h .. 32 h + 31 into LDS
@@ -460,8 +468,8 @@ __device__ __forceinline__ void sa_block_steps(const SaJob& j, int8_t* lds, cons
 		for (int u = 0; u < PT; ++u) {
 			const int c = min((int)threadIdx.x + u * BS, CH - 1);
 			const int64_t at = i64min(p + c / PER, last) * D + c % PER * 16;
-			k[u] = load16(j.k + at);
-			if (WITH_V) v[u] = load16(j.v + at);
+			k[u] = global16(j.k + at);
+			if (WITH_V) v[u] = global16(j.v + at);
 		}
 	};
 #pragma unroll
@@ -497,6 +505,9 @@ __device__ __forceinline__ void sa_steps(const SaJob& j, int8_t* lds, const v4i 
 	else sa_block_steps<D, WITH_V>(j, lds, q, step);
 }
 
+// How many of the step's positions, counted from the lane's first (4 g), its row has.
+__device__ __forceinline__ int sa_left(int64_t p, int64_t end) { return (int)i64min(end - p, 64) - ((threadIdx.x & 63) >> 4) * 4; }
+
 template <int D>
 __global__ __launch_bounds__(64 * kSaWaves) void k_sa_max(sslm_launch::SharedAttnArgs a, SaPlan pl, SaWork w) {
 	constexpr int NC = (D + 63) / 64;
@@ -519,10 +530,11 @@ __global__ __launch_bounds__(64 * kSaWaves) void k_sa_max(sslm_launch::SharedAtt
 		sa_load_q<D>(a, j, q);
 		int32_t m = INT32_MIN;
 		sa_steps<D, false>(j, lds, q, [&](int64_t p, v4i (&s)[4], auto&&) {
+			const int left = sa_left(p, end);
 #pragma unroll
 			for (int t = 0; t < 4; ++t)
 #pragma unroll
-				for (int v = 0; v < 4; ++v) m = max(m, p + t * 16 + g * 4 + v < end ? s[t][v] : INT32_MIN);
+				for (int v = 0; v < 4; ++v) m = max(m, t * 16 + v < left ? s[t][v] : INT32_MIN);
 		});
 		m = max(m, __shfl_xor(m, 16, 64));
 		m = max(m, __shfl_xor(m, 32, 64));
@@ -569,12 +581,13 @@ __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 4 : 2) void k_sa_sum(sslm
 		const SaExp e = sa_exp_of(live ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
 		double acc = 0.0;
 		sa_steps<D, false>(j, lds, q, [&](int64_t p, v4i (&s)[4], auto&&) {
+			const int left = sa_left(p, end);
 #pragma unroll
 			for (int t = 0; t < 4; ++t)
 #pragma unroll
 				for (int v = 0; v < 4; ++v) {
 					const double x = sa_exp(e, s[t][v]);
-					acc += p + t * 16 + g * 4 + v < end ? x : 0.0;
+					acc += t * 16 + v < left ? x : 0.0;
 				}
 		});
 		sum = (int64_t)acc;
@@ -658,10 +671,11 @@ __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 2 : 1) void k_sa_pv(sslm_
 			constexpr bool SMALL = decltype(small)::value;
 			const SaProb pb = sa_prob_of((double)den, SMALL);
 			sa_steps<D, true>(j, lds, q, [&](int64_t p, v4i (&s)[4], auto&& multiply) {
+				const int left = sa_left(p, end);
 #pragma unroll
 				for (int i = 0; i < 16; ++i) {
 					const int32_t x = sa_prob<SMALL>(pb, sa_exp(e, s[i >> 2][i & 3]));
-					pr[i] = p + (i >> 2) * 16 + g * 4 + (i & 3) < end ? x : 0;
+					pr[i] = (i >> 2) * 16 + (i & 3) < left ? x : 0;
 				}
 				sa_pack(pr, &lo, &nhi);
 				multiply(lo, nhi, acc);
@@ -1004,7 +1018,7 @@ __device__ __forceinline__ void row_u(const LoraRef& ad, const int8_t* x, int k,
 		for (int i = 0; i < kUChunks; ++i) {
 			const int c = min(c0 + 1024 * i, k - 16);
 			p[i] = load16(x + c);
-			q[i] = load16(w + c);
+			q[i] = global16(w + c);
 		}
 		__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -1016,7 +1030,7 @@ __device__ __forceinline__ void row_u(const LoraRef& ad, const int8_t* x, int k,
 	}
 	acc = wave_sum32(acc);
 	if (lane == 0) {
-		const int32_t* fd = ad.ufold + 3 * rk;
+		const auto* fd = global_ptr(ad.ufold + 3 * rk);
 		u[rk] = (int8_t)clamp_code(apply_amp_fold((int64_t)acc, fd[0], fd[1], fd[2]));
 	}
 }
@@ -1183,7 +1197,7 @@ __global__ __launch_bounds__(BS) void k_lora_funnel(sslm_launch::LoraGemmArgs g,
 #pragma unroll
 		for (int k = 0; k < EPT; ++k)
 #pragma unroll
-			for (int i = 0; i < 3; ++i) df[k][i] = ref.dfold[3 * col(k) + i];
+			for (int i = 0; i < 3; ++i) df[k][i] = global_ptr(ref.dfold)[3 * col(k) + i];
 		const int span = lora_span(rank, rank % 4 ? 3 : 0);
 		__syncthreads();
 		if (rank >= 16) {
@@ -1192,7 +1206,7 @@ __global__ __launch_bounds__(BS) void k_lora_funnel(sslm_launch::LoraGemmArgs g,
 #pragma unroll
 				for (int k = 0; k < EPT; ++k) {
 					const int off = col(k) * rank;
-					x[k] = ((const unaligned16*)(ref.b + (uint32_t)((off & ~3) + lora_piece(q, rank, off & 3, 16))))->v;
+					x[k] = global_ptr((const unaligned16*)(ref.b + (uint32_t)((off & ~3) + lora_piece(q, rank, off & 3, 16))))->v;
 				}
 #pragma unroll
 				for (int k = 0; k < EPT; ++k) {
@@ -1207,7 +1221,7 @@ __global__ __launch_bounds__(BS) void k_lora_funnel(sslm_launch::LoraGemmArgs g,
 #pragma unroll
 				for (int k = 0; k < EPT; ++k) {
 					const int off = col(k) * rank;
-					x[k] = ((const unaligned4*)(ref.b + (uint32_t)((off & ~3) + lora_piece(q, rank, off & 3, 4))))->v;
+					x[k] = global_ptr((const unaligned4*)(ref.b + (uint32_t)((off & ~3) + lora_piece(q, rank, off & 3, 4))))->v;
 				}
 #pragma unroll
 				for (int k = 0; k < EPT; ++k) d[k] = __builtin_amdgcn_sdot4(x[k], *(const int32_t*)(s_u[col(k) * rank & 3] + 4 * q), d[k], false);
@@ -1295,7 +1309,7 @@ __global__ __launch_bounds__(kPickBlock) void k_pick_slice(sslm_launch::PickArgs
 #pragma unroll
 	for (int u = 0; u < U; ++u) {
 		const int id = v0 + 4 * ((int)threadIdx.x + u * kPickBlock);
-		legal[u] = ru.mask ? ru.mask[min(id, a.vocab - 1) >> 3] >> (id & 4) : 15u;
+		legal[u] = ru.mask ? global_ptr(ru.mask)[min(id, a.vocab - 1) >> 3] >> (id & 4) : 15u;
 	}
 	if (seen) {
 #pragma unroll
@@ -1304,7 +1318,7 @@ __global__ __launch_bounds__(kPickBlock) void k_pick_slice(sslm_launch::PickArgs
 		for (int i = threadIdx.x; i < ru.history_len; i += 4 * kPickBlock) {
 			int32_t h[4];
 #pragma unroll
-			for (int e = 0; e < 4; ++e) h[e] = ru.history[min(i + e * kPickBlock, ru.history_len - 1)];
+			for (int e = 0; e < 4; ++e) h[e] = global_ptr(ru.history)[min(i + e * kPickBlock, ru.history_len - 1)];
 #pragma unroll
 			for (int e = 0; e < 4; ++e) {
 				const int64_t j = (int64_t)h[e] - v0;
@@ -1324,8 +1338,8 @@ __global__ __launch_bounds__(kPickBlock) void k_pick_slice(sslm_launch::PickArgs
 			for (int i = threadIdx.x; i < kPickSlice / 4; i += kPickBlock) ((v4i*)s_bias)[i] = v4i{0, 0, 0, 0};
 			__syncthreads();
 			for (int i = threadIdx.x; i < ru.bias_count; i += kPickBlock) {
-				const int64_t t = (int64_t)ru.bias_ids[i] - v0;
-				if (t >= h0 && t < h0 + kPickSlice / 2 && t < n) atomicAdd(&s_bias[t - h0], (unsigned long long)(int64_t)ru.bias_values[i]);
+				const int64_t t = (int64_t)global_ptr(ru.bias_ids)[i] - v0;
+				if (t >= h0 && t < h0 + kPickSlice / 2 && t < n) atomicAdd(&s_bias[t - h0], (unsigned long long)(int64_t)global_ptr(ru.bias_values)[i]);
 			}
 			__syncthreads();
 		}
