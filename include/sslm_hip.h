@@ -367,8 +367,8 @@ sslm_status sslm_hip_shared_attention(const sslm_hip_shared_attention_args* args
 /* sslm_hip_gemm_requant for a batch whose rows each carry a low-rank adapter of their own (reference
  * forward_sites.cpp:1051-1154: fold, adapter delta, funnel): row t has adapters[row_adapter[t]], a
  * negative index none, and the incoming scale in_scale[t].  adapters is a device array; rank in
- * [1, 64], ranks may differ.  out status -1: an index or rank outside those.  1 <= m <= 512, n a multiple
- * of 16 up to 8192, k a multiple of 16 up to 32768. */
+ * [1, 64], ranks may differ.  out status -1: an index or rank outside those, a null pointer, an `a` that is
+ * not aligned.  1 <= m <= 512, n a multiple of 16 up to 8192, k a multiple of 16 up to 32768. */
 #define SSLM_HIP_GEMM_LORA_MAX_M 512
 #define SSLM_HIP_GEMM_LORA_MAX_K 32768
 typedef struct sslm_hip_lora {

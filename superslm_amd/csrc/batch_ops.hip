@@ -47,6 +47,13 @@ __device__ __forceinline__ const __attribute__((address_space(1))) T* global_ptr
 }
 __device__ __forceinline__ v4i global16(const int8_t* p) { return *global_ptr((const v4i*)p); }
 
+struct __attribute__((packed)) unaligned16 {
+	v4i v;
+};
+struct __attribute__((packed)) unaligned4 {
+	int32_t v;
+};
+
 // Where a row's positions lie: [0, start) in its prefix's block, [start, width) in its own.
 struct RowSpan {
 	int64_t width, start;
@@ -766,7 +773,7 @@ __device__ __forceinline__ void sa_finish(const sslm_launch::SharedAttnArgs& a, 
 			uint32_t o = 0;
 #pragma unroll
 			for (int x = 0; x < 4; ++x) o |= (uint32_t)(uint8_t)requant_code_f(v[u][x], plan.f) << 8 * x;
-			*(uint32_t*)(a.codes + (size_t)r * N + 4 * i) = o;
+			((unaligned4*)(a.codes + (size_t)r * N + 4 * i))->v = (int32_t)o;
 		}
 	}
 }
@@ -999,7 +1006,9 @@ __device__ __forceinline__ bool row_adapter(const sslm_launch::LoraGemmArgs& g, 
 	const int i = g.row_adapter[t];
 	*out = nullptr;
 	if (i < 0) return true;
-	if (i >= g.count || g.adapters[i].rank < 1 || g.adapters[i].rank > kMaxRank) return false;
+	if (i >= g.count) return false;
+	const LoraRef& r = g.adapters[i];
+	if (r.rank < 1 || r.rank > kMaxRank || !r.a || (uintptr_t)r.a % 16 || !r.ufold || !r.b || !r.dfold) return false;
 	*out = g.adapters + i;
 	return true;
 }
@@ -1123,13 +1132,6 @@ __global__ __launch_bounds__(256) void k_lora_proj(sslm_launch::LoraGemmArgs g, 
 __device__ __forceinline__ int lora_span(int rank, int f) { return (f + rank + 3) & ~3; }
 __device__ __forceinline__ int lora_piece(int q, int rank, int f, int w) { return min(w * q, lora_span(rank, f) - w); }
 constexpr int kLoraU = 80;  // bytes of a copy: a span of 68 in 16-byte pieces
-
-struct __attribute__((packed)) unaligned16 {
-	v4i v;
-};
-struct __attribute__((packed)) unaligned4 {
-	int32_t v;
-};
 
 // A column's folded accumulator plus its adapter's apply_amp_fold(d), |d| <= 128 127 64 < 2^20.  There the
 // doubling high multiplication cannot saturate and keeps |x| < 2^20, so that for exponents in [-10, 31] the
@@ -1598,7 +1600,7 @@ void rows_u(const RowsUArgs& a, hipStream_t s) {
 	hipLaunchKernelGGL(k_refs_u, dim3(a.M, kMaxRank / 4, a.nproj), dim3(256), 0, s, a);
 }
 
-static int pick_slices(int vocab) { return (vocab + kPickSlice - 1) / kPickSlice; }
+static int pick_slices(int vocab) { return (int)(((int64_t)vocab + kPickSlice - 1) / kPickSlice); }
 
 void append_tokens(int32_t* const* at, const int32_t* token, int n, hipStream_t s) {
 	hipLaunchKernelGGL(k_append_tokens, dim3((n + 63) / 64), dim3(64), 0, s, at, token, n);

@@ -443,6 +443,7 @@ namespace {
 
 std::mutex g_registry_mu;
 std::set<sslm_seq_s*> g_live_seqs;
+std::set<sslm_prefix_s*> g_live_prefixes;  // begun and not released
 
 // sequence blob constants (src/sslm_abi.cpp:102, :2585-2618)
 constexpr uint8_t kBlobMagic[4] = {'S', 'S', 'B', '3'};
@@ -2357,7 +2358,7 @@ static void share_prompts(sslm_model m, sslm_seq* seqs, std::vector<int>* idx, s
 	for (size_t k = 0; k < ps.size(); ++k)
 		rows->push_back(rows->back() + (int32_t)std::count_if(idx->begin(), idx->end(), [&](int i) { return seqs[i]->prefix == ps[k]; }));
 	*prefixes = std::move(ps);
-	*max_prefix = longest;
+	*max_prefix = (longest + 63) / 64 * 64;  // the steps of a launch: one graph for prompts of as many
 	*max_own = std::min(m->cap, (own + 255) / 256 * 256);
 }
 
@@ -2489,9 +2490,10 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 		set_shared(w, un);
 		if (w.shared.rows) {
 			const size_t need = sslm_launch::shared_attn_workspace(M, m->NH, m->NKV, m->D, w.shared.prefixes, un.max_prefix, un.max_own);
-			if (need > w.shared.ws_bytes) {  // the old one stays: graphs recorded with it are sized for it
-				w.shared.ws = dalloc<uint8_t>(need, &w.own);
-				w.shared.ws_bytes = need;
+			if (need > w.shared.ws_bytes) {  // the old ones stay, together less than the new one: recorded graphs use them
+				const size_t bytes = std::max(need, 2 * w.shared.ws_bytes);
+				w.shared.ws = dalloc<uint8_t>(bytes, &w.own);
+				w.shared.ws_bytes = bytes;
 			}
 			h_i32.emplace_back(M);
 			std::vector<int32_t>& blocks = h_i32.back();
@@ -3193,6 +3195,10 @@ sslm_status sslm_hip_seq_set_rules(sslm_seq seq, const sslm_hip_rules* rules) {
 }
 
 // ---- shared prompts ----
+static bool prefix_live(sslm_prefix prefix) {
+	std::lock_guard<std::mutex> g(g_registry_mu);
+	return g_live_prefixes.count(prefix) != 0;
+}
 sslm_status sslm_prefix_begin(sslm_model model, sslm_kv_pool* pool, sslm_prefix* out) {
 	if (!out) return SSLM_INVALID_ARGUMENT;
 	*out = nullptr;
@@ -3201,27 +3207,36 @@ sslm_status sslm_prefix_begin(sslm_model model, sslm_kv_pool* pool, sslm_prefix*
 	const sslm_status st = sslm_seq_create(model, pool, &p->seq);
 	if (st != SSLM_OK) return st;
 	p->model = model;
+	try {
+		std::lock_guard<std::mutex> g(g_registry_mu);
+		g_live_prefixes.insert(p.get());
+	} catch (const std::bad_alloc&) {
+		(void)sslm_seq_release(p->seq);
+		return SSLM_ALLOCATION_FAILED;
+	}
 	*out = p.release();
 	return SSLM_OK;
 }
 sslm_status sslm_prefix_prefill(sslm_model model, sslm_prefix prefix, const int32_t* tokens, int32_t count,
                                 int32_t chunk_budget, sslm_span_kind kind, sslm_workspace ws, int32_t* consumed) {
 	if (consumed) *consumed = 0;
-	if (!prefix || prefix->released) return SSLM_INVALID_ARGUMENT;
+	if (!prefix_live(prefix)) return SSLM_INVALID_ARGUMENT;
 	if (prefix->frozen) return SSLM_PREFIX_FROZEN_REJECTED;
 	return sslm_prefill(model, prefix->seq, tokens, count, chunk_budget, kind, ws, consumed);
 }
 sslm_status sslm_prefix_freeze(sslm_prefix prefix) {
-	if (!prefix || prefix->released) return SSLM_INVALID_ARGUMENT;
+	if (!prefix_live(prefix)) return SSLM_INVALID_ARGUMENT;
 	std::lock_guard<std::mutex> lk(prefix->model->mu);
 	prefix->frozen = true;
 	return SSLM_OK;
 }
 sslm_status sslm_prefix_release(sslm_prefix prefix) {
-	if (!prefix) return SSLM_INVALID_ARGUMENT;
+	{
+		std::lock_guard<std::mutex> g(g_registry_mu);
+		if (!g_live_prefixes.erase(prefix)) return SSLM_INVALID_ARGUMENT;
+	}
 	{
 		std::lock_guard<std::mutex> lk(prefix->model->mu);
-		if (prefix->released) return SSLM_INVALID_ARGUMENT;
 		prefix->released = true;
 		if (prefix->adopters > 0) return SSLM_OK;  // the last adopter takes it down
 	}
@@ -3230,7 +3245,7 @@ sslm_status sslm_prefix_release(sslm_prefix prefix) {
 // A fresh sequence of the prefix's pool takes over its state: context, stream row, clamp counter, schema
 // walk, and the K/V rows [0, context) of every layer and head.
 sslm_status sslm_seq_adopt_prefix(sslm_seq seq, sslm_prefix prefix) {
-	if (!seq || !prefix) return SSLM_INVALID_ARGUMENT;
+	if (!seq || !prefix_live(prefix)) return SSLM_INVALID_ARGUMENT;
 	sslm_model m = seq->model;
 	if (prefix->model != m) return SSLM_INVALID_ARGUMENT;
 	return guarded([&]() -> sslm_status {
@@ -3407,7 +3422,7 @@ sslm_status sslm_seq_set_schema(sslm_seq seq, sslm_schema schema) {
 	return SSLM_OK;
 }
 sslm_status sslm_prefix_set_schema(sslm_prefix prefix, sslm_schema schema) {
-	if (!prefix || prefix->released) return SSLM_INVALID_ARGUMENT;
+	if (!prefix_live(prefix)) return SSLM_INVALID_ARGUMENT;
 	return prefix->frozen ? SSLM_PREFIX_FROZEN_REJECTED : sslm_seq_set_schema(prefix->seq, schema);
 }
 sslm_status sslm_detokenize_stream(sslm_model, sslm_detok_state*, const int32_t*, int32_t, char*, int32_t* out_n) {

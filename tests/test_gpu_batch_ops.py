@@ -340,6 +340,20 @@ def test_lora_refuses_rows_by_their_status(ops, dev, host):
     b.check(host, got)
 
 
+@pytest.mark.parametrize("field", ["a", "ufold", "b", "dfold", "misaligned"])
+def test_lora_refuses_pointers_by_the_row(field, ops, dev, host):
+    b = LoraBatch(6, 4, 64, 64, [4, 8], [0, 1, -1, 1])
+
+    def edit(table):
+        if field == "misaligned":
+            table[1].a += 8
+        else:
+            setattr(table[1], field, None)
+
+    print("case lora pointers", field, flush=True)
+    b.check(host, b.run(ops, dev, edit=edit), refused=(1, 3))
+
+
 # ---- the next token under each row's rules ----
 class Pick:
     def __init__(self, seed, vocab, rows):

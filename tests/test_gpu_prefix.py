@@ -267,6 +267,36 @@ def test_prefix_refusals(hip_lib):
     model.close()
 
 
+def test_a_released_prefix_is_refused_everywhere(hip_lib):
+    model = Model(hip_lib, build_synthetic(CONFIGS["tiny"], seed=7).to_bytes())
+    pool = model.pool(2)
+    L = model.lib.lib
+    p, s = pool.prefix(), pool.seq()
+    h = p.handle
+    p.prefill([1, 2, 3])
+    p.freeze()
+    p.release()  # nobody adopted it: it is gone
+    assert L.sslm_prefix_release(h) == INVALID and L.sslm_prefix_freeze(h) == INVALID
+    assert L.sslm_prefix_set_schema(h, None) == INVALID and L.sslm_seq_adopt_prefix(s.handle, h) == INVALID
+    assert L.sslm_prefix_prefill(model.handle, h, None, 0, 1, 0, None, None) == INVALID
+    s.prefill([1])
+    assert model.decode_step([s], 2)[0] >= 0
+    s.release()
+    pool.close()
+    model.close()
+
+
+def test_shared_attention_over_prompts_of_growing_length(hip_lib, oracle_lib, monkeypatch):
+    """Units whose scratch grows from step to step while graphs of the smaller ones are kept and run again."""
+    monkeypatch.setenv("SSLM_HIP_SHARED_ATTN", "1")
+    batch = Batch(hip_lib, oracle_lib, built("kv4"), [5, 64, 65, 300, 520], [(i, 2, None) for i in range(5)] + [(4, 1, None)])
+    for _ in range(2):
+        for order in ([0], [0, 1], [2, 1], [3, 0], [4, 5], [0, 1, 2, 3, 4, 5], [0], [3, 0], [0, 1]):
+            batch.step(order=order)
+    batch.check_kv()
+    batch.close()
+
+
 def test_prefix_under_a_schema_and_reset(hip_lib, oracle_lib):
     """The walk goes with the prefix; a reset sequence lets go of it and is a fresh one."""
     table = {0: {t: 1 for t in range(0, 512, 2)}, 1: {t: 0 for t in range(1, 512, 2)}}
