@@ -163,6 +163,9 @@ __device__ __forceinline__ RowConst row_const(const sslm_launch::SharedAttnArgs&
 // rescaling of partial results is exact: three launches -- maxima, sums, P.V -- recompute the scores,
 // which cost 8 MFMAs a step of 64 positions at D = 128 where the i-exp of the step's scores costs some
 // hundreds of vector instructions, and integer sums join the planes exactly in any order.
+// 96 rows of 28 heads over 4 KV heads of 128, 4096 shared positions and 16 .. 384 own: maxima 9.2 us, sums 15.8,
+// P.V 25.0, join 6.1.  Bound by the vector instructions of i-exp and probability (issued back to back they take 3.0,
+// 7.6 and 11.5 us) at the two waves a SIMD that P.V's registers allow, and by each launch's chain of loads.
 struct SaPlan {
 	int tb;          // blocks of kSaWaves tiles of shared rows: at least those of every prefix together
 	int shared, sb;  // shared planes and the positions of one (a multiple of 64)
@@ -464,7 +467,8 @@ __device__ __forceinline__ void sa_own_steps(const SaJob& j, int8_t* lds, const 
 
 // The same over a shared plane, whose rows all waves of the block use: each thread loads its share of a step's
 // rows, AHEAD steps ahead, and stages it into one of two buffers, so a step costs one barrier (buffer b was
-// last read before the previous one).  LDS: 64 D bytes a buffer, K's two and then V's two.
+// last read before the previous one; waves that take different branches around this make equally many steps).
+// Sums of 96 rows over 4096: 15.8 us, 18.4 with each wave staging its own.  LDS: 64 D bytes a buffer, K's two and then V's two.
 template <int D, bool WITH_V, int NC, typename F>
 __device__ __forceinline__ void sa_block_steps(const SaJob& j, int8_t* lds, const v4i (&q)[NC], F&& step) {
 	constexpr int BS = 64 * kSaWaves, CH = 4 * D, PT = (CH + BS - 1) / BS, PER = D / 16, AHEAD = D <= 128 ? 2 : 1;
@@ -828,6 +832,9 @@ __global__ __launch_bounds__(BS) void k_sa_out(sslm_launch::SharedAttnArgs a, Sa
 // empty, columns 8 .. 15 hold the same heads at the next 64 positions (F = 2), by adding the products of
 // the second 64 with a query operand that is zero in the other half; the i-exp, which bounds the
 // kernel, then works on full waves.  K and V are read once per row here, from L2 for the prefix's.
+// 2 rows of 97 .. 105 positions 11.3 us, 16 of up to 609 18.4 (12 heads over 2 KV heads of 128); in the launches by
+// planes 18.8 and 24.1 of kernel time alone.  The chain of one wave's stages bounds it: span, constants, scores, maxima,
+// sums, probabilities and products, funnel.
 constexpr int kSaRowWaves = 8, kSaRowSteps = 2, kSaRowN = 4096;
 template <int D, int F, int NS>
 __global__ __launch_bounds__(64 * kSaRowWaves, 2) void k_sa_row(sslm_launch::SharedAttnArgs a) {
@@ -1070,7 +1077,9 @@ __global__ __launch_bounds__(64) void k_lora_table(const LoraRef* const* rows, i
 // bytes of its column's weights per 64-byte chunk (KC loads in flight, the weights being what has to be
 // read) against MB MFMA tiles of 16 rows, whose codes come from L2.  The waves' int32 sums are
 // joined in LDS and stored as plane blockIdx / tiles of [planes][m][n].  Blocks past the products' do
-// rows_u: 16 of them per row, four ranks each.
+// rows_u: 16 of them per row, four ranks each.  Bound by the chain of loads of a wave's share: 4 x 1536 x 1536 4.0 us,
+// 32 x 4864 x 896 5.7, 64 x 1536 x 8960 15.3 (16 MB of weights and adapters); as the decode GEMV and a launch of
+// k_rows_u 7.6, 9.6 and 29.5.
 template <int MB, int KC>
 __global__ __launch_bounds__(256) void k_lora_proj(sslm_launch::LoraGemmArgs g, int planes, int32_t* part, int8_t* u) {
 	__shared__ v4i s_acc[3][MB][64];
@@ -1282,8 +1291,10 @@ __device__ __forceinline__ int32_t pick_of(uint64_t key) { return key ? (int32_t
 // One block per (slice of the vocabulary, row).  Histories and biases touch few of a slice's tokens, so the
 // rules' 64-bit arithmetic and its division run over those alone: counts, bias sums and a bit per touched token
 // are gathered in LDS while the logits are in flight, and a thread takes its touched tokens one by one.  Bound by
-// the logits' traffic: a thread's are 16-byte loads and stores (VEC: rows 16-byte aligned), the row's history (read by every
-// slice of it, from L2) four loads at a time.  With one slice to a row the block writes the token itself.
+// the logits' traffic: a thread's are 16-byte loads and stores (VEC: rows 16-byte aligned), the row's history
+// (read by every slice of it, from L2) four loads at a time.  16 rows of 151936 7.4 us, 128 with histories of 3000
+// 40.9 (154 MB: 3.8 TB/s; 47.3 with the arithmetic over every token).  With one slice to a row the block writes
+// the token itself.
 template <bool VEC>
 __global__ __launch_bounds__(kPickBlock) void k_pick_slice(sslm_launch::PickArgs a, unsigned long long* keys) {
 	__shared__ __attribute__((aligned(16))) int32_t s_cnt[kPickSlice];
@@ -1444,7 +1455,8 @@ bool shared_attn_ok(int rows, int NH, int NKV, int D) {
 	       (int64_t)NH * D <= kFunnelMaxN;
 }
 
-// Planes: enough waves for the chip's 1024 SIMDs, a plane at least one step of 64 positions.
+// Planes: enough waves for the chip's 1024 SIMDs, a plane at least one step of 64 positions.  The three launches
+// of 96 rows over 4096 positions at kSaTargetWaves 1024, 1536 and 2048: 60, 52 and 59 us.
 static SaPlan sa_plan(int rows, int NH, int NKV, int prefixes, int64_t max_prefix, int64_t max_own) {
 	SaPlan p{};
 	const int G = NH / NKV;
@@ -1483,7 +1495,8 @@ static size_t sa_work(const SaPlan& p, int rows, int NH, int NKV, int D, char* b
 	return at;
 }
 
-// Steps of a wave of k_sa_row, 0 where it does not take the call.
+// Steps of a wave of k_sa_row, 0 where it does not take the call: more heads, dims or steps than its registers
+// hold (a third step spills), the times on either side at the kernel.
 static int sa_row_steps(int NH, int NKV, int D, int prefixes, int64_t max_prefix, int64_t max_own) {
 	const int G = NH / NKV;
 	if (NKV > kSaRowWaves || kSaRowWaves % NKV || G > 16 || NH * D > kSaRowN || D > 128) return 0;
@@ -1536,7 +1549,8 @@ void shared_attn(const SharedAttnArgs& a, hipStream_t s) {
 }
 
 // Planes of k_lora_proj (a power of two): a wave's share of K at most ten chunks of 64 bytes, where that
-// takes more than one plane (their sums are read back by the funnel).
+// takes more than one plane (their sums are read back by the funnel).  64 x 1536 x 8960: 15.3 us in the four planes
+// that ten chunks give, 16.2 in eight, 24.5 in one.
 static int lora_planes(int k) {
 	int p = 1;
 	while (p < 8 && (k + 63) / 64 > 40 * p) p *= 2;
