@@ -219,6 +219,31 @@ def test_attention_refuses_rows_by_their_status(ops, dev, host):
     a.check(host, got, expect={0: ref.POSITION_OVER_CAP, 2: ref.POSITION_OVER_CAP})
 
 
+@pytest.mark.parametrize("runs,widths", [([(40, 2)], [45, 130, 7]), ([(1900, 3)], [1950, 2100, 1901, 800])])
+def test_attention_in_a_pool_past_32_bits(runs, widths, ops, dev, host):
+    """Blocks of 512 MB: heads, V and blocks lie past 2^31 and 2^32 bytes; one-launch rows and planes."""
+    b = Attention(21, 12, 2, 128, runs, widths)
+    cap = 1 << 20
+    half = 2 * cap * 128
+    alloc, copy = ops.lib.lib.sslm_hip_device_alloc, ops.lib.lib.sslm_hip_copy
+    used = sorted({*b.row_block.tolist(), *b.prefix_block.tolist()})
+    far = {blk: 9 - i for i, blk in enumerate(reversed(used))}  # the last blocks of ten
+    pool = alloc(10 * 2 * half)
+    assert pool
+    try:
+        for blk, at in far.items():
+            for kv in range(2):
+                for h in range(2):
+                    rows = np.ascontiguousarray(b.pool[blk, kv, h])
+                    assert copy(pool + at * 2 * half + kv * half + h * cap * 128, rows.ctypes.data, rows.nbytes, 0) == 0
+        row_block, prefix_block = (dev.upload(np.array([far[x] for x in v.tolist()], np.int32)) for v in (b.row_block, b.prefix_block))
+        print("case pool past 32 bits", runs, flush=True)
+        b.check(host, b.run(ops, dev, kv_pool=pool, block_bytes=2 * half, v_offset=half, cap=cap, blocks=10,
+                            row_block=row_block.ptr, prefix_block=prefix_block.ptr))
+    finally:
+        ops.lib.lib.sslm_hip_device_free(pool)
+
+
 # ---- a projection with an adapter of its own per row ----
 def make_adapter(rng, rank, n, k):
     mid = int(round(np.log2(max(2.0, 0.75 * 127 * 73 * k ** 0.5 / 40.0))))
@@ -413,6 +438,38 @@ class Pick:
             assert tokens[r] == tok, (r, tokens[r], tok)
             assert np.array_equal(out[r, :self.vocab], x), r
             assert (out[r, self.vocab:] == (2 ** 31 - 1 if out.shape[1] > self.vocab and out[r, -1] != LEFT else LEFT)).all()
+
+
+def test_pick_rows_past_32_bits(ops, dev):
+    """A row stride of 2^30 logits: the third row begins 8 GB in."""
+    p = Pick(31, 5000, [dict(history=[3, 4999], presence=7), dict(), dict(history=[17] * 5, frequency=90000, mask=range(0, 5000, 3))])
+    ld, alloc, copy = 1 << 30, ops.lib.lib.sslm_hip_device_alloc, ops.lib.lib.sslm_hip_copy
+    logits = alloc((2 * ld + p.vocab) * 4)
+    assert logits
+    try:
+        for r in range(3):
+            row = np.ascontiguousarray(p.logits[r])
+            assert copy(logits + r * ld * 4, row.ctypes.data, row.nbytes, 0) == 0
+        hist = [dev.upload(np.array(u.get("history", [0]), np.int32)) for u in p.rules]
+        mask = dev.upload(p.mask(2))
+        table = (LogitRule * 3)(*[LogitRule(h.ptr, None, None, mask.ptr if r == 2 else None, len(u.get("history", [])), 0, 65536,
+                                            u.get("presence", 0), u.get("frequency", 0), 0)
+                                  for r, (h, u) in enumerate(zip(hist, p.rules))])
+        dt, tokens = dev.upload(np.frombuffer(bytes(table), np.uint8)), dev.upload(np.full(3, LEFT, np.int32))
+        need = ops.pick_workspace(3, p.vocab)
+        ws = dev.upload(np.zeros(need, np.uint8))
+        print("case rows past 32 bits", flush=True)
+        ops.pick_tokens(workspace=ws.ptr, workspace_bytes=need, rows=3, vocab=p.vocab, logits=logits, logits_ld=ld, rules=dt.ptr,
+                        tokens=tokens.ptr, adjusted=logits, adjusted_ld=ld)()
+        sync(ops)
+        for r, u in enumerate(p.rules):
+            tok, x = ref.pick_row(p.logits[r], np.array(u.get("history", []), np.int64), [], p.mask(r), 65536,
+                                  u.get("presence", 0), u.get("frequency", 0))
+            out = np.empty(p.vocab, np.int32)
+            assert copy(out.ctypes.data, logits + r * ld * 4, out.nbytes, 1) == 0
+            assert tokens.numpy()[r] == tok and np.array_equal(out, x), r
+    finally:
+        ops.lib.lib.sslm_hip_device_free(logits)
 
 
 def some_rules(seed, vocab, rows):
