@@ -3,6 +3,7 @@
 #include <stdio.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "../../include/sslm_hip.h"
@@ -413,7 +414,9 @@ __device__ __forceinline__ double sa_exp(const SaExp& e, int32_t score) {
 	return floor(ldexp(fma(base, base, e.qc), -(int)z));
 }
 
-// the wave's rows joined over their planes; a lane's row is read by the lanes ri, ri + 16, ri + 32, ri + 48
+// The wave's rows joined over their planes; a lane's row is read by the lanes ri, ri + 16, ri + 32, ri + 48,
+// kSaJoin planes each in flight.
+constexpr int kSaJoin = 8;
 __device__ __forceinline__ int sa_plane_count(const SaPlan& pl, const SaJob& j, int* shared) {
 	const int64_t own = j.width - j.start;
 	*shared = (int)((j.start + pl.sb - 1) / pl.sb);
@@ -423,7 +426,16 @@ __device__ __forceinline__ int32_t sa_row_max(const sslm_launch::SharedAttnArgs&
 	int sh, m = INT32_MIN;
 	const int n = live ? sa_plane_count(pl, j, &sh) : 0;
 	const int32_t* at = w.pmax + (size_t)(live ? j.r : 0) * a.NH + j.h;
-	for (int i = (threadIdx.x & 63) >> 4; i < n; i += 4) m = max(m, at[(size_t)(i < sh ? i : pl.shared + i - sh) * a.rows * a.NH]);
+	for (int i = (threadIdx.x & 63) >> 4; i < n; i += 4 * kSaJoin) {
+		int32_t x[kSaJoin];
+#pragma unroll
+		for (int e = 0; e < kSaJoin; ++e) {
+			const int k = min(i + 4 * e, n - 1);
+			x[e] = at[(size_t)(k < sh ? k : pl.shared + k - sh) * a.rows * a.NH];
+		}
+#pragma unroll
+		for (int e = 0; e < kSaJoin; ++e) m = max(m, x[e]);  // the last plane may count twice
+	}
 	m = max(m, __shfl_xor(m, 16, 64));
 	return max(m, __shfl_xor(m, 32, 64));
 }
@@ -433,10 +445,19 @@ __device__ __forceinline__ int64_t sa_row_sum(const sslm_launch::SharedAttnArgs&
 	int64_t m = 0;
 	const int n = live ? sa_plane_count(pl, j, &sh) : 0;
 	const int64_t* at = w.psum + (size_t)(live ? j.r : 0) * a.NH + j.h;
-	for (int i = (threadIdx.x & 63) >> 4; i < n; i += 4) {
-		const int64_t x = at[(size_t)(i < sh ? i : pl.shared + i - sh) * a.rows * a.NH];
-		bad |= x < 0;
-		m += x < 0 ? 0 : x;
+	for (int i = (threadIdx.x & 63) >> 4; i < n; i += 4 * kSaJoin) {
+		int64_t x[kSaJoin];
+#pragma unroll
+		for (int e = 0; e < kSaJoin; ++e) {
+			const int k = min(i + 4 * e, n - 1);
+			x[e] = at[(size_t)(k < sh ? k : pl.shared + k - sh) * a.rows * a.NH];
+		}
+#pragma unroll
+		for (int e = 0; e < kSaJoin; ++e)
+			if (i + 4 * e < n) {
+				bad |= x[e] < 0;
+				m += x[e] < 0 ? 0 : x[e];
+			}
 	}
 	for (int o = 16; o < 64; o *= 2) {
 		m += __shfl_xor(m, o, 64);
@@ -1455,6 +1476,11 @@ bool shared_attn_ok(int rows, int NH, int NKV, int D) {
 	       (int64_t)NH * D <= kFunnelMaxN;
 }
 
+// The most planes of so many steps: they are cut in time and joined by every later launch, and the sum of both is
+// least at a count that grows with the root of the steps.  The four launches, so and in as many planes as fill the
+// chip: one row of 8 heads over 8000 positions of 128 27.6 and 34.4 us, 2 rows of 12 over 96000 71 and 198.
+static int64_t sa_most_planes(int64_t steps) { return std::min<int64_t>(steps, std::max<int64_t>(1, (int64_t)std::sqrt(16.0 * (double)steps))); }
+
 // Planes: enough waves for the chip's 1024 SIMDs, a plane at least one step of 64 positions.  The three launches
 // of 96 rows over 4096 positions at kSaTargetWaves 1024, 1536 and 2048: 60, 52 and 59 us.
 static SaPlan sa_plan(int rows, int NH, int NKV, int prefixes, int64_t max_prefix, int64_t max_own) {
@@ -1463,7 +1489,7 @@ static SaPlan sa_plan(int rows, int NH, int NKV, int prefixes, int64_t max_prefi
 	p.tb = prefixes > 0 && max_prefix > 0 ? rows * G / (16 * kSaWaves) + prefixes : 0;
 	const int64_t steps = (max_prefix + 63) / 64, jobs = std::min<int64_t>((int64_t)p.tb * kSaWaves, (int64_t)rows * G / 16 + prefixes) * NKV;
 	if (jobs > 0) {
-		const int64_t want = std::min<int64_t>(steps, std::max<int64_t>(1, (kSaTargetWaves + jobs - 1) / jobs));
+		const int64_t want = std::min<int64_t>(sa_most_planes(steps), std::max<int64_t>(1, (kSaTargetWaves + jobs - 1) / jobs));
 		p.sb = (int)((steps + want - 1) / want) * 64;
 		p.shared = (int)((max_prefix + p.sb - 1) / p.sb);
 	} else {
@@ -1471,7 +1497,7 @@ static SaPlan sa_plan(int rows, int NH, int NKV, int prefixes, int64_t max_prefi
 	}
 	p.ht = (G + 15) / 16;
 	const int64_t osteps = std::max<int64_t>(1, (max_own + 63) / 64), ojobs = (int64_t)rows * NKV * p.ht;
-	const int64_t owant = std::min<int64_t>(osteps, std::max<int64_t>(1, (kSaTargetWaves + ojobs - 1) / ojobs));
+	const int64_t owant = std::min<int64_t>(sa_most_planes(osteps), std::max<int64_t>(1, (kSaTargetWaves + ojobs - 1) / ojobs));
 	p.ob = (int)((osteps + owant - 1) / owant) * 64;
 	p.owned = (int)std::max<int64_t>(1, (max_own + p.ob - 1) / p.ob);
 	p.shared_blocks = (NKV * p.shared + 7) / 8 * 8 * p.tb;

@@ -219,6 +219,12 @@ def test_attention_refuses_rows_by_their_status(ops, dev, host):
     a.check(host, got, expect={0: ref.POSITION_OVER_CAP, 2: ref.POSITION_OVER_CAP})
 
 
+@pytest.mark.parametrize("runs,widths", [([(9001, 2)], [9051, 9010]), ([], [9001]), ([(20000, 1)], [29000])])
+def test_attention_of_few_rows_over_many_planes(runs, widths, ops, dev, host):
+    b = Attention(23, 4, 1, 32, runs, widths, scale=4e-5)
+    b.check(host, b.run(ops, dev))
+
+
 @pytest.mark.parametrize("runs,widths", [([(40, 2)], [45, 130, 7]), ([(1900, 3)], [1950, 2100, 1901, 800])])
 def test_attention_in_a_pool_past_32_bits(runs, widths, ops, dev, host):
     """Blocks of 512 MB: heads, V and blocks lie past 2^31 and 2^32 bytes; one-launch rows and planes."""
