@@ -43,9 +43,9 @@ constexpr int kSlicedActPrefillRows = 32;
 // The attention of one block per (row, KV head) passes over its row alone, so its time is the longest row's
 // positions, once more where the blocks pass the CUs.  A unit with adopted prefixes reads them shared and cut
 // over the whole chip from this many positions on, and always with more blocks than CUs (a step of four layers
-// of the 7B shape, shared against not: 16 rows of 2080 positions 0.741 / 0.694 ms, 16 of 4128 0.749 / 0.786, 64
-// of 1632 0.934 / 0.910, 64 of 4196 0.97 / 1.88; 96 of 32 positions 0.945 / 0.984, 96 of 1056 1.05 / 1.26).
-constexpr int64_t kSharedPositions = 3500;
+// of the 7B shape, shared against not: 32 rows of 2080 positions 0.775 / 0.758 ms, of 2432 0.798 / 0.786, of 2832
+// 0.797 / 0.808, 64 of 4196 0.95 / 1.88; 96 of 32 positions 0.945 / 0.984, 96 of 1056 1.05 / 1.26).
+constexpr int64_t kSharedPositions = 2600;
 
 struct HipError {
 	hipError_t e;
