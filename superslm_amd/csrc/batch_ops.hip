@@ -14,32 +14,6 @@ namespace sslm {
 
 using sslm_launch::LogitRule;
 
-template <int BS>
-__device__ __forceinline__ int64_t block_sum_i64(int64_t v, int64_t* slots) {
-	for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-	if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
-	__syncthreads();
-	int64_t r = 0;
-#pragma unroll
-	for (int i = 0; i < BS / 64; ++i) r += slots[i];
-	return r;
-}
-
-template <int BS>
-__device__ __forceinline__ uint32_t block_max_u32(uint32_t v, uint32_t* slots) {
-	v = wave_max32(v);
-	if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
-	__syncthreads();
-	uint32_t r = slots[0];
-#pragma unroll
-	for (int i = 1; i < BS / 64; ++i) r = max(r, slots[i]);
-	return __builtin_amdgcn_readfirstlane(r);
-}
-
-// ------------------------------------------------------------------------------------------
-// attention of rows that share prompts
-// ------------------------------------------------------------------------------------------
-
 // A pointer that was read from memory is generic to the compiler, whose flat loads count as LDS operations
 // too: each wait for LDS would then be one for every load in flight.  All of these point to global memory.
 template <typename T>
@@ -54,6 +28,10 @@ struct __attribute__((packed)) unaligned16 {
 struct __attribute__((packed)) unaligned4 {
 	int32_t v;
 };
+
+// ------------------------------------------------------------------------------------------
+// attention of rows that share prompts
+// ------------------------------------------------------------------------------------------
 
 // Where a row's positions lie: [0, start) in its prefix's block, [start, width) in its own.
 struct RowSpan {
@@ -204,7 +182,6 @@ struct SaJob {
 };
 
 __device__ __forceinline__ int64_t i64min(int64_t a, int64_t b) { return a < b ? a : b; }
-__device__ __forceinline__ int64_t i64max(int64_t a, int64_t b) { return a > b ? a : b; }
 
 // A wave of the shared planes: false, for its whole block, when there is nothing to do.  A block's waves have
 // neighbouring tiles of one prefix and the same positions; a wave past the last tile has no live lane.
