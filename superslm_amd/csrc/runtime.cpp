@@ -2675,8 +2675,10 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 					                                   std::to_string(sslm_launch::group_row_halves(
 					                                       (int)un.idx.size(), m->NKV, m->NH / m->NKV))
 					                             : "") +
+					                        // with the block count: another pool may lie at the address of one that is gone
 					                        (un.prefixes.empty() ? "" : "|s" + std::to_string(un.prefixes.size()) + "," +
-					                                                        std::to_string(un.max_prefix) + "," + std::to_string(un.max_own));
+					                                                        std::to_string(un.max_prefix) + "," + std::to_string(un.max_own) + "," +
+					                                                        std::to_string(m->pool_blocks));
 					capturing = true;
 					const hipGraphExec_t ge = graph_of(m, key, w.stream, [&] { launch_unit(u); });
 					capturing = false;
