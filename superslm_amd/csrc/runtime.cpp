@@ -419,7 +419,8 @@ struct sslm_seq_s {
 	uint32_t walk = 0xFFFFFFFFu;        // DFA walk state (0xFFFFFFFF: no schema bound)
 	std::vector<int32_t> context;       // the tokens taken in and produced, what token rules count
 	std::unique_ptr<SeqRules> rules;
-	sslm_prefix prefix = nullptr;       // the adopted prompt: positions below prefix->seq's context are its
+	sslm_prefix prefix = nullptr;       // the adopted prompt, whose block holds positions [0, adopted) too
+	int64_t adopted = 0;
 	std::mutex mu;
 };
 
@@ -429,8 +430,8 @@ struct sslm_seq_s {
 struct sslm_prefix_s {
 	sslm_model model = nullptr;
 	sslm_seq seq = nullptr;
-	bool frozen = false, released = false;
-	int adopters = 0;  // under model->mu
+	bool frozen = false, released = false;  // these and `adopters` under model->mu
+	int adopters = 0;
 };
 
 struct sslm_workspace_s {
@@ -1370,6 +1371,25 @@ sslm_status map_forward_status(int32_t word) {
 	return SSLM_ARTIFACT_REJECTED;  // src/sslm_abi.cpp:1352-1360
 }
 
+// A prefix is used only where it is found live with its model's mutex held: its release takes it from the
+// registry first and waits for the mutex before anything of it goes.
+bool prefix_live(sslm_prefix prefix) {
+	std::lock_guard<std::mutex> g(g_registry_mu);
+	return g_live_prefixes.count(prefix) != 0;
+}
+// `f` with the prefix's model locked; refused unless the prefix is live.
+template <typename F>
+sslm_status with_prefix(sslm_prefix prefix, F&& f) {
+	sslm_model m = nullptr;
+	{
+		std::lock_guard<std::mutex> g(g_registry_mu);
+		if (!g_live_prefixes.count(prefix)) return SSLM_INVALID_ARGUMENT;
+		m = prefix->model;
+	}
+	std::lock_guard<std::mutex> lk(m->mu);
+	return prefix_live(prefix) && prefix->model == m ? f() : SSLM_INVALID_ARGUMENT;
+}
+
 // Runs an entry point's body, turning HIP errors and refused launches into statuses.  `refused`:
 // the status of a launch refused by a launch wrapper (SSLM_INVALID_ARGUMENT at the boundary;
 // the forward verbs pass SSLM_NUMERIC_STEP_REFUSED and leave every sequence's state as it was).
@@ -2164,6 +2184,7 @@ sslm_status sslm_seq_create(sslm_model model, sslm_kv_pool* pool, sslm_seq* out)
 static sslm_prefix unref_prefix(sslm_seq seq) {
 	const sslm_prefix p = seq->prefix;
 	seq->prefix = nullptr;
+	seq->adopted = 0;
 	return p && --p->adopters == 0 && p->released ? p : nullptr;
 }
 static sslm_status destroy_prefix(sslm_prefix p) {
@@ -2226,17 +2247,19 @@ sslm_status sslm_seq_reset(sslm_seq seq) {
 	return st;
 }
 
-sslm_status sslm_prefill(sslm_model model, sslm_seq seq, const int32_t* tokens, int32_t count, int32_t chunk_budget,
-                         sslm_span_kind kind, sslm_workspace ws, int32_t* consumed) {
-	(void)ws;
+static sslm_status prefill_args(sslm_model model, sslm_seq seq, const int32_t* tokens, int32_t count, int32_t chunk_budget,
+                                sslm_span_kind kind, int32_t* consumed) {
 	if (!consumed) return SSLM_INVALID_ARGUMENT;
 	*consumed = 0;
 	if (!model || !seq) return SSLM_INVALID_ARGUMENT;
 	if (count < 0 || chunk_budget < 1 || (count > 0 && !tokens)) return SSLM_INVALID_ARGUMENT;
 	if (kind == SSLM_SPAN_SCHEMA_CONTENT && !seq->schema) return SSLM_SCHEMA_SPAN_UNBOUND;
-	if (seq->model != model) return SSLM_INVALID_ARGUMENT;
+	return seq->model == model ? SSLM_OK : SSLM_INVALID_ARGUMENT;
+}
+// model->mu held
+static sslm_status prefill_locked(sslm_model model, sslm_seq seq, const int32_t* tokens, int32_t count, int32_t chunk_budget,
+                                  sslm_span_kind kind, int32_t* consumed) {
 	return guarded([&]() -> sslm_status {
-		std::lock_guard<std::mutex> lk(model->mu);
 		std::lock_guard<std::mutex> sl(seq->mu);
 		const int32_t n = std::min(count, chunk_budget);
 		if (n == 0) return SSLM_OK;
@@ -2286,6 +2309,15 @@ sslm_status sslm_prefill(sslm_model model, sslm_seq seq, const int32_t* tokens, 
 		}
 		return stop;
 	}, SSLM_NUMERIC_STEP_REFUSED);
+}
+
+sslm_status sslm_prefill(sslm_model model, sslm_seq seq, const int32_t* tokens, int32_t count, int32_t chunk_budget,
+                         sslm_span_kind kind, sslm_workspace ws, int32_t* consumed) {
+	(void)ws;
+	const sslm_status st = prefill_args(model, seq, tokens, count, chunk_budget, kind, consumed);
+	if (st != SSLM_OK) return st;
+	std::lock_guard<std::mutex> lk(model->mu);
+	return prefill_locked(model, seq, tokens, count, chunk_budget, kind, consumed);
 }
 
 sslm_launch::SlotCopyArgs slot_copy_args(sslm_model m, const TokenInfo* tok, int l0, int l1) {
@@ -2346,10 +2378,10 @@ static void share_prompts(sslm_model m, sslm_seq* seqs, std::vector<int>* idx, s
 	auto where = [&](int i) { return std::find(ps.begin(), ps.end(), seqs[i]->prefix) - ps.begin(); };
 	const char* e = getenv("SSLM_HIP_SHARED_ATTN");
 	int64_t longest = 0, own = 0, width = 0;
-	for (sslm_prefix p : ps) longest = std::max(longest, p->seq->context_length);
 	for (int i : *idx) {
 		width = std::max(width, seqs[i]->context_length + 1);
-		own = std::max(own, seqs[i]->context_length + 1 - (seqs[i]->prefix ? seqs[i]->prefix->seq->context_length : 0));
+		own = std::max(own, seqs[i]->context_length + 1 - seqs[i]->adopted);
+		longest = std::max(longest, seqs[i]->adopted);
 	}
 	const int64_t blocks = (int64_t)idx->size() * m->NKV;
 	if (e && (e[0] == '0' || e[0] == '1') ? e[0] == '0' : width < kSharedPositions && blocks <= sslm_launch::device_cus()) return;
@@ -2507,9 +2539,9 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 			std::vector<int32_t>& pb = h_i32.back();
 			h_i64.emplace_back();
 			std::vector<int64_t>& pl = h_i64.back();
-			for (sslm_prefix p : un.prefixes) {
-				pb.push_back((int32_t)p->seq->block);
-				pl.push_back(p->seq->context_length);
+			for (size_t k = 0; k < un.prefixes.size(); ++k) {
+				pb.push_back((int32_t)un.prefixes[k]->seq->block);
+				pl.push_back(seqs[un.idx[un.prefix_rows[k]]]->adopted);  // its first sequence's, as all of theirs
 			}
 			ck(hipMemcpyAsync(w.shared.row_block, blocks.data(), M * 4, hipMemcpyHostToDevice, s));
 			ck(hipMemcpyAsync(w.shared.row_width, widths.data(), M * 8, hipMemcpyHostToDevice, s));
@@ -3197,10 +3229,6 @@ sslm_status sslm_hip_seq_set_rules(sslm_seq seq, const sslm_hip_rules* rules) {
 }
 
 // ---- shared prompts ----
-static bool prefix_live(sslm_prefix prefix) {
-	std::lock_guard<std::mutex> g(g_registry_mu);
-	return g_live_prefixes.count(prefix) != 0;
-}
 sslm_status sslm_prefix_begin(sslm_model model, sslm_kv_pool* pool, sslm_prefix* out) {
 	if (!out) return SSLM_INVALID_ARGUMENT;
 	*out = nullptr;
@@ -3221,16 +3249,19 @@ sslm_status sslm_prefix_begin(sslm_model model, sslm_kv_pool* pool, sslm_prefix*
 }
 sslm_status sslm_prefix_prefill(sslm_model model, sslm_prefix prefix, const int32_t* tokens, int32_t count,
                                 int32_t chunk_budget, sslm_span_kind kind, sslm_workspace ws, int32_t* consumed) {
+	(void)ws;
 	if (consumed) *consumed = 0;
-	if (!prefix_live(prefix)) return SSLM_INVALID_ARGUMENT;
-	if (prefix->frozen) return SSLM_PREFIX_FROZEN_REJECTED;
-	return sslm_prefill(model, prefix->seq, tokens, count, chunk_budget, kind, ws, consumed);
+	return with_prefix(prefix, [&] {
+		if (prefix->frozen) return SSLM_PREFIX_FROZEN_REJECTED;
+		const sslm_status st = prefill_args(model, prefix->seq, tokens, count, chunk_budget, kind, consumed);
+		return st != SSLM_OK ? st : prefill_locked(model, prefix->seq, tokens, count, chunk_budget, kind, consumed);
+	});
 }
 sslm_status sslm_prefix_freeze(sslm_prefix prefix) {
-	if (!prefix_live(prefix)) return SSLM_INVALID_ARGUMENT;
-	std::lock_guard<std::mutex> lk(prefix->model->mu);
-	prefix->frozen = true;
-	return SSLM_OK;
+	return with_prefix(prefix, [&] {
+		prefix->frozen = true;
+		return SSLM_OK;
+	});
 }
 sslm_status sslm_prefix_release(sslm_prefix prefix) {
 	{
@@ -3247,13 +3278,13 @@ sslm_status sslm_prefix_release(sslm_prefix prefix) {
 // A fresh sequence of the prefix's pool takes over its state: context, stream row, clamp counter, schema
 // walk, and the K/V rows [0, context) of every layer and head.
 sslm_status sslm_seq_adopt_prefix(sslm_seq seq, sslm_prefix prefix) {
-	if (!seq || !prefix_live(prefix)) return SSLM_INVALID_ARGUMENT;
+	if (!seq) return SSLM_INVALID_ARGUMENT;
 	sslm_model m = seq->model;
-	if (prefix->model != m) return SSLM_INVALID_ARGUMENT;
 	return guarded([&]() -> sslm_status {
 		std::lock_guard<std::mutex> lk(m->mu);
+		if (!prefix_live(prefix) || prefix->model != m) return SSLM_INVALID_ARGUMENT;
 		const sslm_seq from = prefix->seq;
-		if (!prefix->frozen || prefix->released || from->pool != seq->pool || seq->prefix || seq->context_length != 0 ||
+		if (!prefix->frozen || from->pool != seq->pool || seq->prefix || seq->context_length != 0 ||
 		    seq->layer_index != 0 || seq->current_token != -1 || seq->ready_for_logits)
 			return SSLM_INVALID_ARGUMENT;
 		if (seq->schema != from->schema) return SSLM_PREFIX_SCHEMA_MISMATCH;
@@ -3275,6 +3306,7 @@ sslm_status sslm_seq_adopt_prefix(sslm_seq seq, sslm_prefix prefix) {
 		seq->forced_token_count = from->forced_token_count;
 		seq->walk = from->walk;
 		seq->prefix = prefix;
+		seq->adopted = from->context_length;
 		++prefix->adopters;
 		return SSLM_OK;
 	});
@@ -3424,8 +3456,7 @@ sslm_status sslm_seq_set_schema(sslm_seq seq, sslm_schema schema) {
 	return SSLM_OK;
 }
 sslm_status sslm_prefix_set_schema(sslm_prefix prefix, sslm_schema schema) {
-	if (!prefix_live(prefix)) return SSLM_INVALID_ARGUMENT;
-	return prefix->frozen ? SSLM_PREFIX_FROZEN_REJECTED : sslm_seq_set_schema(prefix->seq, schema);
+	return with_prefix(prefix, [&] { return prefix->frozen ? SSLM_PREFIX_FROZEN_REJECTED : sslm_seq_set_schema(prefix->seq, schema); });
 }
 sslm_status sslm_detokenize_stream(sslm_model, sslm_detok_state*, const int32_t*, int32_t, char*, int32_t* out_n) {
 	if (out_n) *out_n = 0;
