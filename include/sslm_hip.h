@@ -172,8 +172,8 @@ sslm_status sslm_g5_test_only_peek_kv_block_bytes(sslm_kv_pool pool, uint32_t bl
  * same schema bound (else SSLM_PREFIX_SCHEMA_MISMATCH), adopts a frozen prefix: its tokens, KV block, blob
  * and every later result are those of a sequence that took the prompt itself.  Decode steps then read the
  * prompt's K/V once for all of the batch's adopters (sslm_hip_shared_attention) where that is the faster
- * form.  Anything else -- a prefix not frozen, a sequence that holds context, another pool -- is refused
- * (SSLM_INVALID_ARGUMENT).  A released prefix keeps its block until its last adopter is released or reset. */
+ * form.  Anything else -- a prefix not frozen, a sequence that holds context or has an adapter (it may be given
+ * one afterwards, for what follows the prompt), another pool -- is refused (SSLM_INVALID_ARGUMENT).  A released prefix keeps its block until its last adopter is released or reset. */
 sslm_status sslm_prefix_begin(sslm_model model, sslm_kv_pool* pool, sslm_prefix* out);
 sslm_status sslm_prefix_prefill(sslm_model model, sslm_prefix prefix, const int32_t* tokens, int32_t count,
                                 int32_t chunk_budget, sslm_span_kind kind, sslm_workspace ws, int32_t* consumed);

@@ -3284,7 +3284,8 @@ sslm_status sslm_seq_adopt_prefix(sslm_seq seq, sslm_prefix prefix) {
 		std::lock_guard<std::mutex> lk(m->mu);
 		if (!prefix_live(prefix) || prefix->model != m) return SSLM_INVALID_ARGUMENT;
 		const sslm_seq from = prefix->seq;
-		if (!prefix->frozen || from->pool != seq->pool || seq->prefix || seq->context_length != 0 ||
+		// an adapter would have shaped the prompt's K/V, which the prefix has without one
+		if (!prefix->frozen || from->pool != seq->pool || seq->prefix || seq->adapter || seq->context_length != 0 ||
 		    seq->layer_index != 0 || seq->current_token != -1 || seq->ready_for_logits)
 			return SSLM_INVALID_ARGUMENT;
 		if (seq->schema != from->schema) return SSLM_PREFIX_SCHEMA_MISMATCH;

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from superslm_amd.sslm import Model
-from superslm_amd.sslm_artifact import CONFIGS, ModelConfig, build_synthetic
+from superslm_amd.sslm_artifact import CONFIGS, ModelConfig, build_adapter, build_synthetic
 
 pytestmark = pytest.mark.gpu
 
@@ -134,5 +134,39 @@ def test_prefix_verbs_against_a_release(hip_lib):
             s.release()
         for s in [pool.seq() for _ in range(5)]:
             s.release()
+    pool.close()
+    model.close()
+
+
+def test_a_sequence_with_an_adapter_does_not_adopt(hip_lib):
+    """Its prompt's K/V would be without the adapter.  Refused, the sequence is still fresh: it takes the prompt
+    itself, or adopts once the adapter is gone and may have it back for what follows."""
+    sm = build_synthetic(CONFIGS["tiny"], seed=7)
+    model = Model(hip_lib, sm.to_bytes())
+    pool, prompt = model.pool(5), [7, 8, 9, 10]
+    ad = model.adapter(build_adapter(sm, rank=16, targets=("q_proj", "k_proj", "v_proj"), seed=1))
+    p = pool.prefix()
+    p.prefill(prompt)
+    p.freeze()
+    a, b, plain = (pool.seq() for _ in range(3))  # blocks 3, 2 and 1
+    print("case adapter before adoption", flush=True)
+    for s in (a, b):
+        s.set_adapter(ad)
+        assert s.adopt(p, raw=True) == INVALID and context_length(s) == 0
+    a.prefill(prompt)  # with its adapter
+    plain.prefill(prompt)
+    assert not np.array_equal(pool.kv_block(3), pool.kv_block(1))
+    b.set_adapter(None)
+    b.adopt(p)
+    assert b.save() == plain.save()
+    for s in (b, plain):
+        s.set_adapter(ad)
+        s.prefill([3, 4])
+    assert [model.decode_step([b], 2) for _ in range(3)] == [model.decode_step([plain], 2) for _ in range(3)]
+    assert b.save() == plain.save()
+    for s in (a, b, plain):
+        s.release()
+    p.release()
+    ad.release()
     pool.close()
     model.close()
