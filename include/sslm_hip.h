@@ -329,7 +329,8 @@ sslm_status sslm_hip_seq_set_rules(sslm_seq seq, const sslm_hip_rules* rules);
  * read once for all of its rows.  Blocks are the KV pool's: `blocks` of block_bytes bytes from kv_pool, K
  * (V) of (KV head, position) at block + k_offset (v_offset) + (KV head * cap + position) * head_dim.
  * Rows [prefix_rows[p], prefix_rows[p + 1]) have prefix p in block prefix_block[p]; rows outside every
- * run have none.  heads / kv_heads query heads share a KV head; head_dim 32, 64, 128 or 256, heads *
+ * run have none; runs may be empty, prefixes is at most rows, rows at most 65535 (and fewer where tens of thousands
+ * of rows have a prefix each over hundreds of KV heads: the workspace is then of 0 bytes).  heads / kv_heads query heads share a KV head; head_dim 32, 64, 128 or 256, heads *
  * head_dim <= 8192.  ln2_q, b_q, ca_q: the i-exp's Q30 constants; khead: the carried scale of one K code
  * over sqrt(head_dim) per KV head.  Writes per row the codes [heads * head_dim] and scale (m, e) of the
  * context after the per-head ctx_fold [heads, 3] and the funnel at (site_m, site_e), and its status: 0,

@@ -1481,6 +1481,10 @@ static SaPlan sa_plan(int rows, int NH, int NKV, int prefixes, int64_t max_prefi
 	return p;
 }
 
+static int64_t sa_blocks(const SaPlan& p, int rows, int NKV) {
+	return p.shared_blocks + ((int64_t)rows * NKV * p.ht * p.owned + kSaWaves - 1) / kSaWaves;
+}
+
 static size_t sa_work(const SaPlan& p, int rows, int NH, int NKV, int D, char* base, SaWork* w) {
 	size_t at = 0;
 	auto take = [&](size_t n) {
@@ -1510,7 +1514,9 @@ static int sa_row_steps(int NH, int NKV, int D, int prefixes, int64_t max_prefix
 
 size_t shared_attn_workspace(int rows, int NH, int NKV, int D, int prefixes, int64_t max_prefix, int64_t max_own) {
 	SaWork w;
-	return sa_work(sa_plan(rows, NH, NKV, prefixes, max_prefix, max_own), rows, NH, NKV, D, nullptr, &w);
+	const SaPlan p = sa_plan(rows, NH, NKV, prefixes, max_prefix, max_own);
+	if (sa_blocks(p, rows, NKV) * 64 * kSaWaves > UINT32_MAX) return 0;  // a grid's most threads
+	return sa_work(p, rows, NH, NKV, D, nullptr, &w);
 }
 
 template <int D, int F>
@@ -1520,12 +1526,16 @@ static void sa_row_launch(const SharedAttnArgs& a, int steps, hipStream_t s) {
 	else hipLaunchKernelGGL((k_sa_row<D, F, kSaRowSteps>), grid, block, 0, s, a);
 }
 
+// Each launch takes lengths and blocks from what the one before wrote: false when one fails, and none follows it.
 template <int D>
-static void sa_launch(const SharedAttnArgs& a, const SaPlan& p, const SaWork& w, hipStream_t s) {
-	const dim3 grid(p.shared_blocks + (a.rows * a.NKV * p.ht * p.owned + kSaWaves - 1) / kSaWaves), block(64 * kSaWaves);
+static bool sa_launch(const SharedAttnArgs& a, const SaPlan& p, const SaWork& w, hipStream_t s) {
+	const dim3 grid((uint32_t)sa_blocks(p, a.rows, a.NKV)), block(64 * kSaWaves);
 	hipLaunchKernelGGL(k_sa_max<D>, grid, block, 0, s, a, p, w);
+	if (hipPeekAtLastError() != hipSuccess) return false;
 	hipLaunchKernelGGL(k_sa_sum<D>, grid, block, 0, s, a, p, w);
+	if (hipPeekAtLastError() != hipSuccess) return false;
 	hipLaunchKernelGGL(k_sa_pv<D>, grid, block, 0, s, a, p, w);
+	return hipPeekAtLastError() == hipSuccess;
 }
 
 void shared_attn(const SharedAttnArgs& a, hipStream_t s) {
@@ -1539,12 +1549,14 @@ void shared_attn(const SharedAttnArgs& a, hipStream_t s) {
 	const SaPlan p = sa_plan(a.rows, a.NH, a.NKV, a.prefixes, a.max_prefix, a.max_own);
 	SaWork w;
 	sa_work(p, a.rows, a.NH, a.NKV, a.D, (char*)a.ws, &w);
+	bool ok = false;
 	switch (a.D) {
-		case 32: sa_launch<32>(a, p, w, s); break;
-		case 64: sa_launch<64>(a, p, w, s); break;
-		case 128: sa_launch<128>(a, p, w, s); break;
-		default: sa_launch<256>(a, p, w, s); break;
+		case 32: ok = sa_launch<32>(a, p, w, s); break;
+		case 64: ok = sa_launch<64>(a, p, w, s); break;
+		case 128: ok = sa_launch<128>(a, p, w, s); break;
+		default: ok = sa_launch<256>(a, p, w, s); break;
 	}
+	if (!ok) return;  // the caller reads the error
 	const int units = a.NH * a.D / 4;
 	if (units <= 512) hipLaunchKernelGGL((k_sa_out<512, 1>), dim3(a.rows), dim3(512), 0, s, a, p, w);
 	else if (units <= 1024) hipLaunchKernelGGL((k_sa_out<512, 2>), dim3(a.rows), dim3(512), 0, s, a, p, w);
