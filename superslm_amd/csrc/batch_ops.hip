@@ -465,7 +465,7 @@ __device__ __forceinline__ void sa_own_steps(const SaJob& j, int8_t* lds, const 
 
 // The same over a shared plane, whose rows all waves of the block use: each thread loads its share of a step's
 // rows, AHEAD steps ahead, and stages it into one of two buffers, so a step costs one barrier (buffer b was
-// last read before the previous one; waves that take different branches around this make equally many steps).
+// last read before the previous one).  All waves of the block have to come here by the same branch (sa_vote).
 // Sums of 96 rows over 4096: 15.8 us, 18.4 with each wave staging its own.  LDS: 64 D bytes a buffer, K's two and then V's two.
 template <int D, bool WITH_V, int NC, typename F>
 __device__ __forceinline__ void sa_block_steps(const SaJob& j, int8_t* lds, const v4i (&q)[NC], F&& step) {
@@ -512,6 +512,23 @@ template <int D, bool WITH_V, int NC, typename F>
 __device__ __forceinline__ void sa_steps(const SaJob& j, int8_t* lds, const v4i (&q)[NC], F&& step) {
 	if (j.owned) sa_own_steps<D, WITH_V>(j, lds + (threadIdx.x >> 6) * 32 * D, q, step);
 	else sa_block_steps<D, WITH_V>(j, lds, q, step);
+}
+
+// Which bits some live row of a shared plane's block, or of an own plane's wave, has set: what every wave of it then
+// branches on alike.  The block's waves meet in the second buffer of K, which none writes before the first step's barrier.
+template <int D>
+__device__ __forceinline__ int sa_vote(const SaJob& j, int bits, int8_t* lds) {
+	int* s_vote = (int*)(lds + 64 * D);
+	const int wave = threadIdx.x >> 6;
+	int all = (__any(bits & 1) ? 1 : 0) | (__any(bits & 2) ? 2 : 0);
+	if (!j.owned) {
+		if ((threadIdx.x & 63) == 0) s_vote[wave] = all;
+		__syncthreads();
+		all = 0;
+#pragma unroll
+		for (int i = 0; i < kSaWaves; ++i) all |= s_vote[i];
+	}
+	return __builtin_amdgcn_readfirstlane(all);
 }
 
 // How many of the step's positions, counted from the lane's first (4 g), its row has.
@@ -577,7 +594,7 @@ __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 4 : 2) void k_sa_sum(sslm
 	__shared__ __attribute__((aligned(16))) int8_t lds[2 * 64 * D];  // also kSaWaves 32 D
 	const int g = (threadIdx.x & 63) >> 4;
 	SaJob j;
-	if (!sa_job(a, pl, w, &j) || j.p0 >= j.p1) return;
+	if (!sa_job(a, pl, w, &j) || j.p0 >= j.p1) return;  // alike for the waves of a shared plane's block
 	v4i q[NC];
 	sa_load_q<D>(a, j, q);
 	const SaConst c = w.cst[(size_t)max(j.r, 0) * a.NKV + j.kvh];
@@ -586,7 +603,7 @@ __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 4 : 2) void k_sa_sum(sslm
 	const int64_t end = !live ? 0 : (j.owned ? j.p1 : i64min(j.p1, j.start));
 	int64_t sum = 0;
 	int bad = 0;
-	if (!__any(live && !sa_fast(c, j.width))) {
+	if (!sa_vote<D>(j, live && !sa_fast(c, j.width), lds)) {
 		const SaExp e = sa_exp_of(live ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
 		double acc = 0.0;
 		sa_steps<D, false>(j, lds, q, [&](int64_t p, v4i (&s)[4], auto&&) {
@@ -674,7 +691,8 @@ __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 2 : 1) void k_sa_pv(sslm_
 #pragma unroll
 	for (int d = 0; d < DT; ++d) acc[d][0] = acc[d][1] = v4i{0, 0, 0, 0};
 	int32_t pr[16];
-	if (!__any(live && !sa_fast(c, j.width))) {
+	const int form = sa_vote<D>(j, (live && !sa_fast(c, j.width) ? 1 : 0) | (den >= ((int64_t)1 << 36) ? 2 : 0), lds);
+	if (!(form & 1)) {
 		const SaExp e = sa_exp_of(live ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
 		auto run = [&](auto small) {
 			constexpr bool SMALL = decltype(small)::value;
@@ -690,7 +708,7 @@ __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 2 : 1) void k_sa_pv(sslm_
 				multiply(lo, nhi, acc);
 			});
 		};
-		if (!__any(den >= ((int64_t)1 << 36))) run(std::true_type{});
+		if (!(form & 2)) run(std::true_type{});
 		else run(std::false_type{});
 	} else {
 		const double inv = 1.0 / (double)c.q_ln2, dinv = 1.0 / (double)den;
