@@ -37,6 +37,10 @@ struct SharedAttnArgs {
 size_t shared_attn_workspace(int rows, int NH, int NKV, int D, int prefixes, int64_t max_prefix, int64_t max_own);
 bool shared_attn_ok(int rows, int NH, int NKV, int D);
 void shared_attn(const SharedAttnArgs& a, hipStream_t s);
+// Whether a decode unit whose rows have adopted prompts takes it: `width` the most positions of a row, `own` those past
+// the rows' prompts, of all rows together; per_head: otherwise one block per query head would run, the grouped kernel,
+// though chosen, having no room for the scores.
+bool shared_attn_pays(int rows, int NKV, int64_t width, int64_t own, bool per_head, int cus);
 
 // A projection of m rows, row t with adapter row_adapter[t] (negative: none) and incoming scale in_scale[t].
 struct LoraGemmArgs {

@@ -1537,6 +1537,24 @@ size_t shared_attn_workspace(int rows, int NH, int NKV, int D, int prefixes, int
 	return sa_work(p, rows, NH, NKV, D, nullptr, &w);
 }
 
+// The attention of one block per (row, KV head) passes over its row alone, so its time is the longest row's
+// positions, once more where the blocks pass the CUs.  The launches by planes cut all rows over the whole chip: their
+// time hardly grows with the prompts, but with the rows' own positions for each CU.  They are taken with more blocks
+// than CUs, and where the longest row is ahead of those positions by kSharedPositions (one row alone gives up the
+// fused layer too: kSharedPositionsAlone); from there on also where one block per query head would run.
+// Steps of four layers, shared against not, ms.  7B shape: 8 adopters of 1000 positions 0.69 / 0.63, 2 of 2600 0.683 / 0.689,
+// 8 of 4000 0.71 / 0.78; one of 2600 0.687 / 0.651, of 3200 0.690 / 0.686, of 3700 0.69 / 0.71; one of 20 positions beside
+// 7 rows of 3000 without a prompt 0.71 / 0.73, beside 15 of 3000 0.76 / 0.73, 31 of 3000 0.89 / 0.81, 31 of 4400 0.95 / 0.88,
+// 39 of 3000 0.97 / 0.91 and of 3600 (per head) 1.00 / 1.41, 95 of 200 0.94 / 1.00, 95 of 4400 1.57 / 2.21.  1.5B shape:
+// 8 of 2000 0.448 / 0.461, of 8000 0.48 / 0.82; one of 20 beside 15 of 3000 0.47 / 0.53, 47 of 3000 0.62 / 0.59, 63 of 4000
+// 0.73 / 0.67, 127 of 6000 (per head) 1.16 / 2.01.
+constexpr int64_t kSharedPositions = 2600, kSharedPositionsAlone = 3200;
+bool shared_attn_pays(int rows, int NKV, int64_t width, int64_t own, bool per_head, int cus) {
+	if ((int64_t)rows * NKV > cus) return true;
+	if (width < (rows == 1 ? kSharedPositionsAlone : kSharedPositions)) return false;
+	return per_head || width - own * NKV / cus >= kSharedPositions;
+}
+
 template <int D, int F>
 static void sa_row_launch(const SharedAttnArgs& a, int steps, hipStream_t s) {
 	const dim3 grid(a.rows), block(64 * kSaRowWaves);

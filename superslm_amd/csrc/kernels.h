@@ -290,6 +290,8 @@ bool grouped_attention_chosen(int M, int NKV, int64_t cap);
 // blocks per (token, KV group) of the grouped decode attention: 2 splits the group's query heads
 // in halves (SSLM_HIP_GROUP_HALVES=1|2 overrides)
 int group_row_halves(int M, int NKV, int G);
+// Whether the grouped kernel, where chosen, holds the launch's scores in LDS; else one block per head runs.
+bool grouped_attention_fits(int M, int NKV, int G, int D, int32_t wcap);
 // Queries and sets the grouped decode kernel's LDS attributes for head size D and group size G
 // (once per process; call before any capture).  False when the runtime refuses them.
 bool attention_prepare(int D, int G);

@@ -4978,15 +4978,14 @@ static int group_rows(int G, int D) {
 }
 
 // rows per block: the group, or its first half (the second takes the rest)
-static int group_block_rows(const AttnArgs& a) {
-	const int G = a.NH / a.NKV;
-	return a.row_halves == 2 ? (G + 1) / 2 : G;
-}
+static int group_block_rows(int G, int halves) { return halves == 2 ? (G + 1) / 2 : G; }
+static int group_block_rows(const AttnArgs& a) { return group_block_rows(a.NH / a.NKV, a.row_halves); }
+static size_t group_scores_bytes(int rows, int32_t wcap) { return (size_t)rows * (size_t)wcap * sizeof(int32_t); }
 
 template <int D, int GM>
 static bool launch_attention_group_gm(const AttnArgs& a, hipStream_t s) {
 	if (a.wcap < 1 || a.wcap % 128 != 0 || !(a.row_halves == 1 || a.row_halves == 2)) return false;
-	const size_t dyn = (size_t)group_block_rows(a) * (size_t)a.wcap * sizeof(int32_t);  // the [rows][wcap] int32 scores
+	const size_t dyn = group_scores_bytes(group_block_rows(a), a.wcap);  // the [rows][wcap] int32 scores
 	if (group_attention_static_lds<D, GM>() + dyn > kCuLds) return false;
 	const int groups = a.M * a.NKV;
 	const int grid = a.row_halves == 2 ? (groups + 7) / 8 * 16 : groups;  // see the block numbering
@@ -5012,18 +5011,24 @@ bool attention_prepare(int D, int G) {
 	return true;
 }
 
+// the static LDS of the kernel for `rows` query rows per block; 0: none takes them
+static size_t group_static_lds(int D, int rows) {
+	const int gm = group_rows(rows, D);
+	if (D == 32 && gm == 4) return group_attention_static_lds<32, 4>();
+	if (D == 32 && gm == 8) return group_attention_static_lds<32, 8>();
+	if (D == 32 && gm == 16) return group_attention_static_lds<32, 16>();
+	if (D == 64 && gm == 4) return group_attention_static_lds<64, 4>();
+	if (D == 64 && gm == 8) return group_attention_static_lds<64, 8>();
+	if (D == 64 && gm == 16) return group_attention_static_lds<64, 16>();
+	if (D == 128 && gm == 4) return group_attention_static_lds<128, 4>();
+	if (D == 128 && gm == 8) return group_attention_static_lds<128, 8>();
+	if (D == 256 && gm == 4) return group_attention_static_lds<256, 4>();
+	return 0;
+}
+
 static bool attention_prepare_rows(int D, int G) {
 	try {
-		const int gm = group_rows(G, D);
-		if (D == 32 && gm == 4) (void)group_attention_static_lds<32, 4>();
-		if (D == 32 && gm == 8) (void)group_attention_static_lds<32, 8>();
-		if (D == 32 && gm == 16) (void)group_attention_static_lds<32, 16>();
-		if (D == 64 && gm == 4) (void)group_attention_static_lds<64, 4>();
-		if (D == 64 && gm == 8) (void)group_attention_static_lds<64, 8>();
-		if (D == 64 && gm == 16) (void)group_attention_static_lds<64, 16>();
-		if (D == 128 && gm == 4) (void)group_attention_static_lds<128, 4>();
-		if (D == 128 && gm == 8) (void)group_attention_static_lds<128, 8>();
-		if (D == 256 && gm == 4) (void)group_attention_static_lds<256, 4>();
+		(void)group_static_lds(D, G);
 	} catch (const LaunchRefused&) {
 		return false;
 	}
@@ -5035,6 +5040,12 @@ int group_row_halves(int M, int NKV, int G) {
 	if (e && e[0]) return e[0] == '2' && G >= 2 ? 2 : 1;
 	// two blocks per group while that still leaves no CU with two
 	return G >= 2 && 2 * M * NKV <= 256 ? 2 : 1;
+}
+
+bool grouped_attention_fits(int M, int NKV, int G, int D, int32_t wcap) {
+	const int rows = group_block_rows(G, group_row_halves(M, NKV, G));
+	const size_t fixed = group_static_lds(D, rows);
+	return fixed && fixed + group_scores_bytes(rows, wcap) <= kCuLds;
 }
 
 bool grouped_attention_chosen(int M, int NKV, int64_t cap) {

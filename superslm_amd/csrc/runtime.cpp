@@ -40,13 +40,6 @@ constexpr int kSlotCapacity = 1024;  // live sequences per model
 // (8 prompts 23.2 against 23.5 and 23.6 against 24.9 ms).
 constexpr int kSlicedActPrefillRows = 32;
 
-// The attention of one block per (row, KV head) passes over its row alone, so its time is the longest row's
-// positions, once more where the blocks pass the CUs.  A unit with adopted prefixes reads them shared and cut
-// over the whole chip from this many positions on, and always with more blocks than CUs (a step of four layers
-// of the 7B shape, shared against not: 32 rows of 2080 positions 0.775 / 0.758 ms, of 2432 0.798 / 0.786, of 2832
-// 0.797 / 0.808, 64 of 4196 0.95 / 1.88; 96 of 32 positions 0.945 / 0.984, 96 of 1056 1.05 / 1.26).
-constexpr int64_t kSharedPositions = 2600;
-
 struct HipError {
 	hipError_t e;
 };
@@ -2377,14 +2370,21 @@ static void share_prompts(sslm_model m, sslm_seq* seqs, std::vector<int>* idx, s
 	if (ps.empty() || !sslm_launch::shared_attn_ok((int)idx->size(), m->NH, m->NKV, m->D)) return;
 	auto where = [&](int i) { return std::find(ps.begin(), ps.end(), seqs[i]->prefix) - ps.begin(); };
 	const char* e = getenv("SSLM_HIP_SHARED_ATTN");
-	int64_t longest = 0, own = 0, width = 0;
+	int64_t longest = 0, own = 0, all_own = 0, width = 0;
 	for (int i : *idx) {
+		const int64_t n = seqs[i]->context_length + 1 - seqs[i]->adopted;
 		width = std::max(width, seqs[i]->context_length + 1);
-		own = std::max(own, seqs[i]->context_length + 1 - seqs[i]->adopted);
+		own = std::max(own, n);
+		all_own += n;
 		longest = std::max(longest, seqs[i]->adopted);
 	}
-	const int64_t blocks = (int64_t)idx->size() * m->NKV;
-	if (e && (e[0] == '0' || e[0] == '1') ? e[0] == '0' : width < kSharedPositions && blocks <= sslm_launch::device_cus()) return;
+	const int rows_n = (int)idx->size();
+	auto pays = [&] {
+		const bool per_head = sslm_launch::grouped_attention_chosen(rows_n, m->NKV, m->cap) &&
+		                      !sslm_launch::grouped_attention_fits(rows_n, m->NKV, m->NH / m->NKV, m->D, sslm_launch::group_width_cap(width, m->cap));
+		return sslm_launch::shared_attn_pays(rows_n, m->NKV, width, all_own, per_head, sslm_launch::device_cus());
+	};
+	if (e && (e[0] == '0' || e[0] == '1') ? e[0] == '0' : !pays()) return;
 	std::stable_sort(idx->begin(), idx->end(), [&](int x, int y) { return where(x) < where(y); });
 	rows->push_back(0);
 	for (size_t k = 0; k < ps.size(); ++k)
