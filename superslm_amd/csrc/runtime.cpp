@@ -2444,10 +2444,13 @@ static sslm_status decode_batch(sslm_model m, sslm_seq* seqs, int32_t n, const s
 	for (auto& g : groups) {
 		const uint32_t l0 = g.first;
 		const uint32_t l1 = std::min<uint32_t>(m->L, l0 + budget);
-		const std::vector<int>& members = g.second;
+		std::vector<int> members = g.second;
 		const int total = (int)members.size();
 		int parts = std::max(1, std::min(track_limit(), total / track_min()));
 		parts = std::max(parts, (total + kTrackTokens - 1) / kTrackTokens);
+		// Of several units as few as can be hold sequences without an adapter beside adapted ones, whose projections they
+		// would go through (1.5B shape, 256 sequences, every other one adapted: 7.41 ms in call order, 7.08 so).
+		if (parts > 1) std::stable_partition(members.begin(), members.end(), [&](int i) { return !seqs[i]->adapter; });
 		for (int p = 0; p < parts; ++p) {
 			const int b = (int)((int64_t)total * p / parts), e = (int)((int64_t)total * (p + 1) / parts);
 			if (e <= b) continue;
