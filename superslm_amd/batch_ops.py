@@ -8,6 +8,7 @@ the default stream) enqueues the operator on the buffers' present contents."""
 from __future__ import annotations
 
 import ctypes
+from numbers import Integral
 
 from .sslm import SslmLib
 
@@ -87,6 +88,8 @@ class BatchOps:
             if not hasattr(args, k):
                 raise TypeError(f"{type(args).__name__} has no field {k}")
             setattr(args, k, v)
+            if isinstance(v, Integral) and (getattr(args, k) or 0) != v:  # ctypes keeps the low bits alone
+                raise OverflowError(f"{type(args).__name__}.{k} does not hold {v}")
         return args
 
     def shared_attention_workspace(self, rows, heads, kv_heads, head_dim, prefixes, max_prefix, max_own) -> int:

@@ -356,10 +356,13 @@ class Seq:
     def set_rules(self, repetition: float = 1.0, presence: int = 0, frequency: int = 0, bias=(), raw: bool = False):
         """sslm_hip_seq_set_rules: a penalty factor for tokens the context holds (rounded to Q16), its
         additive penalties in logit units, and (token, value) biases."""
+        penalties = int(round(repetition * 65536)), presence, frequency
+        if not all(-1 << 31 <= x < 1 << 31 for x in penalties):  # ctypes would keep the low bits alone
+            raise OverflowError(f"rules outside 32 bits: {penalties}")
         pairs = list(bias.items()) if isinstance(bias, dict) else list(bias)
         ids = np.array([t for t, _ in pairs], dtype=np.int32)
         values = np.array([v for _, v in pairs], dtype=np.int32)
-        r = Rules(ctypes.sizeof(Rules), int(round(repetition * 65536)), presence, frequency, len(pairs), 0,
+        r = Rules(ctypes.sizeof(Rules), *penalties, len(pairs), 0,
                   ids.ctypes.data, values.ctypes.data)
         return self._rules(ctypes.byref(r), raw)
 

@@ -2,6 +2,7 @@
 import pytest
 
 from superslm_amd.batch_ops import BatchOps
+from superslm_amd.sslm import Seq
 
 INVALID, SMALL = 1, 2
 ANY = 1 << 20  # a non-null, aligned address that no refused call reads
@@ -44,3 +45,24 @@ def test_attention_workspace_holds_its_planes(rows, heads, kv_heads, dim, ops):
         assert n >= 2 * 4 * rows * heads * dim
         assert n >= last
         last = n
+
+
+@pytest.mark.parametrize("field,value", [("rows", (1 << 32) + 3), ("heads", 1 << 31), ("blocks", -(1 << 31) - 1), ("cap", 1 << 63)])
+def test_an_integer_past_its_field_is_an_error(field, value, ops):
+    """Not the call with the integer's low bits."""
+    half = 2 * 64 * 32
+    f = dict(rows=3, heads=4, kv_heads=2, head_dim=32, prefixes=0, blocks=4, max_prefix=0, max_own=1, kv_pool=ANY, block_bytes=2 * half,
+             k_offset=0, v_offset=half, cap=64, q=None, workspace=ANY, workspace_bytes=1 << 30, site=(1 << 30, -45))
+    ops.shared_attention(**f)
+    with pytest.raises(OverflowError):
+        ops.shared_attention(**{**f, field: value})
+
+
+@pytest.mark.parametrize("rules", [{"repetition": 32768.0}, {"repetition": 1e6}, {"presence": 1 << 31}, {"frequency": -(1 << 31) - 1},
+                                   {"bias": [(3, 1 << 31)]}, {"bias": {1 << 32: 5}}])
+def test_rules_past_32_bits_are_an_error(rules):
+    seq = Seq.__new__(Seq)
+    seq._rules = lambda ref, raw: "called"
+    assert seq.set_rules(repetition=1.5, presence=-7, frequency=3, bias={4: -9}) == "called"
+    with pytest.raises(OverflowError):
+        seq.set_rules(**rules)
