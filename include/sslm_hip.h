@@ -170,10 +170,11 @@ sslm_status sslm_g5_test_only_peek_kv_block_bytes(sslm_kv_pool pool, uint32_t bl
  * A prefix takes a block of its pool and is prefilled like a sequence without an adapter (in any number
  * of calls) until it is frozen (then SSLM_PREFIX_FROZEN_REJECTED).  A fresh sequence of the same pool, with the
  * same schema bound (else SSLM_PREFIX_SCHEMA_MISMATCH), adopts a frozen prefix: its tokens, KV block, blob
- * and every later result are those of a sequence that took the prompt itself.  Decode steps then read the
- * prompt's K/V once for all of the batch's adopters (sslm_hip_shared_attention) where that is the faster
- * form.  Anything else -- a prefix not frozen, a sequence that holds context or has an adapter (it may be given
- * one afterwards, for what follows the prompt), another pool -- is refused (SSLM_INVALID_ARGUMENT).  A released prefix keeps its block until its last adopter is released or reset. */
+ * and every later result are those of a sequence that took the prompt itself.  Decode steps then attend to
+ * the prefix's one copy of the prompt's K/V (sslm_hip_shared_attention) where that is the faster form.  Anything
+ * else -- a prefix not frozen, a sequence that holds context or has an adapter (it may be given one
+ * afterwards, for what follows the prompt), another pool -- is refused (SSLM_INVALID_ARGUMENT).  A released
+ * prefix keeps its block until its last adopter is released or reset. */
 sslm_status sslm_prefix_begin(sslm_model model, sslm_kv_pool* pool, sslm_prefix* out);
 sslm_status sslm_prefix_prefill(sslm_model model, sslm_prefix prefix, const int32_t* tokens, int32_t count,
                                 int32_t chunk_budget, sslm_span_kind kind, sslm_workspace ws, int32_t* consumed);
@@ -325,13 +326,14 @@ sslm_status sslm_hip_seq_set_rules(sslm_seq seq, const sslm_hip_rules* rules);
 /* Decode attention of rows that share prompts (reference src/forward/forward_sites.cpp:1791-1905 and
  * checked_chain_funnel.cpp:257-364, one row's result the same as if it held its whole context).
  * Row r attends to positions [0, row_width[r]) of its context.  Those below its prefix's length lie in
- * the prefix's KV block, the others in the row's own block, each at its own position; a prefix's K/V are
- * read once for all of its rows.  Blocks are the KV pool's: `blocks` of block_bytes bytes from kv_pool, K
+ * the prefix's KV block, the others in the row's own block, each at its own position.  Up to 64 query rows
+ * (row, head) of a prefix and KV head share each reading of its K/V; short rows, which run one to a block, read
+ * them each.  Blocks are the KV pool's: `blocks` of block_bytes bytes from kv_pool, K
  * (V) of (KV head, position) at block + k_offset (v_offset) + (KV head * cap + position) * head_dim.
  * Rows [prefix_rows[p], prefix_rows[p + 1]) have prefix p in block prefix_block[p]; rows outside every
- * run have none; runs may be empty, prefixes is at most rows, rows at most 65535 (and fewer where tens of thousands
- * of rows have a prefix each over hundreds of KV heads: the workspace is then of 0 bytes).  heads / kv_heads query heads share a KV head; head_dim 32, 64, 128 or 256, heads *
- * head_dim <= 8192.  ln2_q, b_q, ca_q: the i-exp's Q30 constants; khead: the carried scale of one K code
+ * run have none; runs may be empty, prefixes is at most rows, rows at most 65535 (and fewer where tens of
+ * thousands of rows have a prefix each over hundreds of KV heads: the workspace is then of 0 bytes).  heads /
+ * kv_heads query heads share a KV head; head_dim 32, 64, 128 or 256, heads * head_dim <= 8192.  ln2_q, b_q, ca_q: the i-exp's Q30 constants; khead: the carried scale of one K code
  * over sqrt(head_dim) per KV head.  Writes per row the codes [heads * head_dim] and scale (m, e) of the
  * context after the per-head ctx_fold [heads, 3] and the funnel at (site_m, site_e), and its status: 0,
  * or the reference's SslmForwardStatus value (7: no position to attend to; 9: a length or block index

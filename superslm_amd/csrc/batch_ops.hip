@@ -136,15 +136,15 @@ __device__ __forceinline__ RowConst row_const(const sslm_launch::SharedAttnArgs&
 
 // The layout of one call's launches.  The unit of work is a wave with a tile of 16 query rows and a
 // range of positions, a "plane": shared planes cut a prefix into sb positions each and their tiles hold
-// the query heads of one KV head of 16 / G neighbouring rows (G heads share a KV head), so a K or V row
-// is read once for all of them; own planes cut a row's own positions, their tiles hold the row's G heads.
+// the query heads of one KV head of 16 / G neighbouring rows (G heads share a KV head), and the tiles of a block's
+// four waves share each K or V row that it loads; own planes cut a row's own positions, their tiles hold the row's G heads.
 // The softmax's maximum and sum run over the whole row and every probability is rounded by itself, so no
 // rescaling of partial results is exact: three launches -- maxima, sums, P.V -- recompute the scores,
 // which cost 8 MFMAs a step of 64 positions at D = 128 where the i-exp of the step's scores costs some
 // hundreds of vector instructions, and integer sums join the planes exactly in any order.
-// 96 rows of 28 heads over 4 KV heads of 128, 4096 shared positions and 16 .. 384 own: maxima 9.2 us, sums 15.8,
-// P.V 25.0, join 6.1.  Bound by the vector instructions of i-exp and probability (issued back to back they take 3.0,
-// 7.6 and 11.5 us) at the two waves a SIMD that P.V's registers allow, and by each launch's chain of loads.
+// 96 rows of 28 heads over 4 KV heads of 128, 4096 shared positions and 16 .. 384 own: maxima 9.4 us, sums 15.7,
+// P.V 25.4, join 5.9.  Bound by the vector instructions of i-exp and probability (issued back to back they take 3.0,
+// 7.8 and 12.2 us) at the two waves a SIMD that P.V's registers allow, and by each launch's chain of loads.
 struct SaPlan {
 	int tb;          // blocks of kSaWaves tiles of shared rows: at least those of every prefix together
 	int shared, sb;  // shared planes and the positions of one (a multiple of 64)
@@ -1094,7 +1094,8 @@ __global__ __launch_bounds__(64) void k_lora_table(const LoraRef* const* rows, i
 // read) against MB MFMA tiles of 16 rows, whose codes come from L2.  The waves' int32 sums are
 // joined in LDS and stored as plane blockIdx / tiles of [planes][m][n].  Blocks past the products' do
 // rows_u: 16 of them per row, four ranks each.  Bound by the chain of loads of a wave's share: 4 x 1536 x 1536 4.0 us,
-// 32 x 4864 x 896 5.7, 64 x 1536 x 8960 15.3 (16 MB of weights and adapters); as the decode GEMV and a launch of
+// 32 x 4864 x 896 5.7, 64 x 1536 x 8960 15.3 (28 MB: 13.8 of weights, 13.5 of the A of the 41 adapters
+// that 64 rows drawn from 64 have on average, 0.5 of codes); as the decode GEMV and a launch of
 // k_rows_u 7.6, 9.6 and 29.5.
 template <int MB, int KC>
 __global__ __launch_bounds__(256) void k_lora_proj(sslm_launch::LoraGemmArgs g, int planes, int32_t* part, int8_t* u) {

@@ -419,7 +419,7 @@ struct sslm_seq_s {
 
 // A shared prompt: a sequence of its own, whose block holds the prompt's K/V.  Sequences that adopt it
 // copy its state and K/V rows (so each one's block, blob and every verb are as if it had taken the prompt
-// itself) and a decode step reads the shared positions from this block, once for all of them.
+// itself) and a decode step reads the shared positions from this block.
 struct sslm_prefix_s {
 	sslm_model model = nullptr;
 	sslm_seq seq = nullptr;
@@ -2358,7 +2358,7 @@ int track_min() {
 	return v;
 }
 
-// Whether a decode unit's attention reads its shared prompts once for all of their sequences, and if so
+// Whether a decode unit's attention reads its shared prompts from the prefixes' blocks, and if so
 // the unit's order (the prefixes' sequences first, run by run) and the launch's sizes: own positions in
 // steps of 256, so that a graph is re-recorded once per 256 tokens.  Otherwise *prefixes stays empty.
 // SSLM_HIP_SHARED_ATTN=1 (0) takes it wherever a prefix is adopted (never); read per call.
