@@ -37,10 +37,14 @@ struct SharedAttnArgs {
 size_t shared_attn_workspace(int rows, int NH, int NKV, int D, int prefixes, int64_t max_prefix, int64_t max_own);
 bool shared_attn_ok(int rows, int NH, int NKV, int D);
 void shared_attn(const SharedAttnArgs& a, hipStream_t s);
-// Whether a decode unit whose rows have adopted prompts takes it: `width` the most positions of a row, `own` those past
-// the rows' prompts, of all rows together; per_head: otherwise one block per query head would run, the grouped kernel,
-// though chosen, having no room for the scores.
-bool shared_attn_pays(int rows, int NKV, int64_t width, int64_t own, bool per_head, int cus);
+// Whether a decode unit whose rows have adopted prompts takes it.
+struct SharedUnit {
+	int rows, NH, NKV, D;
+	int64_t width;         // the most positions of a row
+	int64_t adopted, own;  // positions in the rows' prompts and past them, of all rows together
+	bool per_head;         // otherwise one block per query head runs for want of the fused launch or of LDS for the scores
+};
+bool shared_attn_pays(const SharedUnit& u, int cus);
 
 // A projection of m rows, row t with adapter row_adapter[t] (negative: none) and incoming scale in_scale[t].
 struct LoraGemmArgs {

@@ -1538,22 +1538,39 @@ size_t shared_attn_workspace(int rows, int NH, int NKV, int D, int prefixes, int
 	return sa_work(p, rows, NH, NKV, D, nullptr, &w);
 }
 
-// The attention of one block per (row, KV head) passes over its row alone, so its time is the longest row's
-// positions, once more where the blocks pass the CUs.  The launches by planes cut all rows over the whole chip: their
-// time hardly grows with the prompts, but with the rows' own positions for each CU.  They are taken with more blocks
-// than CUs, and where the longest row is ahead of those positions by kSharedPositions (one row alone gives up the
-// fused layer too: kSharedPositionsAlone); from there on also where one block per query head would run.
-// Steps of four layers, shared against not, ms.  7B shape: 8 adopters of 1000 positions 0.69 / 0.63, 2 of 2600 0.683 / 0.689,
-// 8 of 4000 0.71 / 0.78; one of 2600 0.687 / 0.651, of 3200 0.690 / 0.686, of 3700 0.69 / 0.71; one of 20 positions beside
-// 7 rows of 3000 without a prompt 0.71 / 0.73, beside 15 of 3000 0.76 / 0.73, 31 of 3000 0.89 / 0.81, 31 of 4400 0.95 / 0.88,
-// 39 of 3000 0.97 / 0.91 and of 3600 (per head) 1.00 / 1.41, 95 of 200 0.94 / 1.00, 95 of 4400 1.57 / 2.21.  1.5B shape:
-// 8 of 2000 0.448 / 0.461, of 8000 0.48 / 0.82; one of 20 beside 15 of 3000 0.47 / 0.53, 47 of 3000 0.62 / 0.59, 63 of 4000
-// 0.73 / 0.67, 127 of 6000 (per head) 1.16 / 2.01.
-constexpr int64_t kSharedPositions = 2600, kSharedPositionsAlone = 3200;
-bool shared_attn_pays(int rows, int NKV, int64_t width, int64_t own, bool per_head, int cus) {
-	if ((int64_t)rows * NKV > cus) return true;
-	if (width < (rows == 1 ? kSharedPositionsAlone : kSharedPositions)) return false;
-	return per_head || width - own * NKV / cus >= kSharedPositions;
+// Steps of four layers, shared against not, in ms: shapes as heads / KV heads x dims, `n of p` rows with a prompt of p and
+// 16 or 32 positions of their own, `beside n of p` one row with a prompt of 20 beside n rows of p without one.
+//
+// The launches by planes cut all rows over the whole chip: their time hardly grows with the prompts, but with the
+// rows' own positions for each CU.  The other attention takes a block per (row, KV head), or per query head, over
+// its row alone: its time is the longest row's, once more where the blocks pass the CUs.
+//
+// Up to one block per (row, KV head) for each CU: where the longest row is ahead of the own positions for each CU by
+// kSharedPositions (kSharedPositions64 for less than 128 dims, whose rows the other form passes over faster; a quarter
+// more for one row, whose fused layers end), and where it is that long and a block per query head would run.
+//   28/4x128: 8 of 1000 0.69 / 0.63, 2 of 2600 0.683 / 0.689, 8 of 4000 0.71 / 0.78, one of 2600 0.687 / 0.651, of 3200 0.690 /
+//   0.686, of 3700 0.69 / 0.71; beside 7 of 3000 0.71 / 0.73, 15 of 3000 0.76 / 0.73, 31 of 3000 0.89 / 0.81, 31 of 4400
+//   0.95 / 0.88, 39 of 3000 0.97 / 0.91, 39 of 3600 (per head) 1.00 / 1.41.
+//   12/2x128: 2 of 2600 0.45 / 0.48, 8 of 2000 0.448 / 0.461, of 8000 0.48 / 0.82; beside 15 of 3000 0.47 / 0.53,
+//   47 of 3000 0.62 / 0.59, 63 of 4000 0.73 / 0.67, 127 of 6000 (per head) 1.16 / 2.01.
+//   32/8x64: one of 3300 0.408 / 0.375, 2 of 2700 0.406 / 0.379, of 3300 0.405 / 0.401, 8 of 2700 0.420 / 0.425.
+//   16/4x256: 2 of 2700 0.56 / 0.69.
+// Past it: blocks per query head of at least four to a KV head, up to 128 dims, cost more than the planes whatever
+// the lengths once there are kSharedHeadDims for each CU; else the planes have to save kSharedSaved positions for each CU.
+//   28/4x128: 65 of 32 0.624 / 0.644, 128 of 32 0.69 / 0.75; beside 64 of 300 0.68 / 0.68, 95 of 4400 1.57 / 2.21.
+//   32/8x64: 65 of 32 0.53 / 0.50, 100 of 32 0.57 / 0.58; beside 64 of 300 0.56 / 0.54, 127 of 300 0.65 / 0.69.
+//   32/8x128: 33 of 300 0.63 / 0.60, of 1000 0.666 / 0.669, 64 of 1000 0.71 / 0.73; beside 63 of 1000 0.84 / 0.70.
+//   16/8x128: 100 of 32 0.57 / 0.54, of 1000 0.62 / 0.78; beside 99 of 1000 0.85 / 0.76.
+//   16/4x256: 65 of 32 0.76 / 0.69, 100 of 300 0.851 / 0.859; beside 127 of 300 0.95 / 0.90.
+constexpr int64_t kSharedPositions = 2600, kSharedPositions64 = 3400, kSharedHeadDims = 800, kSharedSaved = 1000;
+bool shared_attn_pays(const SharedUnit& u, int cus) {
+	if ((int64_t)u.rows * u.NKV > cus) {
+		if (u.per_head && u.D <= 128 && u.NH >= 4 * u.NKV && (int64_t)u.rows * u.NH * u.D >= kSharedHeadDims * cus) return true;
+		return (u.adopted - u.own) * u.NKV / cus >= kSharedSaved;
+	}
+	const int64_t least = u.D < 128 ? kSharedPositions64 : kSharedPositions;
+	if (u.width < (u.rows == 1 ? least + least / 4 : least)) return false;
+	return u.per_head || u.width - u.own * u.NKV / cus >= least;
 }
 
 template <int D, int F>

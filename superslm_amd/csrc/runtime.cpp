@@ -2370,19 +2370,23 @@ static void share_prompts(sslm_model m, sslm_seq* seqs, std::vector<int>* idx, s
 	if (ps.empty() || !sslm_launch::shared_attn_ok((int)idx->size(), m->NH, m->NKV, m->D)) return;
 	auto where = [&](int i) { return std::find(ps.begin(), ps.end(), seqs[i]->prefix) - ps.begin(); };
 	const char* e = getenv("SSLM_HIP_SHARED_ATTN");
-	int64_t longest = 0, own = 0, all_own = 0, width = 0;
+	int64_t longest = 0, own = 0;
+	sslm_launch::SharedUnit unit{(int)idx->size(), m->NH, m->NKV, m->D, 0, 0, 0, false};
 	for (int i : *idx) {
 		const int64_t n = seqs[i]->context_length + 1 - seqs[i]->adopted;
-		width = std::max(width, seqs[i]->context_length + 1);
+		unit.width = std::max(unit.width, seqs[i]->context_length + 1);
+		unit.adopted += seqs[i]->adopted;
+		unit.own += n;
 		own = std::max(own, n);
-		all_own += n;
 		longest = std::max(longest, seqs[i]->adopted);
 	}
-	const int rows_n = (int)idx->size();
 	auto pays = [&] {
-		const bool per_head = sslm_launch::grouped_attention_chosen(rows_n, m->NKV, m->cap) &&
-		                      !sslm_launch::grouped_attention_fits(rows_n, m->NKV, m->NH / m->NKV, m->D, sslm_launch::group_width_cap(width, m->cap));
-		return sslm_launch::shared_attn_pays(rows_n, m->NKV, width, all_own, per_head, sslm_launch::device_cus());
+		const bool fused = fused_attention_enabled() &&
+		                   sslm_launch::decode_fused_ok(unit.rows, m->H, m->NKV, m->KVH, m->cap, m->layers[0].p_qkv != nullptr);
+		unit.per_head = !fused || (sslm_launch::grouped_attention_chosen(unit.rows, m->NKV, m->cap) &&
+		                           !sslm_launch::grouped_attention_fits(unit.rows, m->NKV, m->NH / m->NKV, m->D,
+		                                                                sslm_launch::group_width_cap(unit.width, m->cap)));
+		return sslm_launch::shared_attn_pays(unit, sslm_launch::device_cus());
 	};
 	if (e && (e[0] == '0' || e[0] == '1') ? e[0] == '0' : !pays()) return;
 	std::stable_sort(idx->begin(), idx->end(), [&](int x, int y) { return where(x) < where(y); });
