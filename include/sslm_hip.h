@@ -426,6 +426,164 @@ typedef struct sslm_hip_pick_args {
 size_t sslm_hip_pick_workspace(int32_t rows, int32_t vocab);
 sslm_status sslm_hip_pick_tokens(const sslm_hip_pick_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The next token of rows of int32 logits by sampling, from a given random number per row.  With the legal tokens
+ * (mask page bit set; null: all) ordered by logit, largest first, equal ones by the lower index, x0 the first's:
+ *   d = x0 - x;  z = d / q_ln2;  w = z < 30 ? ((q_b - d mod q_ln2)^2 + q_c) >> z : 0     (the framework's i-exp)
+ *   the first top_k tokens (0: all); of those the shortest run of first ones whose w sum to at least
+ *   ceil(top_p_q16 / 2^16 of theirs), one token at least; of those the ones with w >= ceil(min_p_q16 (q_b^2 + q_c) / 2^16)
+ * the token is the first one of these in the order whose running sum of w exceeds floor(random total / 2^32), total
+ * the sum of all of theirs.  q_ln2, q_b, q_c are ln 2, 1.353 and 0.344 / 0.3585 (squared unit) in units of
+ * logits times temperature.  tokens[r]: the token, -1 when no token is legal, -2 when the rule is outside its
+ * domain: 1 <= q_ln2 <= 2 q_b + 1, q_b >= 0, q_c >= 0, w0 = q_b^2 + q_c in [1, 2^47], w0 vocab < 2^62, top_k >= 0,
+ * top_p_q16 and min_p_q16 in [0, 65536].  mass (optional): the token's w and the total, so w / total is the
+ * probability it was drawn with; 0, 0 beside a negative token.  rules is a device array.  Scale, penalties and
+ * biases come before: sslm_hip_pick_tokens' `adjusted` is this one's `logits`. */
+typedef struct sslm_hip_sampling {
+	const uint8_t* mask; /* (vocab + 7) / 8 bytes, or null */
+	int64_t q_ln2, q_b, q_c;
+	int32_t top_k, top_p_q16, min_p_q16;
+	uint32_t random;
+} sslm_hip_sampling;
+typedef struct sslm_hip_sample_args {
+	uint32_t struct_size;
+	int32_t rows, vocab, reserved;
+	const int32_t* logits;
+	int64_t logits_ld; /* row stride in elements, at least vocab */
+	const sslm_hip_sampling* rules;
+	int32_t* tokens; /* [rows] */
+	int64_t* mass;   /* [rows, 2] or null */
+} sslm_hip_sample_args;
+#define SSLM_HIP_SAMPLE_MAX_VOCAB (1 << 24)
+size_t sslm_hip_sample_workspace(int32_t rows, int32_t vocab);
+sslm_status sslm_hip_sample_tokens(const sslm_hip_sample_args* args, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* ---- a cache in pages, for requests that fork (no reference counterpart) ----
+ *
+ * `pages` pages of page_bytes from `pool`, each for page_tokens (16, 32, 64, 128 or 256) positions of a context, in 8 bits
+ * with a scale per page, KV head and K or V: of (KV head h, slot j) K's code d at page + k_offset + (h page_tokens + j)
+ * head_dim + d, V's at v_offset likewise, and the exponents of K (kv_heads bytes) and V (kv_heads) at exp_offset; a code c
+ * under exponent s stands for c 2^s units, s <= 8 (a larger one counts as 8).  Several layers may share a page, each with offsets of its own.
+ * Row r's position p lies in slot p % page_tokens of page tables[r table_ld + p / page_tokens]; rows may share pages.
+ * Streams, workspaces, graphs and refusals as for the operators above: sizes, null pointers and alignment are refused
+ * before the launch, what stands in device memory is checked by the kernels.  pool, page_bytes, k_offset and v_offset are
+ * multiples of 16. */
+#define SSLM_HIP_CACHE_MAX_PAGES (1 << 18)
+#define SSLM_HIP_CACHE_MAX_ROWS 4096
+#define SSLM_HIP_CACHE_MAX_SHIFT 8
+#define SSLM_HIP_CACHE_MAX_WIDTH ((int64_t)1 << 24)
+
+/* Pages change hands: row r becomes a context that has the first keep[r] positions of row source[r]'s (itself, another
+ * row, or -1: none, keep 0) and pages for room[r] >= keep[r] positions.  A row that shares a page it will write into (keep
+ * inside the page and room past keep) gets a copy of it, but where every row that holds the page would write
+ * into it the lowest of them keeps it.  Pages that no row and no `held` byte (optional) keeps are free and given out in
+ * ascending order, row by row, a row's copy before its new pages.  new_tables (entries past a row's pages: -1) and
+ * new_lengths (= room) may be tables and lengths themselves.  All or nothing: result[0] is 0, SSLM_INVALID_ARGUMENT
+ * (result[3]: the first row whose source, keep, room, length or table is out of range) or SSLM_KV_POOL_EXHAUSTED, and then nothing
+ * else is written; result[1]: pages free afterwards (negative: short by), result[2]: pages copied, result[3] else -1. */
+typedef struct sslm_hip_cache_update_args {
+	uint32_t struct_size;
+	int32_t rows, pages, page_tokens, table_ld, reserved;
+	int8_t* pool;
+	int64_t page_bytes;
+	const int32_t* tables;  /* [rows, table_ld] */
+	const int64_t* lengths; /* [rows] */
+	const int32_t* source;  /* [rows] */
+	const int64_t* keep;    /* [rows] */
+	const int64_t* room;    /* [rows] */
+	const uint8_t* held;    /* [pages] or null */
+	int32_t* new_tables;
+	int64_t* new_lengths;
+	int32_t* result; /* [4] */
+} sslm_hip_cache_update_args;
+size_t sslm_hip_cache_update_workspace(int32_t rows, int32_t pages, int32_t table_ld);
+sslm_status sslm_hip_cache_update(const sslm_hip_cache_update_args* args, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
+/* The pages that the rows' lengths reach move to the lowest numbers that `held` (optional: pages that stay where they
+ * are) leaves: those past the last of these, in ascending order, to the free ones before it, in ascending order.  map[p]:
+ * page p's new number, -1 if no row has it.  new_tables may be tables itself; entries past a row's pages become -1.
+ * result as above, but result[1]: one past the highest page in use or held, result[2]: pages moved. */
+typedef struct sslm_hip_cache_compact_args {
+	uint32_t struct_size;
+	int32_t rows, pages, page_tokens, table_ld, reserved;
+	int8_t* pool;
+	int64_t page_bytes;
+	const int32_t* tables;
+	const int64_t* lengths;
+	const uint8_t* held;
+	int32_t* new_tables;
+	int32_t* map;    /* [pages] */
+	int32_t* result; /* [4] */
+} sslm_hip_cache_compact_args;
+size_t sslm_hip_cache_compact_workspace(int32_t rows, int32_t pages, int32_t table_ld);
+sslm_status sslm_hip_cache_compact(const sslm_hip_cache_compact_args* args, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* New tokens of a ragged batch: q and k rotated, k and v landed in the rows' pages.  Row r has the tokens
+ * [row_tokens[r], row_tokens[r + 1]), at positions row_start[r] on (row_tokens ascends within [0, tokens]; at most max_new each;
+ * pages that rows write into are their own).  Codes
+ * are int8 with carried scales k_scale, v_scale (m, e) per token.  The reference's landing (forward_sites.cpp:513-653) with the
+ * KV head's constants r_t, e_t gives units, clamped to +-127 2^8; pairs of the head's first rope_dim (a multiple of 8, 0:
+ * none) dims, (2 i, 2 i + 1) or with rope_halves (i, i + rope_dim / 2), turn by the Q30 tables [rope_rows, rope_dim / 2] (src/intmath.cpp:782-792),
+ * q's codes clamped to +-127, k's units to +-127 2^8.  A page's exponent for a KV head's K or V is 0 at its first slot and
+ * grows to what a token needs, the least that keeps the token's codes within +-127; codes already there are then divided
+ * by the power of two once more.  All roundings go to the nearest, ties away from zero.  Every split of a span into calls leaves
+ * the same bytes; slots past the last token stay as they were.  clamped[r]: values clamped.  status[r]: 0, 9 (a
+ * length, position or page out of range) or 4 (a scale's mantissa), the row's q_out and pages then left as they were.
+ * q null: no queries.  q_out may be q. */
+typedef struct sslm_hip_cache_store_args {
+	uint32_t struct_size;
+	int32_t rows, tokens, max_new, heads, kv_heads, head_dim, pages, page_tokens, table_ld, rope_dim, rope_halves;
+	int8_t* pool;
+	int64_t page_bytes, k_offset, v_offset, exp_offset;
+	const int32_t* tables;
+	const int32_t* row_tokens; /* [rows + 1] */
+	const int64_t* row_start;  /* [rows] */
+	int64_t rope_rows;
+	const int64_t* rope_cos;
+	const int64_t* rope_sin;
+	const int8_t *q, *k, *v;  /* [tokens, heads | kv_heads * head_dim], strides q_ld, k_ld, v_ld */
+	int64_t q_ld, k_ld, v_ld;
+	const int64_t *k_scale, *v_scale; /* [tokens, 2] */
+	const int64_t *r_t_k, *e_t_k, *r_t_v, *e_t_v; /* [kv_heads] */
+	int8_t* q_out; /* [tokens, heads * head_dim] */
+	int32_t* clamped; /* [rows] */
+	int32_t* status; /* [rows] */
+} sslm_hip_cache_store_args;
+sslm_status sslm_hip_cache_store(const sslm_hip_cache_store_args* args, void* stream);
+
+/* Attention over the pages: token i of row r, at position row_start[r] + i, attends to the positions up to its own
+ * (single tokens: decode steps; several: a prompt's chunk, whose rows sslm_hip_cache_store has landed before).
+ * score = (q . k) 2^s of k's page; the softmax, its constants (khead: the carried scale of one K unit over sqrt(head_dim)), the Q15
+ * probabilities, fold and funnel are sslm_hip_shared_attention's; context = sum of p v 2^s of v's page.  max_width: at least
+ * every row's positions.  Per token its codes, scale and status: 0, 9 (the row's lengths or a page of it out of range) or the
+ * reference's SslmForwardStatus value; tokens that no row has stay as they were. */
+typedef struct sslm_hip_cache_attention_args {
+	uint32_t struct_size;
+	int32_t rows, tokens, max_new, heads, kv_heads, head_dim, pages, page_tokens, table_ld, reserved;
+	int64_t max_width;
+	const int8_t* pool;
+	int64_t page_bytes, k_offset, v_offset, exp_offset;
+	const int32_t* tables;
+	const int32_t* row_tokens;
+	const int64_t* row_start;
+	const int8_t* q;        /* [tokens, heads * head_dim] rotated codes */
+	const int64_t* q_scale; /* [tokens, 2] */
+	const int64_t* khead_m; /* [kv_heads] */
+	const int64_t* khead_e;
+	int64_t ln2_q, b_q, ca_q;
+	const int32_t* ctx_fold; /* [heads, 3] */
+	int64_t site_m, site_e;
+	int8_t* codes;   /* [tokens, heads * head_dim] */
+	int64_t* scales; /* [tokens, 2] */
+	int32_t* status; /* [tokens] */
+} sslm_hip_cache_attention_args;
+size_t sslm_hip_cache_attention_workspace(int32_t rows, int32_t tokens, int32_t max_new, int32_t heads, int32_t kv_heads,
+                                          int32_t head_dim, int32_t page_tokens, int64_t max_width);
+sslm_status sslm_hip_cache_attention(const sslm_hip_cache_attention_args* args, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

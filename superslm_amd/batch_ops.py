@@ -51,6 +51,24 @@ class PickArgs(ctypes.Structure):
                 ("logits_ld", _I64), ("adjusted_ld", _I64), ("rules", _P), ("adjusted", _P), ("tokens", _P)]
 
 
+class Sampling(ctypes.Structure):
+    """sslm_hip_sampling: how one row of logits is sampled."""
+    _fields_ = [("mask", _P), ("q_ln2", _I64), ("q_b", _I64), ("q_c", _I64), ("top_k", _I32), ("top_p_q16", _I32),
+                ("min_p_q16", _I32), ("random", _U32)]
+
+
+class SampleArgs(ctypes.Structure):
+    """sslm_hip_sample_args."""
+    _fields_ = [("struct_size", _U32), ("rows", _I32), ("vocab", _I32), ("reserved", _I32), ("logits", _P),
+                ("logits_ld", _I64), ("rules", _P), ("tokens", _P), ("mass", _P)]
+
+
+def sampling_constants(unit: float) -> dict:
+    """q_ln2, q_b and q_c for logits of which `unit` make one natural unit at the wanted temperature: the
+    temperature over the real value of one integer step."""
+    return {"q_ln2": int(0.6931471805599453 * unit), "q_b": int(1.353 * unit), "q_c": int(0.344 / 0.3585 * unit * unit)}
+
+
 class Call:
     """One operator over bound buffers.  `args` is its struct, whose fields may be changed between calls."""
 
@@ -72,13 +90,14 @@ class BatchOps:
         self.lib = lib
         L = lib.lib
         for name, struct in (("sslm_hip_shared_attention", SharedAttentionArgs),
-                             ("sslm_hip_gemm_lora_requant", GemmLoraArgs), ("sslm_hip_pick_tokens", PickArgs)):
+                             ("sslm_hip_gemm_lora_requant", GemmLoraArgs), ("sslm_hip_pick_tokens", PickArgs),
+                             ("sslm_hip_sample_tokens", SampleArgs)):
             f = getattr(L, name)
             f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(struct), _P, _SZ, _P]
         L.sslm_hip_shared_attention_workspace.argtypes = [_I32] * 5 + [_I64] * 2
         L.sslm_hip_gemm_lora_workspace.argtypes = [_I32] * 3
-        L.sslm_hip_pick_workspace.argtypes = [_I32] * 2
-        for name in ("shared_attention", "gemm_lora", "pick"):
+        L.sslm_hip_pick_workspace.argtypes = L.sslm_hip_sample_workspace.argtypes = [_I32] * 2
+        for name in ("shared_attention", "gemm_lora", "pick", "sample"):
             getattr(L, f"sslm_hip_{name}_workspace").restype = _SZ
 
     @staticmethod
@@ -117,3 +136,11 @@ class BatchOps:
         args = self._fill(PickArgs(), dict(fields, vocab=vocab, logits_ld=vocab if logits_ld is None else logits_ld,
                                            adjusted_ld=vocab if adjusted_ld is None else adjusted_ld))
         return Call(self.lib, "sslm_hip_pick_tokens", args, workspace, workspace_bytes)
+
+    def sample_workspace(self, rows, vocab) -> int:
+        return self.lib.lib.sslm_hip_sample_workspace(rows, vocab)
+
+    def sample_tokens(self, *, workspace, workspace_bytes, vocab, logits_ld=None, **fields) -> Call:
+        """sslm_hip_sample_tokens; `rules` is a device array of Sampling, the row stride defaults to the vocabulary."""
+        args = self._fill(SampleArgs(), dict(fields, vocab=vocab, logits_ld=vocab if logits_ld is None else logits_ld))
+        return Call(self.lib, "sslm_hip_sample_tokens", args, workspace, workspace_bytes)

@@ -1,33 +1,18 @@
 // Operators of a decode step whose rows differ (batch_ops.h): kernels, launches and C entries.
 #include <hip/hip_runtime.h>
-#include <stdio.h>
 
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
 
 #include "../../include/sslm_hip.h"
+#include "attention_util.h"
 #include "batch_ops.h"
-#include "device_util.h"
+#include "entry_util.h"
 
 namespace sslm {
 
 using sslm_launch::LogitRule;
-
-// A pointer that was read from memory is generic to the compiler, whose flat loads count as LDS operations
-// too: each wait for LDS would then be one for every load in flight.  All of these point to global memory.
-template <typename T>
-__device__ __forceinline__ const __attribute__((address_space(1))) T* global_ptr(const T* p) {
-	return (const __attribute__((address_space(1))) T*)p;
-}
-__device__ __forceinline__ v4i global16(const int8_t* p) { return *global_ptr((const v4i*)p); }
-
-struct __attribute__((packed)) unaligned16 {
-	v4i v;
-};
-struct __attribute__((packed)) unaligned4 {
-	int32_t v;
-};
 
 // ------------------------------------------------------------------------------------------
 // attention of rows that share prompts
@@ -74,66 +59,9 @@ __device__ __forceinline__ RowSpan row_span(const sslm_launch::SharedAttnArgs& a
 	return s;
 }
 
-struct RowConst {
-	int64_t q_ln2, q_b, q_c, ceil;
-	int32_t st;
-};
-
-// The softmax constants of (row, KV head) (forward_sites.cpp:1805-1830): the general form.
-__device__ __forceinline__ RowConst row_const_general(Scale sm, int64_t ln2_q, int64_t b_q, int64_t ca_q, int64_t width) {
-	RowConst c{0, 0, 0, 0, kOk};
-	if (iexp_scale_constants(sm.m, sm.e, ln2_q, b_q, ca_q, &c.q_ln2, &c.q_b, &c.q_c) != 0) c.st = kIExpScaleDerivationOutOfDomain;
-	else c.st = check_softmax_width(c.q_b, c.q_c, width);
-	if (c.st == kOk) c.ceil = softmax_ceiling(c.q_b, c.q_c);
-	return c;
-}
-
-// The same in 64 bits where it fits (iexp_scale_constants' products below 2^63 and 2^126, its shifts in
-// [1, 63], check_softmax_width's q_b below 2^24): some forty scalar instructions in the row's chain of
-// latencies instead of several hundred.
-struct RowScales {
-	Scale q;
-	int64_t km, ke;
-};
 __device__ __forceinline__ RowScales row_scales(const sslm_launch::SharedAttnArgs& a, int r, int kvh) {
 	return RowScales{a.q_scale[r], a.khead_m[kvh], a.khead_e[kvh]};
 }
-__device__ __forceinline__ RowConst row_const(const sslm_launch::SharedAttnArgs& a, const RowScales& rs, int64_t width) {
-	RowConst c{0, 0, 0, 0, kOk};
-	const Scale qs = rs.q;
-	const int64_t km = rs.km, ke = rs.ke;
-	if (!fits_i32(qs.m) || !fits_i32(km)) {
-		c.st = kCarriedScaleMantissaOutOfDomain;
-		return c;
-	}
-	const Scale sm = combine_scale(qs, Scale{km, ke});
-	if (!fits_i32(sm.m)) {
-		c.st = kCarriedScaleMantissaOutOfDomain;
-		return c;
-	}
-	const int64_t lim = (int64_t)1 << 30;
-	// 92 + e and 154 + 2 e in [1, 63] (e <= -46 already gives the latter's bound, e >= -76 its least)
-	if (sm.m >= lim && a.ln2_q > 0 && a.ln2_q < lim && a.b_q > 0 && a.b_q < 2 * lim && a.ca_q > 0 && a.ca_q < lim && sm.e >= -76 && sm.e <= -46) {
-		const uint64_t rc = (uint64_t)reciprocal_norm(sm.m);  // in (2^31, 2^32]
-		const uint64_t ca = (uint64_t)a.ca_q * rc, lo = ca * rc, hi = __umul64hi(ca, rc);
-		const int sh = (int)(92 + sm.e), sc = (int)(154 + 2 * sm.e);  // sc even, in [2, 62]
-		const uint64_t b = (uint64_t)a.b_q * rc >> sh;
-		if ((hi >> sc) == 0 && b < ((uint64_t)1 << 24)) {
-			const uint64_t qc = hi << (64 - sc) | lo >> sc, m = b * b + qc;
-			if (qc < ((uint64_t)1 << 62) && m >= 1) {
-				c.q_ln2 = (int64_t)((uint64_t)a.ln2_q * rc >> sh);
-				c.q_b = (int64_t)b;
-				c.q_c = (int64_t)qc;
-				const bool wide = m > (uint64_t)kSoftmaxMaxSafe || width <= 0 || __umul64hi(m, (uint64_t)width) != 0 || (int64_t)(m * (uint64_t)width) < 0;
-				c.st = wide ? kSoftmaxRowWidthOutOfDomain : kOk;
-				c.ceil = wide ? 0 : (int64_t)m;
-				return c;
-			}
-		}
-	}
-	return row_const_general(sm, a.ln2_q, a.b_q, a.ca_q, width);
-}
-
 // The layout of one call's launches.  The unit of work is a wave with a tile of 16 query rows and a
 // range of positions, a "plane": shared planes cut a prefix into sb positions each and their tiles hold
 // the query heads of one KV head of 16 / G neighbouring rows (G heads share a KV head), and the tiles of a block's
@@ -151,12 +79,6 @@ struct SaPlan {
 	int owned, ob;   // own planes and the positions of one
 	int ht;          // tiles of a row's own heads
 	int shared_blocks;
-};
-
-// (row, KV head): the softmax constants and whether the row is computed at all
-struct SaConst {
-	int64_t q_ln2, q_b, q_c, ceil;
-	int32_t st, pad;
 };
 
 struct SaWork {
@@ -180,8 +102,6 @@ struct SaJob {
 	int64_t start, width; // by lane: where the row's own positions begin, and its width
 	bool owned, first;    // an own plane; the row's first
 };
-
-__device__ __forceinline__ int64_t i64min(int64_t a, int64_t b) { return a < b ? a : b; }
 
 // A wave of the shared planes: false, for its whole block, when there is nothing to do.  A block's waves have
 // neighbouring tiles of one prefix and the same positions; a wave past the last tile has no live lane.
@@ -258,80 +178,6 @@ __device__ __forceinline__ void sa_load_q(const sslm_launch::SharedAttnArgs& a, 
 	}
 }
 
-// K or V rows of 64 positions on their way through LDS (32 D bytes of the wave's own, half the rows at a
-// time).  An MFMA operand has a row per lane, which as a global load touches 64 lines an instruction; loaded
-// D / 16 lanes to a row and turned in LDS it touches D / 2 (the maxima of 96 rows over 4096 positions: 20 us
-// with direct loads, whatever the waves and the loads in flight).  LDS operations of one wave take effect in
-// order, so no barrier but the compiler's stands between them.
-template <int D>
-struct SaRows {
-	static constexpr int PER = D / 16;
-	v4i r[PER];
-	// where 16-byte chunk `ch` of row `row` lies: chunks change places by row, so that one chunk of
-	// neighbouring rows covers all banks
-	static __device__ __forceinline__ int at(int row, int ch) { return row * D + ((ch ^ (row & (PER - 1))) << 4); }
-	// row(p): position p's row; positions past `last` repeat it
-	template <typename F>
-	__device__ __forceinline__ void load(int64_t p, int64_t last, F&& row) {
-		const int lane = threadIdx.x & 63;
-#pragma unroll
-		for (int u = 0; u < PER; ++u) {
-			const int i = lane + 64 * u;
-			r[u] = global16(row(i64min(p + i / PER, last)) + i % PER * 16);
-		}
-	}
-	// rows 32 h .. 32 h + 31 into LDS
-	__device__ __forceinline__ void stage(int8_t* lds, int h) const {
-		const int lane = threadIdx.x & 63;
-		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-		for (int u = 0; u < PER / 2; ++u) {
-			const int c = lane + 64 * u;
-			*(v4i*)(lds + at(c / PER, c % PER)) = r[h * (PER / 2) + u];
-		}
-		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-		__builtin_amdgcn_wave_barrier();
-	}
-	// As K: the scores of query operand q, added to s.  Lane (ri, g) gets those of query row ri at positions
-	// 16 t + 4 g + v.
-	template <int NC>
-	__device__ __forceinline__ void scores(int8_t* lds, const v4i (&q)[NC], v4i (&s)[4]) const {
-		const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4;
-#pragma unroll
-		for (int h = 0; h < 2; ++h) {
-			stage(lds, h);
-#pragma unroll
-			for (int t = 2 * h; t < 2 * h + 2; ++t) {
-#pragma unroll
-				for (int c = 0; c < NC; ++c) {
-					const int ch = c * 4 + g;  // q is zero past D
-					const v4i k = *(const v4i*)(lds + at((t & 1) * 16 + ri, D < 64 ? ch & (PER - 1) : ch));
-					s[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, q[c], s[t], 0, 0, 0);
-				}
-			}
-		}
-	}
-	// As V: context += P V by the byte-transposing LDS read, which gives lane (ri, g) dim 16 dt + ri of the
-	// positions in sa_pack's order.  Lane (ri, g) of acc[dt][part] holds dims 16 dt + 4 g .. + 3 of query row ri.
-	__device__ __forceinline__ void multiply(int8_t* lds, const v4i& lo, const v4i& nhi, v4i (&acc)[D / 16][2]) const {
-		const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4, i = ri >> 1, row = (i >> 2) * 16 + g * 4 + (i & 3);
-		v2i half[2][D / 16];
-#pragma unroll
-		for (int h = 0; h < 2; ++h) {
-			stage(lds, h);
-#pragma unroll
-			for (int dt = 0; dt < D / 16; ++dt)
-				half[h][dt] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(lds + at(row, dt) + 8 * (ri & 1)));
-		}
-#pragma unroll
-		for (int dt = 0; dt < D / 16; ++dt) {
-			const v4i b = v4i{half[0][dt].x, half[0][dt].y, half[1][dt].x, half[1][dt].y};
-			acc[dt][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, lo, acc[dt][0], 0, 0, 0);
-			acc[dt][1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, nhi, acc[dt][1], 0, 0, 0);
-		}
-	}
-};
-
 // The same from 64 rows that a whole block staged.
 template <int D, int NC>
 __device__ __forceinline__ void sa_block_scores(const int8_t* lds, const v4i (&q)[NC], v4i (&s)[4]) {
@@ -359,36 +205,6 @@ __device__ __forceinline__ void sa_block_multiply(const int8_t* lds, const v4i& 
 		acc[dt][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, lo, acc[dt][0], 0, 0, 0);
 		acc[dt][1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, nhi, acc[dt][1], 0, 0, 0);
 	}
-}
-
-// The i-exp of one query row in doubles, each value exact: with y = q_b - x for a score x below the
-// maximum (x <= 30 q_ln2 by the clip), z = floor(x / q_ln2) = floor((x + 1/2) / q_ln2), whose argument is at
-// least 1 / (2 q_ln2) from an integer and estimated within (q_b + 30 q_ln2) 2^-51 / q_ln2 of its value;
-// base = y + z q_ln2, and base^2 + q_c <= q_b^2 + q_c <= 2^47 by the softmax gate.  `fast` rows have
-// 0 <= q_b, q_ln2 <= 2 q_b + 1 (then base^2 <= q_b^2, so no value leaves the domain) and a sum
-// below 2^53, exact in doubles.  Eleven instructions a value; the integer form takes some forty.
-struct SaExp {
-	double ninv, c0, l, qc;
-	int32_t add, ymin;
-};
-__device__ __forceinline__ bool sa_fast(const SaConst& c, int64_t width) {
-	return c.q_b >= 0 && c.q_ln2 >= 1 && c.ceil >= 1 && c.q_ln2 <= 2 * c.q_b + 1 && (double)c.ceil * (double)width < 0x1p53;
-}
-__device__ __forceinline__ SaExp sa_exp_of(const SaConst& c, int32_t top) {
-	SaExp e;
-	e.l = (double)c.q_ln2;
-	e.ninv = -1.0 / e.l;
-	e.c0 = -((double)c.q_b + 0.5) * e.ninv;
-	e.qc = (double)c.q_c;
-	e.add = (int32_t)c.q_b - top;
-	e.ymin = (int32_t)(c.q_b - 30 * c.q_ln2);
-	return e;
-}
-__device__ __forceinline__ double sa_exp(const SaExp& e, int32_t score) {
-	const double y = (double)max(score + e.add, e.ymin);
-	const double z = floor(fma(y, e.ninv, e.c0));
-	const double base = fma(z, e.l, y);
-	return floor(ldexp(fma(base, base, e.qc), -(int)z));
 }
 
 // The wave's rows joined over their planes; a lane's row is read by the lanes ri, ri + 16, ri + 32, ri + 48,
@@ -569,7 +385,7 @@ __global__ __launch_bounds__(64 * kSaWaves) void k_sa_max(sslm_launch::SharedAtt
 	if (!j.owned || !j.first) return;
 	SaConst c{0, 0, 0, 0, sp.st, 0};
 	if (c.st == kOk) {
-		const RowConst rc = row_const(a, rs, sp.width);
+		const RowConst rc = row_const(rs, a.ln2_q, a.b_q, a.ca_q, sp.width);
 		c = SaConst{rc.q_ln2, rc.q_b, rc.q_c, rc.ceil, rc.st, 0};
 	}
 	if (lane == 0) {
@@ -634,40 +450,6 @@ __global__ __launch_bounds__(64 * kSaWaves, D <= 128 ? 4 : 2) void k_sa_sum(sslm
 		bad |= __shfl_xor(bad, o, 64);
 	}
 	if (g == 0 && live) w.psum[(size_t)j.plane * a.rows * a.NH + (size_t)j.r * a.NH + j.h] = bad ? -1 : sum;
-}
-
-// The Q15 probability floor(2^15 e / d) in doubles, d the row's sum: for d < 2^36 the truncation of
-// (2^15 e + 1/2) / d, which is at least 2^-37 from an integer and estimated within 2^-37; else an estimate
-// from below, off by less than one, and the exact remainder (a multiple of 2^-15 below 2^38).
-struct SaProb {
-	double c1, c2, d;  // small sums: 2^15 / d, 1 / (2 d); else the estimate's factor, unused, d / 2^15
-};
-__device__ __forceinline__ SaProb sa_prob_of(double d, bool small) {
-	SaProb p;
-	p.d = d * 0x1p-15;
-	p.c1 = small ? 32768.0 / d : (1.0 - 0x1p-50) / p.d;
-	p.c2 = 0.5 / d;
-	return p;
-}
-template <bool SMALL>
-__device__ __forceinline__ int32_t sa_prob(const SaProb& p, double e) {
-	if constexpr (SMALL) return (int32_t)fma(e, p.c1, p.c2);
-	const double q = floor(e * p.c1);
-	return (int32_t)q + (fma(-q, p.d, e) >= p.d ? 1 : 0);
-}
-
-// Probabilities p of 64 positions as two int8 MFMA operands with p = 256 hi + lo: lo is p's low byte taken
-// as signed, -hi = floor((127 - p) / 256) in [-128, 0] (hi itself reaches 128).  Byte 4 t + v of lane
-// (ri, g) is position 16 t + 4 g + v: the products sum over positions, so the scores' own order serves.
-__device__ __forceinline__ void sa_pack(const int32_t (&p)[16], v4i* lo, v4i* nhi) {
-#pragma unroll
-	for (int t = 0; t < 4; ++t) {
-		const uint32_t a = __builtin_amdgcn_perm(p[4 * t + 1], p[4 * t], 0x0c0c0400), b = __builtin_amdgcn_perm(p[4 * t + 3], p[4 * t + 2], 0x0c0c0400);
-		(*lo)[t] = (int)(a | b << 16);
-		const uint32_t c = __builtin_amdgcn_perm(127 - p[4 * t + 1], 127 - p[4 * t], 0x0c0c0501),
-		               d = __builtin_amdgcn_perm(127 - p[4 * t + 3], 127 - p[4 * t + 2], 0x0c0c0501);
-		(*nhi)[t] = (int)(c | d << 16);
-	}
 }
 
 template <int D>
@@ -899,7 +681,7 @@ __global__ __launch_bounds__(64 * kSaRowWaves, 2) void k_sa_row(sslm_launch::Sha
 	sa_folds<BS>(a, fc);
 	if (threadIdx.x == 0) s_first = 0xffffffffu;
 	for (int i = threadIdx.x; i < a.NH * D / 4; i += BS) ((v4i*)s_ctx)[i] = v4i{0, 0, 0, 0};
-	const RowConst rc = row_const(a, rs, sp.width);
+	const RowConst rc = row_const(rs, a.ln2_q, a.b_q, a.ca_q, sp.width);
 	const SaConst c{rc.q_ln2, rc.q_b, rc.q_c, rc.ceil, rc.st, 0};
 	int32_t m = INT32_MIN;
 #pragma unroll
@@ -1465,8 +1247,6 @@ namespace sslm_launch {
 
 constexpr int kSaTargetWaves = 1536;
 
-static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-
 bool shared_attn_ok(int rows, int NH, int NKV, int D) {
 	return rows >= 1 && NKV >= 1 && NH >= NKV && NH % NKV == 0 && (D == 32 || D == 64 || D == 128 || D == 256) &&
 	       (int64_t)NH * D <= kFunnelMaxN;
@@ -1705,38 +1485,7 @@ void pick_tokens(const PickArgs& a, hipStream_t s) {
 // ------------------------------------------------------------------------------------------
 // C entries
 // ------------------------------------------------------------------------------------------
-namespace {
-
 using namespace sslm_launch;
-
-constexpr int kMaxRows = 65535;  // a grid's y extent
-
-// A launch on the caller's stream: the stream belongs to the current device, and nothing throws
-// past the boundary.
-template <typename F>
-sslm_status on_stream(void* stream, F&& launch) {
-	int cur = -1;
-	hipDevice_t of = -1;
-	if (hipGetDevice(&cur) != hipSuccess) return SSLM_INVALID_ARGUMENT;
-	if (stream && (hipStreamGetDevice((hipStream_t)stream, &of) != hipSuccess || of != cur)) return SSLM_INVALID_ARGUMENT;
-	(void)hipGetLastError();  // an error left by an unrelated earlier call is not this call's
-	try {
-		launch((hipStream_t)stream);
-	} catch (const LaunchRefused& e) {
-		fprintf(stderr, "sslm_hip: launch refused (%s)\n", e.what);
-		return SSLM_HIP_LAUNCH_FAILED;
-	} catch (...) {
-		return SSLM_HIP_LAUNCH_FAILED;
-	}
-	return hipGetLastError() == hipSuccess ? SSLM_OK : SSLM_HIP_LAUNCH_FAILED;
-}
-
-bool workspace_ok(const void* ws, size_t have, size_t need, sslm_status* st) {
-	*st = !ws ? SSLM_INVALID_ARGUMENT : (((uintptr_t)ws % 256) ? SSLM_MISALIGNED_BUFFER : SSLM_BUFFER_TOO_SMALL);
-	return ws && (uintptr_t)ws % 256 == 0 && have >= need;
-}
-
-}  // namespace
 
 extern "C" {
 

@@ -1,0 +1,1021 @@
+// A cache in pages (cache_ops.h): kernels, launches and C entries.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/sslm_hip.h"
+#include "attention_util.h"
+#include "cache_ops.h"
+#include "entry_util.h"
+
+namespace sslm {
+
+using sslm_launch::CacheAttnArgs;
+using sslm_launch::CacheStoreArgs;
+using sslm_launch::kMaxShift;
+using sslm_launch::kMaxUnits;
+using sslm_launch::PageCompactArgs;
+using sslm_launch::Pages;
+using sslm_launch::PageUpdateArgs;
+
+__device__ __forceinline__ int64_t pages_for(int64_t positions, int lp) { return (positions + ((int64_t)1 << lp) - 1) >> lp; }
+
+// ------------------------------------------------------------------------------------------
+// pages change hands
+// ------------------------------------------------------------------------------------------
+constexpr int kPlanBlock = 1024;
+
+// The sum of v over the threads before this one; *total: over all.  s: kPlanBlock / 64 words.
+__device__ __forceinline__ int block_before(int v, int* total, int* s) {
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+	int x = v;
+	for (int o = 1; o < 64; o *= 2) {
+		const int y = __shfl_up(x, o, 64);
+		x += lane >= o ? y : 0;
+	}
+	__syncthreads();
+	if (lane == 63) s[wave] = x;
+	__syncthreads();
+	int before = 0, all = 0;
+	for (int i = 0; i < kPlanBlock / 64; ++i) {
+		before += i < wave ? s[i] : 0;
+		all += s[i];
+	}
+	*total = all;
+	return before + x - v;
+}
+
+// What a plan leaves for the launch that carries it out.
+struct PlanWork {
+	int32_t* state;   // [0]: whether there is anything to do, [1]: pages to copy
+	int32_t* off;     // [rows] a row's first free page in `free`
+	int32_t* tail;    // [rows] the page it gets a copy of, or -1
+	int32_t* low;     // [pages] the lowest row that writes into a page
+	int32_t* free;    // [pages] free pages in the order they are given out (compaction: the holes)
+	int32_t *from, *to;  // pages to copy
+	int32_t* old;     // [rows, table_ld] the tables as they were, where the new ones take their place
+};
+
+__global__ __launch_bounds__(256) void k_table_copy(const int32_t* from, int32_t* to, int64_t n) {
+	for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) to[i] = from[i];
+}
+
+// One block: bitmaps of the pages that rows hold (seen), hold more than once (multi), and hold without writing
+// into them or keep from outside (fixed), in LDS; then who gets a copy, how many pages each row takes, and the free
+// pages in ascending order.
+__global__ __launch_bounds__(kPlanBlock) void k_update_plan(PageUpdateArgs a, const int32_t* tables, PlanWork w) {
+	extern __shared__ uint32_t lds[];
+	__shared__ int s_scan[kPlanBlock / 64], s_bad, s_most;
+	const int tid = threadIdx.x, words = (a.pages + 31) / 32;
+	uint32_t *seen = lds, *multi = seen + words, *fixed = multi + words;
+	int32_t *s_src = (int32_t*)(fixed + words), *s_kept = s_src + a.rows;  // kept pages, bit 30: the row writes into the last
+	const int64_t cap = (int64_t)a.table_ld << a.lp;
+	if (tid == 0) {
+		s_bad = a.rows;
+		s_most = 0;
+	}
+	for (int i = tid; i < 3 * words; i += kPlanBlock) lds[i] = 0;
+	__syncthreads();
+	for (int r = tid; r < a.rows; r += kPlanBlock) {
+		const int s = a.source[r];
+		const int64_t keep = a.keep[r], room = a.room[r], len = s >= 0 && s < a.rows ? a.lengths[s] : 0;
+		const bool ok = s >= -1 && s < a.rows && len >= 0 && len <= cap && keep >= 0 && keep <= len && room >= keep && room <= cap;
+		if (!ok) atomicMin(&s_bad, r);
+		const int kept = ok ? (int)pages_for(keep, a.lp) : 0;
+		const bool writes = ok && (keep & (((int64_t)1 << a.lp) - 1)) && room > keep;
+		s_src[r] = s;
+		s_kept[r] = kept | (writes ? 1 << 30 : 0);
+		atomicMax(&s_most, kept);
+	}
+	if (a.held)
+		for (int p = tid; p < a.pages; p += kPlanBlock)
+			if (a.held[p]) atomicOr(&fixed[p >> 5], 1u << (p & 31));
+	__syncthreads();
+	const int most = s_most;
+	const int64_t cells = (int64_t)a.rows * most;
+	for (int64_t c = tid; c < cells; c += kPlanBlock) {
+		const int r = (int)(c / most), i = (int)(c - (int64_t)r * most), k = s_kept[r] & ~(1 << 30);
+		if (i >= k) continue;
+		const int p = tables[(int64_t)s_src[r] * a.table_ld + i];
+		if (p < 0 || p >= a.pages) {
+			atomicMin(&s_bad, r);
+			continue;
+		}
+		const uint32_t bit = 1u << (p & 31);
+		if (atomicOr(&seen[p >> 5], bit) & bit) atomicOr(&multi[p >> 5], bit);
+		if (!(s_kept[r] >> 30) || i < k - 1) atomicOr(&fixed[p >> 5], bit);
+	}
+	__syncthreads();
+	if (s_bad < a.rows) {
+		if (tid == 0) {
+			a.result[0] = SSLM_INVALID_ARGUMENT;
+			a.result[1] = a.result[2] = 0;
+			a.result[3] = s_bad;
+			w.state[0] = 0;
+		}
+		return;
+	}
+	// pages that only rows which write into them hold stay with the lowest of these
+	auto tail_of = [&](int r) { return tables[(int64_t)s_src[r] * a.table_ld + (s_kept[r] & ~(1 << 30)) - 1]; };
+	for (int r = tid; r < a.rows; r += kPlanBlock)
+		if (s_kept[r] >> 30) __hip_atomic_store(&w.low[tail_of(r)], a.rows, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+	__threadfence();
+	__syncthreads();
+	for (int r = tid; r < a.rows; r += kPlanBlock)
+		if (s_kept[r] >> 30) atomicMin(&w.low[tail_of(r)], r);
+	__threadfence();
+	__syncthreads();
+	int wants = 0, copies = 0;
+	for (int r0 = 0; r0 < a.rows; r0 += kPlanBlock) {
+		const int r = r0 + tid;
+		int n = 0, t = -1;
+		if (r < a.rows) {
+			if (s_kept[r] >> 30) {
+				const int p = tail_of(r);
+				const uint32_t bit = 1u << (p & 31);
+				if ((fixed[p >> 5] & bit) || ((multi[p >> 5] & bit) && __hip_atomic_load(&w.low[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < r)) t = p;
+			}
+			n = (int)pages_for(a.room[r], a.lp) - (s_kept[r] & ~(1 << 30)) + (t >= 0);
+		}
+		int all;
+		const int before = block_before(n, &all, s_scan) + wants;
+		int those;
+		const int mine = block_before(t >= 0, &those, s_scan) + copies;
+		if (r < a.rows) {
+			w.off[r] = before;
+			w.tail[r] = t;
+			if (t >= 0) {
+				w.from[mine] = t;
+				w.to[mine] = before;  // its place among the free pages
+			}
+		}
+		wants += all;
+		copies += those;
+	}
+	// free pages: neither seen nor held; a thread's are those of neighbouring words
+	const int per = (words + kPlanBlock - 1) / kPlanBlock;
+	auto free_bits = [&](int i) {
+		const uint32_t valid = a.pages - 32 * i >= 32 ? ~0u : (1u << (a.pages - 32 * i)) - 1;
+		return ~(seen[i] | fixed[i]) & valid;
+	};
+	int mine = 0, total;
+	for (int i = tid * per; i < min(words, (tid + 1) * per); ++i) mine += __popc(free_bits(i));
+	int at = block_before(mine, &total, s_scan);
+	const bool ok = wants <= total;
+	if (ok)
+		for (int i = tid * per; i < min(words, (tid + 1) * per) && at < wants; ++i)
+			for (uint32_t b = free_bits(i); b && at < wants; b &= b - 1) w.free[at++] = 32 * i + __builtin_ctz(b);
+	if (tid == 0) {
+		a.result[0] = ok ? SSLM_OK : SSLM_KV_POOL_EXHAUSTED;
+		a.result[1] = total - wants;
+		a.result[2] = ok ? copies : 0;
+		a.result[3] = -1;
+		w.state[0] = ok;
+		w.state[1] = ok ? copies : 0;
+	}
+}
+
+// Pages from one place of the pool to another, 16 KB to a block and step: no page is both read and written.
+constexpr int kCopyChunk = 16384;
+template <typename F>
+__device__ __forceinline__ void copy_pages(int8_t* pool, int64_t page_bytes, int n, F&& pair) {
+	const int chunks = (int)((page_bytes + kCopyChunk - 1) / kCopyChunk);
+	for (int64_t i = blockIdx.x; i < (int64_t)n * chunks; i += gridDim.x) {
+		const int c = (int)(i / chunks);
+		const int64_t at = (i - (int64_t)c * chunks) * kCopyChunk;
+		int from, to;
+		pair(c, &from, &to);
+		const int8_t* src = pool + from * page_bytes + at;
+		int8_t* dst = pool + to * page_bytes + at;
+		const int left = (int)i64min(page_bytes - at, kCopyChunk) / 16;
+		v4i x[kCopyChunk / 4096];
+#pragma unroll
+		for (int u = 0; u < kCopyChunk / 4096; ++u) x[u] = load16(src + 16 * min((int)threadIdx.x + 256 * u, left - 1));
+#pragma unroll
+		for (int u = 0; u < kCopyChunk / 4096; ++u)
+			if ((int)threadIdx.x + 256 * u < left) *(v4i*)(dst + 16 * (threadIdx.x + 256 * u)) = x[u];
+	}
+}
+
+__global__ __launch_bounds__(256) void k_update_apply(PageUpdateArgs a, const int32_t* tables, PlanWork w) {
+	if (!w.state[0]) return;
+	const int64_t cells = (int64_t)a.rows * a.table_ld;
+	for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < cells; c += (int64_t)gridDim.x * 256) {
+		const int r = (int)(c / a.table_ld), i = (int)(c - (int64_t)r * a.table_ld);
+		const int kept = (int)pages_for(a.keep[r], a.lp), need = (int)pages_for(a.room[r], a.lp), off = w.off[r];
+		const bool copied = w.tail[r] >= 0;
+		int p = -1;
+		if (i < kept) p = copied && i == kept - 1 ? w.free[off] : tables[(int64_t)a.source[r] * a.table_ld + i];
+		else if (i < need) p = w.free[off + copied + i - kept];
+		a.new_tables[c] = p;
+		if (i == 0) a.new_lengths[r] = a.room[r];
+	}
+	copy_pages(a.pool, a.page_bytes, w.state[1], [&](int c, int* from, int* to) {
+		*from = w.from[c];
+		*to = w.free[w.to[c]];
+	});
+}
+
+// One block: the pages in use and those held as bitmaps; the boundary before which the movable ones come to lie;
+// the holes before it and the movers after it, both in ascending order.
+__global__ __launch_bounds__(kPlanBlock) void k_compact_plan(PageCompactArgs a, PlanWork w) {
+	extern __shared__ uint32_t lds[];
+	__shared__ int s_scan[kPlanBlock / 64], s_bad, s_most, s_edge, s_top;
+	const int tid = threadIdx.x, words = (a.pages + 31) / 32;
+	uint32_t *live = lds, *held = live + words;
+	int32_t* rank = (int32_t*)(held + words);
+	const int64_t cap = (int64_t)a.table_ld << a.lp;
+	if (tid == 0) {
+		s_bad = a.rows;
+		s_most = 0;
+		s_edge = a.pages;
+		s_top = 0;
+	}
+	for (int i = tid; i < 2 * words; i += kPlanBlock) lds[i] = 0;
+	__syncthreads();
+	for (int r = tid; r < a.rows; r += kPlanBlock) {
+		const int64_t len = a.lengths[r];
+		const bool ok = len >= 0 && len <= cap;
+		if (!ok) atomicMin(&s_bad, r);
+		else atomicMax(&s_most, (int)pages_for(len, a.lp));
+	}
+	if (a.held)
+		for (int p = tid; p < a.pages; p += kPlanBlock)
+			if (a.held[p]) atomicOr(&held[p >> 5], 1u << (p & 31));
+	__syncthreads();
+	const int most = s_most;
+	const int64_t cells = s_bad < a.rows ? 0 : (int64_t)a.rows * most;
+	for (int64_t c = tid; c < cells; c += kPlanBlock) {
+		const int r = (int)(c / most), i = (int)(c - (int64_t)r * most);
+		if (i >= pages_for(a.lengths[r], a.lp)) continue;
+		const int p = a.tables[(int64_t)r * a.table_ld + i];
+		if (p < 0 || p >= a.pages) atomicMin(&s_bad, r);
+		else atomicOr(&live[p >> 5], 1u << (p & 31));
+	}
+	__syncthreads();
+	if (s_bad < a.rows) {
+		if (tid == 0) {
+			a.result[0] = SSLM_INVALID_ARGUMENT;
+			a.result[1] = a.result[2] = 0;
+			a.result[3] = s_bad;
+			w.state[0] = 0;
+		}
+		return;
+	}
+	const int per = (words + kPlanBlock - 1) / kPlanBlock, w0 = tid * per, w1 = min(words, w0 + per);
+	auto valid = [&](int i) { return a.pages - 32 * i >= 32 ? ~0u : (1u << (a.pages - 32 * i)) - 1; };
+	int mine = 0, movable, open;
+	for (int i = w0; i < w1; ++i) mine += __popc(live[i] & ~held[i]);
+	block_before(mine, &movable, s_scan);
+	mine = 0;
+	for (int i = w0; i < w1; ++i) mine += __popc(~held[i] & valid(i));
+	int at = block_before(mine, &open, s_scan);
+	for (int i = w0; i < w1; ++i) {  // the boundary: one past the last of the first `movable` pages that nobody holds
+		const uint32_t b = ~held[i] & valid(i);
+		const int n = __popc(b);
+		if (at < movable && at + n >= movable) {
+			uint32_t x = b;
+			for (int k = movable - at; k > 1; --k) x &= x - 1;
+			s_edge = 32 * i + __builtin_ctz(x) + 1;
+		}
+		at += n;
+	}
+	if (tid == 0 && movable == 0) s_edge = 0;
+	__syncthreads();
+	const int edge = s_edge;
+	auto below = [&](int i) { return 32 * i + 32 <= edge ? ~0u : (32 * i >= edge ? 0u : (1u << (edge - 32 * i)) - 1); };
+	auto holes = [&](int i) { return ~live[i] & ~held[i] & below(i) & valid(i); };
+	auto movers = [&](int i) { return live[i] & ~held[i] & ~below(i); };
+	mine = 0;
+	int nholes = 0, n2;
+	for (int i = w0; i < w1; ++i) mine += __popc(holes(i));
+	at = block_before(mine, &nholes, s_scan);
+	for (int i = w0; i < w1; ++i)
+		for (uint32_t b = holes(i); b; b &= b - 1) w.free[at++] = 32 * i + __builtin_ctz(b);
+	mine = 0;
+	for (int i = w0; i < w1; ++i) mine += __popc(movers(i));
+	at = block_before(mine, &n2, s_scan);
+	for (int i = w0; i < w1; ++i) {
+		rank[i] = at;
+		for (uint32_t b = movers(i); b; b &= b - 1) w.from[at++] = 32 * i + __builtin_ctz(b);
+	}
+	__syncthreads();  // the block's own writes of w.free are seen past it
+	int top = 0;
+	for (int p = tid; p < a.pages; p += kPlanBlock) {
+		const int i = p >> 5;
+		const uint32_t bit = 1u << (p & 31);
+		int to = -1;
+		if (movers(i) & bit) to = w.free[rank[i] + __popc(movers(i) & (bit - 1))];
+		else if (live[i] & bit) to = p;
+		a.map[p] = to;
+		if (to >= 0) top = max(top, to + 1);
+		if (held[i] & bit) top = max(top, p + 1);
+	}
+	atomicMax(&s_top, top);
+	__syncthreads();
+	if (tid == 0) {
+		a.result[0] = SSLM_OK;
+		a.result[1] = s_top;
+		a.result[2] = n2;
+		a.result[3] = -1;
+		w.state[0] = 1;
+		w.state[1] = n2;
+	}
+}
+
+__global__ __launch_bounds__(256) void k_compact_apply(PageCompactArgs a, PlanWork w) {
+	if (!w.state[0]) return;
+	const int64_t cells = (int64_t)a.rows * a.table_ld;
+	for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < cells; c += (int64_t)gridDim.x * 256) {
+		const int r = (int)(c / a.table_ld), i = (int)(c - (int64_t)r * a.table_ld);
+		const int p = i < pages_for(a.lengths[r], a.lp) ? a.map[a.tables[c]] : -1;
+		a.new_tables[c] = p;
+	}
+	copy_pages(a.pool, a.page_bytes, w.state[1], [&](int c, int* from, int* to) {
+		*from = w.from[c];
+		*to = w.free[c];
+	});
+}
+
+// ------------------------------------------------------------------------------------------
+// new tokens land in pages
+// ------------------------------------------------------------------------------------------
+
+// A row's tokens, as far as the tables and lengths admit them.
+struct CacheRow {
+	int64_t start;
+	int t0, n;
+	bool ok;
+};
+__device__ __forceinline__ CacheRow cache_row(const int32_t* row_tokens, const int64_t* row_start, int r, int tokens, int max_new, int64_t cap) {
+	CacheRow c;
+	c.t0 = row_tokens[r];
+	const int t1 = row_tokens[r + 1];
+	c.start = row_start[r];
+	c.n = t1 - c.t0;
+	c.ok = c.t0 >= 0 && t1 >= c.t0 && t1 <= tokens;
+	if (!c.ok) c.n = 0;
+	c.ok = c.ok && c.n <= max_new && c.start >= 0 && c.start <= cap - c.n;
+	return c;
+}
+
+// A block per row: whether its tokens can land.
+__global__ __launch_bounds__(256) void k_store_check(CacheStoreArgs a) {
+	__shared__ int s_st;
+	const int r = blockIdx.x;
+	int64_t cap = (int64_t)a.pg.table_ld << a.pg.lp;
+	if (a.rope_dim) cap = i64min(cap, a.rope_rows);
+	const CacheRow c = cache_row(a.row_tokens, a.row_start, r, a.tokens, a.max_new, cap);
+	if (threadIdx.x == 0) s_st = c.ok ? 0 : 2;
+	__syncthreads();
+	if (c.ok && c.n > 0) {
+		int st = 0;
+		const int p0 = (int)(c.start >> a.pg.lp), p1 = (int)((c.start + c.n - 1) >> a.pg.lp);
+		for (int i = p0 + (int)threadIdx.x; i <= p1; i += 256) {
+			const int p = a.pg.tables[(int64_t)r * a.pg.table_ld + i];
+			if (p < 0 || p >= a.pg.pages) st = 2;
+		}
+		for (int i = threadIdx.x; i < c.n; i += 256)
+			if (!fits_i32(a.k_scale[c.t0 + i].m) || !fits_i32(a.v_scale[c.t0 + i].m)) st = max(st, 1);
+		if (st) atomicMax(&s_st, st);
+	}
+	__syncthreads();
+	if (threadIdx.x == 0) {
+		a.clamped[r] = 0;
+		a.status[r] = s_st == 2 ? kPositionOverCap : (s_st == 1 ? kCarriedScaleMantissaOutOfDomain : kOk);
+	}
+}
+
+struct __attribute__((packed)) unaligned8 {
+	uint64_t v;
+};
+
+// Eight dims of a head that turn or stay together, group g of D / 8: with halves, dims 4 g .. + 3 and the ones
+// rope_dim / 2 further on; else 8 g .. + 7.  Element i of a pair is x[2 i], x[2 i + 1].
+struct Octet {
+	int32_t x[8];
+};
+__device__ __forceinline__ bool octet_split(const CacheStoreArgs& a, int g) { return a.halves && 8 * g < a.rope_dim; }
+__device__ __forceinline__ Octet octet_load(const CacheStoreArgs& a, const int8_t* head, int g) {
+	Octet o;
+	uint64_t w;
+	if (octet_split(a, g)) {
+		const uint32_t lo = (uint32_t)((const unaligned4*)(head + 4 * g))->v, hi = (uint32_t)((const unaligned4*)(head + a.rope_dim / 2 + 4 * g))->v;
+#pragma unroll
+		for (int i = 0; i < 4; ++i) {
+			o.x[2 * i] = (int8_t)(lo >> 8 * i);
+			o.x[2 * i + 1] = (int8_t)(hi >> 8 * i);
+		}
+		return o;
+	}
+	w = ((const unaligned8*)(head + 8 * g))->v;
+#pragma unroll
+	for (int i = 0; i < 8; ++i) o.x[i] = (int8_t)(w >> 8 * i);
+	return o;
+}
+__device__ __forceinline__ void octet_store(const CacheStoreArgs& a, int8_t* head, int g, const Octet& o) {
+	if (octet_split(a, g)) {
+		uint32_t lo = 0, hi = 0;
+#pragma unroll
+		for (int i = 0; i < 4; ++i) {
+			lo |= (uint32_t)(uint8_t)o.x[2 * i] << 8 * i;
+			hi |= (uint32_t)(uint8_t)o.x[2 * i + 1] << 8 * i;
+		}
+		((unaligned4*)(head + 4 * g))->v = (int32_t)lo;
+		((unaligned4*)(head + a.rope_dim / 2 + 4 * g))->v = (int32_t)hi;
+		return;
+	}
+	uint64_t w = 0;
+#pragma unroll
+	for (int i = 0; i < 8; ++i) w |= (uint64_t)(uint8_t)o.x[i] << 8 * i;
+	((unaligned8*)(head + 8 * g))->v = w;
+}
+// The four pairs turned at `pos`, clamped to +-top; returns how many values were.
+struct Turn {
+	int32_t c[4], s[4];
+};
+__device__ __forceinline__ Turn turn_at(const CacheStoreArgs& a, int64_t pos, int g) {
+	Turn t;
+	const int64_t at = pos * (a.rope_dim / 2) + 4 * g;
+#pragma unroll
+	for (int i = 0; i < 4; ++i) {
+		t.c[i] = (int32_t)a.rope_cos[at + i];
+		t.s[i] = (int32_t)a.rope_sin[at + i];
+	}
+	return t;
+}
+__device__ __forceinline__ int octet_turn(Octet& o, const Turn& t, int32_t top) {
+	int n = 0;
+#pragma unroll
+	for (int i = 0; i < 4; ++i) {
+		int64_t y[2];
+		rope_pair(o.x[2 * i], o.x[2 * i + 1], t.c[i], t.s[i], &y[0], &y[1]);
+#pragma unroll
+		for (int j = 0; j < 2; ++j) {
+			n += y[j] > top || y[j] < -top;
+			o.x[2 * i + j] = (int32_t)(y[j] > top ? top : (y[j] < -top ? -top : y[j]));
+		}
+	}
+	return n;
+}
+
+// x / 2^e in units, ties away from zero, at exponent `at` and then at each of `levels` past it: a page's codes are
+// rounded once more whenever it grows.
+__device__ __forceinline__ int32_t grown_code(int32_t x, int at, uint32_t levels) {
+	x = rdbpot32(x, at);
+	for (uint32_t m = levels & ~((2u << at) - 1); m; m &= m - 1) {
+		const int to = __builtin_ctz(m);
+		x = rdbpot32(x, to - at);
+		at = to;
+	}
+	return x;
+}
+// the least exponent that keeps a code of magnitude m within 127
+__device__ __forceinline__ int exponent_for(int32_t m) {
+	int e = 0;
+	while (rdbpot32(m, e) > 127) ++e;
+	return e;
+}
+
+// K or V of one KV head (z) in one page (x) of one row (y): the page's tokens land in LDS, their exponents run up the
+// page, then the codes are written; blocks past the last page take q's tokens, four each, and an equal share of the heads.
+constexpr int kStoreBlock = 256;
+template <int D>
+__global__ __launch_bounds__(kStoreBlock) void k_store_span(CacheStoreArgs a, int pages) {
+	extern __shared__ __attribute__((aligned(16))) int16_t s_x[];  // [page's tokens][D], groups of eight in octet order
+	__shared__ uint8_t s_need[256];
+	__shared__ uint32_t s_levels;
+	__shared__ int s_init, s_clamped;
+	constexpr int GP = D / 8;
+	const int r = blockIdx.y, z = blockIdx.z, tid = threadIdx.x;
+	if (a.status[r] != kOk) return;
+	const int t0 = a.row_tokens[r], n = a.row_tokens[r + 1] - t0;
+	const int64_t start = a.row_start[r];
+	if ((int)blockIdx.x >= pages) {
+		const int i = ((int)blockIdx.x - pages) * (kStoreBlock / 64) + (tid >> 6);
+		if (i >= n) return;
+		const int g = tid % GP;
+		const bool turns = 8 * g < a.rope_dim;
+		Turn t;
+		if (turns) t = turn_at(a, start + i, g);
+		for (int h = z + (int)gridDim.z * ((tid & 63) / GP); h < a.NH; h += (int)gridDim.z * (64 / GP)) {
+			Octet o = octet_load(a, a.q + (int64_t)(t0 + i) * a.q_ld + h * D, g);
+			if (turns) octet_turn(o, t, 127);
+			octet_store(a, a.q_out + ((int64_t)(t0 + i) * a.NH + h) * D, g, o);
+		}
+		return;
+	}
+	const int P = 1 << a.pg.lp;
+	const int64_t page0 = start >> a.pg.lp, first = (page0 + blockIdx.x) << a.pg.lp;
+	const int i0 = (int)(first > start ? first - start : 0), i1 = (int)i64min(n, first + P - start);  // the row's tokens in the page
+	if (i0 >= i1) return;
+	const int slot0 = (int)(start + i0 - first), cnt = i1 - i0, kvh = z >> 1;
+	const bool isv = z & 1;
+	int8_t* page = a.pg.pool + a.pg.tables[(int64_t)r * a.pg.table_ld + page0 + blockIdx.x] * a.pg.page_bytes;
+	int8_t* head = page + (isv ? a.pg.v_off : a.pg.k_off) + ((int64_t)kvh << a.pg.lp) * D;
+	uint8_t* exp = (uint8_t*)page + a.pg.e_off + (isv ? a.pg.NKV : 0) + kvh;
+	if (tid == 0) {
+		s_levels = 0;
+		s_clamped = 0;
+		s_init = slot0 ? min((int)*exp, kMaxShift) : 0;
+	}
+	__syncthreads();
+	const int64_t rt = isv ? a.r_t_v[kvh] : a.r_t_k[kvh], et = isv ? a.e_t_v[kvh] : a.e_t_k[kvh];
+	int clamped = 0;
+	for (int u = tid; u < (cnt * GP + kStoreBlock - 1) / kStoreBlock * kStoreBlock; u += kStoreBlock) {
+		const bool in = u < cnt * GP;
+		const int i = in ? u / GP : 0, g = u % GP, t = t0 + i0 + i;
+		const Scale sc = isv ? a.v_scale[t] : a.k_scale[t];
+		const int8_t* from = isv ? a.v + t * a.v_ld : a.k + t * a.k_ld;
+		Octet o = octet_load(a, from + kvh * D, g);
+		const int64_t k = composed_exponent(sc.e, et);
+		const double f = landing_scale(sc.m, rt, k).f;
+		int32_t mx = 0, over = 0;
+#pragma unroll
+		for (int j = 0; j < 8; ++j) {
+			const double x = residual_land(o.x[j], sc.m, rt, k, f);
+			const double lim = kMaxUnits;
+			over += fabs(x) > lim;
+			o.x[j] = (int32_t)fmin(fmax(x, -lim), lim);
+		}
+		if (!isv && 8 * g < a.rope_dim) over += octet_turn(o, turn_at(a, start + i0 + i, g), kMaxUnits);
+		union {
+			int16_t h[8];
+			v4i v;
+		} pk;
+#pragma unroll
+		for (int j = 0; j < 8; ++j) {
+			mx = max(mx, abs(o.x[j]));
+			pk.h[j] = (int16_t)o.x[j];
+		}
+		for (int d = 1; d < GP; d *= 2) mx = max(mx, __shfl_xor(mx, d, 64));
+		if (in) {
+			*(v4i*)(s_x + (int64_t)u * 8) = pk.v;
+			if (g == 0) s_need[i] = (uint8_t)exponent_for(mx);
+			clamped += over;
+		}
+	}
+	clamped = wave_sum32(clamped);
+	if ((tid & 63) == 0 && clamped) atomicAdd(&s_clamped, clamped);
+	__syncthreads();
+	if (tid < 64) {  // the exponents the page has after each of its tokens
+		int e[4], m = 0;
+#pragma unroll
+		for (int j = 0; j < 4; ++j) {
+			if (4 * tid + j < cnt) m = max(m, (int)s_need[4 * tid + j]);
+			e[j] = m;
+		}
+		for (int d = 1; d < 64; d *= 2) {
+			const int y = __shfl_up(m, d, 64);
+			m = tid >= d ? max(m, y) : m;
+		}
+		int before = __shfl_up(m, 1, 64);
+		before = max(tid ? before : 0, s_init);
+		uint32_t levels = 0;
+#pragma unroll
+		for (int j = 0; j < 4; ++j)
+			if (4 * tid + j < cnt) {
+				e[j] = max(e[j], before);
+				s_need[4 * tid + j] = (uint8_t)e[j];
+				levels |= 1u << e[j];
+			}
+		if (levels) atomicOr(&s_levels, levels);
+	}
+	__syncthreads();
+	const uint32_t levels = s_levels;
+	for (int u = tid; u < cnt * GP; u += kStoreBlock) {
+		const int i = u / GP, g = u % GP;
+		Octet o;
+		union {
+			int16_t h[8];
+			v4i v;
+		} pk;
+		pk.v = *(const v4i*)(s_x + (int64_t)u * 8);
+#pragma unroll
+		for (int j = 0; j < 8; ++j) o.x[j] = grown_code(pk.h[j], s_need[i], levels);
+		octet_store(a, head + (int64_t)(slot0 + i) * D, g, o);
+	}
+	const int init = s_init;
+	if (slot0 && levels >> (init + 1)) {
+		for (int u = tid; u < slot0 * GP; u += kStoreBlock) {
+			int8_t* at = head + (int64_t)u * 8;
+			uint64_t w = ((const unaligned8*)at)->v, out = 0;
+#pragma unroll
+			for (int j = 0; j < 8; ++j) {
+				int32_t x = (int8_t)(w >> 8 * j);
+				x = grown_code(x, 0, levels >> init & ~1u);
+				out |= (uint64_t)(uint8_t)x << 8 * j;
+			}
+			((unaligned8*)at)->v = out;
+		}
+	}
+	if (tid == 0) {
+		*exp = (uint8_t)(31 - __builtin_clz(levels));
+		if (s_clamped) atomicAdd(&a.clamped[r], s_clamped);
+	}
+}
+
+// ------------------------------------------------------------------------------------------
+// attention over pages
+// ------------------------------------------------------------------------------------------
+
+// A block per (token, head): maxima, sums and P V in three passes over the row's positions.
+template <int D>
+__global__ __launch_bounds__(256) void k_ca_head(CacheAttnArgs a, int32_t* ctx, int32_t* hst) {
+	__shared__ __attribute__((aligned(16))) int8_t s_q[D];
+	__shared__ int32_t s_p[256], s_m[4], s_bad;
+	__shared__ int64_t s_sum[4];
+	__shared__ int32_t s_ctx[256];
+	const int r = blockIdx.y, h = blockIdx.z, tid = threadIdx.x, kvh = h / (a.NH / a.pg.NKV);
+	const CacheRow c = cache_row(a.row_tokens, a.row_start, r, a.tokens, a.max_new, i64min((int64_t)a.pg.table_ld << a.pg.lp, a.max_width));
+	if ((int)blockIdx.x >= c.n) return;
+	const int t = c.t0 + blockIdx.x, lane = tid & 63, wave = tid >> 6;
+	const int64_t width = c.start + blockIdx.x + 1;
+	int32_t* out = hst + (size_t)t * a.NH + h;
+	if (tid == 0) s_bad = c.ok ? 0 : 1;
+	__syncthreads();
+	if (c.ok)
+		for (int64_t i = tid; i < (c.start + c.n + (1 << a.pg.lp) - 1) >> a.pg.lp; i += 256) {
+			const int p = a.pg.tables[(int64_t)r * a.pg.table_ld + i];
+			if (p < 0 || p >= a.pg.pages) s_bad = 1;
+		}
+	if (tid < D / 16) ((v4i*)s_q)[tid] = ((const unaligned16*)(a.q + ((size_t)t * a.NH + h) * D + 16 * tid))->v;
+	__syncthreads();
+	if (s_bad) {
+		if (tid == 0) *out = kPositionOverCap;
+		return;
+	}
+	const RowConst rc = row_const(RowScales{a.q_scale[t], a.khead_m[kvh], a.khead_e[kvh]}, a.ln2_q, a.b_q, a.ca_q, width);
+	if (rc.st != kOk) {
+		if (tid == 0) *out = rc.st;
+		return;
+	}
+	auto page_of = [&](int64_t p) { return a.pg.pool + a.pg.tables[(int64_t)r * a.pg.table_ld + (p >> a.pg.lp)] * a.pg.page_bytes; };
+	auto slot = [&](int64_t p) { return (((int64_t)kvh << a.pg.lp) + (p & ((1 << a.pg.lp) - 1))) * D; };
+	auto score = [&](int64_t p) {
+		const int8_t *pg = page_of(p), *k = pg + a.pg.k_off + slot(p);
+		int32_t s = 0;
+		for (int d = 0; d < D; d += 4) {
+			const int x = *(const int*)(k + d), y = *(const int*)(s_q + d);
+			s = __builtin_amdgcn_sdot4(x, y, s, false);
+		}
+		return s << min((int)((const uint8_t*)pg)[a.pg.e_off + kvh], kMaxShift);
+	};
+	int32_t m = INT32_MIN;
+	for (int64_t p = tid; p < width; p += 256) m = max(m, score(p));
+	for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o, 64));
+	if (lane == 0) s_m[wave] = m;
+	__syncthreads();
+	m = max(max(s_m[0], s_m[1]), max(s_m[2], s_m[3]));
+	const double inv = 1.0 / (double)rc.q_ln2;
+	int64_t sum = 0;
+	bool bad = false;
+	for (int64_t p = tid; p < width; p += 256) {
+		const int64_t x = iexp_fast_cold((int64_t)score(p) - m, rc.q_ln2, inv, rc.q_b, rc.q_c, rc.ceil);
+		bad |= x < 0;
+		sum += x < 0 ? 0 : x;
+	}
+	for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+	if (lane == 0) s_sum[wave] = sum;
+	if (bad) s_bad = 1;
+	__syncthreads();
+	if (s_bad) {
+		if (tid == 0) *out = kSoftmaxKernelRefusedAfterGateAccepted;
+		return;
+	}
+	sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+	const int64_t den = sum > 1 ? sum : 1;
+	const double dinv = 1.0 / (double)den;
+	int32_t acc = 0;
+	const int dim = tid % D, part = tid / D;
+	for (int64_t p0 = 0; p0 < width; p0 += 256) {
+		__syncthreads();
+		s_p[tid] = p0 + tid < width ? (int32_t)div_rcp_cold(iexp_fast_cold((int64_t)score(p0 + tid) - m, rc.q_ln2, inv, rc.q_b, rc.q_c, rc.ceil) << 15, den, dinv, 32768) : 0;
+		__syncthreads();
+		for (int64_t p = p0 + part; p < i64min(width, p0 + 256); p += 256 / D) {
+			const int8_t* pg = page_of(p);
+			acc += s_p[p - p0] * (pg[a.pg.v_off + slot(p) + dim] << min((int)((const uint8_t*)pg)[a.pg.e_off + a.pg.NKV + kvh], kMaxShift));
+		}
+	}
+	s_ctx[tid] = acc;
+	__syncthreads();
+	if (tid < D) {
+		for (int i = 1; i < 256 / D; ++i) acc += s_ctx[tid + i * D];
+		ctx[((size_t)t * a.NH + h) * D + tid] = acc;
+	}
+	if (tid == 0) *out = kOk;
+}
+
+// The fold and funnel of one token's context, a block per token.
+__global__ __launch_bounds__(256) void k_ca_out(CacheAttnArgs a, const int32_t* ctx, const int32_t* hst) {
+	__shared__ uint32_t s_first, s_max;
+	const int r = blockIdx.y, tid = threadIdx.x, N = a.NH * a.pg.D;
+	const CacheRow c = cache_row(a.row_tokens, a.row_start, r, a.tokens, a.max_new, i64min((int64_t)a.pg.table_ld << a.pg.lp, a.max_width));
+	if ((int)blockIdx.x >= c.n) return;
+	const int t = c.t0 + blockIdx.x;
+	if (tid == 0) {
+		s_first = 0xffffffffu;
+		s_max = 0;
+	}
+	__syncthreads();
+	for (int h = tid; h < a.NH; h += 256) {
+		const int32_t st = hst[(size_t)t * a.NH + h];
+		if (st != kOk) atomicMin(&s_first, (uint32_t)h << 8 | (uint32_t)st);
+	}
+	__syncthreads();
+	if (s_first != 0xffffffffu) {
+		if (tid == 0) a.status[t] = (int32_t)(s_first & 0xff);
+		return;
+	}
+	auto value = [&](int i) {
+		const int32_t* f = a.ctx_fold + 3 * (i / a.pg.D);
+		return fold_bounded(ctx[(size_t)t * N + i], fold_consts(f[0], f[1], f[2]));
+	};
+	uint32_t mx = 0;
+	for (int i = tid; i < N; i += 256) {
+		const int32_t v = value(i);
+		mx = max(mx, (uint32_t)(v < 0 ? -v : v));
+	}
+	atomicMax(&s_max, mx);
+	__syncthreads();
+	FunnelPlan plan;
+	const int32_t st = funnel_plan(__builtin_amdgcn_readfirstlane(s_max), nullptr, 0, a.site, &plan);
+	if (tid == 0) {
+		a.status[t] = st;
+		if (st == kOk) a.scales[t] = plan.out;
+	}
+	if (st != kOk) return;
+	for (int i = tid; i < N; i += 256) a.codes[(size_t)t * N + i] = requant_code_f(value(i), plan.f);
+}
+
+}  // namespace sslm
+
+// ------------------------------------------------------------------------------------------
+// launches
+// ------------------------------------------------------------------------------------------
+namespace sslm_launch {
+
+static size_t plan_work(int rows, int pages, int table_ld, char* base, PlanWork* w) {
+	size_t at = 0;
+	auto take = [&](size_t n) {
+		int32_t* p = (int32_t*)(base + at);
+		at += up256(n * 4);
+		return p;
+	};
+	w->state = take(2);
+	w->off = take(rows);
+	w->tail = take(rows);
+	w->low = take(pages);
+	w->free = take(pages);
+	w->from = take(std::max(rows, pages));
+	w->to = take(rows);
+	w->old = take((size_t)rows * table_ld);
+	return at;
+}
+
+size_t page_update_workspace(int rows, int pages, int table_ld) {
+	PlanWork w;
+	return plan_work(rows, pages, table_ld, nullptr, &w);
+}
+size_t page_compact_workspace(int rows, int pages, int table_ld) {
+	PlanWork w;
+	return plan_work(rows, pages, table_ld, nullptr, &w);
+}
+
+template <typename K>
+static void allow_lds(K kernel, size_t bytes) {
+	if (bytes > 65536 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess)
+		throw LaunchRefused{"dynamic LDS"};
+}
+
+// blocks for a launch over `cells` entries and up to `copies` pages
+static int apply_blocks(int64_t cells, int64_t copies, int64_t page_bytes) {
+	const int64_t want = std::max((cells + 255) / 256, copies * ((page_bytes + kCopyChunk - 1) / kCopyChunk));
+	return (int)std::min<int64_t>(2048, std::max<int64_t>(1, want));
+}
+
+void page_update(const PageUpdateArgs& a, hipStream_t s) {
+	PlanWork w;
+	plan_work(a.rows, a.pages, a.table_ld, (char*)a.ws, &w);
+	const int64_t cells = (int64_t)a.rows * a.table_ld;
+	const int32_t* tables = a.tables;
+	if (a.new_tables < a.tables + cells && a.tables < a.new_tables + cells) {  // in place: rows are read by others' blocks
+		hipLaunchKernelGGL(k_table_copy, dim3((int)std::min<int64_t>(1024, (cells + 255) / 256)), dim3(256), 0, s, a.tables, w.old, cells);
+		tables = w.old;
+	}
+	const size_t lds = 3 * (size_t)((a.pages + 31) / 32) * 4 + (size_t)a.rows * 8;
+	allow_lds(k_update_plan, lds);
+	hipLaunchKernelGGL(k_update_plan, dim3(1), dim3(kPlanBlock), lds, s, a, tables, w);
+	hipLaunchKernelGGL(k_update_apply, dim3(apply_blocks(cells, a.rows, a.page_bytes)), dim3(256), 0, s, a, tables, w);
+}
+
+void page_compact(const PageCompactArgs& a, hipStream_t s) {
+	PlanWork w;
+	plan_work(a.rows, a.pages, a.table_ld, (char*)a.ws, &w);
+	const size_t lds = 3 * (size_t)((a.pages + 31) / 32) * 4;
+	allow_lds(k_compact_plan, lds);
+	hipLaunchKernelGGL(k_compact_plan, dim3(1), dim3(kPlanBlock), lds, s, a, w);
+	hipLaunchKernelGGL(k_compact_apply, dim3(apply_blocks((int64_t)a.rows * a.table_ld, a.pages, a.page_bytes)), dim3(256), 0, s, a, w);
+}
+
+template <int D>
+static void store_launch(const CacheStoreArgs& a, hipStream_t s) {
+	const int P = 1 << a.pg.lp, pages = (a.max_new + P - 2) / P + 1;
+	const int qs = a.q ? (a.max_new + kStoreBlock / 64 - 1) / (kStoreBlock / 64) : 0;
+	const size_t lds = (size_t)std::min(P, a.max_new) * D * 2;
+	allow_lds(k_store_span<D>, lds);
+	hipLaunchKernelGGL(k_store_check, dim3(a.rows), dim3(256), 0, s, a);
+	hipLaunchKernelGGL(k_store_span<D>, dim3(pages + qs, a.rows, 2 * a.pg.NKV), dim3(kStoreBlock), lds, s, a, pages);
+}
+
+void cache_store(const CacheStoreArgs& a, hipStream_t s) {
+	switch (a.pg.D) {
+		case 32: return store_launch<32>(a, s);
+		case 64: return store_launch<64>(a, s);
+		case 128: return store_launch<128>(a, s);
+		default: return store_launch<256>(a, s);
+	}
+}
+
+size_t cache_attn_workspace(int rows, int tokens, int max_new, int NH, int NKV, int D, int lp, int64_t max_width) {
+	return up256((size_t)tokens * NH * D * 4) + up256((size_t)tokens * NH * 4);
+}
+
+template <int D>
+static void attn_launch(const CacheAttnArgs& a, hipStream_t s) {
+	int32_t* ctx = (int32_t*)a.ws;
+	int32_t* hst = (int32_t*)((char*)a.ws + up256((size_t)a.tokens * a.NH * D * 4));
+	hipLaunchKernelGGL(k_ca_head<D>, dim3(a.max_new, a.rows, a.NH), dim3(256), 0, s, a, ctx, hst);
+	hipLaunchKernelGGL(k_ca_out, dim3(a.max_new, a.rows), dim3(256), 0, s, a, ctx, hst);
+}
+
+void cache_attn(const CacheAttnArgs& a, hipStream_t s) {
+	switch (a.pg.D) {
+		case 32: return attn_launch<32>(a, s);
+		case 64: return attn_launch<64>(a, s);
+		case 128: return attn_launch<128>(a, s);
+		default: return attn_launch<256>(a, s);
+	}
+}
+
+}  // namespace sslm_launch
+
+// ------------------------------------------------------------------------------------------
+// C entries
+// ------------------------------------------------------------------------------------------
+using namespace sslm_launch;
+
+static int log2_page(int32_t positions) {
+	for (int lp = 4; lp <= 8; ++lp)
+		if (positions == 1 << lp) return lp;
+	return -1;
+}
+
+static bool plan_ok(int32_t rows, int32_t pages, int32_t table_ld) {
+	return rows >= 1 && rows <= SSLM_HIP_CACHE_MAX_ROWS && pages >= 1 && pages <= SSLM_HIP_CACHE_MAX_PAGES && table_ld >= 1 &&
+	       table_ld <= SSLM_HIP_CACHE_MAX_WIDTH / 16;
+}
+
+static bool pool_ok(const void* pool, int64_t page_bytes, int32_t pages) {
+	return pool && (uintptr_t)pool % 16 == 0 && page_bytes >= 16 && page_bytes % 16 == 0 && page_bytes <= ((int64_t)1 << 40) / pages;
+}
+
+// One layer's view: K, V and the exponents within a page.
+static bool layer_ok(const Pages& g) {
+	const int64_t half = ((int64_t)g.NKV << g.lp) * g.D;
+	return g.k_off >= 0 && g.v_off >= 0 && g.e_off >= 0 && g.k_off % 16 == 0 && g.v_off % 16 == 0 && g.page_bytes >= half &&
+	       g.k_off <= g.page_bytes - half && g.v_off <= g.page_bytes - half && g.e_off <= g.page_bytes - 2 * (int64_t)g.NKV;
+}
+
+static bool heads_ok(int32_t heads, int32_t kv_heads, int32_t d) {
+	return heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 && (d == 32 || d == 64 || d == 128 || d == 256) && (int64_t)heads * d <= 8192;
+}
+
+extern "C" {
+
+size_t sslm_hip_cache_update_workspace(int32_t rows, int32_t pages, int32_t table_ld) {
+	return plan_ok(rows, pages, table_ld) ? page_update_workspace(rows, pages, table_ld) : 0;
+}
+
+sslm_status sslm_hip_cache_update(const sslm_hip_cache_update_args* p, void* workspace, size_t workspace_bytes, void* stream) {
+	if (!p || p->struct_size != sizeof(*p)) return SSLM_INVALID_ARGUMENT;
+	const size_t need = sslm_hip_cache_update_workspace(p->rows, p->pages, p->table_ld);
+	const int lp = log2_page(p->page_tokens);
+	if (!need || lp < 0 || !pool_ok(p->pool, p->page_bytes, p->pages) || !p->tables || !p->lengths || !p->source || !p->keep || !p->room ||
+	    !p->new_tables || !p->new_lengths || !p->result)
+		return SSLM_INVALID_ARGUMENT;
+	sslm_status st;
+	if (!workspace_ok(workspace, workspace_bytes, need, &st)) return st;
+	const PageUpdateArgs a{p->rows, p->pages, lp, p->table_ld, p->pool, p->page_bytes, p->tables, p->lengths, p->source, p->keep, p->room,
+	                       p->held, p->new_tables, p->new_lengths, p->result, workspace};
+	return on_stream(stream, [&](hipStream_t s) { page_update(a, s); });
+}
+
+size_t sslm_hip_cache_compact_workspace(int32_t rows, int32_t pages, int32_t table_ld) {
+	return plan_ok(rows, pages, table_ld) ? page_compact_workspace(rows, pages, table_ld) : 0;
+}
+
+sslm_status sslm_hip_cache_compact(const sslm_hip_cache_compact_args* p, void* workspace, size_t workspace_bytes, void* stream) {
+	if (!p || p->struct_size != sizeof(*p)) return SSLM_INVALID_ARGUMENT;
+	const size_t need = sslm_hip_cache_compact_workspace(p->rows, p->pages, p->table_ld);
+	const int lp = log2_page(p->page_tokens);
+	if (!need || lp < 0 || !pool_ok(p->pool, p->page_bytes, p->pages) || !p->tables || !p->lengths || !p->new_tables || !p->map || !p->result)
+		return SSLM_INVALID_ARGUMENT;
+	sslm_status st;
+	if (!workspace_ok(workspace, workspace_bytes, need, &st)) return st;
+	const PageCompactArgs a{p->rows, p->pages, lp, p->table_ld, p->pool, p->page_bytes, p->tables, p->lengths, p->held, p->new_tables,
+	                        p->map, p->result, workspace};
+	return on_stream(stream, [&](hipStream_t s) { page_compact(a, s); });
+}
+
+sslm_status sslm_hip_cache_store(const sslm_hip_cache_store_args* p, void* stream) {
+	if (!p || p->struct_size != sizeof(*p)) return SSLM_INVALID_ARGUMENT;
+	const int lp = log2_page(p->page_tokens);
+	if (lp < 0 || p->rows < 1 || p->rows > kMaxRows || p->tokens < 1 || p->max_new < 1 || p->max_new > p->tokens || p->pages < 1 ||
+	    p->table_ld < 1 || p->table_ld > SSLM_HIP_CACHE_MAX_WIDTH / 16 || !heads_ok(p->heads, p->kv_heads, p->head_dim) || p->rope_dim < 0 ||
+	    p->rope_dim % 8 || p->rope_dim > p->head_dim || !pool_ok(p->pool, p->page_bytes, p->pages) || !p->tables || !p->row_tokens ||
+	    !p->row_start || !p->k || !p->v || !p->k_scale || !p->v_scale || !p->r_t_k || !p->e_t_k || !p->r_t_v || !p->e_t_v || !p->clamped || !p->status)
+		return SSLM_INVALID_ARGUMENT;
+	if (p->rope_dim && (!p->rope_cos || !p->rope_sin || p->rope_rows < 1 || p->rope_rows > SSLM_HIP_CACHE_MAX_WIDTH)) return SSLM_INVALID_ARGUMENT;
+	const int64_t width = (int64_t)p->heads * p->head_dim, kv = (int64_t)p->kv_heads * p->head_dim;
+	if (p->k_ld < kv || p->v_ld < kv || (p->q && (!p->q_out || p->q_ld < width || (p->q == p->q_out && p->q_ld != width))))
+		return SSLM_INVALID_ARGUMENT;
+	CacheStoreArgs a{};
+	a.pg = Pages{p->pool, p->page_bytes, p->k_offset, p->v_offset, p->exp_offset, p->pages, lp, p->table_ld, p->kv_heads, p->head_dim, p->tables};
+	if (!layer_ok(a.pg)) return SSLM_INVALID_ARGUMENT;
+	a.rows = p->rows;
+	a.tokens = p->tokens;
+	a.max_new = p->max_new;
+	a.NH = p->heads;
+	a.rope_dim = p->rope_dim;
+	a.halves = p->rope_halves != 0;
+	a.row_tokens = p->row_tokens;
+	a.row_start = p->row_start;
+	a.rope_rows = p->rope_rows;
+	a.rope_cos = p->rope_cos;
+	a.rope_sin = p->rope_sin;
+	a.q = p->q;
+	a.k = p->k;
+	a.v = p->v;
+	a.q_ld = p->q_ld;
+	a.k_ld = p->k_ld;
+	a.v_ld = p->v_ld;
+	a.k_scale = (const Scale*)p->k_scale;
+	a.v_scale = (const Scale*)p->v_scale;
+	a.r_t_k = p->r_t_k;
+	a.e_t_k = p->e_t_k;
+	a.r_t_v = p->r_t_v;
+	a.e_t_v = p->e_t_v;
+	a.q_out = p->q_out;
+	a.clamped = p->clamped;
+	a.status = p->status;
+	return on_stream(stream, [&](hipStream_t s) { cache_store(a, s); });
+}
+
+size_t sslm_hip_cache_attention_workspace(int32_t rows, int32_t tokens, int32_t max_new, int32_t heads, int32_t kv_heads,
+                                          int32_t head_dim, int32_t page_tokens, int64_t max_width) {
+	const int lp = log2_page(page_tokens);
+	if (lp < 0 || rows < 1 || rows > kMaxRows || tokens < 1 || max_new < 1 || max_new > tokens || !heads_ok(heads, kv_heads, head_dim) ||
+	    max_width < 1 || max_width > SSLM_HIP_CACHE_MAX_WIDTH)
+		return 0;
+	return cache_attn_workspace(rows, tokens, max_new, heads, kv_heads, head_dim, lp, max_width);
+}
+
+sslm_status sslm_hip_cache_attention(const sslm_hip_cache_attention_args* p, void* workspace, size_t workspace_bytes, void* stream) {
+	if (!p || p->struct_size != sizeof(*p)) return SSLM_INVALID_ARGUMENT;
+	const size_t need = sslm_hip_cache_attention_workspace(p->rows, p->tokens, p->max_new, p->heads, p->kv_heads, p->head_dim,
+	                                                       p->page_tokens, p->max_width);
+	if (!need || p->pages < 1 || p->table_ld < 1 || p->table_ld > SSLM_HIP_CACHE_MAX_WIDTH / 16 || !pool_ok(p->pool, p->page_bytes, p->pages) ||
+	    !p->tables || !p->row_tokens || !p->row_start || !p->q || !p->q_scale || !p->khead_m || !p->khead_e || !p->ctx_fold || !p->codes ||
+	    !p->scales || !p->status || (uintptr_t)p->q % 16)
+		return SSLM_INVALID_ARGUMENT;
+	CacheAttnArgs a{};
+	a.pg = Pages{(int8_t*)p->pool, p->page_bytes, p->k_offset, p->v_offset, p->exp_offset, p->pages, log2_page(p->page_tokens), p->table_ld,
+	             p->kv_heads, p->head_dim, p->tables};
+	if (!layer_ok(a.pg)) return SSLM_INVALID_ARGUMENT;
+	sslm_status st;
+	if (!workspace_ok(workspace, workspace_bytes, need, &st)) return st;
+	a.rows = p->rows;
+	a.tokens = p->tokens;
+	a.max_new = p->max_new;
+	a.NH = p->heads;
+	a.max_width = p->max_width;
+	a.row_tokens = p->row_tokens;
+	a.row_start = p->row_start;
+	a.q = p->q;
+	a.q_scale = (const Scale*)p->q_scale;
+	a.khead_m = p->khead_m;
+	a.khead_e = p->khead_e;
+	a.ln2_q = p->ln2_q;
+	a.b_q = p->b_q;
+	a.ca_q = p->ca_q;
+	a.ctx_fold = p->ctx_fold;
+	a.site = Scale{p->site_m, p->site_e};
+	a.codes = p->codes;
+	a.scales = (Scale*)p->scales;
+	a.status = p->status;
+	a.ws = workspace;
+	return on_stream(stream, [&](hipStream_t s) { cache_attn(a, s); });
+}
+
+}  // extern "C"
