@@ -477,6 +477,14 @@ __device__ __forceinline__ int exponent_for(int32_t m) {
 	return e;
 }
 
+// A code landed in units and clamped; whether it had to be.  residual_land's infinity has no sign.
+__device__ __forceinline__ int land_units(int32_t& x, int64_t m, int64_t r_t, int64_t k, double f) {
+	const double y = fabs(residual_land(x, m, r_t, k, f));
+	const int32_t u = (int32_t)fmin(y, (double)kMaxUnits);
+	x = (x < 0) != (m < 0) ? -u : u;
+	return y > (double)kMaxUnits;
+}
+
 // K or V of one KV head (z) in one page (x) of one row (y): the page's tokens land in LDS, their exponents run up the
 // page, then the codes are written; blocks past the last page take q's tokens, four each, and an equal share of the heads.
 constexpr int kStoreBlock = 256;
@@ -533,10 +541,7 @@ __global__ __launch_bounds__(kStoreBlock) void k_store_span(CacheStoreArgs a, in
 		int32_t mx = 0, over = 0;
 #pragma unroll
 		for (int j = 0; j < 8; ++j) {
-			const double x = residual_land(o.x[j], sc.m, rt, k, f);
-			const double lim = kMaxUnits;
-			over += fabs(x) > lim;
-			o.x[j] = (int32_t)fmin(fmax(x, -lim), lim);
+			over += land_units(o.x[j], sc.m, rt, k, f);
 		}
 		if (!isv && 8 * g < a.rope_dim) over += octet_turn(o, turn_at(a, start + i0 + i, g), kMaxUnits);
 		union {
@@ -628,17 +633,16 @@ __global__ __launch_bounds__(256) void k_ca_head(CacheAttnArgs a, int32_t* ctx, 
 	__shared__ int32_t s_ctx[256];
 	const int r = blockIdx.y, h = blockIdx.z, tid = threadIdx.x, kvh = h / (a.NH / a.pg.NKV);
 	const CacheRow c = cache_row(a.row_tokens, a.row_start, r, a.tokens, a.max_new, i64min((int64_t)a.pg.table_ld << a.pg.lp, a.max_width));
-	if ((int)blockIdx.x >= c.n) return;
+	if (!c.ok || (int)blockIdx.x >= c.n) return;
 	const int t = c.t0 + blockIdx.x, lane = tid & 63, wave = tid >> 6;
 	const int64_t width = c.start + blockIdx.x + 1;
 	int32_t* out = hst + (size_t)t * a.NH + h;
-	if (tid == 0) s_bad = c.ok ? 0 : 1;
+	if (tid == 0) s_bad = 0;
 	__syncthreads();
-	if (c.ok)
-		for (int64_t i = tid; i < (c.start + c.n + (1 << a.pg.lp) - 1) >> a.pg.lp; i += 256) {
-			const int p = a.pg.tables[(int64_t)r * a.pg.table_ld + i];
-			if (p < 0 || p >= a.pg.pages) s_bad = 1;
-		}
+	for (int64_t i = tid; i < (c.start + c.n + (1 << a.pg.lp) - 1) >> a.pg.lp; i += 256) {
+		const int p = a.pg.tables[(int64_t)r * a.pg.table_ld + i];
+		if (p < 0 || p >= a.pg.pages) s_bad = 1;
+	}
 	if (tid < D / 16) ((v4i*)s_q)[tid] = ((const unaligned16*)(a.q + ((size_t)t * a.NH + h) * D + 16 * tid))->v;
 	__syncthreads();
 	if (s_bad) {
@@ -711,6 +715,10 @@ __global__ __launch_bounds__(256) void k_ca_out(CacheAttnArgs a, const int32_t* 
 	__shared__ uint32_t s_first, s_max;
 	const int r = blockIdx.y, tid = threadIdx.x, N = a.NH * a.pg.D;
 	const CacheRow c = cache_row(a.row_tokens, a.row_start, r, a.tokens, a.max_new, i64min((int64_t)a.pg.table_ld << a.pg.lp, a.max_width));
+	if (!c.ok) {
+		for (int i = blockIdx.x * 256 + tid; i < c.n; i += gridDim.x * 256) a.status[c.t0 + i] = kPositionOverCap;
+		return;
+	}
 	if ((int)blockIdx.x >= c.n) return;
 	const int t = c.t0 + blockIdx.x;
 	if (tid == 0) {
