@@ -108,6 +108,12 @@ struct SaRows {
 			r[u] = global16(row(i64min(p + i / PER, last)) + i % PER * 16);
 		}
 	}
+	// at(u): where this lane's chunk u lies, byte 16 (i % PER) of row i / PER, i = lane + 64 u
+	template <typename F>
+	__device__ __forceinline__ void load_at(F&& at) {
+#pragma unroll
+		for (int u = 0; u < PER; ++u) r[u] = global16(at(u));
+	}
 	// rows 32 h .. 32 h + 31 into LDS
 	__device__ __forceinline__ void stage(int8_t* lds, int h) const {
 		const int lane = threadIdx.x & 63;
@@ -142,6 +148,11 @@ struct SaRows {
 	// As V: context += P V by the byte-transposing LDS read, which gives lane (ri, g) dim 16 dt + ri of the
 	// positions in sa_pack's order.  Lane (ri, g) of acc[dt][part] holds dims 16 dt + 4 g .. + 3 of query row ri.
 	__device__ __forceinline__ void multiply(int8_t* lds, const v4i& lo, const v4i& nhi, v4i (&acc)[D / 16][2]) const {
+		const v4i x[2] = {lo, nhi};
+		multiply(lds, x, acc);
+	}
+	template <int NP>
+	__device__ __forceinline__ void multiply(int8_t* lds, const v4i (&x)[NP], v4i (&acc)[D / 16][NP]) const {
 		const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4, i = ri >> 1, row = (i >> 2) * 16 + g * 4 + (i & 3);
 		v2i half[2][D / 16];
 #pragma unroll
@@ -154,8 +165,8 @@ struct SaRows {
 #pragma unroll
 		for (int dt = 0; dt < D / 16; ++dt) {
 			const v4i b = v4i{half[0][dt].x, half[0][dt].y, half[1][dt].x, half[1][dt].y};
-			acc[dt][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, lo, acc[dt][0], 0, 0, 0);
-			acc[dt][1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, nhi, acc[dt][1], 0, 0, 0);
+#pragma unroll
+			for (int i = 0; i < NP; ++i) acc[dt][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, x[i], acc[dt][i], 0, 0, 0);
 		}
 	}
 };
@@ -221,6 +232,23 @@ __device__ __forceinline__ void sa_pack(const int32_t (&p)[16], v4i* lo, v4i* nh
 		const uint32_t c = __builtin_amdgcn_perm(127 - p[4 * t + 1], 127 - p[4 * t], 0x0c0c0501),
 		               d = __builtin_amdgcn_perm(127 - p[4 * t + 3], 127 - p[4 * t + 2], 0x0c0c0501);
 		(*nhi)[t] = (int)(c | d << 16);
+	}
+}
+
+// The same for p up to 2^23 (a probability times 2^e, e <= 8) as three operands, p = x[0] - 256 x[1] - 65536 x[2]: p's
+// low byte taken as signed, and n = floor((127 - p) / 256) in [-2^15, 0] as its own signed low byte and the rest in [-128, 0].
+__device__ __forceinline__ void sa_pack3(const int32_t (&p)[16], v4i (&x)[3]) {
+#pragma unroll
+	for (int t = 0; t < 4; ++t) {
+		int32_t n[4];
+#pragma unroll
+		for (int i = 0; i < 4; ++i) n[i] = 127 - p[4 * t + i];
+		const uint32_t a = __builtin_amdgcn_perm(p[4 * t + 1], p[4 * t], 0x0c0c0400), b = __builtin_amdgcn_perm(p[4 * t + 3], p[4 * t + 2], 0x0c0c0400);
+		x[0][t] = (int)(a | b << 16);
+		const uint32_t c = __builtin_amdgcn_perm(n[1], n[0], 0x0c0c0501), d = __builtin_amdgcn_perm(n[3], n[2], 0x0c0c0501);
+		x[1][t] = (int)(c | d << 16);
+		const uint32_t e = __builtin_amdgcn_perm(n[1] + 32768, n[0] + 32768, 0x0c0c0602), f = __builtin_amdgcn_perm(n[3] + 32768, n[2] + 32768, 0x0c0c0602);
+		x[2][t] = (int)(e | f << 16);
 	}
 }
 

@@ -81,7 +81,7 @@ struct CacheAttnArgs {
 	int32_t* status;
 	void* ws;
 };
-size_t cache_attn_workspace(int rows, int tokens, int max_new, int NH, int NKV, int D, int lp, int64_t max_width);
+size_t cache_attn_workspace(int rows, int tokens, int max_new, int NH, int NKV, int D, int64_t max_width);
 void cache_attn(const CacheAttnArgs& a, hipStream_t s);
 
 struct Sampling {

@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/sslm_hip.h"
 #include "attention_util.h"
@@ -624,136 +625,727 @@ __global__ __launch_bounds__(kStoreBlock) void k_store_span(CacheStoreArgs a, in
 // attention over pages
 // ------------------------------------------------------------------------------------------
 
-// A block per (token, head): maxima, sums and P V in three passes over the row's positions.
-template <int D>
-__global__ __launch_bounds__(256) void k_ca_head(CacheAttnArgs a, int32_t* ctx, int32_t* hst) {
-	__shared__ __attribute__((aligned(16))) int8_t s_q[D];
-	__shared__ int32_t s_p[256], s_m[4], s_bad;
-	__shared__ int64_t s_sum[4];
-	__shared__ int32_t s_ctx[256];
-	const int r = blockIdx.y, h = blockIdx.z, tid = threadIdx.x, kvh = h / (a.NH / a.pg.NKV);
-	const CacheRow c = cache_row(a.row_tokens, a.row_start, r, a.tokens, a.max_new, i64min((int64_t)a.pg.table_ld << a.pg.lp, a.max_width));
-	if (!c.ok || (int)blockIdx.x >= c.n) return;
-	const int t = c.t0 + blockIdx.x, lane = tid & 63, wave = tid >> 6;
-	const int64_t width = c.start + blockIdx.x + 1;
-	int32_t* out = hst + (size_t)t * a.NH + h;
-	if (tid == 0) s_bad = 0;
-	__syncthreads();
-	for (int64_t i = tid; i < (c.start + c.n + (1 << a.pg.lp) - 1) >> a.pg.lp; i += 256) {
-		const int p = a.pg.tables[(int64_t)r * a.pg.table_ld + i];
-		if (p < 0 || p >= a.pg.pages) s_bad = 1;
-	}
-	if (tid < D / 16) ((v4i*)s_q)[tid] = ((const unaligned16*)(a.q + ((size_t)t * a.NH + h) * D + 16 * tid))->v;
-	__syncthreads();
-	if (s_bad) {
-		if (tid == 0) *out = kPositionOverCap;
-		return;
-	}
-	const RowConst rc = row_const(RowScales{a.q_scale[t], a.khead_m[kvh], a.khead_e[kvh]}, a.ln2_q, a.b_q, a.ca_q, width);
-	if (rc.st != kOk) {
-		if (tid == 0) *out = rc.st;
-		return;
-	}
-	auto page_of = [&](int64_t p) { return a.pg.pool + a.pg.tables[(int64_t)r * a.pg.table_ld + (p >> a.pg.lp)] * a.pg.page_bytes; };
-	auto slot = [&](int64_t p) { return (((int64_t)kvh << a.pg.lp) + (p & ((1 << a.pg.lp) - 1))) * D; };
-	auto score = [&](int64_t p) {
-		const int8_t *pg = page_of(p), *k = pg + a.pg.k_off + slot(p);
-		int32_t s = 0;
-		for (int d = 0; d < D; d += 4) {
-			const int x = *(const int*)(k + d), y = *(const int*)(s_q + d);
-			s = __builtin_amdgcn_sdot4(x, y, s, false);
-		}
-		return s << min((int)((const uint8_t*)pg)[a.pg.e_off + kvh], kMaxShift);
-	};
-	int32_t m = INT32_MIN;
-	for (int64_t p = tid; p < width; p += 256) m = max(m, score(p));
-	for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o, 64));
-	if (lane == 0) s_m[wave] = m;
-	__syncthreads();
-	m = max(max(s_m[0], s_m[1]), max(s_m[2], s_m[3]));
-	const double inv = 1.0 / (double)rc.q_ln2;
-	int64_t sum = 0;
-	bool bad = false;
-	for (int64_t p = tid; p < width; p += 256) {
-		const int64_t x = iexp_fast_cold((int64_t)score(p) - m, rc.q_ln2, inv, rc.q_b, rc.q_c, rc.ceil);
-		bad |= x < 0;
-		sum += x < 0 ? 0 : x;
-	}
-	for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-	if (lane == 0) s_sum[wave] = sum;
-	if (bad) s_bad = 1;
-	__syncthreads();
-	if (s_bad) {
-		if (tid == 0) *out = kSoftmaxKernelRefusedAfterGateAccepted;
-		return;
-	}
-	sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-	const int64_t den = sum > 1 ? sum : 1;
-	const double dinv = 1.0 / (double)den;
-	int32_t acc = 0;
-	const int dim = tid % D, part = tid / D;
-	for (int64_t p0 = 0; p0 < width; p0 += 256) {
-		__syncthreads();
-		s_p[tid] = p0 + tid < width ? (int32_t)div_rcp_cold(iexp_fast_cold((int64_t)score(p0 + tid) - m, rc.q_ln2, inv, rc.q_b, rc.q_c, rc.ceil) << 15, den, dinv, 32768) : 0;
-		__syncthreads();
-		for (int64_t p = p0 + part; p < i64min(width, p0 + 256); p += 256 / D) {
-			const int8_t* pg = page_of(p);
-			acc += s_p[p - p0] * (pg[a.pg.v_off + slot(p) + dim] << min((int)((const uint8_t*)pg)[a.pg.e_off + a.pg.NKV + kvh], kMaxShift));
-		}
-	}
-	s_ctx[tid] = acc;
-	__syncthreads();
-	if (tid < D) {
-		for (int i = 1; i < 256 / D; ++i) acc += s_ctx[tid + i * D];
-		ctx[((size_t)t * a.NH + h) * D + tid] = acc;
-	}
-	if (tid == 0) *out = kOk;
+// The layout of one call's launches.  The unit of work is a wave with a tile of 16 query rows (token, head) of one KV
+// head and a range of positions, a "plane" of sp.  The softmax's maximum and sum run over the whole row and each
+// probability is rounded by itself, so nothing is rescaled: maxima, sums and P V are launches of their own, and the
+// planes' integers join exactly in any order.
+// Single tokens: a tile is one token's heads, waves work alone, scores are kept for the later launches (4 G bytes a
+// position beside the 2 D of its K and V).  Chunks: four neighbouring tiles of a row share each step of 64 positions that
+// their block stages, and the scores are computed again, 8 MFMAs a step at D = 128.
+struct CaPlan {
+	int ht;          // single tokens: tiles of a token's heads
+	int groups;      // chunks: blocks of 64 query rows, at least those of every row together
+	int sp, planes;  // positions of a plane (a multiple of 128), planes of the widest row
+	int ps, parts;   // positions of one block of sums, blocks of the widest row
+	int64_t wpad;    // kept scores of a (token, head)
+};
+
+struct CaWork {
+	SaConst* cst;     // [tokens, NKV]
+	int32_t* pmax;    // [planes][tokens NH]
+	int32_t* top;     // [tokens NH] single tokens: the row's maximum
+	int64_t* psum;    // [parts or planes][tokens NH]; negative: an i-exp value was refused
+	int32_t* part;    // [planes][tokens][NH D]
+	int32_t* hst;     // [tokens NH] refusals of the softmax
+	int32_t* scores;  // [tokens NH][wpad] single tokens
+};
+
+constexpr int kCaWaves = 4;
+
+__device__ __forceinline__ CacheRow attn_row(const CacheAttnArgs& a, int r) {
+	return cache_row(a.row_tokens, a.row_start, r, a.tokens, a.max_new, i64min((int64_t)a.pg.table_ld << a.pg.lp, a.max_width));
 }
 
-// The fold and funnel of one token's context, a block per token.
-__global__ __launch_bounds__(256) void k_ca_out(CacheAttnArgs a, const int32_t* ctx, const int32_t* hst) {
-	__shared__ uint32_t s_first, s_max;
-	const int r = blockIdx.y, tid = threadIdx.x, N = a.NH * a.pg.D;
-	const CacheRow c = cache_row(a.row_tokens, a.row_start, r, a.tokens, a.max_new, i64min((int64_t)a.pg.table_ld << a.pg.lp, a.max_width));
+// A wave's next 64 pages of a row, one to a lane, from position p0's on (lanes past position `last`'s page repeat it), with the
+// KV head's exponents; false for the whole wave when one is not a page.
+struct LanePages {
+	int32_t page, ke, ve;
+	int64_t first;
+};
+__device__ __forceinline__ bool lane_pages(const Pages& g, int r, int kvh, int64_t p0, int64_t last, LanePages* o) {
+	o->first = p0 >> g.lp;
+	const int64_t n = (last >> g.lp) - o->first;
+	o->page = g.tables[(int64_t)r * g.table_ld + o->first + i64min(threadIdx.x & 63, n)];
+	if (__any(o->page < 0 || o->page >= g.pages)) return false;
+	const uint8_t* e = (const uint8_t*)g.pool + o->page * g.page_bytes + g.e_off;
+	o->ke = min((int)e[kvh], kMaxShift);
+	o->ve = min((int)e[g.NKV + kvh], kMaxShift);
+	return true;
+}
+// where the 64 pages from position p's on end
+__device__ __forceinline__ int64_t pages_end(const Pages& g, int64_t p) { return ((p >> g.lp) + 64) << g.lp; }
+// whether every page of the row's first `width` positions is one (by all lanes of a wave)
+__device__ __forceinline__ bool row_pages_ok(const Pages& g, int r, int64_t width) {
+	bool bad = false;
+	for (int64_t i = threadIdx.x & 63; i < pages_for(width, g.lp); i += 64) {
+		const int p = g.tables[(int64_t)r * g.table_ld + i];
+		bad |= p < 0 || p >= g.pages;
+	}
+	return !__any(bad);
+}
+
+// Rows of 64 positions from p (a multiple of 64) as a wave loads them: the page of each 16 of them is the same for the
+// wave, slots past the row's end are still the page's own.
+template <int D>
+__device__ __forceinline__ void load_rows(SaRows<D>& x, const Pages& g, const LanePages& lp, int64_t p, int64_t last, int64_t off) {
+	constexpr int PER = D / 16, R = 64 / PER;  // rows of one load
+	const int lane = threadIdx.x & 63, mask = min(1 << g.lp, 64) - 1, high = (int)(p & ((1 << g.lp) - 1));
+	auto page = [&](int row) {
+		const int i = (int)((i64min(p + row, last) >> g.lp) - lp.first);
+		return g.pool + __builtin_amdgcn_readlane(lp.page, i) * g.page_bytes + off;
+	};
+	x.load_at([&](int u) {
+		const int row = u * R + lane / PER;
+		const int8_t* at = page(u * R);
+		if (R > 16) {
+			const int8_t* next = page(u * R + 16);
+			at = lane / PER >= 16 ? next : at;
+		}
+		return at + ((high & ~63) + (row & mask)) * D + lane % PER * 16;
+	});
+}
+// the exponents of 16 positions from p
+__device__ __forceinline__ int page_exp(const Pages& g, const LanePages& lp, int32_t e, int64_t p, int64_t last) {
+	return __builtin_amdgcn_readlane(e, (int)((i64min(p, last) >> g.lp) - lp.first));
+}
+
+// A single token's wave: number w of the launch's.
+struct CdJob {
+	int r, t, kvh, tile, plane, h0, heads;  // h0: the tile's first head
+	int64_t width, p0, p1;
+	CacheRow row;
+};
+__device__ __forceinline__ bool cd_job(const CacheAttnArgs& a, const CaPlan& pl, CdJob* j) {
+	const int w = (int)blockIdx.x * kCaWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), G = a.NH / a.pg.NKV;
+	j->plane = w % pl.planes;
+	j->tile = w / pl.planes % pl.ht;
+	j->kvh = w / pl.planes / pl.ht % a.pg.NKV;
+	j->r = w / pl.planes / pl.ht / a.pg.NKV;
+	if (j->r >= a.rows) return false;
+	j->row = attn_row(a, j->r);
+	if (!j->row.ok || j->row.n < 1) return false;
+	j->t = j->row.t0;
+	j->h0 = j->kvh * G + j->tile * 16;
+	j->heads = min(16, G - j->tile * 16);
+	j->width = j->row.start + 1;
+	j->p0 = (int64_t)j->plane * pl.sp;
+	j->p1 = i64min(j->width, j->p0 + pl.sp);
+	return j->p0 < j->p1;
+}
+
+// The scores of a plane, kept, and their maxima.  The wave of a row's first plane also settles its constants.
+template <int D>
+__global__ __launch_bounds__(64 * kCaWaves) void k_cd_scores(CacheAttnArgs a, CaPlan pl, CaWork w) {
+	constexpr int NC = (D + 63) / 64;
+	__shared__ __attribute__((aligned(16))) int8_t s_k[kCaWaves][32 * D];
+	const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4;
+	CdJob j;
+	if (!cd_job(a, pl, &j)) return;
+	int8_t* lds = s_k[threadIdx.x >> 6];
+	const bool mine = ri < j.heads;
+	const int h = j.h0 + (mine ? ri : 0);
+	v4i q[NC];
+#pragma unroll
+	for (int c = 0; c < NC; ++c) q[c] = mine && c * 64 + g * 16 < D ? load16(a.q + ((size_t)j.t * a.NH + h) * D + c * 64 + g * 16) : v4i{0, 0, 0, 0};
+	if (j.plane == 0 && j.tile == 0) {
+		SaConst c{0, 0, 0, 0, kPositionOverCap, 0};
+		if (row_pages_ok(a.pg, j.r, j.width)) {
+			const RowConst rc = row_const(RowScales{a.q_scale[j.t], a.khead_m[j.kvh], a.khead_e[j.kvh]}, a.ln2_q, a.b_q, a.ca_q, j.width);
+			c = SaConst{rc.q_ln2, rc.q_b, rc.q_c, rc.ceil, rc.st, 0};
+		}
+		if (lane == 0) w.cst[(size_t)j.t * a.pg.NKV + j.kvh] = c;
+	}
+	int32_t* out = w.scores + ((size_t)j.t * a.NH + h) * pl.wpad + 4 * g;
+	const int64_t off = a.pg.k_off + ((int64_t)j.kvh << a.pg.lp) * D;
+	int32_t m = INT32_MIN;
+	for (int64_t s0 = j.p0; s0 < j.p1; s0 = pages_end(a.pg, s0)) {
+		const int64_t s1 = i64min(j.p1, pages_end(a.pg, s0)), last = s1 - 1;
+		LanePages lp;
+		if (!lane_pages(a.pg, j.r, j.kvh, s0, last, &lp)) return;
+		SaRows<D> k[2];
+		load_rows(k[0], a.pg, lp, s0, last, off);
+		if (s0 + 64 < s1) load_rows(k[1], a.pg, lp, s0 + 64, last, off);
+		for (int64_t p0 = s0; p0 < s1; p0 += 128) {
+#pragma unroll
+			for (int b = 0; b < 2; ++b) {
+				const int64_t p = p0 + 64 * b;
+				if (p >= s1) break;
+				v4i s[4] = {};
+				k[b].scores(lds, q, s);
+				if (p + 128 < s1) load_rows(k[b], a.pg, lp, p + 128, last, off);
+				const int left = (int)i64min(s1 - p, 64) - 4 * g;
+#pragma unroll
+				for (int t = 0; t < 4; ++t) {
+					const int e = page_exp(a.pg, lp, lp.ke, p + 16 * t, last);
+#pragma unroll
+					for (int v = 0; v < 4; ++v) {
+						s[t][v] <<= e;
+						m = max(m, t * 16 + v < left ? s[t][v] : INT32_MIN);
+					}
+					if (mine) *(v4i*)(out + p + 16 * t) = s[t];
+				}
+			}
+		}
+	}
+	m = max(m, __shfl_xor(m, 16, 64));
+	m = max(m, __shfl_xor(m, 32, 64));
+	if (g == 0 && mine) w.pmax[((size_t)j.plane * a.tokens + j.t) * a.NH + h] = m;
+}
+
+// The sum of one (token, head) over a part of its positions, from the kept scores.
+__global__ __launch_bounds__(256) void k_cd_sum(CacheAttnArgs a, CaPlan pl, CaWork w) {
+	__shared__ int32_t s_m[4];
+	__shared__ int64_t s_s[4];
+	const int part = blockIdx.x, h = blockIdx.y, r = blockIdx.z, tid = threadIdx.x, kvh = h / (a.NH / a.pg.NKV);
+	const CacheRow row = attn_row(a, r);
+	if (!row.ok || row.n < 1) return;
+	const int t = row.t0;
+	const int64_t width = row.start + 1, p0 = (int64_t)part * pl.ps, p1 = i64min(width, p0 + pl.ps);
+	if (p0 >= p1) return;
+	const int32_t* sc = w.scores + ((size_t)t * a.NH + h) * pl.wpad;
+	const SaConst c = w.cst[(size_t)t * a.pg.NKV + kvh];
+	if (c.st != kOk) return;
+	int32_t top = INT32_MIN;
+	const int n = (int)((width + pl.sp - 1) / pl.sp);
+	for (int i = tid; i < n; i += 256) top = max(top, w.pmax[((size_t)i * a.tokens + t) * a.NH + h]);
+	for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
+	if ((tid & 63) == 0) s_m[tid >> 6] = top;
+	__syncthreads();
+	top = max(max(s_m[0], s_m[1]), max(s_m[2], s_m[3]));
+	int64_t sum = 0;
+	int bad = 0;
+	if (sa_fast(c, width)) {
+		const SaExp e = sa_exp_of(c, top);
+		double acc = 0.0;
+		for (int64_t p = p0 + 4 * tid; p < p1; p += 1024) {
+			const v4i x = *(const v4i*)(sc + p);
+#pragma unroll
+			for (int i = 0; i < 4; ++i) {
+				const double y = sa_exp(e, x[i]);
+				acc += p + i < p1 ? y : 0.0;
+			}
+		}
+		sum = (int64_t)acc;
+	} else {
+		const double inv = 1.0 / (double)c.q_ln2;
+		for (int64_t p = p0 + tid; p < p1; p += 256) {
+			const int64_t x = iexp_fast_cold((int64_t)sc[p] - top, c.q_ln2, inv, c.q_b, c.q_c, c.ceil);
+			bad |= x < 0;
+			sum += x < 0 ? 0 : x;
+		}
+	}
+	for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+	bad = __any(bad);
+	if ((tid & 63) == 0) s_s[tid >> 6] = bad ? -1 : sum;
+	__syncthreads();
+	if (tid == 0) {
+		sum = 0;
+		for (int i = 0; i < 4; ++i) {
+			bad |= s_s[i] < 0;
+			sum += s_s[i];
+		}
+		w.psum[((size_t)part * a.tokens + t) * a.NH + h] = bad ? -1 : sum;
+		if (part == 0) w.top[(size_t)t * a.NH + h] = top;
+	}
+}
+
+// P V of a plane.  Where at most eight heads would leave half of a tile's columns empty, columns 8 .. 15 hold
+// the same heads at the next 64 positions (F = 2), so that i-exp and probabilities run on full waves.
+template <int D, int F>
+__global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cd_pv(CacheAttnArgs a, CaPlan pl, CaWork w) {
+	constexpr int DT = D / 16, GP = 16 / F;
+	__shared__ __attribute__((aligned(16))) int8_t s_v[kCaWaves][32 * D];
+	const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4, col = ri % GP, half = ri / GP;
+	CdJob j;
+	if (!cd_job(a, pl, &j)) return;
+	int8_t* lds = s_v[threadIdx.x >> 6];
+	const SaConst c = w.cst[(size_t)j.t * a.pg.NKV + j.kvh];
+	if (c.st != kOk) return;
+	bool live = col < j.heads;
+	const int h = j.h0 + (live ? col : 0);
+	const size_t th = (size_t)j.t * a.NH + h;
+	const int32_t top = w.top[th];
+	int64_t sum = 0;
+	bool bad = false;
+	const int parts = (int)((j.width + pl.ps - 1) / pl.ps);
+	for (int i = 0; i < parts; ++i) {
+		const int64_t x = w.psum[(size_t)i * a.tokens * a.NH + th];
+		bad |= x < 0;
+		sum += x;
+	}
+	if (j.plane == 0 && g == 0 && half == 0 && live) w.hst[th] = bad ? kSoftmaxKernelRefusedAfterGateAccepted : kOk;
+	live = live && !bad;
+	const int64_t den = live && sum > 1 ? sum : 1;
+	const bool fast = sa_fast(c, j.width), small = fast && !__any(den >= ((int64_t)1 << 36));
+	const int64_t off = a.pg.v_off + ((int64_t)j.kvh << a.pg.lp) * D;
+	const int32_t* sc = w.scores + th * pl.wpad + half * 64 + 4 * g;
+	const SaExp e = sa_exp_of(fast ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
+	const SaProb pb = sa_prob_of((double)den, small);
+	const double inv = 1.0 / (double)c.q_ln2, dinv = 1.0 / (double)den;
+	v4i acc[DT][3];
+#pragma unroll
+	for (int d = 0; d < DT; ++d) acc[d][0] = acc[d][1] = acc[d][2] = v4i{0, 0, 0, 0};
+	for (int64_t s0 = j.p0; s0 < j.p1; s0 = pages_end(a.pg, s0)) {
+		const int64_t s1 = i64min(j.p1, pages_end(a.pg, s0)), last = s1 - 1;
+		LanePages lp;
+		if (!lane_pages(a.pg, j.r, j.kvh, s0, last, &lp)) return;
+		SaRows<D> v[F];
+		v4i s[4];
+		auto scores = [&](int64_t p) {
+#pragma unroll
+			for (int t = 0; t < 4; ++t) s[t] = *(const v4i*)(sc + p + 16 * t);
+		};
+		scores(s0);
+#pragma unroll
+		for (int f = 0; f < F; ++f) load_rows(v[f], a.pg, lp, i64min(s0 + 64 * f, last & ~63ll), last, off);
+		for (int64_t p = s0; p < s1; p += 64 * F) {
+			const int left = (int)i64min(s1 - p - half * 64, 64) - 4 * g;
+			int32_t pr[16];
+			auto exps = [&](auto&& value) {
+#pragma unroll
+				for (int t = 0; t < 4; ++t) {
+					int sh = page_exp(a.pg, lp, lp.ve, p + 16 * t, last);
+					if (F == 2) sh = half ? page_exp(a.pg, lp, lp.ve, p + 64 + 16 * t, last) : sh;
+#pragma unroll
+					for (int i = 0; i < 4; ++i) {
+						const int32_t x = value(s[t][i], 16 * t + i < left);
+						pr[4 * t + i] = 16 * t + i < left && live ? x << sh : 0;
+					}
+				}
+			};
+			if (small) exps([&](int32_t x, bool) { return sa_prob<true>(pb, sa_exp(e, x)); });
+			else if (fast) exps([&](int32_t x, bool) { return sa_prob<false>(pb, sa_exp(e, x)); });
+			else
+				exps([&](int32_t x, bool in) {
+					return in && live ? (int32_t)div_rcp_cold(iexp_fast_cold((int64_t)x - top, c.q_ln2, inv, c.q_b, c.q_c, c.ceil) << 15, den, dinv, 32768) : 0;
+				});
+			if (p + 64 * F < s1) scores(p + 64 * F);
+			v4i x[3];
+			sa_pack3(pr, x);
+#pragma unroll
+			for (int f = 0; f < F; ++f) {
+				if (p + 64 * f >= s1) break;
+				v4i y[3];
+#pragma unroll
+				for (int i = 0; i < 3; ++i) y[i] = F == 1 || half == f ? x[i] : v4i{0, 0, 0, 0};
+				v[f].multiply(lds, y, acc);
+				if (p + 64 * (f + F) < s1) load_rows(v[f], a.pg, lp, p + 64 * (f + F), last, off);
+			}
+		}
+	}
+	int32_t* out = w.part + (((size_t)j.plane * a.tokens + j.t) * a.NH + h) * D + 4 * g;
+#pragma unroll
+	for (int d = 0; d < DT; ++d) {
+		v4i y = acc[d][0] - 256 * acc[d][1] - 65536 * acc[d][2];
+		if (F == 2) {
+#pragma unroll
+			for (int i = 0; i < 4; ++i) y[i] += __shfl_xor(y[i], 8, 64);
+		}
+		if (col < j.heads && half == 0) *(v4i*)(out + 16 * d) = y;
+	}
+}
+
+// A chunk's block: number `b` of the row groups, 64 query rows from the group's, and a plane.
+struct CcJob {
+	int r, kvh, plane, i0, count;  // i0: the block's first query row of `count` in the row
+	int64_t width, p0, p1;         // width: of the block's last token
+	CacheRow row;
+};
+// The rows' groups are counted 64 rows at a time, a row to a lane.
+__device__ __forceinline__ bool cc_job(const CacheAttnArgs& a, const CaPlan& pl, CcJob* j) {
+	const int G = a.NH / a.pg.NKV, blk = blockIdx.x, lane = threadIdx.x & 63;
+	// blocks go to the XCDs in turn: a (KV head, plane)'s groups stay on one, whose L2 then holds its K/V
+	const int grp = (blk / 8 / pl.groups) * 8 + blk % 8;
+	int b = (blk / 8) % pl.groups;
+	if (grp >= a.pg.NKV * pl.planes) return false;
+	j->plane = grp / a.pg.NKV;
+	j->kvh = grp % a.pg.NKV;
+	for (int r0 = 0;; r0 += 64) {
+		if (r0 >= a.rows) return false;
+		int n = 0;
+		if (r0 + lane < a.rows) {
+			const CacheRow row = attn_row(a, r0 + lane);
+			n = row.ok ? (row.n * G + 63) / 64 : 0;
+		}
+		int x = n;
+		for (int o = 1; o < 64; o *= 2) {
+			const int y = __shfl_up(x, o, 64);
+			x += lane >= o ? y : 0;
+		}
+		const uint64_t hit = __ballot(b < x);
+		if (hit) {
+			const int at = __builtin_ctzll(hit);
+			b -= __builtin_amdgcn_readlane(x, at) - __builtin_amdgcn_readlane(n, at);
+			j->r = r0 + at;
+			break;
+		}
+		b -= __builtin_amdgcn_readlane(x, 63);
+	}
+	j->row = attn_row(a, j->r);
+	j->i0 = b * 64;
+	j->count = j->row.n * G;
+	j->width = j->row.start + (min(j->i0 + 64, j->count) - 1) / G + 1;
+	j->p0 = (int64_t)j->plane * pl.sp;
+	j->p1 = i64min(j->width, j->p0 + pl.sp);
+	return j->p0 < j->p1;
+}
+// what a lane of the block has: its token, head and width (t < 0: none)
+struct CcLane {
+	int t, h;
+	int64_t width;
+};
+__device__ __forceinline__ CcLane cc_lane(const CacheAttnArgs& a, const CcJob& j) {
+	const int G = a.NH / a.pg.NKV, i = j.i0 + (int)(threadIdx.x >> 6) * 16 + (int)(threadIdx.x & 15);
+	CcLane l{-1, j.kvh * G, 0};
+	if (i < j.count) {
+		l.t = j.row.t0 + i / G;
+		l.h += i % G;
+		l.width = j.row.start + i / G + 1;
+	}
+	return l;
+}
+template <int D, int NC>
+__device__ __forceinline__ void cc_load_q(const CacheAttnArgs& a, const CcLane& l, v4i (&q)[NC]) {
+	const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+	for (int c = 0; c < NC; ++c)
+		q[c] = l.t >= 0 && c * 64 + g * 16 < D ? load16(a.q + ((size_t)l.t * a.NH + l.h) * D + c * 64 + g * 16) : v4i{0, 0, 0, 0};
+}
+
+// Steps of 64 positions over the block's plane: `step(p, last, scores, pages, multiply)`.  Each thread loads its share of a
+// step's rows two steps ahead and stages it into one of two buffers, so a step costs one barrier.  LDS: 64 D bytes a buffer, K's two and then V's
+// two.  False, for the whole block, when one of the plane's pages is none.
+template <int D, bool WITH_V, int NC, typename F>
+__device__ __forceinline__ bool cc_steps(const CacheAttnArgs& a, const CcJob& j, int8_t* lds, const v4i (&q)[NC], F&& step) {
+	constexpr int BS = 64 * kCaWaves, CH = 4 * D, PT = (CH + BS - 1) / BS, PER = D / 16, AHEAD = D <= 128 ? 2 : 1;
+	const Pages& g = a.pg;
+	const int64_t head = ((int64_t)j.kvh << g.lp) * D;
+	const int mask = min(1 << g.lp, 64) - 1;
+	int b = 0;
+	for (int64_t s0 = j.p0; s0 < j.p1; s0 = pages_end(g, s0)) {
+		const int64_t s1 = i64min(j.p1, pages_end(g, s0)), last = s1 - 1;
+		LanePages lp;
+		if (!lane_pages(g, j.r, j.kvh, s0, last, &lp)) return false;
+		v4i kr[AHEAD][PT], vr[AHEAD][PT], s[4];
+		auto load = [&](int64_t p, v4i (&k)[PT], v4i (&v)[PT]) {
+#pragma unroll
+			for (int u = 0; u < PT; ++u) {
+				const int c = min((int)threadIdx.x + u * BS, CH - 1), row = c / PER;
+				const int page = __shfl(lp.page, (int)((i64min(p + row, last) >> g.lp) - lp.first), 64);
+				const int8_t* at = g.pool + page * g.page_bytes + head + (((int)(p & ((1 << g.lp) - 1)) & ~63) + (row & mask)) * D + c % PER * 16;
+				k[u] = global16(at + g.k_off);
+				if (WITH_V) v[u] = global16(at + g.v_off);
+			}
+		};
+#pragma unroll
+		for (int i = 0; i < AHEAD; ++i) load(s0 + 64 * i, kr[i], vr[i]);
+		for (int64_t p0 = s0; p0 < s1; p0 += 64 * AHEAD) {
+#pragma unroll
+			for (int i = 0; i < AHEAD; ++i) {
+				const int64_t p = p0 + 64 * i;
+				if (i && p >= s1) break;
+				int8_t *kb = lds + b * 64 * D, *vb = lds + (2 + b) * 64 * D;
+#pragma unroll
+				for (int u = 0; u < PT; ++u) {
+					const int c = (int)threadIdx.x + u * BS;
+					if (CH % BS == 0 || c < CH) {
+						*(v4i*)(kb + SaRows<D>::at(c / PER, c % PER)) = kr[i][u];
+						if (WITH_V) *(v4i*)(vb + SaRows<D>::at(c / PER, c % PER)) = vr[i][u];
+					}
+				}
+				load(p + 64 * AHEAD, kr[i], vr[i]);
+				__syncthreads();
+				const int lane = threadIdx.x & 63, ri = lane & 15, gg = lane >> 4;
+#pragma unroll
+				for (int t = 0; t < 4; ++t) {
+					s[t] = v4i{0, 0, 0, 0};
+#pragma unroll
+					for (int c = 0; c < NC; ++c) {
+						const int ch = c * 4 + gg;
+						const v4i k = *(const v4i*)(kb + SaRows<D>::at(t * 16 + ri, D < 64 ? ch & (PER - 1) : ch));
+						s[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, q[c], s[t], 0, 0, 0);
+					}
+					const int e = page_exp(g, lp, lp.ke, p + 16 * t, last);
+#pragma unroll
+					for (int v = 0; v < 4; ++v) s[t][v] <<= e;
+				}
+				step(p, last, s, lp, [&](const v4i (&x)[3], v4i (&acc)[D / 16][3]) {
+					const int k = ri >> 1, row = (k >> 2) * 16 + gg * 4 + (k & 3);
+#pragma unroll
+					for (int dt = 0; dt < D / 16; ++dt) {
+						const int8_t* from = vb + SaRows<D>::at(row, dt) + 8 * (ri & 1);  // rows 32 apart change places alike
+						const v2i y = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)from);
+						const v2i z = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(from + 32 * D));
+						const v4i m = v4i{y.x, y.y, z.x, z.y};
+#pragma unroll
+						for (int n = 0; n < 3; ++n) acc[dt][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(m, x[n], acc[dt][n], 0, 0, 0);
+					}
+				});
+				b ^= 1;
+			}
+		}
+	}
+	return true;
+}
+
+// how many of a step's positions, counted from the lane's first (4 g), lie before `end`
+__device__ __forceinline__ int ca_left(int64_t p, int64_t end) { return (int)i64min(end - p, 64) - ((threadIdx.x & 63) >> 4) * 4; }
+
+// Which bits some live lane of the block has set: what its waves branch on alike.
+__device__ __forceinline__ int block_vote(int bits, int* s) {
+	const int all = (__any(bits & 1) ? 1 : 0) | (__any(bits & 2) ? 2 : 0);
+	if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = all;
+	__syncthreads();
+	return __builtin_amdgcn_readfirstlane(s[0] | s[1] | s[2] | s[3]);
+}
+
+// a (token, head)'s maximum or sum over its planes; the lanes ri, ri + 16, ri + 32, ri + 48 share the work
+__device__ __forceinline__ int32_t cc_top(const CacheAttnArgs& a, const CaPlan& pl, const CaWork& w, const CcLane& l, bool live) {
+	const int n = live ? (int)((l.width + pl.sp - 1) / pl.sp) : 0;
+	int32_t m = INT32_MIN;
+	for (int i = (threadIdx.x & 63) >> 4; i < n; i += 4) m = max(m, w.pmax[((size_t)i * a.tokens + l.t) * a.NH + l.h]);
+	m = max(m, __shfl_xor(m, 16, 64));
+	return max(m, __shfl_xor(m, 32, 64));
+}
+__device__ __forceinline__ int64_t cc_sum(const CacheAttnArgs& a, const CaPlan& pl, const CaWork& w, const CcLane& l, bool live) {
+	const int n = live ? (int)((l.width + pl.sp - 1) / pl.sp) : 0;
+	int64_t sum = 0;
+	int bad = 0;
+	for (int i = (threadIdx.x & 63) >> 4; i < n; i += 4) {
+		const int64_t x = w.psum[((size_t)i * a.tokens + l.t) * a.NH + l.h];
+		bad |= x < 0;
+		sum += x;
+	}
+	for (int o = 16; o < 64; o *= 2) {
+		sum += __shfl_xor(sum, o, 64);
+		bad |= __shfl_xor(bad, o, 64);
+	}
+	return bad ? -1 : sum;
+}
+
+template <int D>
+__global__ __launch_bounds__(64 * kCaWaves) void k_cc_max(CacheAttnArgs a, CaPlan pl, CaWork w) {
+	constexpr int NC = (D + 63) / 64;
+	__shared__ __attribute__((aligned(16))) int8_t lds[2 * 64 * D];
+	CcJob j;
+	if (!cc_job(a, pl, &j)) return;
+	const CcLane l = cc_lane(a, j);
+	const int g = (threadIdx.x & 63) >> 4;
+	v4i q[NC];
+	cc_load_q<D>(a, l, q);
+	if (j.plane == 0) {  // a token's constants, by every lane that has a head of it
+		SaConst c{0, 0, 0, 0, kPositionOverCap, 0};
+		if (row_pages_ok(a.pg, j.r, j.row.start + j.row.n) && l.t >= 0) {
+			const RowConst rc = row_const(RowScales{a.q_scale[l.t], a.khead_m[j.kvh], a.khead_e[j.kvh]}, a.ln2_q, a.b_q, a.ca_q, l.width);
+			c = SaConst{rc.q_ln2, rc.q_b, rc.q_c, rc.ceil, rc.st, 0};
+		}
+		if (g == 0 && l.t >= 0) w.cst[(size_t)l.t * a.pg.NKV + j.kvh] = c;
+	}
+	const int64_t end = i64min(j.p1, l.width);
+	int32_t m = INT32_MIN;
+	cc_steps<D, false>(a, j, lds, q, [&](int64_t p, int64_t, v4i (&s)[4], const LanePages&, auto&&) {
+		const int left = ca_left(p, end);
+#pragma unroll
+		for (int t = 0; t < 4; ++t)
+#pragma unroll
+			for (int v = 0; v < 4; ++v) m = max(m, t * 16 + v < left ? s[t][v] : INT32_MIN);
+	});
+	m = max(m, __shfl_xor(m, 16, 64));
+	m = max(m, __shfl_xor(m, 32, 64));
+	if (g == 0 && l.t >= 0) w.pmax[((size_t)j.plane * a.tokens + l.t) * a.NH + l.h] = m;
+}
+
+template <int D>
+__global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 4 : 2) void k_cc_sum(CacheAttnArgs a, CaPlan pl, CaWork w) {
+	constexpr int NC = (D + 63) / 64;
+	__shared__ __attribute__((aligned(16))) int8_t lds[2 * 64 * D];
+	__shared__ int s_vote[kCaWaves];
+	CcJob j;
+	if (!cc_job(a, pl, &j)) return;
+	const CcLane l = cc_lane(a, j);
+	const int g = (threadIdx.x & 63) >> 4;
+	const SaConst c = w.cst[(size_t)max(l.t, 0) * a.pg.NKV + j.kvh];
+	const bool live = l.t >= 0 && c.st == kOk;
+	v4i q[NC];
+	cc_load_q<D>(a, l, q);
+	const int32_t top = cc_top(a, pl, w, l, live);
+	const int64_t end = live ? i64min(j.p1, l.width) : 0;
+	int64_t sum = 0;
+	int bad = 0;
+	if (!block_vote(live && !sa_fast(c, l.width), s_vote)) {
+		const SaExp e = sa_exp_of(live ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
+		double acc = 0.0;
+		cc_steps<D, false>(a, j, lds, q, [&](int64_t p, int64_t, v4i (&s)[4], const LanePages&, auto&&) {
+			const int left = ca_left(p, end);
+#pragma unroll
+			for (int t = 0; t < 4; ++t)
+#pragma unroll
+				for (int v = 0; v < 4; ++v) {
+					const double x = sa_exp(e, s[t][v]);
+					acc += t * 16 + v < left ? x : 0.0;
+				}
+		});
+		sum = (int64_t)acc;
+	} else {
+		const double inv = 1.0 / (double)c.q_ln2;
+		cc_steps<D, false>(a, j, lds, q, [&](int64_t p, int64_t, v4i (&s)[4], const LanePages&, auto&&) {
+			const int left = ca_left(p, end);
+#pragma unroll
+			for (int i = 0; i < 16; ++i) {
+				if ((i >> 2) * 16 + (i & 3) >= left) continue;
+				const int64_t x = iexp_fast_cold((int64_t)s[i >> 2][i & 3] - top, c.q_ln2, inv, c.q_b, c.q_c, c.ceil);
+				bad |= x < 0;
+				sum += x < 0 ? 0 : x;
+			}
+		});
+	}
+	for (int o = 16; o < 64; o *= 2) {
+		sum += __shfl_xor(sum, o, 64);
+		bad |= __shfl_xor(bad, o, 64);
+	}
+	if (g == 0 && live) w.psum[((size_t)j.plane * a.tokens + l.t) * a.NH + l.h] = bad ? -1 : sum;
+}
+
+template <int D>
+__global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cc_pv(CacheAttnArgs a, CaPlan pl, CaWork w) {
+	constexpr int NC = (D + 63) / 64, DT = D / 16;
+	__shared__ __attribute__((aligned(16))) int8_t lds[4 * 64 * D];
+	__shared__ int s_vote[kCaWaves];
+	CcJob j;
+	if (!cc_job(a, pl, &j)) return;
+	const CcLane l = cc_lane(a, j);
+	const int g = (threadIdx.x & 63) >> 4;
+	const SaConst c = w.cst[(size_t)max(l.t, 0) * a.pg.NKV + j.kvh];
+	bool live = l.t >= 0 && c.st == kOk;
+	v4i q[NC], acc[DT][3];
+	cc_load_q<D>(a, l, q);
+	const int32_t top = cc_top(a, pl, w, l, live);
+	const int64_t sum = cc_sum(a, pl, w, l, live);
+	if (j.plane == 0 && g == 0 && live) w.hst[(size_t)l.t * a.NH + l.h] = sum < 0 ? kSoftmaxKernelRefusedAfterGateAccepted : kOk;
+	live = live && sum >= 0;
+	const int64_t den = live && sum > 1 ? sum : 1;
+	const int64_t end = live ? i64min(j.p1, l.width) : 0;
+#pragma unroll
+	for (int d = 0; d < DT; ++d) acc[d][0] = acc[d][1] = acc[d][2] = v4i{0, 0, 0, 0};
+	const int form = block_vote((live && !sa_fast(c, l.width) ? 1 : 0) | (den >= ((int64_t)1 << 36) ? 2 : 0), s_vote);
+	auto run = [&](auto&& value) {
+		cc_steps<D, true>(a, j, lds, q, [&](int64_t p, int64_t last, v4i (&s)[4], const LanePages& lp, auto&& multiply) {
+			const int left = ca_left(p, end);
+			int32_t pr[16];
+#pragma unroll
+			for (int t = 0; t < 4; ++t) {
+				const int sh = page_exp(a.pg, lp, lp.ve, p + 16 * t, last);
+#pragma unroll
+				for (int i = 0; i < 4; ++i) {
+					const int32_t x = value(s[t][i], 16 * t + i < left);
+					pr[4 * t + i] = 16 * t + i < left ? x << sh : 0;
+				}
+			}
+			v4i x[3];
+			sa_pack3(pr, x);
+			multiply(x, acc);
+		});
+	};
+	const SaExp e = sa_exp_of(live && !(form & 1) ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
+	const SaProb pb = sa_prob_of((double)den, !(form & 2));
+	if (form == 0) run([&](int32_t x, bool) { return sa_prob<true>(pb, sa_exp(e, x)); });
+	else if (form == 2) run([&](int32_t x, bool) { return sa_prob<false>(pb, sa_exp(e, x)); });
+	else {
+		const double inv = 1.0 / (double)c.q_ln2, dinv = 1.0 / (double)den;
+		run([&](int32_t x, bool in) {
+			return in ? (int32_t)div_rcp_cold(iexp_fast_cold((int64_t)x - top, c.q_ln2, inv, c.q_b, c.q_c, c.ceil) << 15, den, dinv, 32768) : 0;
+		});
+	}
+	if (l.t < 0) return;
+	int32_t* out = w.part + (((size_t)j.plane * a.tokens + l.t) * a.NH + l.h) * D + 4 * g;
+#pragma unroll
+	for (int d = 0; d < DT; ++d) *(v4i*)(out + 16 * d) = acc[d][0] - 256 * acc[d][1] - 65536 * acc[d][2];
+}
+
+// The planes' contexts of one token joined, folded and requantized (checked_chain_funnel.cpp:257-364), U units of
+// four dims to a thread.
+template <int BS, int U>
+__global__ __launch_bounds__(BS) void k_ca_out(CacheAttnArgs a, CaPlan pl, CaWork w) {
+	__shared__ uint32_t s_red[2 * BS / 64];
+	const int r = blockIdx.y, tid = threadIdx.x, N = a.NH * a.pg.D, G = a.NH / a.pg.NKV;
+	const CacheRow c = attn_row(a, r);
 	if (!c.ok) {
-		for (int i = blockIdx.x * 256 + tid; i < c.n; i += gridDim.x * 256) a.status[c.t0 + i] = kPositionOverCap;
+		for (int i = blockIdx.x * BS + tid; i < c.n; i += gridDim.x * BS) a.status[c.t0 + i] = kPositionOverCap;
 		return;
 	}
 	if ((int)blockIdx.x >= c.n) return;
 	const int t = c.t0 + blockIdx.x;
-	if (tid == 0) {
-		s_first = 0xffffffffu;
-		s_max = 0;
+	const int n = (int)((c.start + blockIdx.x + pl.sp) / pl.sp);
+	// the first refusing head, heads of one KV head sharing its constants' status
+	uint32_t first = 0xffffffffu;
+	for (int h = tid; h < a.NH; h += BS) {
+		const int32_t st = w.cst[(size_t)t * a.pg.NKV + h / G].st, x = st != kOk ? st : w.hst[(size_t)t * a.NH + h];
+		if (x != kOk) first = min(first, (uint32_t)h << 8 | (uint32_t)x);
+	}
+	FoldConsts fc[U];
+	v4i v[U];
+	const int32_t* at[U];
+#pragma unroll
+	for (int u = 0; u < U; ++u) {
+		const int i = 4 * min(tid + u * BS, N / 4 - 1);
+		const int32_t* cf = a.ctx_fold + 3 * (i / a.pg.D);
+		fc[u] = fold_consts(cf[0], cf[1], cf[2]);
+		v[u] = v4i{0, 0, 0, 0};
+		at[u] = w.part + (size_t)t * N + i;
+	}
+	constexpr int PK = 8 / U;  // planes in flight
+	for (int k = 0; k < n; k += PK) {
+		v4i x[PK][U];
+#pragma unroll
+		for (int e = 0; e < PK; ++e)
+#pragma unroll
+			for (int u = 0; u < U; ++u) x[e][u] = *(const v4i*)(at[u] + (size_t)min(k + e, n - 1) * a.tokens * N);
+#pragma unroll
+		for (int e = 0; e < PK; ++e)
+#pragma unroll
+			for (int u = 0; u < U; ++u) v[u] += k + e < n ? x[e][u] : v4i{0, 0, 0, 0};
+	}
+	uint32_t mx = 0;
+#pragma unroll
+	for (int u = 0; u < U; ++u)  // a clamped unit repeats the last one
+#pragma unroll
+		for (int x = 0; x < 4; ++x) {
+			v[u][x] = fold_bounded(v[u][x], fc[u]);  // |context| <= 2^15 kMaxUnits, and half of a fold's 2^31 more stays in 32 bits
+			mx = max(mx, (uint32_t)(v[u][x] < 0 ? -v[u][x] : v[u][x]));
+		}
+	mx = wave_max32(mx);
+	first = ~wave_max32(~first);
+	if ((tid & 63) == 0) {
+		s_red[tid >> 6] = mx;
+		s_red[BS / 64 + (tid >> 6)] = first;
 	}
 	__syncthreads();
-	for (int h = tid; h < a.NH; h += 256) {
-		const int32_t st = hst[(size_t)t * a.NH + h];
-		if (st != kOk) atomicMin(&s_first, (uint32_t)h << 8 | (uint32_t)st);
+#pragma unroll
+	for (int i = 0; i < BS / 64; ++i) {
+		mx = max(mx, s_red[i]);
+		first = min(first, s_red[BS / 64 + i]);
 	}
-	__syncthreads();
-	if (s_first != 0xffffffffu) {
-		if (tid == 0) a.status[t] = (int32_t)(s_first & 0xff);
+	if (first != 0xffffffffu) {
+		if (tid == 0) a.status[t] = (int32_t)(first & 0xff);
 		return;
 	}
-	auto value = [&](int i) {
-		const int32_t* f = a.ctx_fold + 3 * (i / a.pg.D);
-		return fold_bounded(ctx[(size_t)t * N + i], fold_consts(f[0], f[1], f[2]));
-	};
-	uint32_t mx = 0;
-	for (int i = tid; i < N; i += 256) {
-		const int32_t v = value(i);
-		mx = max(mx, (uint32_t)(v < 0 ? -v : v));
-	}
-	atomicMax(&s_max, mx);
-	__syncthreads();
 	FunnelPlan plan;
-	const int32_t st = funnel_plan(__builtin_amdgcn_readfirstlane(s_max), nullptr, 0, a.site, &plan);
+	const int32_t st = funnel_plan(__builtin_amdgcn_readfirstlane(mx), nullptr, 0, a.site, &plan);
 	if (tid == 0) {
 		a.status[t] = st;
 		if (st == kOk) a.scales[t] = plan.out;
 	}
 	if (st != kOk) return;
-	for (int i = tid; i < N; i += 256) a.codes[(size_t)t * N + i] = requant_code_f(value(i), plan.f);
+#pragma unroll
+	for (int u = 0; u < U; ++u) {
+		const int i = tid + u * BS;
+		if (4 * i < N) {
+			uint32_t o = 0;
+#pragma unroll
+			for (int x = 0; x < 4; ++x) o |= (uint32_t)(uint8_t)requant_code_f(v[u][x], plan.f) << 8 * x;
+			((unaligned4*)(a.codes + (size_t)t * N + 4 * i))->v = (int32_t)o;
+		}
+	}
 }
 
 }  // namespace sslm
@@ -845,16 +1437,79 @@ void cache_store(const CacheStoreArgs& a, hipStream_t s) {
 	}
 }
 
-size_t cache_attn_workspace(int rows, int tokens, int max_new, int NH, int NKV, int D, int lp, int64_t max_width) {
-	return up256((size_t)tokens * NH * D * 4) + up256((size_t)tokens * NH * 4);
+constexpr int kCaTargetWaves = 4096;  // single tokens; chunks aim at as many as kCaTargetBlocks blocks of four
+constexpr int kCaTargetBlocks = 1024;
+
+// Planes: as many as fill the chip, at most some 4 sqrt(steps) of them, as their maxima and contexts are joined by
+// each (token, head) and token.
+static CaPlan ca_plan(int rows, int tokens, int max_new, int NH, int NKV, int64_t max_width) {
+	CaPlan p{};
+	const int G = NH / NKV;
+	p.ht = (G + 15) / 16;
+	p.groups = (int)((int64_t)tokens * G / 64 + rows);
+	const int64_t units = max_new == 1 ? (int64_t)rows * NKV * p.ht : (int64_t)p.groups * NKV;
+	const int64_t target = max_new == 1 ? kCaTargetWaves : kCaTargetBlocks;
+	const int64_t steps = (max_width + 127) / 128;
+	int64_t planes = std::min(steps, std::max<int64_t>(1, target / units));
+	planes = std::min(planes, std::max<int64_t>(1, (int64_t)std::sqrt(16.0 * (double)steps)));
+	p.sp = (int)((steps + planes - 1) / planes * 128);
+	p.planes = (int)((max_width + p.sp - 1) / p.sp);
+	p.ps = 8192;
+	p.parts = max_new == 1 ? (int)((max_width + p.ps - 1) / p.ps) : p.planes;
+	p.wpad = steps * 128;
+	return p;
+}
+
+static size_t ca_work(const CaPlan& p, int tokens, int max_new, int NH, int NKV, int D, char* base, CaWork* w) {
+	size_t at = 0;
+	auto take = [&](size_t n) {
+		char* q = base + at;
+		at += up256(n);
+		return q;
+	};
+	const size_t th = (size_t)tokens * NH;
+	w->cst = (SaConst*)take((size_t)tokens * NKV * sizeof(SaConst));
+	w->pmax = (int32_t*)take(p.planes * th * 4);
+	w->top = (int32_t*)take(th * 4);
+	w->psum = (int64_t*)take(p.parts * th * 8);
+	w->part = (int32_t*)take(p.planes * th * D * 4);
+	w->hst = (int32_t*)take(th * 4);
+	w->scores = (int32_t*)take(max_new == 1 ? th * p.wpad * 4 : 0);
+	return at;
+}
+
+size_t cache_attn_workspace(int rows, int tokens, int max_new, int NH, int NKV, int D, int64_t max_width) {
+	const CaPlan p = ca_plan(rows, tokens, max_new, NH, NKV, max_width);
+	// a launch's blocks
+	if ((int64_t)rows * NKV * p.ht * p.planes / kCaWaves >= 1ll << 30 || ((int64_t)p.planes * NKV + 8) * p.groups >= 1ll << 30) return 0;
+	CaWork w;
+	return ca_work(p, tokens, max_new, NH, NKV, D, nullptr, &w);
 }
 
 template <int D>
 static void attn_launch(const CacheAttnArgs& a, hipStream_t s) {
-	int32_t* ctx = (int32_t*)a.ws;
-	int32_t* hst = (int32_t*)((char*)a.ws + up256((size_t)a.tokens * a.NH * D * 4));
-	hipLaunchKernelGGL(k_ca_head<D>, dim3(a.max_new, a.rows, a.NH), dim3(256), 0, s, a, ctx, hst);
-	hipLaunchKernelGGL(k_ca_out, dim3(a.max_new, a.rows), dim3(256), 0, s, a, ctx, hst);
+	const int NKV = a.pg.NKV, N = a.NH * D;
+	const CaPlan p = ca_plan(a.rows, a.tokens, a.max_new, a.NH, NKV, a.max_width);
+	CaWork w;
+	ca_work(p, a.tokens, a.max_new, a.NH, NKV, D, (char*)a.ws, &w);
+	const dim3 bs(64 * kCaWaves);
+	if (a.max_new == 1) {
+		const dim3 grid((unsigned)(((int64_t)a.rows * NKV * p.ht * p.planes + kCaWaves - 1) / kCaWaves));
+		hipLaunchKernelGGL(k_cd_scores<D>, grid, bs, 0, s, a, p, w);
+		hipLaunchKernelGGL(k_cd_sum, dim3(p.parts, a.NH, a.rows), dim3(256), 0, s, a, p, w);
+		if (a.NH / NKV <= 8) hipLaunchKernelGGL((k_cd_pv<D, 2>), grid, bs, 0, s, a, p, w);
+		else hipLaunchKernelGGL((k_cd_pv<D, 1>), grid, bs, 0, s, a, p, w);
+	} else {
+		const dim3 grid((unsigned)((p.planes * NKV + 7) / 8 * 8 * p.groups));
+		hipLaunchKernelGGL(k_cc_max<D>, grid, bs, 0, s, a, p, w);
+		hipLaunchKernelGGL(k_cc_sum<D>, grid, bs, 0, s, a, p, w);
+		hipLaunchKernelGGL(k_cc_pv<D>, grid, bs, 0, s, a, p, w);
+	}
+	const dim3 out(a.max_new, a.rows);
+	if (N <= 1024) hipLaunchKernelGGL((k_ca_out<256, 1>), out, dim3(256), 0, s, a, p, w);
+	else if (N <= 2048) hipLaunchKernelGGL((k_ca_out<512, 1>), out, dim3(512), 0, s, a, p, w);
+	else if (N <= 4096) hipLaunchKernelGGL((k_ca_out<1024, 1>), out, dim3(1024), 0, s, a, p, w);
+	else hipLaunchKernelGGL((k_ca_out<1024, 2>), out, dim3(1024), 0, s, a, p, w);
 }
 
 void cache_attn(const CacheAttnArgs& a, hipStream_t s) {
@@ -986,7 +1641,7 @@ size_t sslm_hip_cache_attention_workspace(int32_t rows, int32_t tokens, int32_t 
 	if (lp < 0 || rows < 1 || rows > kMaxRows || tokens < 1 || max_new < 1 || max_new > tokens || !heads_ok(heads, kv_heads, head_dim) ||
 	    max_width < 1 || max_width > SSLM_HIP_CACHE_MAX_WIDTH)
 		return 0;
-	return cache_attn_workspace(rows, tokens, max_new, heads, kv_heads, head_dim, lp, max_width);
+	return cache_attn_workspace(rows, tokens, max_new, heads, kv_heads, head_dim, max_width);
 }
 
 sslm_status sslm_hip_cache_attention(const sslm_hip_cache_attention_args* p, void* workspace, size_t workspace_bytes, void* stream) {
