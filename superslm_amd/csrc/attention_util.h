@@ -237,18 +237,19 @@ __device__ __forceinline__ void sa_pack(const int32_t (&p)[16], v4i* lo, v4i* nh
 
 // The same for p up to 2^23 (a probability times 2^e, e <= 8) as three operands, p = x[0] - 256 x[1] - 65536 x[2]: p's
 // low byte taken as signed, and n = floor((127 - p) / 256) in [-2^15, 0] as its own signed low byte and the rest in [-128, 0].
+__device__ __forceinline__ void sa_pack3_word(int32_t p0, int32_t p1, int32_t p2, int32_t p3, uint32_t (&x)[3]) {
+	const int32_t n0 = 127 - p0, n1 = 127 - p1, n2 = 127 - p2, n3 = 127 - p3;
+	x[0] = __builtin_amdgcn_perm(p1, p0, 0x0c0c0400) | __builtin_amdgcn_perm(p3, p2, 0x0c0c0400) << 16;
+	x[1] = __builtin_amdgcn_perm(n1, n0, 0x0c0c0501) | __builtin_amdgcn_perm(n3, n2, 0x0c0c0501) << 16;
+	x[2] = __builtin_amdgcn_perm(n1 + 32768, n0 + 32768, 0x0c0c0602) | __builtin_amdgcn_perm(n3 + 32768, n2 + 32768, 0x0c0c0602) << 16;
+}
 __device__ __forceinline__ void sa_pack3(const int32_t (&p)[16], v4i (&x)[3]) {
 #pragma unroll
 	for (int t = 0; t < 4; ++t) {
-		int32_t n[4];
+		uint32_t y[3];
+		sa_pack3_word(p[4 * t], p[4 * t + 1], p[4 * t + 2], p[4 * t + 3], y);
 #pragma unroll
-		for (int i = 0; i < 4; ++i) n[i] = 127 - p[4 * t + i];
-		const uint32_t a = __builtin_amdgcn_perm(p[4 * t + 1], p[4 * t], 0x0c0c0400), b = __builtin_amdgcn_perm(p[4 * t + 3], p[4 * t + 2], 0x0c0c0400);
-		x[0][t] = (int)(a | b << 16);
-		const uint32_t c = __builtin_amdgcn_perm(n[1], n[0], 0x0c0c0501), d = __builtin_amdgcn_perm(n[3], n[2], 0x0c0c0501);
-		x[1][t] = (int)(c | d << 16);
-		const uint32_t e = __builtin_amdgcn_perm(n[1] + 32768, n[0] + 32768, 0x0c0c0602), f = __builtin_amdgcn_perm(n[3] + 32768, n[2] + 32768, 0x0c0c0602);
-		x[2][t] = (int)(e | f << 16);
+		for (int n = 0; n < 3; ++n) x[n][t] = (int)y[n];
 	}
 }
 

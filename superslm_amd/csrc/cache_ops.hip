@@ -629,13 +629,13 @@ __global__ __launch_bounds__(kStoreBlock) void k_store_span(CacheStoreArgs a, in
 // head and a range of positions, a "plane" of sp.  The softmax's maximum and sum run over the whole row and each
 // probability is rounded by itself, so nothing is rescaled: maxima, sums and P V are launches of their own, and the
 // planes' integers join exactly in any order.
-// Single tokens: a tile is one token's heads, waves work alone, scores are kept for the later launches (4 G bytes a
-// position beside the 2 D of its K and V).  Chunks: four neighbouring tiles of a row share each step of 64 positions that
+// Single tokens: a tile is one token's heads, four waves take the positions in turn, scores are kept for the later
+// launches (4 G bytes a position beside the 2 D of its K and V).  Chunks: four neighbouring tiles of a row share each step of 64 positions that
 // their block stages, and the scores are computed again, 8 MFMAs a step at D = 128.
 struct CaPlan {
 	int ht;          // single tokens: tiles of a token's heads
 	int groups;      // chunks: blocks of 64 query rows, at least those of every row together
-	int sp, planes;  // positions of a plane (a multiple of 128), planes of the widest row
+	int sp, planes;  // positions of a plane (a multiple of 256), planes of the widest row
 	int ps, parts;   // positions of one block of sums, blocks of the widest row
 	int64_t wpad;    // kept scores of a (token, head)
 };
@@ -685,9 +685,10 @@ __device__ __forceinline__ bool row_pages_ok(const Pages& g, int r, int64_t widt
 }
 
 // Rows of 64 positions from p (a multiple of 64) as a wave loads them: the page of each 16 of them is the same for the
-// wave, slots past the row's end are still the page's own.
+// wave, slots past the row's end are still the page's own.  Not `real`: 16 bytes of a page once, whatever they are, so that the loads in
+// flight are the same number on every path.
 template <int D>
-__device__ __forceinline__ void load_rows(SaRows<D>& x, const Pages& g, const LanePages& lp, int64_t p, int64_t last, int64_t off) {
+__device__ __forceinline__ void load_rows(SaRows<D>& x, const Pages& g, const LanePages& lp, int64_t p, int64_t last, int64_t off, bool real) {
 	constexpr int PER = D / 16, R = 64 / PER;  // rows of one load
 	const int lane = threadIdx.x & 63, mask = min(1 << g.lp, 64) - 1, high = (int)(p & ((1 << g.lp) - 1));
 	auto page = [&](int row) {
@@ -701,7 +702,7 @@ __device__ __forceinline__ void load_rows(SaRows<D>& x, const Pages& g, const La
 			const int8_t* next = page(u * R + 16);
 			at = lane / PER >= 16 ? next : at;
 		}
-		return at + ((high & ~63) + (row & mask)) * D + lane % PER * 16;
+		return at + (real ? ((high & ~63) + (row & mask)) * D + lane % PER * 16 : 0);
 	});
 }
 // the exponents of 16 positions from p
@@ -709,19 +710,27 @@ __device__ __forceinline__ int page_exp(const Pages& g, const LanePages& lp, int
 	return __builtin_amdgcn_readlane(e, (int)((i64min(p, last) >> g.lp) - lp.first));
 }
 
-// A single token's wave: number w of the launch's.
+// Which bits some live lane of the block has set: what its waves branch on alike.
+__device__ __forceinline__ int block_vote(int bits, int* s) {
+	const int all = (__any(bits & 1) ? 1 : 0) | (__any(bits & 2) ? 2 : 0);
+	if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = all;
+	__syncthreads();
+	return __builtin_amdgcn_readfirstlane(s[0] | s[1] | s[2] | s[3]);
+}
+
+// A single token's block: a plane of a (row, KV head, tile of heads).  A step is 256 positions, 64 to a wave.
+constexpr int kCdStep = 64 * kCaWaves;
 struct CdJob {
 	int r, t, kvh, tile, plane, h0, heads;  // h0: the tile's first head
 	int64_t width, p0, p1;
 	CacheRow row;
 };
 __device__ __forceinline__ bool cd_job(const CacheAttnArgs& a, const CaPlan& pl, CdJob* j) {
-	const int w = (int)blockIdx.x * kCaWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), G = a.NH / a.pg.NKV;
+	const int w = blockIdx.x, G = a.NH / a.pg.NKV;
 	j->plane = w % pl.planes;
 	j->tile = w / pl.planes % pl.ht;
 	j->kvh = w / pl.planes / pl.ht % a.pg.NKV;
 	j->r = w / pl.planes / pl.ht / a.pg.NKV;
-	if (j->r >= a.rows) return false;
 	j->row = attn_row(a, j->r);
 	if (!j->row.ok || j->row.n < 1) return false;
 	j->t = j->row.t0;
@@ -733,46 +742,39 @@ __device__ __forceinline__ bool cd_job(const CacheAttnArgs& a, const CaPlan& pl,
 	return j->p0 < j->p1;
 }
 
-// The scores of a plane, kept, and their maxima.  The wave of a row's first plane also settles its constants.
+// The scores of a plane, kept, and their maxima.  The first wave of a row's first plane also settles its constants.
 template <int D>
 __global__ __launch_bounds__(64 * kCaWaves) void k_cd_scores(CacheAttnArgs a, CaPlan pl, CaWork w) {
 	constexpr int NC = (D + 63) / 64;
 	__shared__ __attribute__((aligned(16))) int8_t s_k[kCaWaves][32 * D];
-	const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4;
+	__shared__ int32_t s_m[kCaWaves][16];
+	const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	CdJob j;
 	if (!cd_job(a, pl, &j)) return;
-	int8_t* lds = s_k[threadIdx.x >> 6];
+	int8_t* lds = s_k[wave];
 	const bool mine = ri < j.heads;
 	const int h = j.h0 + (mine ? ri : 0);
 	v4i q[NC];
 #pragma unroll
 	for (int c = 0; c < NC; ++c) q[c] = mine && c * 64 + g * 16 < D ? load16(a.q + ((size_t)j.t * a.NH + h) * D + c * 64 + g * 16) : v4i{0, 0, 0, 0};
-	if (j.plane == 0 && j.tile == 0) {
-		SaConst c{0, 0, 0, 0, kPositionOverCap, 0};
-		if (row_pages_ok(a.pg, j.r, j.width)) {
-			const RowConst rc = row_const(RowScales{a.q_scale[j.t], a.khead_m[j.kvh], a.khead_e[j.kvh]}, a.ln2_q, a.b_q, a.ca_q, j.width);
-			c = SaConst{rc.q_ln2, rc.q_b, rc.q_c, rc.ceil, rc.st, 0};
-		}
-		if (lane == 0) w.cst[(size_t)j.t * a.pg.NKV + j.kvh] = c;
-	}
 	int32_t* out = w.scores + ((size_t)j.t * a.NH + h) * pl.wpad + 4 * g;
 	const int64_t off = a.pg.k_off + ((int64_t)j.kvh << a.pg.lp) * D;
 	int32_t m = INT32_MIN;
 	for (int64_t s0 = j.p0; s0 < j.p1; s0 = pages_end(a.pg, s0)) {
 		const int64_t s1 = i64min(j.p1, pages_end(a.pg, s0)), last = s1 - 1;
 		LanePages lp;
-		if (!lane_pages(a.pg, j.r, j.kvh, s0, last, &lp)) return;
+		if (!lane_pages(a.pg, j.r, j.kvh, s0, last, &lp)) break;
 		SaRows<D> k[2];
-		load_rows(k[0], a.pg, lp, s0, last, off);
-		if (s0 + 64 < s1) load_rows(k[1], a.pg, lp, s0 + 64, last, off);
-		for (int64_t p0 = s0; p0 < s1; p0 += 128) {
+#pragma unroll
+		for (int b = 0; b < 2; ++b) load_rows(k[b], a.pg, lp, s0 + 64 * wave + b * kCdStep, last, off, s0 + 64 * wave + b * kCdStep < s1);
+		for (int64_t p0 = s0 + 64 * wave; p0 < s1; p0 += 2 * kCdStep) {
 #pragma unroll
 			for (int b = 0; b < 2; ++b) {
-				const int64_t p = p0 + 64 * b;
+				const int64_t p = p0 + b * kCdStep;
 				if (p >= s1) break;
 				v4i s[4] = {};
 				k[b].scores(lds, q, s);
-				if (p + 128 < s1) load_rows(k[b], a.pg, lp, p + 128, last, off);
+				load_rows(k[b], a.pg, lp, p + 2 * kCdStep, last, off, p + 2 * kCdStep < s1);
 				const int left = (int)i64min(s1 - p, 64) - 4 * g;
 #pragma unroll
 				for (int t = 0; t < 4; ++t) {
@@ -787,12 +789,25 @@ __global__ __launch_bounds__(64 * kCaWaves) void k_cd_scores(CacheAttnArgs a, Ca
 			}
 		}
 	}
+	if (j.plane == 0 && j.tile == 0 && wave == 0) {
+		SaConst c{0, 0, 0, 0, kPositionOverCap, 0};
+		if (row_pages_ok(a.pg, j.r, j.width)) {
+			const RowConst rc = row_const(RowScales{a.q_scale[j.t], a.khead_m[j.kvh], a.khead_e[j.kvh]}, a.ln2_q, a.b_q, a.ca_q, j.width);
+			c = SaConst{rc.q_ln2, rc.q_b, rc.q_c, rc.ceil, rc.st, 0};
+		}
+		if (lane == 0) w.cst[(size_t)j.t * a.pg.NKV + j.kvh] = c;
+	}
 	m = max(m, __shfl_xor(m, 16, 64));
 	m = max(m, __shfl_xor(m, 32, 64));
-	if (g == 0 && mine) w.pmax[((size_t)j.plane * a.tokens + j.t) * a.NH + h] = m;
+	if (g == 0) s_m[wave][ri] = m;
+	__syncthreads();
+	if (threadIdx.x < j.heads)
+		w.pmax[((size_t)j.plane * a.tokens + j.t) * a.NH + j.h0 + threadIdx.x] = max(max(s_m[0][threadIdx.x], s_m[1][threadIdx.x]), max(s_m[2][threadIdx.x], s_m[3][threadIdx.x]));
 }
 
-// The sum of one (token, head) over a part of its positions, from the kept scores.
+// The sum of one (token, head) over a part of its positions, from the kept scores: all of a thread's are loaded ahead of the
+// constants and maxima that they wait for.
+constexpr int kCdSumLoads = 4, kCdSum = 1024 * kCdSumLoads;
 __global__ __launch_bounds__(256) void k_cd_sum(CacheAttnArgs a, CaPlan pl, CaWork w) {
 	__shared__ int32_t s_m[4];
 	__shared__ int64_t s_s[4];
@@ -803,35 +818,42 @@ __global__ __launch_bounds__(256) void k_cd_sum(CacheAttnArgs a, CaPlan pl, CaWo
 	const int64_t width = row.start + 1, p0 = (int64_t)part * pl.ps, p1 = i64min(width, p0 + pl.ps);
 	if (p0 >= p1) return;
 	const int32_t* sc = w.scores + ((size_t)t * a.NH + h) * pl.wpad;
+	v4i x[kCdSumLoads];
+#pragma unroll
+	for (int i = 0; i < kCdSumLoads; ++i) x[i] = *(const v4i*)(sc + i64min(p0 + 1024 * i + 4 * tid, (p1 - 1) & ~3ll));
 	const SaConst c = w.cst[(size_t)t * a.pg.NKV + kvh];
-	if (c.st != kOk) return;
 	int32_t top = INT32_MIN;
 	const int n = (int)((width + pl.sp - 1) / pl.sp);
 	for (int i = tid; i < n; i += 256) top = max(top, w.pmax[((size_t)i * a.tokens + t) * a.NH + h]);
 	for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
 	if ((tid & 63) == 0) s_m[tid >> 6] = top;
 	__syncthreads();
+	if (c.st != kOk) return;
 	top = max(max(s_m[0], s_m[1]), max(s_m[2], s_m[3]));
 	int64_t sum = 0;
 	int bad = 0;
 	if (sa_fast(c, width)) {
 		const SaExp e = sa_exp_of(c, top);
 		double acc = 0.0;
-		for (int64_t p = p0 + 4 * tid; p < p1; p += 1024) {
-			const v4i x = *(const v4i*)(sc + p);
 #pragma unroll
-			for (int i = 0; i < 4; ++i) {
-				const double y = sa_exp(e, x[i]);
-				acc += p + i < p1 ? y : 0.0;
+		for (int i = 0; i < kCdSumLoads; ++i) {
+			const int64_t p = p0 + 1024 * i + 4 * tid;
+			if (p0 + 1024 * i >= p1) break;
+#pragma unroll
+			for (int k = 0; k < 4; ++k) {
+				const double y = sa_exp(e, x[i][k]);
+				acc += p + k < p1 ? y : 0.0;
 			}
 		}
 		sum = (int64_t)acc;
 	} else {
 		const double inv = 1.0 / (double)c.q_ln2;
-		for (int64_t p = p0 + tid; p < p1; p += 256) {
-			const int64_t x = iexp_fast_cold((int64_t)sc[p] - top, c.q_ln2, inv, c.q_b, c.q_c, c.ceil);
-			bad |= x < 0;
-			sum += x < 0 ? 0 : x;
+#pragma unroll
+		for (int i = 0; i < 4 * kCdSumLoads; ++i) {
+			if (p0 + 1024 * (i >> 2) + 4 * tid + (i & 3) >= p1) continue;
+			const int64_t y = iexp_fast_cold((int64_t)x[i >> 2][i & 3] - top, c.q_ln2, inv, c.q_b, c.q_c, c.ceil);
+			bad |= y < 0;
+			sum += y < 0 ? 0 : y;
 		}
 	}
 	for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -849,99 +871,131 @@ __global__ __launch_bounds__(256) void k_cd_sum(CacheAttnArgs a, CaPlan pl, CaWo
 	}
 }
 
-// P V of a plane.  Where at most eight heads would leave half of a tile's columns empty, columns 8 .. 15 hold
-// the same heads at the next 64 positions (F = 2), so that i-exp and probabilities run on full waves.
-template <int D, int F>
+// P V of a plane, a block of four waves: probabilities of 256 positions at a time, a wave to a head, go to LDS as three
+// int8 operands (sa_pack3) in the order the MFMAs read them, then each wave multiplies 64 of the positions; the waves'
+// contexts are joined at the end.  The next 256 positions' scores and V rows are in flight meanwhile.
+template <int D, int R>
 __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cd_pv(CacheAttnArgs a, CaPlan pl, CaWork w) {
-	constexpr int DT = D / 16, GP = 16 / F;
-	__shared__ __attribute__((aligned(16))) int8_t s_v[kCaWaves][32 * D];
-	const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4, col = ri % GP, half = ri / GP;
+	constexpr int DT = D / 16;
+	// [parity][operand][64 positions' bytes of 16 heads], V staged by each wave; the join reuses it: [wave][dt][lane]
+	struct Step {
+		uint32_t p[2][3][kCaWaves][256];
+		int8_t v[kCaWaves][32 * D];
+	};
+	union Lds {
+		Step s;
+		v4i join[kCaWaves][DT][64];
+	};
+	__shared__ __attribute__((aligned(16))) Lds lds;
+	__shared__ int s_vote[kCaWaves];
+	const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	CdJob j;
 	if (!cd_job(a, pl, &j)) return;
-	int8_t* lds = s_v[threadIdx.x >> 6];
-	const SaConst c = w.cst[(size_t)j.t * a.pg.NKV + j.kvh];
-	if (c.st != kOk) return;
-	bool live = col < j.heads;
-	const int h = j.h0 + (live ? col : 0);
-	const size_t th = (size_t)j.t * a.NH + h;
-	const int32_t top = w.top[th];
-	int64_t sum = 0;
-	bool bad = false;
-	const int parts = (int)((j.width + pl.ps - 1) / pl.ps);
-	for (int i = 0; i < parts; ++i) {
-		const int64_t x = w.psum[(size_t)i * a.tokens * a.NH + th];
-		bad |= x < 0;
-		sum += x;
-	}
-	if (j.plane == 0 && g == 0 && half == 0 && live) w.hst[th] = bad ? kSoftmaxKernelRefusedAfterGateAccepted : kOk;
-	live = live && !bad;
-	const int64_t den = live && sum > 1 ? sum : 1;
-	const bool fast = sa_fast(c, j.width), small = fast && !__any(den >= ((int64_t)1 << 36));
 	const int64_t off = a.pg.v_off + ((int64_t)j.kvh << a.pg.lp) * D;
-	const int32_t* sc = w.scores + th * pl.wpad + half * 64 + 4 * g;
-	const SaExp e = sa_exp_of(fast ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
-	const SaProb pb = sa_prob_of((double)den, small);
-	const double inv = 1.0 / (double)c.q_ln2, dinv = 1.0 / (double)den;
+	const SaConst c = w.cst[(size_t)j.t * a.pg.NKV + j.kvh];
+	const int parts = (int)((j.width + pl.ps - 1) / pl.ps);
+	// this wave's heads wave, wave + 4, ..: the maximum and the sum
+	int32_t top[R];
+	int64_t den[R];
+	int refused = 0, form = 0;
+#pragma unroll
+	for (int i = 0; i < R; ++i) {
+		const size_t th = (size_t)j.t * a.NH + j.h0 + min(wave + 4 * i, j.heads - 1);
+		top[i] = w.top[th];
+		int64_t sum = 0;
+		bool bad = false;
+		for (int k = 0; k < parts; ++k) {
+			const int64_t x = w.psum[(size_t)k * a.tokens * a.NH + th];
+			bad |= x < 0;
+			sum += x;
+		}
+		refused |= bad ? 1 << i : 0;
+		den[i] = !bad && sum > 1 ? sum : 1;
+		form |= den[i] >= (int64_t)1 << 36 ? 2 : 0;
+		if (c.st == kOk && j.plane == 0 && lane == 0 && wave + 4 * i < j.heads) w.hst[th] = bad ? kSoftmaxKernelRefusedAfterGateAccepted : kOk;
+	}
+	if (c.st != kOk) return;
+	form = block_vote(form | !sa_fast(c, j.width), s_vote);
 	v4i acc[DT][3];
 #pragma unroll
 	for (int d = 0; d < DT; ++d) acc[d][0] = acc[d][1] = acc[d][2] = v4i{0, 0, 0, 0};
-	for (int64_t s0 = j.p0; s0 < j.p1; s0 = pages_end(a.pg, s0)) {
-		const int64_t s1 = i64min(j.p1, pages_end(a.pg, s0)), last = s1 - 1;
-		LanePages lp;
-		if (!lane_pages(a.pg, j.r, j.kvh, s0, last, &lp)) return;
-		SaRows<D> v[F];
-		v4i s[4];
-		auto scores = [&](int64_t p) {
+	// value(i, score, in): the probability of a score of head wave + 4 i
+	auto run = [&](auto&& value) {
+		int b = 0;
+		for (int64_t s0 = j.p0; s0 < j.p1; s0 = pages_end(a.pg, s0)) {
+			const int64_t s1 = i64min(j.p1, pages_end(a.pg, s0)), last = s1 - 1;
+			LanePages lp;
+			if (!lane_pages(a.pg, j.r, j.kvh, s0, last, &lp)) return;  // alike for the block's waves
+			SaRows<D> v;
+			v4i s[R];
+			auto scores = [&](int64_t p) {
 #pragma unroll
-			for (int t = 0; t < 4; ++t) s[t] = *(const v4i*)(sc + p + 16 * t);
-		};
-		scores(s0);
-#pragma unroll
-		for (int f = 0; f < F; ++f) load_rows(v[f], a.pg, lp, i64min(s0 + 64 * f, last & ~63ll), last, off);
-		for (int64_t p = s0; p < s1; p += 64 * F) {
-			const int left = (int)i64min(s1 - p - half * 64, 64) - 4 * g;
-			int32_t pr[16];
-			auto exps = [&](auto&& value) {
-#pragma unroll
-				for (int t = 0; t < 4; ++t) {
-					int sh = page_exp(a.pg, lp, lp.ve, p + 16 * t, last);
-					if (F == 2) sh = half ? page_exp(a.pg, lp, lp.ve, p + 64 + 16 * t, last) : sh;
-#pragma unroll
-					for (int i = 0; i < 4; ++i) {
-						const int32_t x = value(s[t][i], 16 * t + i < left);
-						pr[4 * t + i] = 16 * t + i < left && live ? x << sh : 0;
-					}
-				}
+				for (int i = 0; i < R; ++i)
+					s[i] = *(const v4i*)(w.scores + ((size_t)j.t * a.NH + j.h0 + min(wave + 4 * i, j.heads - 1)) * pl.wpad + p + 4 * lane);
 			};
-			if (small) exps([&](int32_t x, bool) { return sa_prob<true>(pb, sa_exp(e, x)); });
-			else if (fast) exps([&](int32_t x, bool) { return sa_prob<false>(pb, sa_exp(e, x)); });
-			else
-				exps([&](int32_t x, bool in) {
-					return in && live ? (int32_t)div_rcp_cold(iexp_fast_cold((int64_t)x - top, c.q_ln2, inv, c.q_b, c.q_c, c.ceil) << 15, den, dinv, 32768) : 0;
-				});
-			if (p + 64 * F < s1) scores(p + 64 * F);
-			v4i x[3];
-			sa_pack3(pr, x);
+			scores(s0);
+			load_rows(v, a.pg, lp, s0 + 64 * wave, last, off, s0 + 64 * wave < s1);
+			for (int64_t p = s0; p < s1; p += kCdStep) {
+				const int left = (int)i64min(s1 - p - 4 * lane, 4);
+				// lane 4 i + k of a head has positions 16 i + 4 k .. + 3: word i of the operand's lane (head, k)
+				const int sh = __shfl(lp.ve, (int)((i64min(p + 4 * lane, last) >> a.pg.lp) - lp.first), 64);
 #pragma unroll
-			for (int f = 0; f < F; ++f) {
-				if (p + 64 * f >= s1) break;
-				v4i y[3];
+				for (int i = 0; i < R; ++i) {
+					const int head = wave + 4 * i;
+					if (head >= j.heads) break;
+					int32_t pr[4];
 #pragma unroll
-				for (int i = 0; i < 3; ++i) y[i] = F == 1 || half == f ? x[i] : v4i{0, 0, 0, 0};
-				v[f].multiply(lds, y, acc);
-				if (p + 64 * (f + F) < s1) load_rows(v[f], a.pg, lp, p + 64 * (f + F), last, off);
+					for (int k = 0; k < 4; ++k) {
+						const int32_t y = value(i, s[i][k], k < left);
+						pr[k] = k < left && !(refused >> i & 1) ? y << sh : 0;
+					}
+					uint32_t x[3];
+					sa_pack3_word(pr[0], pr[1], pr[2], pr[3], x);
+					const int at = head * 16 + (lane & 3) * 4 + (lane >> 2 & 3);
+#pragma unroll
+					for (int n = 0; n < 3; ++n) lds.s.p[b][n][lane >> 4][at] = x[n];
+				}
+				scores(p + kCdStep < s1 ? p + kCdStep : p);
+				__syncthreads();
+				v4i x[3];
+#pragma unroll
+				for (int n = 0; n < 3; ++n) x[n] = *(const v4i*)&lds.s.p[b][n][wave][ri * 16 + g * 4];
+				v.multiply(lds.s.v[wave], x, acc);
+				load_rows(v, a.pg, lp, p + kCdStep + 64 * wave, last, off, p + kCdStep + 64 * wave < s1);
+				b ^= 1;
 			}
 		}
+	};
+	if (!(form & 1)) {
+		SaExp e = sa_exp_of(c, 0);
+		const int32_t add = e.add;
+		SaProb pb[R];
+#pragma unroll
+		for (int i = 0; i < R; ++i) pb[i] = sa_prob_of((double)den[i], form == 0);
+		auto exp = [&](int i, int32_t x) {
+			e.add = add - top[i];
+			return sa_exp(e, x);
+		};
+		if (form == 0) run([&](int i, int32_t x, bool) { return sa_prob<true>(pb[i], exp(i, x)); });
+		else run([&](int i, int32_t x, bool) { return sa_prob<false>(pb[i], exp(i, x)); });
+	} else {
+		const double inv = 1.0 / (double)c.q_ln2;
+		run([&](int i, int32_t x, bool in) {
+			return in ? (int32_t)div_rcp_cold(iexp_fast_cold((int64_t)x - top[i], c.q_ln2, inv, c.q_b, c.q_c, c.ceil) << 15, den[i], 1.0 / (double)den[i], 32768) : 0;
+		});
 	}
-	int32_t* out = w.part + (((size_t)j.plane * a.tokens + j.t) * a.NH + h) * D + 4 * g;
+	__syncthreads();
 #pragma unroll
-	for (int d = 0; d < DT; ++d) {
-		v4i y = acc[d][0] - 256 * acc[d][1] - 65536 * acc[d][2];
-		if (F == 2) {
+	for (int d = 0; d < DT; ++d) lds.join[wave][d][lane] = acc[d][0] - 256 * acc[d][1] - 65536 * acc[d][2];
+	__syncthreads();
 #pragma unroll
-			for (int i = 0; i < 4; ++i) y[i] += __shfl_xor(y[i], 8, 64);
-		}
-		if (col < j.heads && half == 0) *(v4i*)(out + 16 * d) = y;
+	for (int i = 0; i < (DT + kCaWaves - 1) / kCaWaves; ++i) {
+		const int d = wave + kCaWaves * i;
+		if (DT % kCaWaves && d >= DT) break;
+		v4i y = lds.join[0][d][lane];
+#pragma unroll
+		for (int k = 1; k < kCaWaves; ++k) y += lds.join[k][d][lane];
+		if (ri < j.heads) *(v4i*)(w.part + (((size_t)j.plane * a.tokens + j.t) * a.NH + j.h0 + ri) * D + 16 * d + 4 * g) = y;
 	}
 }
 
@@ -1090,14 +1144,6 @@ __device__ __forceinline__ bool cc_steps(const CacheAttnArgs& a, const CcJob& j,
 
 // how many of a step's positions, counted from the lane's first (4 g), lie before `end`
 __device__ __forceinline__ int ca_left(int64_t p, int64_t end) { return (int)i64min(end - p, 64) - ((threadIdx.x & 63) >> 4) * 4; }
-
-// Which bits some live lane of the block has set: what its waves branch on alike.
-__device__ __forceinline__ int block_vote(int bits, int* s) {
-	const int all = (__any(bits & 1) ? 1 : 0) | (__any(bits & 2) ? 2 : 0);
-	if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = all;
-	__syncthreads();
-	return __builtin_amdgcn_readfirstlane(s[0] | s[1] | s[2] | s[3]);
-}
 
 // a (token, head)'s maximum or sum over its planes; the lanes ri, ri + 16, ri + 32, ri + 48 share the work
 __device__ __forceinline__ int32_t cc_top(const CacheAttnArgs& a, const CaPlan& pl, const CaWork& w, const CcLane& l, bool live) {
@@ -1437,7 +1483,6 @@ void cache_store(const CacheStoreArgs& a, hipStream_t s) {
 	}
 }
 
-constexpr int kCaTargetWaves = 4096;  // single tokens; chunks aim at as many as kCaTargetBlocks blocks of four
 constexpr int kCaTargetBlocks = 1024;
 
 // Planes: as many as fill the chip, at most some 4 sqrt(steps) of them, as their maxima and contexts are joined by
@@ -1448,15 +1493,14 @@ static CaPlan ca_plan(int rows, int tokens, int max_new, int NH, int NKV, int64_
 	p.ht = (G + 15) / 16;
 	p.groups = (int)((int64_t)tokens * G / 64 + rows);
 	const int64_t units = max_new == 1 ? (int64_t)rows * NKV * p.ht : (int64_t)p.groups * NKV;
-	const int64_t target = max_new == 1 ? kCaTargetWaves : kCaTargetBlocks;
-	const int64_t steps = (max_width + 127) / 128;
-	int64_t planes = std::min(steps, std::max<int64_t>(1, target / units));
+	const int64_t steps = (max_width + kCdStep - 1) / kCdStep;
+	int64_t planes = std::min(steps, std::max<int64_t>(1, kCaTargetBlocks / units));
 	planes = std::min(planes, std::max<int64_t>(1, (int64_t)std::sqrt(16.0 * (double)steps)));
-	p.sp = (int)((steps + planes - 1) / planes * 128);
+	p.sp = (int)((steps + planes - 1) / planes * kCdStep);
 	p.planes = (int)((max_width + p.sp - 1) / p.sp);
-	p.ps = 8192;
+	p.ps = kCdSum;
 	p.parts = max_new == 1 ? (int)((max_width + p.ps - 1) / p.ps) : p.planes;
-	p.wpad = steps * 128;
+	p.wpad = steps * kCdStep;
 	return p;
 }
 
@@ -1481,7 +1525,7 @@ static size_t ca_work(const CaPlan& p, int tokens, int max_new, int NH, int NKV,
 size_t cache_attn_workspace(int rows, int tokens, int max_new, int NH, int NKV, int D, int64_t max_width) {
 	const CaPlan p = ca_plan(rows, tokens, max_new, NH, NKV, max_width);
 	// a launch's blocks
-	if ((int64_t)rows * NKV * p.ht * p.planes / kCaWaves >= 1ll << 30 || ((int64_t)p.planes * NKV + 8) * p.groups >= 1ll << 30) return 0;
+	if ((int64_t)rows * NKV * p.ht * p.planes >= 1ll << 30 || ((int64_t)p.planes * NKV + 8) * p.groups >= 1ll << 30) return 0;
 	CaWork w;
 	return ca_work(p, tokens, max_new, NH, NKV, D, nullptr, &w);
 }
@@ -1494,11 +1538,13 @@ static void attn_launch(const CacheAttnArgs& a, hipStream_t s) {
 	ca_work(p, a.tokens, a.max_new, a.NH, NKV, D, (char*)a.ws, &w);
 	const dim3 bs(64 * kCaWaves);
 	if (a.max_new == 1) {
-		const dim3 grid((unsigned)(((int64_t)a.rows * NKV * p.ht * p.planes + kCaWaves - 1) / kCaWaves));
+		const dim3 grid((unsigned)(a.rows * NKV * p.ht * p.planes));
 		hipLaunchKernelGGL(k_cd_scores<D>, grid, bs, 0, s, a, p, w);
 		hipLaunchKernelGGL(k_cd_sum, dim3(p.parts, a.NH, a.rows), dim3(256), 0, s, a, p, w);
-		if (a.NH / NKV <= 8) hipLaunchKernelGGL((k_cd_pv<D, 2>), grid, bs, 0, s, a, p, w);
-		else hipLaunchKernelGGL((k_cd_pv<D, 1>), grid, bs, 0, s, a, p, w);
+		const int G = a.NH / NKV;
+		if (G <= 4) hipLaunchKernelGGL((k_cd_pv<D, 1>), grid, bs, 0, s, a, p, w);
+		else if (G <= 8) hipLaunchKernelGGL((k_cd_pv<D, 2>), grid, bs, 0, s, a, p, w);
+		else hipLaunchKernelGGL((k_cd_pv<D, 4>), grid, bs, 0, s, a, p, w);
 	} else {
 		const dim3 grid((unsigned)((p.planes * NKV + 7) / 8 * 8 * p.groups));
 		hipLaunchKernelGGL(k_cc_max<D>, grid, bs, 0, s, a, p, w);
