@@ -710,6 +710,32 @@ __device__ __forceinline__ int page_exp(const Pages& g, const LanePages& lp, int
 	return __builtin_amdgcn_readlane(e, (int)((i64min(p, last) >> g.lp) - lp.first));
 }
 
+// Whether a row's i-exp values are the doubles' (sa_exp): 0 <= q_b and q_ln2 <= 2 q_b + 1, then no value leaves [0, ceil],
+// ceil <= 2^47.  A unit of score is small here (a page's exponents are above it), so sums pass 2^53 often: a lane adds 16 values in
+// a double, below 2^51, and those to an integer.
+__device__ __forceinline__ bool ca_fast(const SaConst& c) { return c.q_b >= 0 && c.q_ln2 >= 1 && c.ceil >= 1 && c.q_ln2 <= 2 * c.q_b + 1; }
+
+// sa_prob for sums d of up to 2^62.  From 2^36 on: q, the estimate from below, is the quotient or one less; with
+// d = dh + dl, dh a multiple of 2^20, e - (q + 1) dh 2^-15 is an integer below 2^49 and (q + 1) dl 2^-15 has 36 bits, both exact.
+struct CaProb {
+	double c1, c2, dh, dl;
+};
+__device__ __forceinline__ CaProb ca_prob_of(int64_t d, bool small) {
+	const int64_t low = d & ((1 << 20) - 1);
+	CaProb p;
+	p.dh = (double)(d - low) * 0x1p-15;
+	p.dl = (double)low * 0x1p-15;
+	p.c1 = small ? 32768.0 / (double)d : (1.0 - 0x1p-50) * 32768.0 / (double)d;
+	p.c2 = 0.5 / (double)d;
+	return p;
+}
+template <bool SMALL>
+__device__ __forceinline__ int32_t ca_prob(const CaProb& p, double e) {
+	if constexpr (SMALL) return (int32_t)fma(e, p.c1, p.c2);
+	const double q = floor(e * p.c1), n = q + 1.0;
+	return (int32_t)q + (fma(-n, p.dh, e) >= n * p.dl ? 1 : 0);
+}
+
 // Which bits some live lane of the block has set: what its waves branch on alike.
 __device__ __forceinline__ int block_vote(int bits, int* s) {
 	const int all = (__any(bits & 1) ? 1 : 0) | (__any(bits & 2) ? 2 : 0);
@@ -832,9 +858,9 @@ __global__ __launch_bounds__(256) void k_cd_sum(CacheAttnArgs a, CaPlan pl, CaWo
 	top = max(max(s_m[0], s_m[1]), max(s_m[2], s_m[3]));
 	int64_t sum = 0;
 	int bad = 0;
-	if (sa_fast(c, width)) {
+	if (ca_fast(c)) {
 		const SaExp e = sa_exp_of(c, top);
-		double acc = 0.0;
+		double acc = 0.0;  // 16 values
 #pragma unroll
 		for (int i = 0; i < kCdSumLoads; ++i) {
 			const int64_t p = p0 + 1024 * i + 4 * tid;
@@ -915,7 +941,7 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cd_pv(Cache
 		if (c.st == kOk && j.plane == 0 && lane == 0 && wave + 4 * i < j.heads) w.hst[th] = bad ? kSoftmaxKernelRefusedAfterGateAccepted : kOk;
 	}
 	if (c.st != kOk) return;
-	form = block_vote(form | !sa_fast(c, j.width), s_vote);
+	form = block_vote(form | !ca_fast(c), s_vote);
 	v4i acc[DT][3];
 #pragma unroll
 	for (int d = 0; d < DT; ++d) acc[d][0] = acc[d][1] = acc[d][2] = v4i{0, 0, 0, 0};
@@ -969,15 +995,15 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cd_pv(Cache
 	if (!(form & 1)) {
 		SaExp e = sa_exp_of(c, 0);
 		const int32_t add = e.add;
-		SaProb pb[R];
+		CaProb pb[R];
 #pragma unroll
-		for (int i = 0; i < R; ++i) pb[i] = sa_prob_of((double)den[i], form == 0);
+		for (int i = 0; i < R; ++i) pb[i] = ca_prob_of(den[i], form == 0);
 		auto exp = [&](int i, int32_t x) {
 			e.add = add - top[i];
 			return sa_exp(e, x);
 		};
-		if (form == 0) run([&](int i, int32_t x, bool) { return sa_prob<true>(pb[i], exp(i, x)); });
-		else run([&](int i, int32_t x, bool) { return sa_prob<false>(pb[i], exp(i, x)); });
+		if (form == 0) run([&](int i, int32_t x, bool) { return ca_prob<true>(pb[i], exp(i, x)); });
+		else run([&](int i, int32_t x, bool) { return ca_prob<false>(pb[i], exp(i, x)); });
 	} else {
 		const double inv = 1.0 / (double)c.q_ln2;
 		run([&](int i, int32_t x, bool in) {
@@ -1218,11 +1244,11 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 4 : 2) void k_cc_sum(Cach
 	const int64_t end = live ? i64min(j.p1, l.width) : 0;
 	int64_t sum = 0;
 	int bad = 0;
-	if (!block_vote(live && !sa_fast(c, l.width), s_vote)) {
+	if (!block_vote(live && !ca_fast(c), s_vote)) {
 		const SaExp e = sa_exp_of(live ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
-		double acc = 0.0;
 		cc_steps<D, false>(a, j, lds, q, [&](int64_t p, int64_t, v4i (&s)[4], const LanePages&, auto&&) {
 			const int left = ca_left(p, end);
+			double acc = 0.0;
 #pragma unroll
 			for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -1230,8 +1256,8 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 4 : 2) void k_cc_sum(Cach
 					const double x = sa_exp(e, s[t][v]);
 					acc += t * 16 + v < left ? x : 0.0;
 				}
+			sum += (int64_t)acc;
 		});
-		sum = (int64_t)acc;
 	} else {
 		const double inv = 1.0 / (double)c.q_ln2;
 		cc_steps<D, false>(a, j, lds, q, [&](int64_t p, int64_t, v4i (&s)[4], const LanePages&, auto&&) {
@@ -1273,7 +1299,7 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cc_pv(Cache
 	const int64_t end = live ? i64min(j.p1, l.width) : 0;
 #pragma unroll
 	for (int d = 0; d < DT; ++d) acc[d][0] = acc[d][1] = acc[d][2] = v4i{0, 0, 0, 0};
-	const int form = block_vote((live && !sa_fast(c, l.width) ? 1 : 0) | (den >= ((int64_t)1 << 36) ? 2 : 0), s_vote);
+	const int form = block_vote((live && !ca_fast(c) ? 1 : 0) | (den >= ((int64_t)1 << 36) ? 2 : 0), s_vote);
 	auto run = [&](auto&& value) {
 		cc_steps<D, true>(a, j, lds, q, [&](int64_t p, int64_t last, v4i (&s)[4], const LanePages& lp, auto&& multiply) {
 			const int left = ca_left(p, end);
@@ -1293,9 +1319,9 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cc_pv(Cache
 		});
 	};
 	const SaExp e = sa_exp_of(live && !(form & 1) ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
-	const SaProb pb = sa_prob_of((double)den, !(form & 2));
-	if (form == 0) run([&](int32_t x, bool) { return sa_prob<true>(pb, sa_exp(e, x)); });
-	else if (form == 2) run([&](int32_t x, bool) { return sa_prob<false>(pb, sa_exp(e, x)); });
+	const CaProb pb = ca_prob_of(den, !(form & 2));
+	if (form == 0) run([&](int32_t x, bool) { return ca_prob<true>(pb, sa_exp(e, x)); });
+	else if (form == 2) run([&](int32_t x, bool) { return ca_prob<false>(pb, sa_exp(e, x)); });
 	else {
 		const double inv = 1.0 / (double)c.q_ln2, dinv = 1.0 / (double)den;
 		run([&](int32_t x, bool in) {
@@ -1483,24 +1509,30 @@ void cache_store(const CacheStoreArgs& a, hipStream_t s) {
 	}
 }
 
-constexpr int kCaTargetBlocks = 1024;
+#ifndef T_CD
+#define T_CD 4096
+#endif
+#ifndef T_CC
+#define T_CC 768
+#endif
+constexpr int kCdTargetBlocks = T_CD, kCcTargetBlocks = T_CC;
 
 // Planes: as many as fill the chip, at most some 4 sqrt(steps) of them, as their maxima and contexts are joined by
 // each (token, head) and token.
 static CaPlan ca_plan(int rows, int tokens, int max_new, int NH, int NKV, int64_t max_width) {
 	CaPlan p{};
-	const int G = NH / NKV;
+	const int G = NH / NKV, step = max_new == 1 ? kCdStep : 64;
 	p.ht = (G + 15) / 16;
 	p.groups = (int)((int64_t)tokens * G / 64 + rows);
 	const int64_t units = max_new == 1 ? (int64_t)rows * NKV * p.ht : (int64_t)p.groups * NKV;
-	const int64_t steps = (max_width + kCdStep - 1) / kCdStep;
-	int64_t planes = std::min(steps, std::max<int64_t>(1, kCaTargetBlocks / units));
+	const int64_t steps = (max_width + step - 1) / step;
+	int64_t planes = std::min(steps, std::max<int64_t>(1, (max_new == 1 ? kCdTargetBlocks : kCcTargetBlocks) / units));
 	planes = std::min(planes, std::max<int64_t>(1, (int64_t)std::sqrt(16.0 * (double)steps)));
-	p.sp = (int)((steps + planes - 1) / planes * kCdStep);
+	p.sp = (int)((steps + planes - 1) / planes * step);
 	p.planes = (int)((max_width + p.sp - 1) / p.sp);
 	p.ps = kCdSum;
 	p.parts = max_new == 1 ? (int)((max_width + p.ps - 1) / p.ps) : p.planes;
-	p.wpad = steps * kCdStep;
+	p.wpad = (max_width + kCdStep - 1) / kCdStep * kCdStep;
 	return p;
 }
 
