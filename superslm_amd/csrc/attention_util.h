@@ -22,6 +22,7 @@ struct __attribute__((packed)) unaligned4 {
 };
 
 __device__ __forceinline__ int64_t i64min(int64_t a, int64_t b) { return a < b ? a : b; }
+__device__ __forceinline__ int64_t i64max(int64_t a, int64_t b) { return a < b ? b : a; }
 
 struct RowConst {
 	int64_t q_ln2, q_b, q_c, ceil;
@@ -108,11 +109,11 @@ struct SaRows {
 			r[u] = global16(row(i64min(p + i / PER, last)) + i % PER * 16);
 		}
 	}
-	// at(u): where this lane's chunk u lies, byte 16 (i % PER) of row i / PER, i = lane + 64 u
+	// at(u): this lane's chunk u, byte 16 (i % PER) of row i / PER, i = lane + 64 u
 	template <typename F>
 	__device__ __forceinline__ void load_at(F&& at) {
 #pragma unroll
-		for (int u = 0; u < PER; ++u) r[u] = global16(at(u));
+		for (int u = 0; u < PER; ++u) r[u] = at(u);
 	}
 	// rows 32 h .. 32 h + 31 into LDS
 	__device__ __forceinline__ void stage(int8_t* lds, int h) const {

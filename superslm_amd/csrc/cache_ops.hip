@@ -657,15 +657,13 @@ __device__ __forceinline__ CacheRow attn_row(const CacheAttnArgs& a, int r) {
 }
 
 // A wave's next 64 pages of a row, one to a lane, from position p0's on (lanes past position `last`'s page repeat it), with the
-// KV head's exponents; false for the whole wave when one is not a page.
+// KV head's exponents; false for the whole wave when one is not a page.  Positions are below 2^24 from here on.
 struct LanePages {
-	int32_t page, ke, ve;
-	int64_t first;
+	int32_t page, ke, ve, first;
 };
-__device__ __forceinline__ bool lane_pages(const Pages& g, int r, int kvh, int64_t p0, int64_t last, LanePages* o) {
+__device__ __forceinline__ bool lane_pages(const Pages& g, int r, int kvh, int p0, int last, LanePages* o) {
 	o->first = p0 >> g.lp;
-	const int64_t n = (last >> g.lp) - o->first;
-	o->page = g.tables[(int64_t)r * g.table_ld + o->first + i64min(threadIdx.x & 63, n)];
+	o->page = g.tables[(int64_t)r * g.table_ld + o->first + min((int)threadIdx.x & 63, (last >> g.lp) - o->first)];
 	if (__any(o->page < 0 || o->page >= g.pages)) return false;
 	const uint8_t* e = (const uint8_t*)g.pool + o->page * g.page_bytes + g.e_off;
 	o->ke = min((int)e[kvh], kMaxShift);
@@ -673,7 +671,7 @@ __device__ __forceinline__ bool lane_pages(const Pages& g, int r, int kvh, int64
 	return true;
 }
 // where the 64 pages from position p's on end
-__device__ __forceinline__ int64_t pages_end(const Pages& g, int64_t p) { return ((p >> g.lp) + 64) << g.lp; }
+__device__ __forceinline__ int pages_end(const Pages& g, int p) { return ((p >> g.lp) + 64) << g.lp; }
 // whether every page of the row's first `width` positions is one (by all lanes of a wave)
 __device__ __forceinline__ bool row_pages_ok(const Pages& g, int r, int64_t width) {
 	bool bad = false;
@@ -684,30 +682,36 @@ __device__ __forceinline__ bool row_pages_ok(const Pages& g, int r, int64_t widt
 	return !__any(bad);
 }
 
-// Rows of 64 positions from p (a multiple of 64) as a wave loads them: the page of each 16 of them is the same for the
-// wave, slots past the row's end are still the page's own.  Not `real`: 16 bytes of a page once, whatever they are, so that the loads in
-// flight are the same number on every path.
+// K or V of the page under 16 positions from p on, as a buffer: a load is then this in scalars and 32 bits of a lane's own.  Past
+// `last` the buffer is empty: its loads give zeros and move nothing, and the loads in flight are the same number on every path.
+// `off`: the head's K or V in its page.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rows(const Pages& g, const LanePages& lp, int p, int last, int64_t off) {
+	const int page = __builtin_amdgcn_readlane(lp.page, (min(p, last) >> g.lp) - lp.first);
+	return __builtin_amdgcn_make_buffer_rsrc(g.pool + (page * g.page_bytes + off), 0, p <= last ? g.D << g.lp : 0, 0x00020000);
+}
+__device__ __forceinline__ v4i buffer16(__amdgpu_buffer_rsrc_t b, uint32_t at) {
+	return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0));
+}
+// Rows of 64 positions from p on (a multiple of 64) as a wave loads them: 16 positions never leave a page.
 template <int D>
-__device__ __forceinline__ void load_rows(SaRows<D>& x, const Pages& g, const LanePages& lp, int64_t p, int64_t last, int64_t off, bool real) {
+__device__ __forceinline__ void load_rows(SaRows<D>& x, const Pages& g, const LanePages& lp, int p, int last, int64_t off) {
 	constexpr int PER = D / 16, R = 64 / PER;  // rows of one load
-	const int lane = threadIdx.x & 63, mask = min(1 << g.lp, 64) - 1, high = (int)(p & ((1 << g.lp) - 1));
-	auto page = [&](int row) {
-		const int i = (int)((i64min(p + row, last) >> g.lp) - lp.first);
-		return g.pool + __builtin_amdgcn_readlane(lp.page, i) * g.page_bytes + off;
-	};
+	const int lane = threadIdx.x & 63, mask = (1 << g.lp) - 1;
+	__amdgpu_buffer_rsrc_t b[4];
+	b[0] = page_rows(g, lp, p, last, off);
+#pragma unroll
+	for (int t = 1; t < 4; ++t) b[t] = page_rows(g, lp, p + 16 * t, last, off);
 	x.load_at([&](int u) {
 		const int row = u * R + lane / PER;
-		const int8_t* at = page(u * R);
-		if (R > 16) {
-			const int8_t* next = page(u * R + 16);
-			at = lane / PER >= 16 ? next : at;
-		}
-		return at + (real ? ((high & ~63) + (row & mask)) * D + lane % PER * 16 : 0);
+		const uint32_t at = (uint32_t)(((p + row) & mask) * D + lane % PER * 16);
+		if constexpr (R > 16) return buffer16(b[2 * u], lane / PER < 16 ? at : ~0u) | buffer16(b[2 * u + 1], lane / PER < 16 ? ~0u : at);
+		else return buffer16(b[u * R / 16], at);
 	});
+	__builtin_amdgcn_sched_barrier(0);  // loads stay in this order: a wait for the older rows then leaves the newer in flight
 }
 // the exponents of 16 positions from p
-__device__ __forceinline__ int page_exp(const Pages& g, const LanePages& lp, int32_t e, int64_t p, int64_t last) {
-	return __builtin_amdgcn_readlane(e, (int)((i64min(p, last) >> g.lp) - lp.first));
+__device__ __forceinline__ int page_exp(const Pages& g, const LanePages& lp, int32_t e, int p, int last) {
+	return __builtin_amdgcn_readlane(e, (min(p, last) >> g.lp) - lp.first);
 }
 
 // Whether a row's i-exp values are the doubles' (sa_exp): 0 <= q_b and q_ln2 <= 2 q_b + 1, then no value leaves [0, ceil],
@@ -748,7 +752,7 @@ __device__ __forceinline__ int block_vote(int bits, int* s) {
 constexpr int kCdStep = 64 * kCaWaves;
 struct CdJob {
 	int r, t, kvh, tile, plane, h0, heads;  // h0: the tile's first head
-	int64_t width, p0, p1;
+	int width, p0, p1;
 	CacheRow row;
 };
 __device__ __forceinline__ bool cd_job(const CacheAttnArgs& a, const CaPlan& pl, CdJob* j) {
@@ -762,9 +766,9 @@ __device__ __forceinline__ bool cd_job(const CacheAttnArgs& a, const CaPlan& pl,
 	j->t = j->row.t0;
 	j->h0 = j->kvh * G + j->tile * 16;
 	j->heads = min(16, G - j->tile * 16);
-	j->width = j->row.start + 1;
-	j->p0 = (int64_t)j->plane * pl.sp;
-	j->p1 = i64min(j->width, j->p0 + pl.sp);
+	j->width = (int)j->row.start + 1;
+	j->p0 = j->plane * pl.sp;
+	j->p1 = min(j->width, j->p0 + pl.sp);
 	return j->p0 < j->p1;
 }
 
@@ -783,25 +787,27 @@ __global__ __launch_bounds__(64 * kCaWaves) void k_cd_scores(CacheAttnArgs a, Ca
 	v4i q[NC];
 #pragma unroll
 	for (int c = 0; c < NC; ++c) q[c] = mine && c * 64 + g * 16 < D ? load16(a.q + ((size_t)j.t * a.NH + h) * D + c * 64 + g * 16) : v4i{0, 0, 0, 0};
-	int32_t* out = w.scores + ((size_t)j.t * a.NH + h) * pl.wpad + 4 * g;
+	// dead lanes and positions past the plane store outside the descriptor, which drops them: no branch between the loads
+	const auto out = __builtin_amdgcn_make_buffer_rsrc(w.scores + ((size_t)j.t * a.NH + j.h0) * pl.wpad, 0, (int)(j.heads * pl.wpad * 4), 0x00020000);
+	const uint32_t mine_at = mine ? (uint32_t)((ri * pl.wpad + 4 * g) * 4) : ~0u;
 	const int64_t off = a.pg.k_off + ((int64_t)j.kvh << a.pg.lp) * D;
 	int32_t m = INT32_MIN;
-	for (int64_t s0 = j.p0; s0 < j.p1; s0 = pages_end(a.pg, s0)) {
-		const int64_t s1 = i64min(j.p1, pages_end(a.pg, s0)), last = s1 - 1;
+	for (int s0 = j.p0; s0 < j.p1; s0 = pages_end(a.pg, s0)) {
+		const int s1 = min(j.p1, pages_end(a.pg, s0)), last = s1 - 1;
 		LanePages lp;
 		if (!lane_pages(a.pg, j.r, j.kvh, s0, last, &lp)) break;
 		SaRows<D> k[2];
 #pragma unroll
-		for (int b = 0; b < 2; ++b) load_rows(k[b], a.pg, lp, s0 + 64 * wave + b * kCdStep, last, off, s0 + 64 * wave + b * kCdStep < s1);
-		for (int64_t p0 = s0 + 64 * wave; p0 < s1; p0 += 2 * kCdStep) {
+		for (int b = 0; b < 2; ++b) load_rows(k[b], a.pg, lp, s0 + 64 * wave + b * kCdStep, last, off);
+		for (int p0 = s0 + 64 * wave; p0 < s1; p0 += 2 * kCdStep) {
 #pragma unroll
 			for (int b = 0; b < 2; ++b) {
-				const int64_t p = p0 + b * kCdStep;
-				if (p >= s1) break;
+				const int p = p0 + b * kCdStep;
 				v4i s[4] = {};
 				k[b].scores(lds, q, s);
-				load_rows(k[b], a.pg, lp, p + 2 * kCdStep, last, off, p + 2 * kCdStep < s1);
-				const int left = (int)i64min(s1 - p, 64) - 4 * g;
+				load_rows(k[b], a.pg, lp, p + 2 * kCdStep, last, off);
+				const int left = s1 - p - 4 * g;
+				const uint32_t at = p < s1 ? mine_at : ~0u;
 #pragma unroll
 				for (int t = 0; t < 4; ++t) {
 					const int e = page_exp(a.pg, lp, lp.ke, p + 16 * t, last);
@@ -810,7 +816,7 @@ __global__ __launch_bounds__(64 * kCaWaves) void k_cd_scores(CacheAttnArgs a, Ca
 						s[t][v] <<= e;
 						m = max(m, t * 16 + v < left ? s[t][v] : INT32_MIN);
 					}
-					if (mine) *(v4i*)(out + p + 16 * t) = s[t];
+					__builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, s[t]), out, at, (p + 16 * t) * 4, 0);
 				}
 			}
 		}
@@ -841,15 +847,15 @@ __global__ __launch_bounds__(256) void k_cd_sum(CacheAttnArgs a, CaPlan pl, CaWo
 	const CacheRow row = attn_row(a, r);
 	if (!row.ok || row.n < 1) return;
 	const int t = row.t0;
-	const int64_t width = row.start + 1, p0 = (int64_t)part * pl.ps, p1 = i64min(width, p0 + pl.ps);
+	const int width = (int)row.start + 1, p0 = part * pl.ps, p1 = min(width, p0 + pl.ps);
 	if (p0 >= p1) return;
 	const int32_t* sc = w.scores + ((size_t)t * a.NH + h) * pl.wpad;
 	v4i x[kCdSumLoads];
 #pragma unroll
-	for (int i = 0; i < kCdSumLoads; ++i) x[i] = *(const v4i*)(sc + i64min(p0 + 1024 * i + 4 * tid, (p1 - 1) & ~3ll));
+	for (int i = 0; i < kCdSumLoads; ++i) x[i] = *(const v4i*)(sc + min(p0 + 1024 * i + 4 * tid, (p1 - 1) & ~3));
 	const SaConst c = w.cst[(size_t)t * a.pg.NKV + kvh];
 	int32_t top = INT32_MIN;
-	const int n = (int)((width + pl.sp - 1) / pl.sp);
+	const int n = (width + pl.sp - 1) / pl.sp;
 	for (int i = tid; i < n; i += 256) top = max(top, w.pmax[((size_t)i * a.tokens + t) * a.NH + h]);
 	for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
 	if ((tid & 63) == 0) s_m[tid >> 6] = top;
@@ -863,7 +869,7 @@ __global__ __launch_bounds__(256) void k_cd_sum(CacheAttnArgs a, CaPlan pl, CaWo
 		double acc = 0.0;  // 16 values
 #pragma unroll
 		for (int i = 0; i < kCdSumLoads; ++i) {
-			const int64_t p = p0 + 1024 * i + 4 * tid;
+			const int p = p0 + 1024 * i + 4 * tid;
 			if (p0 + 1024 * i >= p1) break;
 #pragma unroll
 			for (int k = 0; k < 4; ++k) {
@@ -919,7 +925,7 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cd_pv(Cache
 	if (!cd_job(a, pl, &j)) return;
 	const int64_t off = a.pg.v_off + ((int64_t)j.kvh << a.pg.lp) * D;
 	const SaConst c = w.cst[(size_t)j.t * a.pg.NKV + j.kvh];
-	const int parts = (int)((j.width + pl.ps - 1) / pl.ps);
+	const int parts = (j.width + pl.ps - 1) / pl.ps;
 	// this wave's heads wave, wave + 4, ..: the maximum and the sum
 	int32_t top[R];
 	int64_t den[R];
@@ -948,23 +954,23 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cd_pv(Cache
 	// value(i, score, in): the probability of a score of head wave + 4 i
 	auto run = [&](auto&& value) {
 		int b = 0;
-		for (int64_t s0 = j.p0; s0 < j.p1; s0 = pages_end(a.pg, s0)) {
-			const int64_t s1 = i64min(j.p1, pages_end(a.pg, s0)), last = s1 - 1;
+		for (int s0 = j.p0; s0 < j.p1; s0 = pages_end(a.pg, s0)) {
+			const int s1 = min(j.p1, pages_end(a.pg, s0)), last = s1 - 1;
 			LanePages lp;
 			if (!lane_pages(a.pg, j.r, j.kvh, s0, last, &lp)) return;  // alike for the block's waves
 			SaRows<D> v;
 			v4i s[R];
-			auto scores = [&](int64_t p) {
+			auto scores = [&](int p) {
 #pragma unroll
 				for (int i = 0; i < R; ++i)
 					s[i] = *(const v4i*)(w.scores + ((size_t)j.t * a.NH + j.h0 + min(wave + 4 * i, j.heads - 1)) * pl.wpad + p + 4 * lane);
 			};
 			scores(s0);
-			load_rows(v, a.pg, lp, s0 + 64 * wave, last, off, s0 + 64 * wave < s1);
-			for (int64_t p = s0; p < s1; p += kCdStep) {
-				const int left = (int)i64min(s1 - p - 4 * lane, 4);
+			load_rows(v, a.pg, lp, s0 + 64 * wave, last, off);
+			for (int p = s0; p < s1; p += kCdStep) {
+				const int left = s1 - p - 4 * lane;
 				// lane 4 i + k of a head has positions 16 i + 4 k .. + 3: word i of the operand's lane (head, k)
-				const int sh = __shfl(lp.ve, (int)((i64min(p + 4 * lane, last) >> a.pg.lp) - lp.first), 64);
+				const int sh = __shfl(lp.ve, (min(p + 4 * lane, last) >> a.pg.lp) - lp.first, 64);
 #pragma unroll
 				for (int i = 0; i < R; ++i) {
 					const int head = wave + 4 * i;
@@ -987,7 +993,7 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cd_pv(Cache
 #pragma unroll
 				for (int n = 0; n < 3; ++n) x[n] = *(const v4i*)&lds.s.p[b][n][wave][ri * 16 + g * 4];
 				v.multiply(lds.s.v[wave], x, acc);
-				load_rows(v, a.pg, lp, p + kCdStep + 64 * wave, last, off, p + kCdStep + 64 * wave < s1);
+				load_rows(v, a.pg, lp, p + kCdStep + 64 * wave, last, off);
 				b ^= 1;
 			}
 		}
@@ -1028,7 +1034,7 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cd_pv(Cache
 // A chunk's block: number `b` of the row groups, 64 query rows from the group's, and a plane.
 struct CcJob {
 	int r, kvh, plane, i0, count;  // i0: the block's first query row of `count` in the row
-	int64_t width, p0, p1;         // width: of the block's last token
+	int width, p0, p1;             // width: of the block's last token
 	CacheRow row;
 };
 // The rows' groups are counted 64 rows at a time, a row to a lane.
@@ -1064,15 +1070,14 @@ __device__ __forceinline__ bool cc_job(const CacheAttnArgs& a, const CaPlan& pl,
 	j->row = attn_row(a, j->r);
 	j->i0 = b * 64;
 	j->count = j->row.n * G;
-	j->width = j->row.start + (min(j->i0 + 64, j->count) - 1) / G + 1;
-	j->p0 = (int64_t)j->plane * pl.sp;
-	j->p1 = i64min(j->width, j->p0 + pl.sp);
+	j->width = (int)j->row.start + (min(j->i0 + 64, j->count) - 1) / G + 1;
+	j->p0 = j->plane * pl.sp;
+	j->p1 = min(j->width, j->p0 + pl.sp);
 	return j->p0 < j->p1;
 }
 // what a lane of the block has: its token, head and width (t < 0: none)
 struct CcLane {
-	int t, h;
-	int64_t width;
+	int t, h, width;
 };
 __device__ __forceinline__ CcLane cc_lane(const CacheAttnArgs& a, const CcJob& j) {
 	const int G = a.NH / a.pg.NKV, i = j.i0 + (int)(threadIdx.x >> 6) * 16 + (int)(threadIdx.x & 15);
@@ -1080,7 +1085,7 @@ __device__ __forceinline__ CcLane cc_lane(const CacheAttnArgs& a, const CcJob& j
 	if (i < j.count) {
 		l.t = j.row.t0 + i / G;
 		l.h += i % G;
-		l.width = j.row.start + i / G + 1;
+		l.width = (int)j.row.start + i / G + 1;
 	}
 	return l;
 }
@@ -1100,29 +1105,37 @@ __device__ __forceinline__ bool cc_steps(const CacheAttnArgs& a, const CcJob& j,
 	constexpr int BS = 64 * kCaWaves, CH = 4 * D, PT = (CH + BS - 1) / BS, PER = D / 16, AHEAD = D <= 128 ? 2 : 1;
 	const Pages& g = a.pg;
 	const int64_t head = ((int64_t)j.kvh << g.lp) * D;
-	const int mask = min(1 << g.lp, 64) - 1;
+	const int mask = (1 << g.lp) - 1;
 	int b = 0;
-	for (int64_t s0 = j.p0; s0 < j.p1; s0 = pages_end(g, s0)) {
-		const int64_t s1 = i64min(j.p1, pages_end(g, s0)), last = s1 - 1;
+	for (int s0 = j.p0; s0 < j.p1; s0 = pages_end(g, s0)) {
+		const int s1 = min(j.p1, pages_end(g, s0)), last = s1 - 1;
 		LanePages lp;
 		if (!lane_pages(g, j.r, j.kvh, s0, last, &lp)) return false;
 		v4i kr[AHEAD][PT], vr[AHEAD][PT], s[4];
-		auto load = [&](int64_t p, v4i (&k)[PT], v4i (&v)[PT]) {
+		auto load = [&](int p, v4i (&k)[PT], v4i (&v)[PT]) {
 #pragma unroll
 			for (int u = 0; u < PT; ++u) {
 				const int c = min((int)threadIdx.x + u * BS, CH - 1), row = c / PER;
-				const int page = __shfl(lp.page, (int)((i64min(p + row, last) >> g.lp) - lp.first), 64);
-				const int8_t* at = g.pool + page * g.page_bytes + head + (((int)(p & ((1 << g.lp) - 1)) & ~63) + (row & mask)) * D + c % PER * 16;
-				k[u] = global16(at + g.k_off);
-				if (WITH_V) v[u] = global16(at + g.v_off);
+				// a wave's rows of one load: within 16 (32 at D = 32)
+				const int r0 = p + (__builtin_amdgcn_readfirstlane(row) & ~15);
+				const uint32_t at = (uint32_t)(((p + row) & mask) * D + c % PER * 16);
+				auto get = [&](int64_t off) {
+					const auto b = page_rows(g, lp, r0, last, off);
+					if constexpr (D == 32) {
+						const bool second = (row & 16) != (__builtin_amdgcn_readfirstlane(row) & 16);
+						return buffer16(b, second ? ~0u : at) | buffer16(page_rows(g, lp, r0 + 16, last, off), second ? at : ~0u);
+					} else return buffer16(b, at);
+				};
+				k[u] = get(g.k_off + head);
+				if (WITH_V) v[u] = get(g.v_off + head);
 			}
 		};
 #pragma unroll
 		for (int i = 0; i < AHEAD; ++i) load(s0 + 64 * i, kr[i], vr[i]);
-		for (int64_t p0 = s0; p0 < s1; p0 += 64 * AHEAD) {
+		for (int p0 = s0; p0 < s1; p0 += 64 * AHEAD) {
 #pragma unroll
 			for (int i = 0; i < AHEAD; ++i) {
-				const int64_t p = p0 + 64 * i;
+				const int p = p0 + 64 * i;
 				if (i && p >= s1) break;
 				int8_t *kb = lds + b * 64 * D, *vb = lds + (2 + b) * 64 * D;
 #pragma unroll
@@ -1169,18 +1182,18 @@ __device__ __forceinline__ bool cc_steps(const CacheAttnArgs& a, const CcJob& j,
 }
 
 // how many of a step's positions, counted from the lane's first (4 g), lie before `end`
-__device__ __forceinline__ int ca_left(int64_t p, int64_t end) { return (int)i64min(end - p, 64) - ((threadIdx.x & 63) >> 4) * 4; }
+__device__ __forceinline__ int ca_left(int p, int end) { return end - p - ((threadIdx.x & 63) >> 4) * 4; }
 
 // a (token, head)'s maximum or sum over its planes; the lanes ri, ri + 16, ri + 32, ri + 48 share the work
 __device__ __forceinline__ int32_t cc_top(const CacheAttnArgs& a, const CaPlan& pl, const CaWork& w, const CcLane& l, bool live) {
-	const int n = live ? (int)((l.width + pl.sp - 1) / pl.sp) : 0;
+	const int n = live ? (l.width + pl.sp - 1) / pl.sp : 0;
 	int32_t m = INT32_MIN;
 	for (int i = (threadIdx.x & 63) >> 4; i < n; i += 4) m = max(m, w.pmax[((size_t)i * a.tokens + l.t) * a.NH + l.h]);
 	m = max(m, __shfl_xor(m, 16, 64));
 	return max(m, __shfl_xor(m, 32, 64));
 }
 __device__ __forceinline__ int64_t cc_sum(const CacheAttnArgs& a, const CaPlan& pl, const CaWork& w, const CcLane& l, bool live) {
-	const int n = live ? (int)((l.width + pl.sp - 1) / pl.sp) : 0;
+	const int n = live ? (l.width + pl.sp - 1) / pl.sp : 0;
 	int64_t sum = 0;
 	int bad = 0;
 	for (int i = (threadIdx.x & 63) >> 4; i < n; i += 4) {
@@ -1213,9 +1226,9 @@ __global__ __launch_bounds__(64 * kCaWaves) void k_cc_max(CacheAttnArgs a, CaPla
 		}
 		if (g == 0 && l.t >= 0) w.cst[(size_t)l.t * a.pg.NKV + j.kvh] = c;
 	}
-	const int64_t end = i64min(j.p1, l.width);
+	const int end = min(j.p1, l.width);
 	int32_t m = INT32_MIN;
-	cc_steps<D, false>(a, j, lds, q, [&](int64_t p, int64_t, v4i (&s)[4], const LanePages&, auto&&) {
+	cc_steps<D, false>(a, j, lds, q, [&](int p, int, v4i (&s)[4], const LanePages&, auto&&) {
 		const int left = ca_left(p, end);
 #pragma unroll
 		for (int t = 0; t < 4; ++t)
@@ -1241,12 +1254,12 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 4 : 2) void k_cc_sum(Cach
 	v4i q[NC];
 	cc_load_q<D>(a, l, q);
 	const int32_t top = cc_top(a, pl, w, l, live);
-	const int64_t end = live ? i64min(j.p1, l.width) : 0;
+	const int end = live ? min(j.p1, l.width) : 0;
 	int64_t sum = 0;
 	int bad = 0;
 	if (!block_vote(live && !ca_fast(c), s_vote)) {
 		const SaExp e = sa_exp_of(live ? c : SaConst{1, 1, 0, 1, 0, 0}, top);
-		cc_steps<D, false>(a, j, lds, q, [&](int64_t p, int64_t, v4i (&s)[4], const LanePages&, auto&&) {
+		cc_steps<D, false>(a, j, lds, q, [&](int p, int, v4i (&s)[4], const LanePages&, auto&&) {
 			const int left = ca_left(p, end);
 			double acc = 0.0;
 #pragma unroll
@@ -1260,7 +1273,7 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 4 : 2) void k_cc_sum(Cach
 		});
 	} else {
 		const double inv = 1.0 / (double)c.q_ln2;
-		cc_steps<D, false>(a, j, lds, q, [&](int64_t p, int64_t, v4i (&s)[4], const LanePages&, auto&&) {
+		cc_steps<D, false>(a, j, lds, q, [&](int p, int, v4i (&s)[4], const LanePages&, auto&&) {
 			const int left = ca_left(p, end);
 #pragma unroll
 			for (int i = 0; i < 16; ++i) {
@@ -1296,12 +1309,12 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cc_pv(Cache
 	if (j.plane == 0 && g == 0 && live) w.hst[(size_t)l.t * a.NH + l.h] = sum < 0 ? kSoftmaxKernelRefusedAfterGateAccepted : kOk;
 	live = live && sum >= 0;
 	const int64_t den = live && sum > 1 ? sum : 1;
-	const int64_t end = live ? i64min(j.p1, l.width) : 0;
+	const int end = live ? min(j.p1, l.width) : 0;
 #pragma unroll
 	for (int d = 0; d < DT; ++d) acc[d][0] = acc[d][1] = acc[d][2] = v4i{0, 0, 0, 0};
 	const int form = block_vote((live && !ca_fast(c) ? 1 : 0) | (den >= ((int64_t)1 << 36) ? 2 : 0), s_vote);
 	auto run = [&](auto&& value) {
-		cc_steps<D, true>(a, j, lds, q, [&](int64_t p, int64_t last, v4i (&s)[4], const LanePages& lp, auto&& multiply) {
+		cc_steps<D, true>(a, j, lds, q, [&](int p, int last, v4i (&s)[4], const LanePages& lp, auto&& multiply) {
 			const int left = ca_left(p, end);
 			int32_t pr[16];
 #pragma unroll
