@@ -633,6 +633,7 @@ __global__ __launch_bounds__(kStoreBlock) void k_store_span(CacheStoreArgs a, in
 // launches (4 G bytes a position beside the 2 D of its K and V).  Chunks: four neighbouring tiles of a row share each step of 64 positions that
 // their block stages, and the scores are computed again, 8 MFMAs a step at D = 128.
 struct CaPlan {
+	int whole;       // single tokens' rows in one launch and the join (k_cr_row): cr_form's answer
 	int ht;          // single tokens: tiles of a token's heads
 	int groups;      // chunks: blocks of 64 query rows, at least those of every row together
 	int sp, planes;  // positions of a plane (a multiple of 256), planes of the widest row
@@ -1028,6 +1029,257 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cd_pv(Cache
 #pragma unroll
 		for (int k = 1; k < kCaWaves; ++k) y += lds.join[k][d][lane];
 		if (ri < j.heads) *(v4i*)(w.part + (((size_t)j.plane * a.tokens + j.t) * a.NH + j.h0 + ri) * D + 16 * d + 4 * g) = y;
+	}
+}
+
+// The whole of a single token's row in one launch, a block per (row, KV head, tile of heads): its waves take 64 positions in
+// turn and keep their scores in LDS, or where these are too many (GS) in the workspace, from which i-exp and probabilities
+// run on full waves, four heads at a time; maxima, sums and contexts are joined in LDS.  k_ca_out finds one plane.
+template <int D>
+struct CrShape {
+	static constexpr int NW = D <= 128 ? 8 : 4, STEP = 64 * NW, LD = 68;  // LD: a head's 64 scores, moved apart by a few banks
+	static constexpr size_t kWave = 32 * D + 3 * 1024, kJoin = (size_t)NW * D * 64;
+	static size_t lds(int heads, int64_t width, bool gs) {
+		const size_t n = NW * kWave + (gs ? 0 : (size_t)((width + STEP - 1) / STEP) * NW * heads * LD * 4);
+		return n > kJoin ? n : kJoin;
+	}
+};
+constexpr int kCrSteps = 16;  // a lane holds the page of 16 positions of one of a wave's next 16 steps
+template <int D, int R, bool GS>
+__global__ __launch_bounds__(64 * CrShape<D>::NW, D <= 128 ? 2 : 1) void k_cr_row(CacheAttnArgs a, CaPlan pl, CaWork w) {
+	constexpr int NW = CrShape<D>::NW, STEP = CrShape<D>::STEP, LD = GS ? 64 : CrShape<D>::LD, DT = D / 16, NC = (D + 63) / 64, PER = D / 16, RL = 64 / PER;
+	extern __shared__ __attribute__((aligned(16))) int8_t row_lds[];
+	__shared__ int32_t s_max[NW][16], s_bad[NW];
+	__shared__ int64_t s_sum[NW][16];
+	const int lane = threadIdx.x & 63, ri = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int G = a.NH / a.pg.NKV, tile = blockIdx.x % pl.ht, kvh = blockIdx.x / pl.ht % a.pg.NKV, r = blockIdx.x / pl.ht / a.pg.NKV;
+	const int h0 = kvh * G + tile * 16, heads = min(16, G - tile * 16);
+	// lane 4 i + t of a segment of kCrSteps steps from n on: positions 64 (wave + NW (n + i)) + 16 t .. + 15
+	auto first_of = [&](int n) { return 64 * (wave + NW * (n + (lane >> 2))) + 16 * (lane & 3); };
+	auto entry_of = [&](int n) { return a.pg.tables[(int64_t)r * a.pg.table_ld + min(first_of(n) >> a.pg.lp, a.pg.table_ld - 1)]; };
+	const int32_t entry0 = entry_of(0);
+	const CacheRow row = attn_row(a, r);
+	if (!row.ok || row.n < 1) return;
+	const int t = row.t0, last = (int)row.start, width = last + 1, steps = (width - 64 * wave + STEP - 1) / STEP;  // the wave's
+	int32_t page = 0, ke = 0, ve = 0;
+	bool wrong = false;
+	auto enter = [&](int n) {
+		const int32_t entry = n ? entry_of(n) : entry0;
+		const bool out = entry < 0 || entry >= a.pg.pages;
+		wrong |= (bool)__any(out && first_of(n) <= last);
+		page = out ? 0 : entry;
+		const uint8_t* ex = (const uint8_t*)a.pg.pool + page * a.pg.page_bytes + a.pg.e_off;
+		ke = min((int)ex[kvh], kMaxShift);
+		ve = min((int)ex[a.pg.NKV + kvh], kMaxShift);
+	};
+	const int64_t head = ((int64_t)kvh << a.pg.lp) * D;
+	const int mask = (1 << a.pg.lp) - 1;
+	// step n's rows, n0 + kCrSteps the segment's end; none past that, the row's end or behind a page that is none
+	auto load = [&](SaRows<D>& x, int n, int n0, int64_t off) {
+		const int p = 64 * (wave + NW * n);
+		__amdgpu_buffer_rsrc_t b[4];
+#pragma unroll
+		for (int i = 0; i < 4; ++i) {
+			const int pg = __builtin_amdgcn_readlane(page, min(4 * (n - n0) + i, 63));
+			b[i] = __builtin_amdgcn_make_buffer_rsrc(a.pg.pool + (pg * a.pg.page_bytes + off + head), 0, p + 16 * i <= last && n - n0 < kCrSteps && !wrong ? D << a.pg.lp : 0, 0x00020000);
+		}
+		x.load_at([&](int u) {
+			const int rr = u * RL + lane / PER;
+			const uint32_t at = (uint32_t)(((p + rr) & mask) * D + lane % PER * 16);
+			if constexpr (RL > 16) return buffer16(b[2 * u], lane / PER < 16 ? at : ~0u) | buffer16(b[2 * u + 1], lane / PER < 16 ? ~0u : at);
+			else return buffer16(b[u * RL / 16], at);
+		});
+		__builtin_amdgcn_sched_barrier(0);
+	};
+	int8_t* stage = row_lds + wave * CrShape<D>::kWave;
+	uint32_t* ops = (uint32_t*)(stage + 32 * D);  // [operand][256]: 64 positions' bytes of 16 heads
+	int32_t* sc = (GS ? w.scores + ((size_t)t * a.NH + h0) * pl.wpad : (int32_t*)(row_lds + NW * CrShape<D>::kWave)) + wave * heads * LD;
+	const int sc_step = NW * heads * LD;
+	v4i q[NC];
+	const int hq = h0 + min(ri, heads - 1);
+#pragma unroll
+	for (int c = 0; c < NC; ++c) q[c] = c * 64 + g * 16 < D ? load16(a.q + ((size_t)t * a.NH + hq) * D + c * 64 + g * 16) : v4i{0, 0, 0, 0};
+	const RowScales rs{a.q_scale[t], a.khead_m[kvh], a.khead_e[kvh]};
+	const RowConst rc = row_const(rs, a.ln2_q, a.b_q, a.ca_q, width);
+	const SaConst c{rc.q_ln2, rc.q_b, rc.q_c, rc.ceil, rc.st, 0};
+	int32_t m = INT32_MIN;
+	int seg = 0;
+	for (;; seg += kCrSteps) {
+		enter(seg);
+		SaRows<D> k[2];
+		load(k[0], seg, seg, a.pg.k_off);
+		load(k[1], seg + 1, seg, a.pg.k_off);
+		for (int n0 = seg; n0 < min(steps, seg + kCrSteps); n0 += 2) {
+#pragma unroll
+			for (int b = 0; b < 2; ++b) {
+				const int n = n0 + b, left = width - 64 * (wave + NW * n) - 4 * g;
+				v4i s[4] = {};
+				k[b].scores(stage, q, s);
+				load(k[b], n + 2, seg, a.pg.k_off);
+#pragma unroll
+				for (int i = 0; i < 4; ++i) {
+					const int e = __builtin_amdgcn_readlane(ke, min(4 * (n - seg) + i, 63));
+#pragma unroll
+					for (int v = 0; v < 4; ++v) {
+						s[i][v] <<= e;
+						m = max(m, 16 * i + v < left ? s[i][v] : INT32_MIN);
+					}
+					if (ri < heads && n < steps) *(v4i*)(sc + n * sc_step + ri * LD + 16 * i + 4 * g) = s[i];
+				}
+			}
+		}
+		if (seg + kCrSteps >= steps) break;
+	}
+	SaRows<D> v;
+	if (seg) {
+		seg = 0;
+		enter(0);
+	}
+	load(v, 0, 0, a.pg.v_off);  // in flight through the softmax
+	m = max(m, __shfl_xor(m, 16, 64));
+	m = max(m, __shfl_xor(m, 32, 64));
+	if (g == 0) s_max[wave][ri] = m;
+	if (lane == 0) s_bad[wave] = wrong;
+	__syncthreads();
+	int st = c.st;
+#pragma unroll
+	for (int i = 0; i < NW; ++i) st = s_bad[i] ? (int)kPositionOverCap : st;
+	if (threadIdx.x == 0 && tile == 0) w.cst[(size_t)t * a.pg.NKV + kvh] = SaConst{0, 0, 0, 0, st, 0};
+	if (st != kOk) return;
+	// from here on a lane has four positions 4 ri .. + 3 of a step and the heads g, g + 4, ..
+	const bool fast = ca_fast(c);
+	const SaExp e0 = sa_exp_of(fast ? c : SaConst{1, 1, 0, 1, 0, 0}, 0);
+	const double inv = 1.0 / (double)c.q_ln2;
+	int32_t top[R];
+#pragma unroll
+	for (int i = 0; i < R; ++i) {
+		const int h = min(g + 4 * i, heads - 1);
+		top[i] = s_max[0][h];
+#pragma unroll
+		for (int x = 1; x < NW; ++x) top[i] = max(top[i], s_max[x][h]);
+	}
+	double acc1[R];
+	int64_t sum[R];
+	int bad = 0;
+#pragma unroll
+	for (int i = 0; i < R; ++i) {
+		acc1[i] = 0.0;
+		sum[i] = 0;
+	}
+	v4i x[R];
+	auto scores = [&](int n) {
+#pragma unroll
+		for (int i = 0; i < R; ++i) x[i] = *(const v4i*)(sc + min(n, steps - 1) * sc_step + min(g + 4 * i, heads - 1) * LD + 4 * ri);
+	};
+	if (steps > 0) scores(0);
+	for (int n = 0; n < steps; ++n) {
+		const int left = width - 64 * (wave + NW * n) - 4 * ri;
+		v4i now[R];
+#pragma unroll
+		for (int i = 0; i < R; ++i) now[i] = x[i];
+		scores(n + 1);
+#pragma unroll
+		for (int i = 0; i < R; ++i) {
+			if (fast) {
+				SaExp e = e0;
+				e.add -= top[i];
+#pragma unroll
+				for (int k4 = 0; k4 < 4; ++k4) {
+					const double y = sa_exp(e, now[i][k4]);
+					acc1[i] += k4 < left ? y : 0.0;
+				}
+				if ((n & 15) == 15) {  // 64 values of 2^47
+					sum[i] += (int64_t)acc1[i];
+					acc1[i] = 0.0;
+				}
+			} else {
+#pragma unroll
+				for (int k4 = 0; k4 < 4; ++k4) {
+					if (k4 >= left) continue;
+					const int64_t y = iexp_fast_cold((int64_t)now[i][k4] - top[i], c.q_ln2, inv, c.q_b, c.q_c, c.ceil);
+					bad |= y < 0 ? 1 << i : 0;
+					sum[i] += y < 0 ? 0 : y;
+				}
+			}
+		}
+	}
+#pragma unroll
+	for (int i = 0; i < R; ++i) {
+		const int64_t x = row16_sum(sum[i] + (int64_t)acc1[i]);
+		const bool b = row16_max(bad >> i & 1) != 0;
+		if (ri == 0 && g + 4 * i < heads) s_sum[wave][g + 4 * i] = b ? -1 : x;
+	}
+	__syncthreads();
+	CaProb pb[R];
+	int64_t den[R];
+	int refused = 0, big = 0;
+#pragma unroll
+	for (int i = 0; i < R; ++i) {
+		const int h = min(g + 4 * i, heads - 1);
+		int64_t x = 0;
+#pragma unroll
+		for (int y = 0; y < NW; ++y) {
+			refused |= s_sum[y][h] < 0 ? 1 << i : 0;
+			x += s_sum[y][h];
+		}
+		den[i] = !(refused >> i & 1) && x > 1 ? x : 1;
+		big |= den[i] >= (int64_t)1 << 36;
+		if (wave == 0 && ri == 0 && g + 4 * i < heads) w.hst[(size_t)t * a.NH + h0 + g + 4 * i] = refused >> i & 1 ? kSoftmaxKernelRefusedAfterGateAccepted : kOk;
+	}
+	const bool small = !__any(big);
+#pragma unroll
+	for (int i = 0; i < R; ++i) pb[i] = ca_prob_of(den[i], small);
+	v4i acc[DT][3];
+#pragma unroll
+	for (int d = 0; d < DT; ++d) acc[d][0] = acc[d][1] = acc[d][2] = v4i{0, 0, 0, 0};
+	if (steps > 0) scores(0);
+	for (int n = 0; n < steps; ++n) {
+		if (n == seg + kCrSteps) {
+			seg = n;
+			enter(n);
+			load(v, n, seg, a.pg.v_off);
+		}
+		const int left = width - 64 * (wave + NW * n) - 4 * ri;
+		const int sh = __shfl(ve, 4 * (n - seg) + (ri >> 2), 64);
+#pragma unroll
+		for (int i = 0; i < R; ++i) {
+			SaExp e = e0;
+			e.add -= top[i];
+			int32_t pr[4];
+#pragma unroll
+			for (int k4 = 0; k4 < 4; ++k4) {
+				if (fast) pr[k4] = small ? ca_prob<true>(pb[i], sa_exp(e, x[i][k4])) : ca_prob<false>(pb[i], sa_exp(e, x[i][k4]));
+				else pr[k4] = k4 < left ? (int32_t)div_rcp_cold(iexp_fast_cold((int64_t)x[i][k4] - top[i], c.q_ln2, inv, c.q_b, c.q_c, c.ceil) << 15, den[i], 1.0 / (double)den[i], 32768) : 0;
+				pr[k4] = k4 < left && !(refused >> i & 1) ? pr[k4] << sh : 0;
+			}
+			uint32_t y[3];
+			sa_pack3_word(pr[0], pr[1], pr[2], pr[3], y);
+			const int at = (g + 4 * i) * 16 + (ri & 3) * 4 + (ri >> 2);
+#pragma unroll
+			for (int z = 0; z < 3; ++z) ops[z * 256 + at] = y[z];
+		}
+		scores(n + 1);
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		__builtin_amdgcn_wave_barrier();
+		v4i op[3];
+#pragma unroll
+		for (int z = 0; z < 3; ++z) op[z] = *(const v4i*)(ops + z * 256 + ri * 16 + g * 4);
+		v.multiply(stage, op, acc);
+		load(v, n + 1, seg, a.pg.v_off);
+	}
+	__syncthreads();
+	v4i* join = (v4i*)row_lds;
+#pragma unroll
+	for (int d = 0; d < DT; ++d) join[(wave * DT + d) * 64 + lane] = acc[d][0] - 256 * acc[d][1] - 65536 * acc[d][2];
+	__syncthreads();
+#pragma unroll
+	for (int i = 0; i < (DT + NW - 1) / NW; ++i) {
+		const int d = wave + NW * i;
+		if (DT % NW && d >= DT) break;
+		v4i y = join[d * 64 + lane];
+#pragma unroll
+		for (int x = 1; x < NW; ++x) y += join[(x * DT + d) * 64 + lane];
+		if (ri < heads) *(v4i*)(w.part + ((size_t)t * a.NH + h0 + ri) * D + 16 * d + 4 * g) = y;
 	}
 }
 
@@ -1522,30 +1774,47 @@ void cache_store(const CacheStoreArgs& a, hipStream_t s) {
 	}
 }
 
-#ifndef T_CD
-#define T_CD 4096
-#endif
-#ifndef T_CC
-#define T_CC 768
-#endif
-constexpr int kCdTargetBlocks = T_CD, kCcTargetBlocks = T_CC;
+// Blocks that fill the chip: more cost their own start, fewer leave CUs idle.  64 rows of 28 heads / 4 KV x 128 with 1000 ..
+// 8000 positions, scores + P V: 81 us at 768 blocks, 86 at 1536, 102 at 2560, 116 at 4096; few rows want them all the same, so the
+// middle.  A chunk of 500 at 2000, its three launches: 62 at 384, 59 at 768, 73 at 1536.
+constexpr int kCdTargetBlocks = 1536, kCcTargetBlocks = 768;
+
+// Rows of up to max_width by k_cr_row: 1 with their scores in LDS, 2 in the workspace, 0 by planes.  A block takes some 6.8 us for 1000
+// positions of 128 dims by itself; the planes' three launches take 8 us more to start and then share the chip, so that they are
+// the faster form the longer the rows and the fewer the (row, KV head)s.  Row kernel / planes, us: 2 x 2 KV heads 19.5 / 21.3 at 1000
+// positions, 26.6 / 20.6 at 2000; 16 x 4 28 / 27 at 2000, 45 / 40 at 4000; 64 x 2 46 / 47 at 4000, 78 / 72 at 8000; 64 x 4 59 / 78 at
+// 4000, 313 / 326 at 20000; 32 x 2 x 64 dims 18 / 20 at 1000, 24 / 23 at 2000; 24 x 2 x 256 25 / 25 at 1000, 38 / 35 at 2000.
+template <int D>
+static int cr_form(int64_t units, int NH, int NKV, int64_t max_width) {
+	if (max_width * (210 - units) > 257000) return 0;
+	return CrShape<D>::lds(std::min(16, NH / NKV), max_width, false) <= 150 * 1024 ? 1 : 2;
+}
+static int cr_form(int64_t units, int NH, int NKV, int D, int64_t max_width) {
+	switch (D) {
+		case 32: return cr_form<32>(units, NH, NKV, max_width);
+		case 64: return cr_form<64>(units, NH, NKV, max_width);
+		case 128: return cr_form<128>(units, NH, NKV, max_width);
+		default: return cr_form<256>(units, NH, NKV, max_width);
+	}
+}
 
 // Planes: as many as fill the chip, at most some 4 sqrt(steps) of them, as their maxima and contexts are joined by
 // each (token, head) and token.
-static CaPlan ca_plan(int rows, int tokens, int max_new, int NH, int NKV, int64_t max_width) {
+static CaPlan ca_plan(int rows, int tokens, int max_new, int NH, int NKV, int D, int64_t max_width) {
 	CaPlan p{};
 	const int G = NH / NKV, step = max_new == 1 ? kCdStep : 64;
 	p.ht = (G + 15) / 16;
 	p.groups = (int)((int64_t)tokens * G / 64 + rows);
 	const int64_t units = max_new == 1 ? (int64_t)rows * NKV * p.ht : (int64_t)p.groups * NKV;
+	p.whole = max_new == 1 ? cr_form(units, NH, NKV, D, max_width) : 0;
 	const int64_t steps = (max_width + step - 1) / step;
-	int64_t planes = std::min(steps, std::max<int64_t>(1, (max_new == 1 ? kCdTargetBlocks : kCcTargetBlocks) / units));
+	int64_t planes = p.whole ? 1 : std::min(steps, std::max<int64_t>(1, (max_new == 1 ? kCdTargetBlocks : kCcTargetBlocks) / units));
 	planes = std::min(planes, std::max<int64_t>(1, (int64_t)std::sqrt(16.0 * (double)steps)));
 	p.sp = (int)((steps + planes - 1) / planes * step);
 	p.planes = (int)((max_width + p.sp - 1) / p.sp);
 	p.ps = kCdSum;
-	p.parts = max_new == 1 ? (int)((max_width + p.ps - 1) / p.ps) : p.planes;
-	p.wpad = (max_width + kCdStep - 1) / kCdStep * kCdStep;
+	p.parts = p.whole ? 0 : (max_new == 1 ? (int)((max_width + p.ps - 1) / p.ps) : p.planes);
+	p.wpad = p.whole == 1 ? 0 : (max_width + 511) / 512 * 512;
 	return p;
 }
 
@@ -1568,7 +1837,7 @@ static size_t ca_work(const CaPlan& p, int tokens, int max_new, int NH, int NKV,
 }
 
 size_t cache_attn_workspace(int rows, int tokens, int max_new, int NH, int NKV, int D, int64_t max_width) {
-	const CaPlan p = ca_plan(rows, tokens, max_new, NH, NKV, max_width);
+	const CaPlan p = ca_plan(rows, tokens, max_new, NH, NKV, D, max_width);
 	// a launch's blocks
 	if ((int64_t)rows * NKV * p.ht * p.planes >= 1ll << 30 || ((int64_t)p.planes * NKV + 8) * p.groups >= 1ll << 30) return 0;
 	CaWork w;
@@ -1578,15 +1847,30 @@ size_t cache_attn_workspace(int rows, int tokens, int max_new, int NH, int NKV, 
 template <int D>
 static void attn_launch(const CacheAttnArgs& a, hipStream_t s) {
 	const int NKV = a.pg.NKV, N = a.NH * D;
-	const CaPlan p = ca_plan(a.rows, a.tokens, a.max_new, a.NH, NKV, a.max_width);
+	const CaPlan p = ca_plan(a.rows, a.tokens, a.max_new, a.NH, NKV, D, a.max_width);
 	CaWork w;
 	ca_work(p, a.tokens, a.max_new, a.NH, NKV, D, (char*)a.ws, &w);
 	const dim3 bs(64 * kCaWaves);
-	if (a.max_new == 1) {
+	const int G = a.NH / NKV;
+	if (p.whole) {
+		const size_t lds = CrShape<D>::lds(std::min(16, G), a.max_width, p.whole == 2);
+		auto run = [&](auto kernel) {
+			allow_lds(kernel, lds);
+			hipLaunchKernelGGL(kernel, dim3((unsigned)(a.rows * NKV * p.ht)), dim3(64 * CrShape<D>::NW), lds, s, a, p, w);
+		};
+		if (p.whole == 1) {
+			if (G <= 4) run(k_cr_row<D, 1, false>);
+			else if (G <= 8) run(k_cr_row<D, 2, false>);
+			else run(k_cr_row<D, 4, false>);
+		} else {
+			if (G <= 4) run(k_cr_row<D, 1, true>);
+			else if (G <= 8) run(k_cr_row<D, 2, true>);
+			else run(k_cr_row<D, 4, true>);
+		}
+	} else if (a.max_new == 1) {
 		const dim3 grid((unsigned)(a.rows * NKV * p.ht * p.planes));
 		hipLaunchKernelGGL(k_cd_scores<D>, grid, bs, 0, s, a, p, w);
 		hipLaunchKernelGGL(k_cd_sum, dim3(p.parts, a.NH, a.rows), dim3(256), 0, s, a, p, w);
-		const int G = a.NH / NKV;
 		if (G <= 4) hipLaunchKernelGGL((k_cd_pv<D, 1>), grid, bs, 0, s, a, p, w);
 		else if (G <= 8) hipLaunchKernelGGL((k_cd_pv<D, 2>), grid, bs, 0, s, a, p, w);
 		else hipLaunchKernelGGL((k_cd_pv<D, 4>), grid, bs, 0, s, a, p, w);
