@@ -55,8 +55,8 @@ __device__ __forceinline__ uint64_t weight(const Weight& w, uint32_t d) { return
 // Rows of one slice are searched in LDS by k_sample_pick alone.
 constexpr int kSampleBlock = 512;
 constexpr int kSampleSlice = 8192, kSampleLoads = kSampleSlice / kSampleBlock / 4;
-constexpr int kBuckets = 2048, kPlanThreads = 1024;
-constexpr int kSampleList = 4096;
+constexpr int kBuckets = 2048;
+constexpr int kSampleList = 4096, kSliceList = 2048;  // elements gathered of a row, of a slice of it
 
 // What the plan found: the borders' bucket ranges [a, b), 0 top-k, 1 top-p, 2 the draw (unused ones empty).
 struct SamplePlan {
@@ -66,8 +66,9 @@ struct SamplePlan {
 	uint32_t goal_k;
 	uint32_t a[3], b[3];
 	uint32_t count;    // elements gathered
-	// sums before range 0 / 1 / 2, of the weights and of the kept ones; over the whole row where the border is none
-	unsigned long long w[2], kept[3];
+	// sums of the weights before ranges 0 and 1, of the kept ones before range 1 (0 without top-p) and range 2; over the whole row
+	// where there is no such border
+	unsigned long long w[2], kept[2];
 };
 
 struct SampleWork {
@@ -155,42 +156,59 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_hist(SampleArgs a, Samp
 	for (int i = tid; i < kBuckets / 2; i += kSampleBlock) out[i] = s_hist[2 * i] | s_hist[2 * i + 1] << 16;
 }
 
-// inclusive sums over a block's threads, and the total
-template <typename T>
-__device__ __forceinline__ T block_scan(T v, T* s, T* total) {
+// What a bucket counts for in the plan, and its sums.
+struct Mass {
+	int32_t c;
+	double e, k, v;  // weight, kept weight, variance of the weight
+};
+__device__ __forceinline__ Mass operator+(const Mass& a, const Mass& b) { return Mass{a.c + b.c, a.e + b.e, a.k + b.k, a.v + b.v}; }
+
+constexpr int kPlanThreads = 512, kPlanBuckets = kBuckets / kPlanThreads;
+
+// sums up to and with each thread's, in thread order, and the total
+__device__ __forceinline__ Mass mass_scan(Mass x, Mass* s, Mass* total) {
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 	for (int o = 1; o < 64; o *= 2) {
-		const T y = __shfl_up(v, o, 64);
-		v += lane >= o ? y : (T)0;
+		const Mass y{__shfl_up(x.c, o, 64), __shfl_up(x.e, o, 64), __shfl_up(x.k, o, 64), __shfl_up(x.v, o, 64)};
+		if (lane >= o) x = x + y;
 	}
+	if (lane == 63) s[wave] = x;
 	__syncthreads();
-	if (lane == 63) s[wave] = v;
-	__syncthreads();
-	T before = 0, all = 0;
-	for (int i = 0; i < (int)blockDim.x / 64; ++i) {
-		before += i < wave ? s[i] : (T)0;
-		all += s[i];
+	Mass before{0, 0.0, 0.0, 0.0}, all{0, 0.0, 0.0, 0.0};
+#pragma unroll
+	for (int i = 0; i < kPlanThreads / 64; ++i) {
+		if (i < wave) before = before + s[i];
+		all = all + s[i];
 	}
 	*total = all;
-	return before + v;
+	return before + x;
 }
 
-// A block per row, two neighbouring buckets a thread.  A bucket's weight is estimated by its count times the weight of its middle; that
-// is off by a few standard deviations of places spread evenly over the buckets, so a border is looked for six of them around.
+// A block per row, a few neighbouring buckets a thread.  A bucket's weight is estimated by its count times the mean of its ends',
+// which is off by what places spread evenly over the bucket deviate.  A border at the share f of a sum lies where the sum P up to
+// it less f of all is nothing: with the errors of what is before and behind it apart, that has the variance (1 - f)^2 V_before +
+// f^2 V_behind, and the border is looked for within six deviations.
 __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, SampleWork w, int slices) {
-	__shared__ int s_i[kPlanThreads / 64], s_a[3], s_b[3];
-	__shared__ double s_d[kPlanThreads / 64];
+	__shared__ uint32_t s_hist[kBuckets];
+	__shared__ Mass s_scan[kPlanThreads / 64];
 	__shared__ long long s_top;
+	__shared__ int s_a[3], s_b[3], s_n;
+	__shared__ uint32_t s_goal;
+	__shared__ double s_sum, s_kept, s_var, s_doubt, s_more;
+	__shared__ int s_few;
 	const int r = blockIdx.x, tid = threadIdx.x;
 	const Sampling s = a.rules[r];
 	if (!sampling_ok(s, a.vocab)) return;
-	if (tid == 0) s_top = kNoLogit;
+	if (tid == 0) {
+		s_top = kNoLogit;
+		s_n = 0;
+		s_goal = 0;
+		s_doubt = 0.0;
+	}
+	if (tid < 3) s_a[tid] = s_b[tid] = kBuckets;
+	for (int i = tid; i < kBuckets; i += kPlanThreads) s_hist[i] = 0;
 	__syncthreads();
 	for (int i = tid; i < slices; i += kPlanThreads) atomicMax(&s_top, (long long)w.smax[(size_t)r * slices + i]);
-	if (tid < 3) {
-		s_a[tid] = kBuckets;
-		s_b[tid] = kBuckets;
-	}
 	__syncthreads();
 	SamplePlan p{};
 	p.state = -1;
@@ -199,90 +217,103 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, Samp
 		p.top = (int32_t)s_top;
 		p.sh = bucket_shift(s);
 		const int rb = p.top >> p.sh;
-		int c[2] = {0, 0};
-		for (int i = 0; i < slices; ++i) {
-			const int64_t m = w.smax[(size_t)r * slices + i];
+		const uint32_t j0 = kPlanBuckets * tid;
+		// a wave to a slice, sixteen bytes of its counts to a lane
+		for (int i = tid >> 6; i < slices; i += kPlanThreads / 64) {
+			const size_t at = (size_t)r * slices + i;
+			const int64_t m = w.smax[at];
+			v4i x[kBuckets / 512];
+#pragma unroll
+			for (int k = 0; k < kBuckets / 512; ++k) x[k] = *(const v4i*)(w.hist + at * kBuckets + 8 * ((tid & 63) + 64 * k));
 			if (m == kNoLogit) continue;
 			const uint32_t off = (uint32_t)rb - (uint32_t)((int32_t)m >> p.sh);  // the slice's first bucket
-			const uint16_t* h = w.hist + ((size_t)r * slices + i) * kBuckets;
 #pragma unroll
-			for (int k = 0; k < 2; ++k) {
-				const uint32_t j = 2 * tid + k;
-				if (j >= off) c[k] += h[j - off];
-			}
-		}
-		const Weight wt = weight_of(s);
-		const double least = (double)share_of((uint64_t)(s.q_b * s.q_b + s.q_c), s.min_p);
-		// a bucket's estimate, kept estimate and variance
-		double e[2], k[2], var = 0.0, doubt = 0.0;
+			for (int k = 0; k < kBuckets / 512; ++k)
 #pragma unroll
-		for (int i = 0; i < 2; ++i) {
-			const int64_t low = ((int64_t)rb - (2 * tid + i)) * ((int64_t)1 << p.sh);  // its least logit
-			const int64_t d1 = p.top - low, d0 = i64max(0, d1 - (((int64_t)1 << p.sh) - 1));
-			const double w0 = (double)weight(wt, (uint32_t)i64min(d0, 0xffffffffll)), w1 = (double)weight(wt, (uint32_t)i64min(d1, 0xffffffffll));
-			const double mid = 0.5 * (w0 + w1), n = (double)c[i];
-			e[i] = n * mid;
-			k[i] = mid >= least ? n * mid : 0.0;
-			if (w0 >= least && w1 < least) doubt += n * w0;
-			var += n * (w0 - w1) * (w0 - w1) * (1.0 / 12);
-		}
-		int all_c;
-		double all_e, all_k, all_v, all_x;
-		const int run_c = block_scan(c[0] + c[1], s_i, &all_c);
-		const double run_e = block_scan(e[0] + e[1], s_d, &all_e), run_k = block_scan(k[0] + k[1], s_d, &all_k);
-		block_scan(var, s_d, &all_v);
-		block_scan(doubt, s_d, &all_x);
-		// one past bucket i of this thread's
-		const int pc[2] = {run_c - c[1], run_c};
-		const double pe[2] = {run_e - e[1], run_e}, pk[2] = {run_k - k[1], run_k};
-		__shared__ double s_sum, s_kept;
-		__shared__ uint32_t s_goal;
-		// top-k: exactly its bucket; the estimates up to its border
-		const bool cut_k = s.top_k > 0 && s.top_k < all_c;
-		if (tid == 0) {
-			s_sum = all_e;
-			s_kept = all_k;
-			s_goal = 0;
+				for (int e = 0; e < 8; ++e) {
+					const uint32_t j = 8 * ((tid & 63) + 64 * k) + e, n = (uint32_t)x[k][e / 2] >> 16 * (e & 1) & 0xffff;
+					if (n && off < kBuckets && j + off < kBuckets) atomicAdd(&s_hist[j + off], n);
+				}
 		}
 		__syncthreads();
+		int c[kPlanBuckets];
+#pragma unroll
+		for (int k = 0; k < kPlanBuckets; ++k) c[k] = s_hist[j0 + k];
+		const Weight wt = weight_of(s);
+		const double least = (double)share_of((uint64_t)(s.q_b * s.q_b + s.q_c), s.min_p);
+		Mass one[kPlanBuckets], run[kPlanBuckets], all, mine{0, 0.0, 0.0, 0.0};
+		double doubt = 0.0;  // what lies in the bucket that min-p cuts
+#pragma unroll
+		for (int i = 0; i < kPlanBuckets; ++i) {
+			const int64_t low = ((int64_t)rb - (j0 + i)) * ((int64_t)1 << p.sh);  // its least logit
+			const int64_t d1 = p.top - low, d0 = i64max(0, d1 - (((int64_t)1 << p.sh) - 1));
+			const double w0 = weight_d(wt, (uint32_t)i64min(d0, 0xffffffffll)), w1 = weight_d(wt, (uint32_t)i64min(d1, 0xffffffffll));
+			const double mid = 0.5 * (w0 + w1), n = (double)c[i];
+			one[i] = Mass{c[i], n * mid, mid >= least ? n * mid : 0.0, n * (w0 - w1) * (w0 - w1) * (1.0 / 12)};
+			doubt += w0 >= least && w1 < least ? n * w0 : 0.0;
+			mine = mine + one[i];
+		}
+		if (s.min_p > 0 && doubt > 0.0) s_doubt = doubt;
+		Mass at = mass_scan(mine, s_scan, &all);
+#pragma unroll
+		for (int i = kPlanBuckets - 1; i >= 0; --i) {
+			run[i] = at;
+			at = Mass{at.c - one[i].c, at.e - one[i].e, at.k - one[i].k, at.v - one[i].v};
+		}
+		if (tid == 0) {
+			s_sum = all.e;
+			s_kept = all.k;
+			s_var = all.v;
+			s_few = all.c;
+			s_more = 0.0;
+		}
+		__syncthreads();
+		// top-k: exactly its bucket; the estimates up to its border
+		const bool cut_k = s.top_k > 0 && s.top_k < all.c, by_p = s.top_p < 65536;
 		if (cut_k)
 #pragma unroll
-			for (int i = 0; i < 2; ++i)
-				if (pc[i] >= s.top_k && pc[i] - c[i] < s.top_k) {
-					const double part = (double)(s.top_k - (pc[i] - c[i])) / (double)c[i];
-					s_a[0] = 2 * tid + i;
-					s_b[0] = 2 * tid + i + 1;
-					s_goal = s.top_k - (pc[i] - c[i]);
-					s_sum = pe[i] - e[i] + part * e[i];
-					s_kept = pk[i] - k[i] + part * k[i];
+			for (int i = 0; i < kPlanBuckets; ++i)
+				if (run[i].c >= s.top_k && run[i].c - one[i].c < s.top_k) {
+					s_goal = s.top_k - (run[i].c - one[i].c);
+					s_few = run[i].c;
+					const double part = (double)s_goal / (double)one[i].c;
+					s_a[0] = (int)j0 + i;
+					s_b[0] = (int)j0 + i + 1;
+					s_sum = run[i].e - (1.0 - part) * one[i].e;
+					s_kept = run[i].k - (1.0 - part) * one[i].k;
+					s_var = run[i].v + one[i].e * one[i].e * 0.01;  // which of the bucket's elements these are
 				}
 		__syncthreads();
 		const int end = s_b[0];  // nothing is taken past it
-		const double slack = 6.0 * sqrt(all_v) + 1e-9 * all_e;
-		double kept = s_kept;
-		auto range = [&](int which, const double (&run)[2], const double (&one)[2], double goal, double off) {
-			if (tid == 0 && goal - off <= 0.0) s_a[which] = 0;
+		const bool few = s_few <= kSampleList / 2;  // of few elements all are gathered
+		const double sum = s_sum, kept_k = s_kept, var = s_var;
+		auto range = [&](int which, bool of_kept, double goal, double whole, double more) {
+			const double f = whole > 0.0 ? fmin(1.0, goal / whole) : 0.0;
 #pragma unroll
-			for (int i = 0; i < 2; ++i) {
-				const int j = 2 * tid + i;
-				if (run[i] >= goal - off && run[i] - one[i] < goal - off) atomicMin(&s_a[which], max(0, j - 1));
-				if (run[i] >= goal + off && run[i] - one[i] < goal + off) atomicMin(&s_b[which], j + 2);
+			for (int i = 0; i < kPlanBuckets; ++i) {
+				const double v = fmin(run[i].v, var), off = 6.0 * sqrt((1.0 - f) * (1.0 - f) * v + f * f * (var - v)) + 1e-9 * whole + more;
+				const double at = (of_kept ? run[i].k : run[i].e) - goal;
+				if (at >= -off) atomicMin(&s_a[which], max(0, (int)j0 + i - 1));
+				if (at >= off) {
+					atomicMin(&s_b[which], (int)j0 + i + 2);
+					break;
+				}
 			}
 		};
-		if (s.top_p < 65536) {
-			const double goal = s_sum * s.top_p * (1.0 / 65536);
-			range(1, pe, e, goal, slack);
-			__syncthreads();
-			s_kept = all_k;
-			__syncthreads();
-			// the kept weight up to there
+		double kept = kept_k;
+		if (by_p) {
+			const double goal = sum * s.top_p * (1.0 / 65536);
+			range(1, false, goal, sum, 0.0);
 #pragma unroll
-			for (int i = 0; i < 2; ++i)
-				if (pe[i] >= goal && pe[i] - e[i] < goal) s_kept = pk[i] - k[i] + (e[i] > 0.0 ? (goal - (pe[i] - e[i])) / e[i] : 0.0) * k[i];
+			for (int i = 0; i < kPlanBuckets; ++i)  // the kept weight up to there
+				if (run[i].e >= goal && run[i].e - one[i].e < goal) {
+					s_kept = fmin(kept_k, run[i].k - (1.0 - (goal - (run[i].e - one[i].e)) / one[i].e) * one[i].k);
+					s_more = 1.2 * one[i].e / (double)one[i].c;  // the run ends with a whole element
+				}
 			__syncthreads();
-			kept = fmin(kept, s_kept);
+			kept = s_kept;
 		}
-		range(2, pk, k, kept * s.random * 0x1p-32, slack + all_x);
+		range(2, true, kept * s.random * 0x1p-32, kept_k, s_doubt + s_more);
 		__syncthreads();
 		p.cut_k = cut_k;
 		p.goal_k = s_goal;
@@ -290,22 +321,24 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, Samp
 		for (int i = 0; i < 3; ++i) {
 			p.a[i] = min(s_a[i], end - 1);
 			p.b[i] = max(min(s_b[i], end), (int)p.a[i]);
+			if (few) {
+				p.a[i] = i ? 0 : p.a[i];
+				p.b[i] = end;
+			}
 		}
 		if (!cut_k) p.a[0] = p.b[0] = kBuckets;
-		if (s.top_p >= 65536) p.a[1] = p.b[1] = kBuckets;
+		if (!by_p) p.a[1] = p.b[1] = kBuckets;
 		// how much would be gathered
 		int n = 0;
 #pragma unroll
-		for (int i = 0; i < 2; ++i) {
-			const uint32_t j = 2 * tid + i;
-			bool in = false;
-#pragma unroll
-			for (int x = 0; x < 3; ++x) in |= j >= p.a[x] && j < p.b[x];
-			n += in ? c[i] : 0;
+		for (int i = 0; i < kPlanBuckets; ++i) {
+			const uint32_t j = j0 + i;
+			n += (j >= p.a[0] && j < p.b[0]) || (j >= p.a[1] && j < p.b[1]) || (j >= p.a[2] && j < p.b[2]) ? c[i] : 0;
 		}
-		int sum;
-		block_scan(n, s_i, &sum);
-		if (sum > kSampleList) p.state = 1;
+		n = wave_sum32(n);
+		if ((tid & 63) == 0 && n) atomicAdd(&s_n, n);
+		__syncthreads();
+		if (s_n > kSampleList) p.state = 1;
 	}
 	if (tid == 0) w.plan[r] = p;
 }
@@ -313,6 +346,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, Samp
 template <bool VEC>
 __global__ __launch_bounds__(kSampleBlock) void k_sample_gather(SampleArgs a, SampleWork w) {
 	__shared__ unsigned long long s_sum[5];
+	__shared__ uint2 s_list[kSliceList];
+	__shared__ uint32_t s_n, s_at;
 	const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
 	const Sampling s = a.rules[r];
 	SampleSlice<VEC> sl;
@@ -322,49 +357,64 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_gather(SampleArgs a, Sa
 	if (p.state != 0) return;
 	const int32_t top = p.top, sh = p.sh, rb = top >> sh;
 	const uint32_t a0 = p.a[0], a1 = p.a[1], a2 = p.a[2], b0 = p.b[0], b1 = p.b[1], b2 = p.b[2];
-	// the sums that the borders need: 0, 1 weights before ranges 0 and 1; 2, 3, 4 kept weights before 0, 1 and 2
-	const bool by_p = s.top_p < 65536;
-	const uint32_t upto[5] = {by_p ? a0 : 0, by_p ? a1 : 0, by_p ? 0 : a0, by_p ? a1 : 0, a2};
-	uint32_t most = 0;
-#pragma unroll
-	for (int i = 0; i < 5; ++i) most = max(most, upto[i]);
+	// the sums that the borders need: weights before ranges 0, 1 and 2, kept ones (where min-p makes them others) before 0 or 1, and 2
+	const bool by_p = s.top_p < 65536, min_p = s.min_p > 0;
+	const uint32_t first = by_p ? a1 : a0, most = by_p ? max(a0, max(a1, a2)) : max(a0, a2);
 	if (tid < 5) s_sum[tid] = 0;
+	if (tid == 0) s_n = 0;
 	__syncthreads();
 	const Weight wt = weight_of(s);
-	const uint64_t w0 = (uint64_t)(s.q_b * s.q_b + s.q_c);
-	const double least = (double)share_of(w0, s.min_p);
-	double acc[5] = {};
+	const double least = (double)share_of((uint64_t)(s.q_b * s.q_b + s.q_c), s.min_p);
+	double acc[5] = {};  // 16 values of 2^47
 #pragma unroll
 	for (int u = 0; u < kSampleLoads; ++u)
 #pragma unroll
 		for (int i = 0; i < 4; ++i) {
-			const uint32_t j = (uint32_t)rb - (uint32_t)(sl.x[u][i] >> sh);
-			const bool has = sl.has(u, i);
-			if (__any(has && j < most)) {
-				const double x = weight_d(wt, (uint32_t)top - (uint32_t)sl.x[u][i]), y = x >= least ? x : 0.0;
-#pragma unroll
-				for (int k = 0; k < 5; ++k) acc[k] += has && j < upto[k] ? (k < 2 ? x : y) : 0.0;  // 16 values of 2^47
+			const uint32_t j = sl.has(u, i) ? (uint32_t)rb - (uint32_t)(sl.x[u][i] >> sh) : ~0u;
+			if (__any(j < most)) {
+				const double x = weight_d(wt, (uint32_t)top - (uint32_t)sl.x[u][i]);
+				acc[0] += j < a0 ? x : 0.0;
+				if (by_p) acc[1] += j < a1 ? x : 0.0;
+				if (!min_p) acc[2] += j < a2 ? x : 0.0;
+				else {
+					const double y = x >= least ? x : 0.0;
+					acc[3] += j < first ? y : 0.0;
+					acc[4] += j < a2 ? y : 0.0;
+				}
 			}
-			const bool in = has && ((j >= a0 && j < b0) || (j >= a1 && j < b1) || (j >= a2 && j < b2));
-			const uint64_t who = __ballot(in);
-			if (who) {
-				uint32_t at = 0;
-				if (lane == __builtin_ctzll(who)) at = atomicAdd(&w.plan[r].count, (uint32_t)__popcll(who));
-				at = __builtin_amdgcn_readlane(at, __builtin_ctzll(who)) + __popcll(who & ((1ull << lane) - 1));
-				if (in && at < kSampleList) w.list[(size_t)r * kSampleList + at] = uint2{(uint32_t)top - (uint32_t)sl.x[u][i], (uint32_t)sl.index(u, i)};
+			const bool in = j - a0 < b0 - a0 || j - a1 < b1 - a1 || j - a2 < b2 - a2;
+			if (__any(in) && in) {
+				const uint32_t at = atomicAdd(&s_n, 1u);
+				if (at < kSliceList) s_list[at] = uint2{(uint32_t)top - (uint32_t)sl.x[u][i], (uint32_t)sl.index(u, i)};
 			}
 		}
 #pragma unroll
 	for (int k = 0; k < 5; ++k) {
-		if (!upto[k]) continue;
+		if (!__any(acc[k] != 0.0)) continue;
 		int64_t x = (int64_t)acc[k];
 		x = row16_sum(x);
 		x += __shfl_xor(x, 16, 64);
 		x += __shfl_xor(x, 32, 64);
-		if (lane == 0 && x) atomicAdd(&s_sum[k], (unsigned long long)x);
+		if (lane == 0) atomicAdd(&s_sum[k], (unsigned long long)x);
 	}
 	__syncthreads();
-	if (tid < 5 && s_sum[tid]) atomicAdd(tid < 2 ? &w.plan[r].w[tid] : &w.plan[r].kept[tid - 2], s_sum[tid]);
+	const uint32_t n = s_n;
+	if (tid == 0) {
+		SamplePlan& o = w.plan[r];
+		// a slice with more than its share: past the row's list, whose search then runs over the row
+		if (n) s_at = atomicAdd(&o.count, n <= kSliceList ? n : kSampleList + 1);
+		auto add = [](unsigned long long* to, unsigned long long x) {
+			if (x) atomicAdd(to, x);
+		};
+		add(&o.w[0], s_sum[0]);
+		add(&o.w[1], s_sum[1]);
+		add(&o.kept[0], min_p ? s_sum[3] : (by_p ? s_sum[1] : s_sum[0]));
+		add(&o.kept[1], min_p ? s_sum[4] : s_sum[2]);
+	}
+	__syncthreads();
+	if (n > kSliceList) return;
+	for (uint32_t i = tid; i < n; i += kSampleBlock)
+		if (s_at + i < kSampleList) w.list[(size_t)r * kSampleList + s_at + i] = s_list[i];
 }
 
 struct BorderShared {
@@ -373,30 +423,44 @@ struct BorderShared {
 	unsigned long long sum[kSampleBlock / 64];
 };
 
-// The element whose running measure reaches `goal` among those that get(i, d, index) admits of `n`, by radix over the key
-// (d - d0, index), d - d0 below 2^bits: a byte a pass until one element is left.  False when there is none.
-template <typename G, typename M>
-__device__ __forceinline__ bool find_border(int n, G&& get, M&& measure, uint64_t goal, uint32_t d0, int bits, BorderShared& s, uint32_t* dcut, uint32_t* icut) {
+// f(d, index) for the elements i < n that fetch(i) gives (no element: kNone), eight of a thread's on their way at a time
+constexpr uint32_t kNone = 0xffffffffu;
+template <typename F, typename X, typename I>
+__device__ __forceinline__ void each_element(int n, F&& fetch, I&& index, X&& f) {
+	for (int i0 = threadIdx.x; i0 < n; i0 += 8 * kSampleBlock) {
+		uint32_t d[8];
+#pragma unroll
+		for (int u = 0; u < 8; ++u) d[u] = i0 + u * kSampleBlock < n ? fetch(i0 + u * kSampleBlock) : kNone;
+#pragma unroll
+		for (int u = 0; u < 8; ++u)
+			if (d[u] != kNone) f(d[u], index(i0 + u * kSampleBlock));
+	}
+}
+
+// The element whose running measure reaches `goal` among those that admit(d, index) lets in, by radix over the key
+// (d - d0, index), d - d0 below 2^bits: eight bits a pass until one element is left.  False when there is none.
+template <typename F, typename I, typename A, typename M>
+__device__ __forceinline__ bool find_border(int n, F&& fetch, I&& index, A&& admit, M&& measure, uint64_t goal, uint32_t d0, int bits, BorderShared& s, uint32_t* dcut,
+                                            uint32_t* icut) {
 	const int tid = threadIdx.x;
 	uint64_t prefix = 0;
-	int shift = 24 + (bits + 7) / 8 * 8;
+	int shift = 24 + bits;
 	for (uint32_t one = 0; shift > 0 && !one;) {
-		shift -= 8;
+		const int above = shift;
+		shift = max(0, shift - 8);
 		__syncthreads();
 		for (int i = tid; i < 256; i += kSampleBlock) {
 			s.m[i] = 0;
 			s.c[i] = 0;
 		}
 		__syncthreads();
-		for (int i = tid; i < n; i += kSampleBlock) {
-			uint32_t d, index;
-			if (!get(i, &d, &index)) continue;
-			const uint64_t key = (uint64_t)(d - d0) << 24 | index;
-			if ((key ^ prefix) >> (shift + 8)) continue;
-			const int b = (int)(key >> shift & 255);
+		each_element(n, fetch, index, [&](uint32_t d, uint32_t i) {
+			const uint64_t key = (uint64_t)(d - d0) << 24 | i;
+			if (((key ^ prefix) >> above) || !admit(d, i)) return;
+			const int b = (int)(key >> shift) & ((1 << (above - shift)) - 1);
 			atomicAdd(&s.m[b], (unsigned long long)measure(d));
 			atomicAdd(&s.c[b], 1u);
-		}
+		});
 		__syncthreads();
 		if (tid < 64) {
 			uint64_t m[4], x = 0;
@@ -424,12 +488,10 @@ __device__ __forceinline__ bool find_border(int n, G&& get, M&& measure, uint64_
 		goal -= s.below;
 		one = s.one;
 	}
-	for (int i = tid; i < n; i += kSampleBlock) {
-		uint32_t d, index;
-		if (!get(i, &d, &index)) continue;
-		const uint64_t key = (uint64_t)(d - d0) << 24 | index;
-		if (!((key ^ prefix) >> shift)) s.key = key;
-	}
+	each_element(n, fetch, index, [&](uint32_t d, uint32_t i) {
+		const uint64_t key = (uint64_t)(d - d0) << 24 | i;
+		if (!((key ^ prefix) >> shift) && admit(d, i)) s.key = key;
+	});
 	__syncthreads();
 	*dcut = (uint32_t)(s.key >> 24) + d0;
 	*icut = (uint32_t)(s.key & 0xffffff);
@@ -437,13 +499,10 @@ __device__ __forceinline__ bool find_border(int n, G&& get, M&& measure, uint64_
 	return true;
 }
 
-template <typename G, typename M>
-__device__ __forceinline__ uint64_t sum_of(int n, G&& get, M&& measure, BorderShared& s) {
+template <typename F, typename I, typename A, typename M>
+__device__ __forceinline__ uint64_t sum_of(int n, F&& fetch, I&& index, A&& admit, M&& measure, BorderShared& s) {
 	uint64_t x = 0;
-	for (int i = threadIdx.x; i < n; i += kSampleBlock) {
-		uint32_t d, index;
-		if (get(i, &d, &index)) x += measure(d);
-	}
+	each_element(n, fetch, index, [&](uint32_t d, uint32_t i) { x += admit(d, i) ? measure(d) : 0; });
 	for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
 	__syncthreads();
 	if ((threadIdx.x & 63) == 0) s.sum[threadIdx.x >> 6] = x;
@@ -491,12 +550,13 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_pick(SampleArgs a, Samp
 			i_of[i] = x.y;
 		}
 		__syncthreads();
+		auto fetch = [&](int i) { return d_of[i]; };
+		auto index = [&](int i) { return i_of[i]; };
 		auto within = [&](int which) {
-			return [&, which](int i, uint32_t* d, uint32_t* index) {
-				*d = d_of[i];
-				*index = i_of[i];
-				const uint32_t j = (uint32_t)rb - (uint32_t)((int32_t)((uint32_t)p.top - *d) >> p.sh);
-				return j >= p.a[which] && j < p.b[which] && (*d < dcut || (*d == dcut && *index <= icut));
+			const uint32_t from = p.a[which], many = p.b[which] - p.a[which];
+			return [&, from, many](uint32_t d, uint32_t i) {
+				const uint32_t j = (uint32_t)rb - (uint32_t)((int32_t)((uint32_t)p.top - d) >> p.sh);
+				return j - from < many && (d < dcut || (d == dcut && i <= icut));
 			};
 		};
 		// the smallest d of a bucket, and the bits of a range
@@ -505,20 +565,20 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_pick(SampleArgs a, Samp
 		uint64_t total = p.w[0], kept = p.kept[0];
 		bool ok = true;
 		if (p.cut_k) {
-			ok = find_border(n, within(0), ones, p.goal_k, first(0), bits(0), sh, &dcut, &icut);
-			if (ok && by_p) total += sum_of(n, within(0), weights, sh);
-			if (ok && !by_p) kept += sum_of(n, within(0), kepts, sh);
+			ok = find_border(n, fetch, index, within(0), ones, p.goal_k, first(0), bits(0), sh, &dcut, &icut);
+			if (ok && by_p) total += sum_of(n, fetch, index, within(0), weights, sh);
+			if (ok && !by_p) kept += sum_of(n, fetch, index, within(0), kepts, sh);
 		}
 		if (ok && by_p) {
 			uint64_t need = share_of(total, s.top_p);
 			need = need < 1 ? 1 : need;
-			ok = need > p.w[1] && find_border(n, within(1), weights, need - p.w[1], first(1), bits(1), sh, &dcut, &icut);
-			if (ok) kept = p.kept[1] + sum_of(n, within(1), kepts, sh);
+			ok = need > p.w[1] && find_border(n, fetch, index, within(1), weights, need - p.w[1], first(1), bits(1), sh, &dcut, &icut);
+			if (ok) kept += sum_of(n, fetch, index, within(1), kepts, sh);
 		}
 		if (ok) {
 			const uint64_t goal = random_of(kept, s.random) + 1;
 			all = kept;
-			ok = goal > p.kept[2] && find_border(n, within(2), kepts, goal - p.kept[2], first(2), bits(2), sh, &dcut, &icut);
+			ok = goal > p.kept[1] && find_border(n, fetch, index, within(2), kepts, goal - p.kept[1], first(2), bits(2), sh, &dcut, &icut);
 		}
 		done = ok;
 		__syncthreads();
@@ -534,11 +594,21 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_pick(SampleArgs a, Samp
 		auto legal = [&](int i) { return !s.mask || (global_ptr(s.mask)[i >> 3] >> (i & 7) & 1); };
 		int top = INT32_MIN;
 		bool any = false;
-		for (int i = tid; i < a.vocab; i += kSampleBlock)
-			if (legal(i)) {
-				top = max(top, row[i]);
-				any = true;
+		for (int i0 = tid; i0 < a.vocab; i0 += 8 * kSampleBlock) {
+			int32_t x[8];
+			bool ok[8];
+#pragma unroll
+			for (int u = 0; u < 8; ++u) {
+				const int i = min(i0 + u * kSampleBlock, a.vocab - 1);
+				x[u] = row[i];
+				ok[u] = legal(i);
 			}
+#pragma unroll
+			for (int u = 0; u < 8; ++u) {  // a clamped one repeats the last
+				top = ok[u] ? max(top, x[u]) : top;
+				any |= ok[u];
+			}
+		}
 		if (any) {
 			atomicMax(&s_top, top);
 			s_any = 1;
@@ -556,25 +626,27 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_pick(SampleArgs a, Samp
 		if (in_lds) {
 			for (int i = tid; i < a.vocab; i += kSampleBlock) {
 				const uint32_t d = (uint32_t)top - (uint32_t)row[i];
-				s_d[i] = legal(i) && (int64_t)d < wt.lim ? d : 0xffffffffu;
+				s_d[i] = legal(i) && (int64_t)d < wt.lim ? d : kNone;
 			}
 			__syncthreads();
 		}
 		dcut = 0xffffffffu;
 		icut = 0xffffffu;
-		auto get = [&](int i, uint32_t* d, uint32_t* index) {
-			*d = in_lds ? s_d[i] : (legal(i) ? (uint32_t)top - (uint32_t)row[i] : 0xffffffffu);
-			*index = i;
-			return (int64_t)*d < wt.lim && (*d < dcut || (*d == dcut && *index <= icut));
+		auto fetch = [&](int i) {
+			if (in_lds) return s_d[i];
+			const uint32_t d = (uint32_t)top - (uint32_t)row[i];
+			return legal(i) && (int64_t)d < wt.lim ? d : kNone;
 		};
+		auto index = [&](int i) { return (uint32_t)i; };
+		auto admit = [&](uint32_t d, uint32_t i) { return d < dcut || (d == dcut && i <= icut); };
 		const int bits = 64 - __builtin_clzll((uint64_t)wt.lim);
-		if (s.top_k > 0 && (uint64_t)s.top_k < sum_of(a.vocab, get, ones, sh)) find_border(a.vocab, get, ones, s.top_k, 0, bits, sh, &dcut, &icut);
+		if (s.top_k > 0 && (uint64_t)s.top_k < sum_of(a.vocab, fetch, index, admit, ones, sh)) find_border(a.vocab, fetch, index, admit, ones, s.top_k, 0, bits, sh, &dcut, &icut);
 		if (by_p) {
-			const uint64_t need = share_of(sum_of(a.vocab, get, weights, sh), s.top_p);
-			find_border(a.vocab, get, weights, need < 1 ? 1 : need, 0, bits, sh, &dcut, &icut);
+			const uint64_t need = share_of(sum_of(a.vocab, fetch, index, admit, weights, sh), s.top_p);
+			find_border(a.vocab, fetch, index, admit, weights, need < 1 ? 1 : need, 0, bits, sh, &dcut, &icut);
 		}
-		all = sum_of(a.vocab, get, kepts, sh);
-		find_border(a.vocab, get, kepts, random_of(all, s.random) + 1, 0, bits, sh, &dcut, &icut);
+		all = sum_of(a.vocab, fetch, index, admit, kepts, sh);
+		find_border(a.vocab, fetch, index, admit, kepts, random_of(all, s.random) + 1, 0, bits, sh, &dcut, &icut);
 	}
 	if (tid == 0) {
 		a.tokens[r] = (int32_t)icut;
