@@ -208,7 +208,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, Samp
 	if (tid < 3) s_a[tid] = s_b[tid] = kBuckets;
 	for (int i = tid; i < kBuckets; i += kPlanThreads) s_hist[i] = 0;
 	__syncthreads();
-	for (int i = tid; i < slices; i += kPlanThreads) atomicMax(&s_top, (long long)w.smax[(size_t)r * slices + i]);
+	long long top = kNoLogit;
+	for (int i = tid; i < slices; i += kPlanThreads) top = max(top, (long long)w.smax[(size_t)r * slices + i]);
+	for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
+	if ((tid & 63) == 0) atomicMax(&s_top, top);
 	__syncthreads();
 	SamplePlan p{};
 	p.state = -1;
@@ -289,16 +292,18 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, Samp
 		const double sum = s_sum, kept_k = s_kept, var = s_var;
 		auto range = [&](int which, bool of_kept, double goal, double whole, double more) {
 			const double f = whole > 0.0 ? fmin(1.0, goal / whole) : 0.0;
+			int from = kBuckets, to = kBuckets;
 #pragma unroll
-			for (int i = 0; i < kPlanBuckets; ++i) {
+			for (int i = kPlanBuckets - 1; i >= 0; --i) {
 				const double v = fmin(run[i].v, var), off = 6.0 * sqrt((1.0 - f) * (1.0 - f) * v + f * f * (var - v)) + 1e-9 * whole + more;
 				const double at = (of_kept ? run[i].k : run[i].e) - goal;
-				if (at >= -off) atomicMin(&s_a[which], max(0, (int)j0 + i - 1));
-				if (at >= off) {
-					atomicMin(&s_b[which], (int)j0 + i + 2);
-					break;
-				}
+				from = at >= -off ? max(0, (int)j0 + i - 1) : from;
+				to = at >= off ? (int)j0 + i + 2 : to;
 			}
+			// buckets ascend with the lanes: a wave's first one is its least
+			const uint64_t fs = __ballot(from < kBuckets), ts = __ballot(to < kBuckets);
+			if (fs && (tid & 63) == __builtin_ctzll(fs)) atomicMin(&s_a[which], from);
+			if (ts && (tid & 63) == __builtin_ctzll(ts)) atomicMin(&s_b[which], to);
 		};
 		double kept = kept_k;
 		if (by_p) {
@@ -343,6 +348,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, Samp
 	if (tid == 0) w.plan[r] = p;
 }
 
+// x, or less than 2^-1000, which no sum of integers notices: one select instead of two
+__device__ __forceinline__ double only(bool take, double x) { return __hiloint2double(take ? __double2hiint(x) : 0, __double2loint(x)); }
+
 template <bool VEC>
 __global__ __launch_bounds__(kSampleBlock) void k_sample_gather(SampleArgs a, SampleWork w) {
 	__shared__ unsigned long long s_sum[5];
@@ -373,19 +381,21 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_gather(SampleArgs a, Sa
 			const uint32_t j = sl.has(u, i) ? (uint32_t)rb - (uint32_t)(sl.x[u][i] >> sh) : ~0u;
 			if (__any(j < most)) {
 				const double x = weight_d(wt, (uint32_t)top - (uint32_t)sl.x[u][i]);
-				acc[0] += j < a0 ? x : 0.0;
-				if (by_p) acc[1] += j < a1 ? x : 0.0;
-				if (!min_p) acc[2] += j < a2 ? x : 0.0;
+				acc[0] += only(j < a0, x);
+				if (by_p) acc[1] += only(j < a1, x);
+				if (!min_p) acc[2] += only(j < a2, x);
 				else {
-					const double y = x >= least ? x : 0.0;
-					acc[3] += j < first ? y : 0.0;
-					acc[4] += j < a2 ? y : 0.0;
+					acc[3] += only(j < first && x >= least, x);
+					acc[4] += only(j < a2 && x >= least, x);
 				}
 			}
 			const bool in = j - a0 < b0 - a0 || j - a1 < b1 - a1 || j - a2 < b2 - a2;
-			if (__any(in) && in) {
-				const uint32_t at = atomicAdd(&s_n, 1u);
-				if (at < kSliceList) s_list[at] = uint2{(uint32_t)top - (uint32_t)sl.x[u][i], (uint32_t)sl.index(u, i)};
+			const uint64_t who = __ballot(in);
+			if (who) {
+				uint32_t at = 0;
+				if (lane == __builtin_ctzll(who)) at = atomicAdd(&s_n, (uint32_t)__popcll(who));
+				at = __builtin_amdgcn_readlane(at, __builtin_ctzll(who)) + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+				if (in && at < kSliceList) s_list[at] = uint2{(uint32_t)top - (uint32_t)sl.x[u][i], (uint32_t)sl.index(u, i)};
 			}
 		}
 #pragma unroll
