@@ -27,17 +27,19 @@ __device__ __forceinline__ int64_t pages_for(int64_t positions, int lp) { return
 constexpr int kPlanBlock = 1024;
 
 // The sum of v over the threads before this one; *total: over all.  s: kPlanBlock / 64 words.
-__device__ __forceinline__ int block_before(int v, int* total, int* s) {
+template <typename T>
+__device__ __forceinline__ T block_before(T v, T* total, T* s) {
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-	int x = v;
+	T x = v;
 	for (int o = 1; o < 64; o *= 2) {
-		const int y = __shfl_up(x, o, 64);
+		const T y = __shfl_up(x, o, 64);
 		x += lane >= o ? y : 0;
 	}
 	__syncthreads();
 	if (lane == 63) s[wave] = x;
 	__syncthreads();
-	int before = 0, all = 0;
+	T before = 0, all = 0;
+#pragma unroll
 	for (int i = 0; i < kPlanBlock / 64; ++i) {
 		before += i < wave ? s[i] : 0;
 		all += s[i];
@@ -51,7 +53,6 @@ struct PlanWork {
 	int32_t* state;   // [0]: whether there is anything to do, [1]: pages to copy
 	int32_t* off;     // [rows] a row's first free page in `free`
 	int32_t* tail;    // [rows] the page it gets a copy of, or -1
-	int32_t* low;     // [pages] the lowest row that writes into a page
 	int32_t* free;    // [pages] free pages in the order they are given out (compaction: the holes)
 	int32_t *from, *to;  // pages to copy
 	int32_t* old;     // [rows, table_ld] the tables as they were, where the new ones take their place
@@ -63,19 +64,23 @@ __global__ __launch_bounds__(256) void k_table_copy(const int32_t* from, int32_t
 
 // One block: bitmaps of the pages that rows hold (seen), hold more than once (multi), and hold without writing
 // into them or keep from outside (fixed), in LDS; then who gets a copy, how many pages each row takes, and the free
-// pages in ascending order.
+// pages in ascending order.  Bound by its chain of loads (a row's numbers, its source's length, the tables) and of block sums.
+constexpr int kLowSlots = 2048;
+constexpr int kWrites = 1 << 30;  // beside a row's number of kept pages: it writes into the last of them
 __global__ __launch_bounds__(kPlanBlock) void k_update_plan(PageUpdateArgs a, const int32_t* tables, PlanWork w) {
 	extern __shared__ uint32_t lds[];
-	__shared__ int s_scan[kPlanBlock / 64], s_bad, s_most;
+	__shared__ int64_t s_scan[kPlanBlock / 64];
+	__shared__ int s_bad, s_most, s_low[kLowSlots];  // s_low: the lowest row that writes into a page of the slot
 	const int tid = threadIdx.x, words = (a.pages + 31) / 32;
 	uint32_t *seen = lds, *multi = seen + words, *fixed = multi + words;
-	int32_t *s_src = (int32_t*)(fixed + words), *s_kept = s_src + a.rows;  // kept pages, bit 30: the row writes into the last
+	int32_t *s_src = (int32_t*)(fixed + words), *s_kept = s_src + a.rows, *s_tail = s_kept + a.rows;
 	const int64_t cap = (int64_t)a.table_ld << a.lp;
 	if (tid == 0) {
 		s_bad = a.rows;
 		s_most = 0;
 	}
 	for (int i = tid; i < 3 * words; i += kPlanBlock) lds[i] = 0;
+	for (int i = tid; i < kLowSlots; i += kPlanBlock) s_low[i] = a.rows;
 	__syncthreads();
 	for (int r = tid; r < a.rows; r += kPlanBlock) {
 		const int s = a.source[r];
@@ -85,26 +90,38 @@ __global__ __launch_bounds__(kPlanBlock) void k_update_plan(PageUpdateArgs a, co
 		const int kept = ok ? (int)pages_for(keep, a.lp) : 0;
 		const bool writes = ok && (keep & (((int64_t)1 << a.lp) - 1)) && room > keep;
 		s_src[r] = s;
-		s_kept[r] = kept | (writes ? 1 << 30 : 0);
-		atomicMax(&s_most, kept);
+		s_kept[r] = kept | (writes ? kWrites : 0);
+		if (kept) atomicMax(&s_most, kept);
 	}
 	if (a.held)
 		for (int p = tid; p < a.pages; p += kPlanBlock)
 			if (a.held[p]) atomicOr(&fixed[p >> 5], 1u << (p & 31));
 	__syncthreads();
-	const int most = s_most;
-	const int64_t cells = (int64_t)a.rows * most;
-	for (int64_t c = tid; c < cells; c += kPlanBlock) {
-		const int r = (int)(c / most), i = (int)(c - (int64_t)r * most), k = s_kept[r] & ~(1 << 30);
-		if (i >= k) continue;
-		const int p = tables[(int64_t)s_src[r] * a.table_ld + i];
-		if (p < 0 || p >= a.pages) {
-			atomicMin(&s_bad, r);
-			continue;
+	const uint32_t most = s_most;
+	const uint64_t cells = (uint64_t)a.rows * most;
+	for (uint64_t c0 = tid; c0 < cells; c0 += 4 * kPlanBlock) {
+		int r[4], i[4], p[4];
+#pragma unroll
+		for (int u = 0; u < 4; ++u) {
+			const uint64_t c = c0 + u * kPlanBlock;
+			r[u] = cells >> 32 ? (int)(c / most) : (int)((uint32_t)c / most);
+			i[u] = (int)(c - (uint64_t)r[u] * most);
+			const bool in = c < cells && i[u] < (s_kept[min(r[u], a.rows - 1)] & ~kWrites);
+			p[u] = in ? tables[(int64_t)s_src[r[u]] * a.table_ld + i[u]] : 0;
+			r[u] = in ? r[u] : -1;
 		}
-		const uint32_t bit = 1u << (p & 31);
-		if (atomicOr(&seen[p >> 5], bit) & bit) atomicOr(&multi[p >> 5], bit);
-		if (!(s_kept[r] >> 30) || i < k - 1) atomicOr(&fixed[p >> 5], bit);
+#pragma unroll
+		for (int u = 0; u < 4; ++u) {
+			if (r[u] < 0) continue;
+			if (p[u] < 0 || p[u] >= a.pages) {
+				atomicMin(&s_bad, r[u]);
+				continue;
+			}
+			const uint32_t bit = 1u << (p[u] & 31);
+			if (atomicOr(&seen[p[u] >> 5], bit) & bit) atomicOr(&multi[p[u] >> 5], bit);
+			if (i[u] == (s_kept[r[u]] ^ kWrites) - 1) s_tail[r[u]] = p[u];
+			else atomicOr(&fixed[p[u] >> 5], bit);
+		}
 	}
 	__syncthreads();
 	if (s_bad < a.rows) {
@@ -117,41 +134,45 @@ __global__ __launch_bounds__(kPlanBlock) void k_update_plan(PageUpdateArgs a, co
 		return;
 	}
 	// pages that only rows which write into them hold stay with the lowest of these
-	auto tail_of = [&](int r) { return tables[(int64_t)s_src[r] * a.table_ld + (s_kept[r] & ~(1 << 30)) - 1]; };
+	auto slot = [](int p) { return (int)((uint32_t)p * 2654435761u >> 21); };
+	auto contested = [&](int r) {
+		const int p = s_tail[r];
+		const uint32_t bit = 1u << (p & 31);
+		return (multi[p >> 5] & bit) && !(fixed[p >> 5] & bit);
+	};
 	for (int r = tid; r < a.rows; r += kPlanBlock)
-		if (s_kept[r] >> 30) __hip_atomic_store(&w.low[tail_of(r)], a.rows, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-	__threadfence();
+		if ((s_kept[r] & kWrites) && contested(r)) atomicMin(&s_low[slot(s_tail[r])], r);
 	__syncthreads();
-	for (int r = tid; r < a.rows; r += kPlanBlock)
-		if (s_kept[r] >> 30) atomicMin(&w.low[tail_of(r)], r);
-	__threadfence();
-	__syncthreads();
-	int wants = 0, copies = 0;
+	int64_t wants = 0, copies = 0;
 	for (int r0 = 0; r0 < a.rows; r0 += kPlanBlock) {
 		const int r = r0 + tid;
-		int n = 0, t = -1;
+		int64_t n = 0;
+		int t = -1;
 		if (r < a.rows) {
-			if (s_kept[r] >> 30) {
-				const int p = tail_of(r);
-				const uint32_t bit = 1u << (p & 31);
-				if ((fixed[p >> 5] & bit) || ((multi[p >> 5] & bit) && __hip_atomic_load(&w.low[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < r)) t = p;
+			if (s_kept[r] & kWrites) {
+				const int p = s_tail[r];
+				bool copy = fixed[p >> 5] >> (p & 31) & 1;
+				if (contested(r)) {
+					const int low = s_low[slot(p)];
+					copy = low != r && s_tail[low] == p;
+					for (int q = low; low != r && !copy && q < r; ++q) copy = (s_kept[q] & kWrites) && s_tail[q] == p;  // another page's slot
+				}
+				if (copy) t = p;
 			}
-			n = (int)pages_for(a.room[r], a.lp) - (s_kept[r] & ~(1 << 30)) + (t >= 0);
+			n = pages_for(a.room[r], a.lp) - (s_kept[r] & ~kWrites) + (t >= 0);
 		}
-		int all;
-		const int before = block_before(n, &all, s_scan) + wants;
-		int those;
-		const int mine = block_before(t >= 0, &those, s_scan) + copies;
+		int64_t all;  // pages below 2^40, copies above
+		const int64_t before = block_before<int64_t>(n + ((int64_t)(t >= 0) << 40), &all, s_scan), mine = (before >> 40) + copies;
 		if (r < a.rows) {
-			w.off[r] = before;
+			w.off[r] = (int)min((before & (((int64_t)1 << 40) - 1)) + wants, (int64_t)INT32_MAX);
 			w.tail[r] = t;
 			if (t >= 0) {
 				w.from[mine] = t;
-				w.to[mine] = before;  // its place among the free pages
+				w.to[mine] = w.off[r];  // its place among the free pages
 			}
 		}
-		wants += all;
-		copies += those;
+		wants += all & (((int64_t)1 << 40) - 1);
+		copies += all >> 40;
 	}
 	// free pages: neither seen nor held; a thread's are those of neighbouring words
 	const int per = (words + kPlanBlock - 1) / kPlanBlock;
@@ -159,20 +180,20 @@ __global__ __launch_bounds__(kPlanBlock) void k_update_plan(PageUpdateArgs a, co
 		const uint32_t valid = a.pages - 32 * i >= 32 ? ~0u : (1u << (a.pages - 32 * i)) - 1;
 		return ~(seen[i] | fixed[i]) & valid;
 	};
-	int mine = 0, total;
+	int64_t mine = 0, total;
 	for (int i = tid * per; i < min(words, (tid + 1) * per); ++i) mine += __popc(free_bits(i));
-	int at = block_before(mine, &total, s_scan);
+	int64_t at = block_before<int64_t>(mine, &total, s_scan);
 	const bool ok = wants <= total;
 	if (ok)
 		for (int i = tid * per; i < min(words, (tid + 1) * per) && at < wants; ++i)
 			for (uint32_t b = free_bits(i); b && at < wants; b &= b - 1) w.free[at++] = 32 * i + __builtin_ctz(b);
 	if (tid == 0) {
 		a.result[0] = ok ? SSLM_OK : SSLM_KV_POOL_EXHAUSTED;
-		a.result[1] = total - wants;
-		a.result[2] = ok ? copies : 0;
+		a.result[1] = (int32_t)i64max(total - wants, INT32_MIN);
+		a.result[2] = ok ? (int32_t)copies : 0;
 		a.result[3] = -1;
 		w.state[0] = ok;
-		w.state[1] = ok ? copies : 0;
+		w.state[1] = ok ? (int32_t)copies : 0;
 	}
 }
 
@@ -221,10 +242,11 @@ __global__ __launch_bounds__(256) void k_update_apply(PageUpdateArgs a, const in
 // the holes before it and the movers after it, both in ascending order.
 __global__ __launch_bounds__(kPlanBlock) void k_compact_plan(PageCompactArgs a, PlanWork w) {
 	extern __shared__ uint32_t lds[];
-	__shared__ int s_scan[kPlanBlock / 64], s_bad, s_most, s_edge, s_top;
+	__shared__ int64_t s_scan[kPlanBlock / 64];
+	__shared__ int s_bad, s_most, s_edge, s_top;
 	const int tid = threadIdx.x, words = (a.pages + 31) / 32;
 	uint32_t *live = lds, *held = live + words;
-	int32_t* rank = (int32_t*)(held + words);
+	int32_t *rank = (int32_t*)(held + words), *s_len = rank + words;  // s_len: a row's pages
 	const int64_t cap = (int64_t)a.table_ld << a.lp;
 	if (tid == 0) {
 		s_bad = a.rows;
@@ -238,20 +260,32 @@ __global__ __launch_bounds__(kPlanBlock) void k_compact_plan(PageCompactArgs a, 
 		const int64_t len = a.lengths[r];
 		const bool ok = len >= 0 && len <= cap;
 		if (!ok) atomicMin(&s_bad, r);
-		else atomicMax(&s_most, (int)pages_for(len, a.lp));
+		s_len[r] = ok ? (int)pages_for(len, a.lp) : 0;
+		if (ok && len) atomicMax(&s_most, s_len[r]);
 	}
 	if (a.held)
 		for (int p = tid; p < a.pages; p += kPlanBlock)
 			if (a.held[p]) atomicOr(&held[p >> 5], 1u << (p & 31));
 	__syncthreads();
-	const int most = s_most;
-	const int64_t cells = s_bad < a.rows ? 0 : (int64_t)a.rows * most;
-	for (int64_t c = tid; c < cells; c += kPlanBlock) {
-		const int r = (int)(c / most), i = (int)(c - (int64_t)r * most);
-		if (i >= pages_for(a.lengths[r], a.lp)) continue;
-		const int p = a.tables[(int64_t)r * a.table_ld + i];
-		if (p < 0 || p >= a.pages) atomicMin(&s_bad, r);
-		else atomicOr(&live[p >> 5], 1u << (p & 31));
+	const uint32_t most = s_most;
+	const uint64_t cells = s_bad < a.rows ? 0 : (uint64_t)a.rows * most;
+	for (uint64_t c0 = tid; c0 < cells; c0 += 4 * kPlanBlock) {
+		int r[4], p[4];
+#pragma unroll
+		for (int u = 0; u < 4; ++u) {
+			const uint64_t c = c0 + u * kPlanBlock;
+			r[u] = cells >> 32 ? (int)(c / most) : (int)((uint32_t)c / most);
+			const int i = (int)(c - (uint64_t)r[u] * most);
+			const bool in = c < cells && i < s_len[min(r[u], a.rows - 1)];
+			p[u] = in ? a.tables[(int64_t)r[u] * a.table_ld + i] : 0;
+			r[u] = in ? r[u] : -1;
+		}
+#pragma unroll
+		for (int u = 0; u < 4; ++u) {
+			if (r[u] < 0) continue;
+			if (p[u] < 0 || p[u] >= a.pages) atomicMin(&s_bad, r[u]);
+			else atomicOr(&live[p[u] >> 5], 1u << (p[u] & 31));
+		}
 	}
 	__syncthreads();
 	if (s_bad < a.rows) {
@@ -265,12 +299,11 @@ __global__ __launch_bounds__(kPlanBlock) void k_compact_plan(PageCompactArgs a, 
 	}
 	const int per = (words + kPlanBlock - 1) / kPlanBlock, w0 = tid * per, w1 = min(words, w0 + per);
 	auto valid = [&](int i) { return a.pages - 32 * i >= 32 ? ~0u : (1u << (a.pages - 32 * i)) - 1; };
-	int mine = 0, movable, open;
-	for (int i = w0; i < w1; ++i) mine += __popc(live[i] & ~held[i]);
-	block_before(mine, &movable, s_scan);
-	mine = 0;
-	for (int i = w0; i < w1; ++i) mine += __popc(~held[i] & valid(i));
-	int at = block_before(mine, &open, s_scan);
+	int at;
+	int64_t both = 0, all;  // movable pages above 2^32, those that nobody holds below
+	for (int i = w0; i < w1; ++i) both += (int64_t)__popc(live[i] & ~held[i]) << 32 | __popc(~held[i] & valid(i));
+	at = (int)block_before<int64_t>(both, &all, s_scan);
+	const int movable = (int)(all >> 32);
 	for (int i = w0; i < w1; ++i) {  // the boundary: one past the last of the first `movable` pages that nobody holds
 		const uint32_t b = ~held[i] & valid(i);
 		const int n = __popc(b);
@@ -287,15 +320,14 @@ __global__ __launch_bounds__(kPlanBlock) void k_compact_plan(PageCompactArgs a, 
 	auto below = [&](int i) { return 32 * i + 32 <= edge ? ~0u : (32 * i >= edge ? 0u : (1u << (edge - 32 * i)) - 1); };
 	auto holes = [&](int i) { return ~live[i] & ~held[i] & below(i) & valid(i); };
 	auto movers = [&](int i) { return live[i] & ~held[i] & ~below(i); };
-	mine = 0;
-	int nholes = 0, n2;
-	for (int i = w0; i < w1; ++i) mine += __popc(holes(i));
-	at = block_before(mine, &nholes, s_scan);
+	both = 0;
+	for (int i = w0; i < w1; ++i) both += (int64_t)__popc(movers(i)) << 32 | __popc(holes(i));
+	both = block_before<int64_t>(both, &all, s_scan);
+	const int n2 = (int)(all >> 32);  // as many as there are holes
+	at = (int)both;
 	for (int i = w0; i < w1; ++i)
 		for (uint32_t b = holes(i); b; b &= b - 1) w.free[at++] = 32 * i + __builtin_ctz(b);
-	mine = 0;
-	for (int i = w0; i < w1; ++i) mine += __popc(movers(i));
-	at = block_before(mine, &n2, s_scan);
+	at = (int)(both >> 32);
 	for (int i = w0; i < w1; ++i) {
 		rank[i] = at;
 		for (uint32_t b = movers(i); b; b &= b - 1) w.from[at++] = 32 * i + __builtin_ctz(b);
@@ -312,7 +344,8 @@ __global__ __launch_bounds__(kPlanBlock) void k_compact_plan(PageCompactArgs a, 
 		if (to >= 0) top = max(top, to + 1);
 		if (held[i] & bit) top = max(top, p + 1);
 	}
-	atomicMax(&s_top, top);
+	for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
+	if ((tid & 63) == 0) atomicMax(&s_top, top);
 	__syncthreads();
 	if (tid == 0) {
 		a.result[0] = SSLM_OK;
@@ -486,9 +519,45 @@ __device__ __forceinline__ int land_units(int32_t& x, int64_t m, int64_t r_t, in
 	return y > (double)kMaxUnits;
 }
 
+// octet g of a token's query head, turned
+__device__ __forceinline__ void q_octet(const CacheStoreArgs& a, int t, int h, int g, bool turns, const Turn& turn) {
+	Octet o = octet_load(a, a.q + (int64_t)t * a.q_ld + h * a.pg.D, g);
+	if (turns) octet_turn(o, turn, 127);
+	octet_store(a, a.q_out + ((int64_t)t * a.NH + h) * a.pg.D, g, o);
+}
+// octet g of token t's K or V in units, turned; the values clamped
+__device__ __forceinline__ int land_octet(const CacheStoreArgs& a, bool isv, int kvh, int t, int64_t pos, int g, const Scale& sc, int64_t rt, int64_t et, Octet* out) {
+	Octet o = octet_load(a, (isv ? a.v + t * a.v_ld : a.k + t * a.k_ld) + kvh * a.pg.D, g);
+	const int64_t k = composed_exponent(sc.e, et);
+	const double f = landing_scale(sc.m, rt, k).f;
+	int over = 0;
+#pragma unroll
+	for (int j = 0; j < 8; ++j) over += land_units(o.x[j], sc.m, rt, k, f);
+	if (!isv && 8 * g < a.rope_dim) over += octet_turn(o, turn_at(a, pos, g), kMaxUnits);
+	*out = o;
+	return over;
+}
+// a KV head's largest magnitude over the lanes of its octets
+template <int GP>
+__device__ __forceinline__ int32_t octets_max(const Octet& o) {
+	int32_t mx = 0;
+#pragma unroll
+	for (int j = 0; j < 8; ++j) mx = max(mx, abs(o.x[j]));
+	for (int d = 1; d < GP; d *= 2) mx = max(mx, __shfl_xor(mx, d, 64));
+	return mx;
+}
+// eight old codes of a page that grows from exponent `init` through `levels`
+__device__ __forceinline__ void regrow(int8_t* at, int init, uint32_t levels) {
+	const uint64_t w = ((const unaligned8*)at)->v;
+	uint64_t out = 0;
+#pragma unroll
+	for (int j = 0; j < 8; ++j) out |= (uint64_t)(uint8_t)grown_code((int8_t)(w >> 8 * j), 0, levels >> init & ~1u) << 8 * j;
+	((unaligned8*)at)->v = out;
+}
+
 // K or V of one KV head (z) in one page (x) of one row (y): the page's tokens land in LDS, their exponents run up the
-// page, then the codes are written; blocks past the last page take q's tokens, four each, and an equal share of the heads.
-constexpr int kStoreBlock = 256;
+// page, then the codes are written; the waves of blocks past the last page take q's tokens, one each.
+constexpr int kStoreBlock = 512;
 template <int D>
 __global__ __launch_bounds__(kStoreBlock) void k_store_span(CacheStoreArgs a, int pages) {
 	extern __shared__ __attribute__((aligned(16))) int16_t s_x[];  // [page's tokens][D], groups of eight in octet order
@@ -501,17 +570,13 @@ __global__ __launch_bounds__(kStoreBlock) void k_store_span(CacheStoreArgs a, in
 	const int t0 = a.row_tokens[r], n = a.row_tokens[r + 1] - t0;
 	const int64_t start = a.row_start[r];
 	if ((int)blockIdx.x >= pages) {
-		const int i = ((int)blockIdx.x - pages) * (kStoreBlock / 64) + (tid >> 6);
+		const int i = (((int)blockIdx.x - pages) * (int)gridDim.z + z) * (kStoreBlock / 64) + (tid >> 6);
 		if (i >= n) return;
 		const int g = tid % GP;
 		const bool turns = 8 * g < a.rope_dim;
 		Turn t;
 		if (turns) t = turn_at(a, start + i, g);
-		for (int h = z + (int)gridDim.z * ((tid & 63) / GP); h < a.NH; h += (int)gridDim.z * (64 / GP)) {
-			Octet o = octet_load(a, a.q + (int64_t)(t0 + i) * a.q_ld + h * D, g);
-			if (turns) octet_turn(o, t, 127);
-			octet_store(a, a.q_out + ((int64_t)(t0 + i) * a.NH + h) * D, g, o);
-		}
+		for (int h = (tid & 63) / GP; h < a.NH; h += 64 / GP) q_octet(a, t0 + i, h, g, turns, t);
 		return;
 	}
 	const int P = 1 << a.pg.lp;
@@ -534,27 +599,15 @@ __global__ __launch_bounds__(kStoreBlock) void k_store_span(CacheStoreArgs a, in
 	for (int u = tid; u < (cnt * GP + kStoreBlock - 1) / kStoreBlock * kStoreBlock; u += kStoreBlock) {
 		const bool in = u < cnt * GP;
 		const int i = in ? u / GP : 0, g = u % GP, t = t0 + i0 + i;
-		const Scale sc = isv ? a.v_scale[t] : a.k_scale[t];
-		const int8_t* from = isv ? a.v + t * a.v_ld : a.k + t * a.k_ld;
-		Octet o = octet_load(a, from + kvh * D, g);
-		const int64_t k = composed_exponent(sc.e, et);
-		const double f = landing_scale(sc.m, rt, k).f;
-		int32_t mx = 0, over = 0;
-#pragma unroll
-		for (int j = 0; j < 8; ++j) {
-			over += land_units(o.x[j], sc.m, rt, k, f);
-		}
-		if (!isv && 8 * g < a.rope_dim) over += octet_turn(o, turn_at(a, start + i0 + i, g), kMaxUnits);
+		Octet o;
+		const int over = land_octet(a, isv, kvh, t, start + i0 + i, g, isv ? a.v_scale[t] : a.k_scale[t], rt, et, &o);
+		const int32_t mx = octets_max<GP>(o);
 		union {
 			int16_t h[8];
 			v4i v;
 		} pk;
 #pragma unroll
-		for (int j = 0; j < 8; ++j) {
-			mx = max(mx, abs(o.x[j]));
-			pk.h[j] = (int16_t)o.x[j];
-		}
-		for (int d = 1; d < GP; d *= 2) mx = max(mx, __shfl_xor(mx, d, 64));
+		for (int j = 0; j < 8; ++j) pk.h[j] = (int16_t)o.x[j];
 		if (in) {
 			*(v4i*)(s_x + (int64_t)u * 8) = pk.v;
 			if (g == 0) s_need[i] = (uint8_t)exponent_for(mx);
@@ -603,21 +656,80 @@ __global__ __launch_bounds__(kStoreBlock) void k_store_span(CacheStoreArgs a, in
 	}
 	const int init = s_init;
 	if (slot0 && levels >> (init + 1)) {
-		for (int u = tid; u < slot0 * GP; u += kStoreBlock) {
-			int8_t* at = head + (int64_t)u * 8;
-			uint64_t w = ((const unaligned8*)at)->v, out = 0;
-#pragma unroll
-			for (int j = 0; j < 8; ++j) {
-				int32_t x = (int8_t)(w >> 8 * j);
-				x = grown_code(x, 0, levels >> init & ~1u);
-				out |= (uint64_t)(uint8_t)x << 8 * j;
-			}
-			((unaligned8*)at)->v = out;
-		}
+		for (int u = tid; u < slot0 * GP; u += kStoreBlock) regrow(head + (int64_t)u * 8, init, levels);
 	}
 	if (tid == 0) {
 		*exp = (uint8_t)(31 - __builtin_clz(levels));
 		if (s_clamped) atomicAdd(&a.clamped[r], s_clamped);
+	}
+}
+
+// Single tokens in one launch, a block per row: K's and V's octets, then q's.  The lanes of a head's octets find its
+// exponent; a page that grows is rounded by the whole block once all heads are known.
+template <int D>
+__global__ __launch_bounds__(kStoreBlock) void k_store_token(CacheStoreArgs a) {
+	__shared__ uint16_t s_grow[2 * 256];  // of each KV head's K and V: the exponents before and after
+	__shared__ int s_clamped;
+	constexpr int GP = D / 8;
+	const int r = blockIdx.x, tid = threadIdx.x, kv = 2 * a.pg.NKV * GP, total = kv + (a.q ? a.NH * GP : 0);
+	int64_t cap = (int64_t)a.pg.table_ld << a.pg.lp;
+	if (a.rope_dim) cap = i64min(cap, a.rope_rows);
+	const CacheRow c = cache_row(a.row_tokens, a.row_start, r, a.tokens, a.max_new, cap);
+	int st = c.ok ? kOk : kPositionOverCap;
+	int32_t entry = 0;
+	if (c.ok && c.n > 0) {
+		entry = a.pg.tables[(int64_t)r * a.pg.table_ld + (c.start >> a.pg.lp)];
+		const bool scales = fits_i32(a.k_scale[c.t0].m) && fits_i32(a.v_scale[c.t0].m);
+		st = entry < 0 || entry >= a.pg.pages ? kPositionOverCap : (scales ? kOk : kCarriedScaleMantissaOutOfDomain);
+	}
+	if (tid == 0) {
+		s_clamped = 0;
+		a.status[r] = st;
+	}
+	__syncthreads();
+	if (st != kOk || c.n == 0) {
+		if (tid == 0) a.clamped[r] = 0;
+		return;
+	}
+	const int slot = (int)(c.start & ((1 << a.pg.lp) - 1)), g = tid % GP;
+	int8_t* page = a.pg.pool + entry * a.pg.page_bytes;
+	const bool turns = 8 * g < a.rope_dim;
+	Turn turn;
+	if (turns) turn = turn_at(a, c.start, g);
+	auto head = [&](int z) { return page + (z & 1 ? a.pg.v_off : a.pg.k_off) + ((int64_t)(z >> 1) << a.pg.lp) * D; };
+	int clamped = 0;
+	for (int u0 = tid - tid % 64; u0 < total; u0 += kStoreBlock) {  // whole waves
+		const int u = u0 + tid % 64;
+		if (u0 < kv) {
+			const bool in = u < kv;
+			const int z = in ? u / GP : 0, kvh = z >> 1;
+			const bool isv = z & 1;
+			Octet o;
+			const int over = land_octet(a, isv, kvh, c.t0, c.start, g, isv ? a.v_scale[c.t0] : a.k_scale[c.t0], isv ? a.r_t_v[kvh] : a.r_t_k[kvh],
+			                            isv ? a.e_t_v[kvh] : a.e_t_k[kvh], &o);
+			const int need = exponent_for(octets_max<GP>(o));
+			if (in) {
+				uint8_t* exp = (uint8_t*)page + a.pg.e_off + (isv ? a.pg.NKV : 0) + kvh;
+				const int was = slot ? min((int)*exp, kMaxShift) : 0, now = max(was, need);
+				clamped += over;
+				if (g == 0) {
+					*exp = (uint8_t)now;
+					s_grow[z] = (uint16_t)(was | now << 8);
+				}
+#pragma unroll
+				for (int j = 0; j < 8; ++j) o.x[j] = rdbpot32(o.x[j], now);
+				octet_store(a, head(z) + (int64_t)slot * D, g, o);
+			}
+		}
+		if (u >= kv && u < total) q_octet(a, c.t0, (u - kv) / GP, g, turns, turn);
+	}
+	if (clamped) atomicAdd(&s_clamped, clamped);
+	__syncthreads();
+	if (tid == 0) a.clamped[r] = s_clamped;
+	for (int z = 0; slot && z < 2 * a.pg.NKV; ++z) {
+		const int was = s_grow[z] & 255, now = s_grow[z] >> 8;
+		if (now == was) continue;
+		for (int u = tid; u < slot * GP; u += kStoreBlock) regrow(head(z) + (int64_t)u * 8, was, 1u << now);
 	}
 }
 
@@ -1702,7 +1814,6 @@ static size_t plan_work(int rows, int pages, int table_ld, char* base, PlanWork*
 	w->state = take(2);
 	w->off = take(rows);
 	w->tail = take(rows);
-	w->low = take(pages);
 	w->free = take(pages);
 	w->from = take(std::max(rows, pages));
 	w->to = take(rows);
@@ -1721,7 +1832,7 @@ size_t page_compact_workspace(int rows, int pages, int table_ld) {
 
 template <typename K>
 static void allow_lds(K kernel, size_t bytes) {
-	if (bytes > 65536 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess)
+	if (bytes > 32768 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess)
 		throw LaunchRefused{"dynamic LDS"};
 }
 
@@ -1740,7 +1851,7 @@ void page_update(const PageUpdateArgs& a, hipStream_t s) {
 		hipLaunchKernelGGL(k_table_copy, dim3((int)std::min<int64_t>(1024, (cells + 255) / 256)), dim3(256), 0, s, a.tables, w.old, cells);
 		tables = w.old;
 	}
-	const size_t lds = 3 * (size_t)((a.pages + 31) / 32) * 4 + (size_t)a.rows * 8;
+	const size_t lds = 3 * (size_t)((a.pages + 31) / 32) * 4 + (size_t)a.rows * 12;
 	allow_lds(k_update_plan, lds);
 	hipLaunchKernelGGL(k_update_plan, dim3(1), dim3(kPlanBlock), lds, s, a, tables, w);
 	hipLaunchKernelGGL(k_update_apply, dim3(apply_blocks(cells, a.rows, a.page_bytes)), dim3(256), 0, s, a, tables, w);
@@ -1749,7 +1860,7 @@ void page_update(const PageUpdateArgs& a, hipStream_t s) {
 void page_compact(const PageCompactArgs& a, hipStream_t s) {
 	PlanWork w;
 	plan_work(a.rows, a.pages, a.table_ld, (char*)a.ws, &w);
-	const size_t lds = 3 * (size_t)((a.pages + 31) / 32) * 4;
+	const size_t lds = 3 * (size_t)((a.pages + 31) / 32) * 4 + (size_t)a.rows * 4;
 	allow_lds(k_compact_plan, lds);
 	hipLaunchKernelGGL(k_compact_plan, dim3(1), dim3(kPlanBlock), lds, s, a, w);
 	hipLaunchKernelGGL(k_compact_apply, dim3(apply_blocks((int64_t)a.rows * a.table_ld, a.pages, a.page_bytes)), dim3(256), 0, s, a, w);
@@ -1757,8 +1868,12 @@ void page_compact(const PageCompactArgs& a, hipStream_t s) {
 
 template <int D>
 static void store_launch(const CacheStoreArgs& a, hipStream_t s) {
+	if (a.max_new == 1) {
+		hipLaunchKernelGGL(k_store_token<D>, dim3(a.rows), dim3(kStoreBlock), 0, s, a);
+		return;
+	}
 	const int P = 1 << a.pg.lp, pages = (a.max_new + P - 2) / P + 1;
-	const int qs = a.q ? (a.max_new + kStoreBlock / 64 - 1) / (kStoreBlock / 64) : 0;
+	const int qs = a.q ? (a.max_new + kStoreBlock / 64 * 2 * a.pg.NKV - 1) / (kStoreBlock / 64 * 2 * a.pg.NKV) : 0;
 	const size_t lds = (size_t)std::min(P, a.max_new) * D * 2;
 	allow_lds(k_store_span<D>, lds);
 	hipLaunchKernelGGL(k_store_check, dim3(a.rows), dim3(256), 0, s, a);

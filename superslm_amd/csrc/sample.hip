@@ -1,6 +1,8 @@
 // The next token by sampling (cache_ops.h): kernels, launches and the C entry.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "../../include/sslm_hip.h"
 #include "attention_util.h"
 #include "cache_ops.h"
@@ -26,7 +28,7 @@ __device__ __forceinline__ bool sampling_ok(const Sampling& s, int vocab) {
 // for a d of up to 2^32, and nothing from 30 q_ln2 on.
 struct Weight {
 	double ninv, half, l, b, c;
-	int64_t lim;
+	uint32_t lim;  // below 2^30
 };
 __device__ __forceinline__ Weight weight_of(const Sampling& s) {
 	Weight w;
@@ -35,12 +37,12 @@ __device__ __forceinline__ Weight weight_of(const Sampling& s) {
 	w.half = 0.5 * w.ninv;
 	w.b = (double)s.q_b;
 	w.c = (double)s.q_c;
-	w.lim = 30 * s.q_ln2;
+	w.lim = (uint32_t)(30 * s.q_ln2);
 	return w;
 }
 __device__ __forceinline__ double weight_d(const Weight& w, uint32_t d) {
 	const double x = (double)d, z = floor(fma(x, w.ninv, w.half)), base = fma(z, w.l, w.b - x);
-	return (int64_t)d >= w.lim ? 0.0 : floor(ldexp(fma(base, base, w.c), -(int)z));
+	return d >= w.lim ? 0.0 : floor(ldexp(fma(base, base, w.c), -(int)z));
 }
 __device__ __forceinline__ uint64_t weight(const Weight& w, uint32_t d) { return (uint64_t)weight_d(w, d); }
 
@@ -364,40 +366,49 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_gather(SampleArgs a, Sa
 	const SamplePlan& p = w.plan[r];
 	if (p.state != 0) return;
 	const int32_t top = p.top, sh = p.sh, rb = top >> sh;
-	const uint32_t a0 = p.a[0], a1 = p.a[1], a2 = p.a[2], b0 = p.b[0], b1 = p.b[1], b2 = p.b[2];
+	const uint32_t a0 = p.a[0], a2 = p.a[2], b0 = p.b[0], b2 = p.b[2];
+	const uint32_t a1 = s.top_p < 65536 ? p.a[1] : 0, b1 = s.top_p < 65536 ? p.b[1] : 0;
 	// the sums that the borders need: weights before ranges 0, 1 and 2, kept ones (where min-p makes them others) before 0 or 1, and 2
 	const bool by_p = s.top_p < 65536, min_p = s.min_p > 0;
-	const uint32_t first = by_p ? a1 : a0, most = by_p ? max(a0, max(a1, a2)) : max(a0, a2);
+	const uint32_t first = by_p ? a1 : a0, most = max(a0, max(by_p ? a1 : 0, a2));
 	if (tid < 5) s_sum[tid] = 0;
 	if (tid == 0) s_n = 0;
 	__syncthreads();
 	const Weight wt = weight_of(s);
 	const double least = (double)share_of((uint64_t)(s.q_b * s.q_b + s.q_c), s.min_p);
-	double acc[5] = {};  // 16 values of 2^47
+	double acc0 = 0.0, acc1 = 0.0, acc2 = 0.0, acc3 = 0.0, acc4 = 0.0;  // 16 values of 2^47
+	const uint32_t n0 = b0 - a0, n1 = b1 - a1, n2 = b2 - a2;
+	auto run = [&](auto with_min_p) {
 #pragma unroll
-	for (int u = 0; u < kSampleLoads; ++u)
+		for (int u = 0; u < kSampleLoads; ++u)
 #pragma unroll
-		for (int i = 0; i < 4; ++i) {
-			const uint32_t j = sl.has(u, i) ? (uint32_t)rb - (uint32_t)(sl.x[u][i] >> sh) : ~0u;
-			if (__any(j < most)) {
-				const double x = weight_d(wt, (uint32_t)top - (uint32_t)sl.x[u][i]);
-				acc[0] += only(j < a0, x);
-				if (by_p) acc[1] += only(j < a1, x);
-				if (!min_p) acc[2] += only(j < a2, x);
-				else {
-					acc[3] += only(j < first && x >= least, x);
-					acc[4] += only(j < a2 && x >= least, x);
+			for (int i = 0; i < 4; ++i) {
+				const uint32_t j = sl.has(u, i) ? (uint32_t)rb - (uint32_t)(sl.x[u][i] >> sh) : ~0u;
+				const uint32_t d = (uint32_t)top - (uint32_t)sl.x[u][i];
+				if (__any(j < most)) {
+					const double x = weight_d(wt, d);
+					acc0 += only(j < a0, x);
+					acc1 += only(j < a1, x);
+					if constexpr (!decltype(with_min_p)::value) acc2 += only(j < a2, x);
+					else {
+						const bool kept = x >= least;
+						acc3 += only((j < first) & kept, x);
+						acc4 += only((j < a2) & kept, x);
+					}
+				}
+				const bool in = (j - a0 < n0) | (j - a1 < n1) | (j - a2 < n2);
+				const uint64_t who = __ballot(in);
+				if (who) {
+					uint32_t at = 0;
+					if (lane == __builtin_ctzll(who)) at = atomicAdd(&s_n, (uint32_t)__popcll(who));
+					at = __builtin_amdgcn_readlane(at, __builtin_ctzll(who)) + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+					if (in && at < kSliceList) s_list[at] = uint2{d, (uint32_t)sl.index(u, i)};
 				}
 			}
-			const bool in = j - a0 < b0 - a0 || j - a1 < b1 - a1 || j - a2 < b2 - a2;
-			const uint64_t who = __ballot(in);
-			if (who) {
-				uint32_t at = 0;
-				if (lane == __builtin_ctzll(who)) at = atomicAdd(&s_n, (uint32_t)__popcll(who));
-				at = __builtin_amdgcn_readlane(at, __builtin_ctzll(who)) + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-				if (in && at < kSliceList) s_list[at] = uint2{(uint32_t)top - (uint32_t)sl.x[u][i], (uint32_t)sl.index(u, i)};
-			}
-		}
+	};
+	if (min_p) run(std::true_type{});
+	else run(std::false_type{});
+	const double acc[5] = {acc0, acc1, acc2, acc3, acc4};
 #pragma unroll
 	for (int k = 0; k < 5; ++k) {
 		if (!__any(acc[k] != 0.0)) continue;
@@ -636,7 +647,7 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_pick(SampleArgs a, Samp
 		if (in_lds) {
 			for (int i = tid; i < a.vocab; i += kSampleBlock) {
 				const uint32_t d = (uint32_t)top - (uint32_t)row[i];
-				s_d[i] = legal(i) && (int64_t)d < wt.lim ? d : kNone;
+				s_d[i] = legal(i) && d < wt.lim ? d : kNone;
 			}
 			__syncthreads();
 		}
@@ -645,7 +656,7 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_pick(SampleArgs a, Samp
 		auto fetch = [&](int i) {
 			if (in_lds) return s_d[i];
 			const uint32_t d = (uint32_t)top - (uint32_t)row[i];
-			return legal(i) && (int64_t)d < wt.lim ? d : kNone;
+			return legal(i) && d < wt.lim ? d : kNone;
 		};
 		auto index = [&](int i) { return (uint32_t)i; };
 		auto admit = [&](uint32_t d, uint32_t i) { return d < dcut || (d == dcut && i <= icut); };
