@@ -223,22 +223,31 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, Samp
 		p.sh = bucket_shift(s);
 		const int rb = p.top >> p.sh;
 		const uint32_t j0 = kPlanBuckets * tid;
-		// a wave to a slice, sixteen bytes of its counts to a lane
-		for (int i = tid >> 6; i < slices; i += kPlanThreads / 64) {
-			const size_t at = (size_t)r * slices + i;
-			const int64_t m = w.smax[at];
-			v4i x[kBuckets / 512];
+		// a wave to a slice, sixteen bytes of its counts to a lane, four slices on their way
+		constexpr int kWaves = kPlanThreads / 64, kAhead = 4;
+		for (int i0 = tid >> 6; i0 < slices; i0 += kAhead * kWaves) {
+			int64_t m[kAhead];
+			v4i x[kAhead][kBuckets / 512];
 #pragma unroll
-			for (int k = 0; k < kBuckets / 512; ++k) x[k] = *(const v4i*)(w.hist + at * kBuckets + 8 * ((tid & 63) + 64 * k));
-			if (m == kNoLogit) continue;
-			const uint32_t off = (uint32_t)rb - (uint32_t)((int32_t)m >> p.sh);  // the slice's first bucket
+			for (int q = 0; q < kAhead; ++q) {
+				const size_t at = (size_t)r * slices + min(i0 + q * kWaves, slices - 1);
+				m[q] = w.smax[at];
 #pragma unroll
-			for (int k = 0; k < kBuckets / 512; ++k)
+				for (int k = 0; k < kBuckets / 512; ++k) x[q][k] = *(const v4i*)(w.hist + at * kBuckets + 8 * ((tid & 63) + 64 * k));
+			}
 #pragma unroll
-				for (int e = 0; e < 8; ++e) {
-					const uint32_t j = 8 * ((tid & 63) + 64 * k) + e, n = (uint32_t)x[k][e / 2] >> 16 * (e & 1) & 0xffff;
-					if (n && off < kBuckets && j + off < kBuckets) atomicAdd(&s_hist[j + off], n);
-				}
+			for (int q = 0; q < kAhead; ++q) {
+				if (m[q] == kNoLogit || i0 + q * kWaves >= slices) continue;
+				const uint32_t off = (uint32_t)rb - (uint32_t)((int32_t)m[q] >> p.sh);  // the slice's first bucket
+				if (off >= kBuckets) continue;
+#pragma unroll
+				for (int k = 0; k < kBuckets / 512; ++k)
+#pragma unroll
+					for (int e = 0; e < 8; ++e) {
+						const uint32_t j = 8 * ((tid & 63) + 64 * k) + e + off, n = (uint32_t)x[q][k][e / 2] >> 16 * (e & 1) & 0xffff;
+						if (n && j < kBuckets) atomicAdd(&s_hist[j], n);
+					}
+			}
 		}
 		__syncthreads();
 		int c[kPlanBuckets];
