@@ -40,10 +40,11 @@ __device__ __forceinline__ Weight weight_of(const Sampling& s) {
 	w.lim = (uint32_t)(30 * s.q_ln2);
 	return w;
 }
-__device__ __forceinline__ double weight_d(const Weight& w, uint32_t d) {
-	const double x = (double)d, z = floor(fma(x, w.ninv, w.half)), base = fma(z, w.l, w.b - x);
-	return d >= w.lim ? 0.0 : floor(ldexp(fma(base, base, w.c), -(int)z));
+__device__ __forceinline__ double weight_below(const Weight& w, uint32_t d) {  // d < lim; past it something
+	const double x = (double)d, z = ceil(fma(x, -w.ninv, -w.half)), base = fma(-z, w.l, w.b - x);
+	return floor(ldexp(fma(base, base, w.c), (int)z));
 }
+__device__ __forceinline__ double weight_d(const Weight& w, uint32_t d) { return d >= w.lim ? 0.0 : weight_below(w, d); }
 __device__ __forceinline__ uint64_t weight(const Weight& w, uint32_t d) { return (uint64_t)weight_d(w, d); }
 
 // Everything a row's sampling asks for is a border in one order, logit descending, then index ascending: the element whose
@@ -98,22 +99,35 @@ struct SampleSlice {
 		v0 = blockIdx.x * kSampleSlice;
 		n = min(kSampleSlice, a.vocab - v0);
 		const int32_t* row = a.logits + (int64_t)blockIdx.y * a.ld + v0;
+		// every load goes out before one is waited for: quads by the row's last whole one, then what stands past it
+		if (VEC && n >= 4) {
+#pragma unroll
+			for (int u = 0; u < kSampleLoads; ++u) x[u] = *(const v4i*)(row + min(place(u), (n & ~3) - 4));
+		}
+		if (!VEC || n < 4 || (n & 3)) {
+#pragma unroll
+			for (int u = 0; u < kSampleLoads; ++u)
+				if (!VEC || place(u) + 4 > n)
+#pragma unroll
+					for (int i = 0; i < 4; ++i) x[u][i] = row[min(place(u) + i, n - 1)];
+		}
+		uint32_t m[kSampleLoads];
+#pragma unroll
+		for (int u = 0; u < kSampleLoads; ++u) m[u] = 0xff;
+		if (mask) {
+#pragma unroll
+			for (int u = 0; u < kSampleLoads; ++u) m[u] = global_ptr(mask)[min(v0 + place(u), a.vocab - 1) >> 3];
+		}
 		legal = 0;
 #pragma unroll
 		for (int u = 0; u < kSampleLoads; ++u) {
-			const int j = 4 * ((int)threadIdx.x + u * kSampleBlock);
-			if (VEC && j + 4 <= n) x[u] = *(const v4i*)(row + j);
-			else {
-#pragma unroll
-				for (int i = 0; i < 4; ++i) x[u][i] = row[min(j + i, n - 1)];
-			}
-			uint32_t m = mask ? global_ptr(mask)[min(v0 + j, a.vocab - 1) >> 3] >> (j & 4) & 15 : 15;
-			m &= j + 4 <= n ? 15u : (j < n ? (1u << (n - j)) - 1 : 0u);
-			legal |= m << 4 * u;
+			const int left = n - place(u);
+			legal |= (m[u] >> (place(u) & 4) & (left >= 4 ? 15u : (left > 0 ? (1u << left) - 1 : 0u))) << 4 * u;
 		}
 	}
+	__device__ __forceinline__ int place(int u) const { return 4 * ((int)threadIdx.x + u * kSampleBlock); }
 	__device__ __forceinline__ bool has(int u, int i) const { return legal >> (4 * u + i) & 1; }
-	__device__ __forceinline__ int index(int u, int i) const { return v0 + 4 * ((int)threadIdx.x + u * kSampleBlock) + i; }
+	__device__ __forceinline__ int index(int u, int i) const { return v0 + place(u) + i; }
 };
 
 template <bool VEC>
@@ -375,48 +389,69 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_gather(SampleArgs a, Sa
 	const SamplePlan& p = w.plan[r];
 	if (p.state != 0) return;
 	const int32_t top = p.top, sh = p.sh, rb = top >> sh;
-	const uint32_t a0 = p.a[0], a2 = p.a[2], b0 = p.b[0], b2 = p.b[2];
-	const uint32_t a1 = s.top_p < 65536 ? p.a[1] : 0, b1 = s.top_p < 65536 ? p.b[1] : 0;
 	// the sums that the borders need: weights before ranges 0, 1 and 2, kept ones (where min-p makes them others) before 0 or 1, and 2
 	const bool by_p = s.top_p < 65536, min_p = s.min_p > 0;
-	const uint32_t first = by_p ? a1 : a0, most = max(a0, max(by_p ? a1 : 0, a2));
 	if (tid < 5) s_sum[tid] = 0;
 	if (tid == 0) s_n = 0;
 	__syncthreads();
 	const Weight wt = weight_of(s);
 	const double least = (double)share_of((uint64_t)(s.q_b * s.q_b + s.q_c), s.min_p);
 	double acc0 = 0.0, acc1 = 0.0, acc2 = 0.0, acc3 = 0.0, acc4 = 0.0;  // 16 values of 2^47
-	const uint32_t n0 = b0 - a0, n1 = b1 - a1, n2 = b2 - a2;
-	auto run = [&](auto with_min_p) {
+	// What bounds the kernel is its instructions, so the places j < x of the buckets are the d below this, one comparison of an element for
+	// each, and what is not legal is moved past them all: 128 rows of 151936 in 29 us, 33 with the buckets' numbers, every sum and
+	// the legal bits looked at for each element.
+	auto below = [&](uint32_t x) { return (uint32_t)i64max(0, (int64_t)top + 1 - ((int64_t)rb - x + 1) * ((int64_t)1 << sh)); };
+	const uint32_t r0 = below(p.a[0]), n0 = below(p.b[0]) - r0, r1 = below(p.a[1]), n1 = below(p.b[1]) - r1, r2 = below(p.a[2]), n2 = below(p.b[2]) - r2;
+	const uint32_t a0 = min(r0, wt.lim), a1 = min(r1, wt.lim), a2 = min(r2, wt.lim), first = by_p ? a1 : a0, most = max(a0, max(by_p ? a1 : 0, a2));
+	if (__any(sl.legal != (1u << 4 * kSampleLoads) - 1)) {
+		// what is not legal goes furthest below the largest, past every range
+#pragma unroll
+		for (int u = 0; u < kSampleLoads; ++u)
+#pragma unroll
+			for (int i = 0; i < 4; ++i) sl.x[u][i] = sl.has(u, i) ? sl.x[u][i] : (int32_t)((uint32_t)top + 1);
+	}
+	uint64_t who[4 * kSampleLoads];  // which lanes' elements lie in a range
+	auto run = [&](auto with_top_p, auto with_min_p) {
+		constexpr bool TP = decltype(with_top_p)::value, MP = decltype(with_min_p)::value;
 #pragma unroll
 		for (int u = 0; u < kSampleLoads; ++u)
 #pragma unroll
 			for (int i = 0; i < 4; ++i) {
-				const uint32_t j = sl.has(u, i) ? (uint32_t)rb - (uint32_t)(sl.x[u][i] >> sh) : ~0u;
 				const uint32_t d = (uint32_t)top - (uint32_t)sl.x[u][i];
-				if (__any(j < most)) {
-					const double x = weight_d(wt, d);
-					acc0 += only(j < a0, x);
-					acc1 += only(j < a1, x);
-					if constexpr (!decltype(with_min_p)::value) acc2 += only(j < a2, x);
+				if (__any(d < most)) {
+					const double x = weight_below(wt, d);
+					acc0 += only(d < a0, x);
+					if constexpr (TP) acc1 += only(d < a1, x);
+					if constexpr (!MP) acc2 += only(d < a2, x);
 					else {
 						const bool kept = x >= least;
-						acc3 += only((j < first) & kept, x);
-						acc4 += only((j < a2) & kept, x);
+						acc3 += only((d < first) & kept, x);
+						acc4 += only((d < a2) & kept, x);
 					}
 				}
-				const bool in = (j - a0 < n0) | (j - a1 < n1) | (j - a2 < n2);
-				const uint64_t who = __ballot(in);
-				if (who) {
-					uint32_t at = 0;
-					if (lane == __builtin_ctzll(who)) at = atomicAdd(&s_n, (uint32_t)__popcll(who));
-					at = __builtin_amdgcn_readlane(at, __builtin_ctzll(who)) + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-					if (in && at < kSliceList) s_list[at] = uint2{d, (uint32_t)sl.index(u, i)};
-				}
+				who[4 * u + i] = __ballot(d - r0 < n0) | __ballot(d - r2 < n2);
+				if constexpr (TP) who[4 * u + i] |= __ballot(d - r1 < n1);
 			}
 	};
-	if (min_p) run(std::true_type{});
-	else run(std::false_type{});
+	if (by_p && min_p) run(std::true_type{}, std::true_type{});
+	else if (by_p) run(std::true_type{}, std::false_type{});
+	else if (min_p) run(std::false_type{}, std::true_type{});
+	else run(std::false_type{}, std::false_type{});
+	uint32_t mine = 0;
+#pragma unroll
+	for (int k = 0; k < 4 * kSampleLoads; ++k) mine += (uint32_t)__popcll(who[k]);
+	if (mine) {
+		uint32_t at = 0;
+		if (lane == 0) at = atomicAdd(&s_n, mine);  // the wave's places in the list
+		at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+		for (int k = 0; k < 4 * kSampleLoads; ++k)
+			if (who[k]) {
+				const uint32_t to = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(who[k] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who[k], 0));
+				if ((who[k] >> lane & 1) && to < kSliceList) s_list[to] = uint2{(uint32_t)top - (uint32_t)sl.x[k / 4][k % 4], (uint32_t)sl.index(k / 4, k % 4)};
+				at += (uint32_t)__popcll(who[k]);
+			}
+	}
 	const double acc[5] = {acc0, acc1, acc2, acc3, acc4};
 #pragma unroll
 	for (int k = 0; k < 5; ++k) {
