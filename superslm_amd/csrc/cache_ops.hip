@@ -64,7 +64,8 @@ __global__ __launch_bounds__(256) void k_table_copy(const int32_t* from, int32_t
 
 // One block: bitmaps of the pages that rows hold (seen), hold more than once (multi), and hold without writing
 // into them or keep from outside (fixed), in LDS; then who gets a copy, how many pages each row takes, and the free
-// pages in ascending order.  Bound by its chain of loads (a row's numbers, its source's length, the tables) and of block sums.
+// pages in ascending order.  Bound by its chain of loads (a row's numbers, its source's length, the tables) and of block sums:
+// 6.2 us for 4 rows and 114 pages, 8.9 for 128 rows of 16 pages; a block per row would need its answers joined by further launches.
 constexpr int kLowSlots = 2048;
 constexpr int kWrites = 1 << 30;  // beside a row's number of kept pages: it writes into the last of them
 __global__ __launch_bounds__(kPlanBlock) void k_update_plan(PageUpdateArgs a, const int32_t* tables, PlanWork w) {
@@ -197,7 +198,8 @@ __global__ __launch_bounds__(kPlanBlock) void k_update_plan(PageUpdateArgs a, co
 	}
 }
 
-// Pages from one place of the pool to another, 16 KB to a block and step: no page is both read and written.
+// Pages from one place of the pool to another, 16 KB to a block and step: no page is both read and written.  Bound by HBM: 283 MB
+// (read + written) in 60 us, 4.7 TB/s (47 where the caches still hold some of them); a handful of pages is a launch's 4 us.
 constexpr int kCopyChunk = 16384;
 template <typename F>
 __device__ __forceinline__ void copy_pages(int8_t* pool, int64_t page_bytes, int n, F&& pair) {
@@ -239,7 +241,8 @@ __global__ __launch_bounds__(256) void k_update_apply(PageUpdateArgs a, const in
 }
 
 // One block: the pages in use and those held as bitmaps; the boundary before which the movable ones come to lie;
-// the holes before it and the movers after it, both in ascending order.
+// the holes before it and the movers after it, both in ascending order.  The same chain as the update's plan: 6.6 us for 6 rows,
+// 9.7 for 100 rows and 800 pages.
 __global__ __launch_bounds__(kPlanBlock) void k_compact_plan(PageCompactArgs a, PlanWork w) {
 	extern __shared__ uint32_t lds[];
 	__shared__ int64_t s_scan[kPlanBlock / 64];
@@ -268,7 +271,7 @@ __global__ __launch_bounds__(kPlanBlock) void k_compact_plan(PageCompactArgs a, 
 			if (a.held[p]) atomicOr(&held[p >> 5], 1u << (p & 31));
 	__syncthreads();
 	const uint32_t most = s_most;
-	const uint64_t cells = s_bad < a.rows ? 0 : (uint64_t)a.rows * most;
+	const uint64_t cells = (uint64_t)a.rows * most;
 	for (uint64_t c0 = tid; c0 < cells; c0 += 4 * kPlanBlock) {
 		int r[4], p[4];
 #pragma unroll
@@ -393,7 +396,7 @@ __device__ __forceinline__ CacheRow cache_row(const int32_t* row_tokens, const i
 	return c;
 }
 
-// A block per row: whether its tokens can land.
+// A block per row: whether its tokens can land, 2.5 us beside the span's 16: the span's blocks would each have to look at every token.
 __global__ __launch_bounds__(256) void k_store_check(CacheStoreArgs a) {
 	__shared__ int s_st;
 	const int r = blockIdx.x;
@@ -467,7 +470,7 @@ __device__ __forceinline__ void octet_store(const CacheStoreArgs& a, int8_t* hea
 // The angles of four pairs at `pos`, and the pairs turned by them (rope_pair), clamped to +-top; returns how many values were.
 // In doubles: a value of 16 bits times a table's 31, and the sum of two of these, are exact at the scale 2^-30, and so is half a
 // unit added away from zero before the conversion truncates.  Five instructions a value, the 64-bit form takes some thirty: 512 tokens of
-// 28 + 2 x 4 heads for each of four rows 18.4 -> 14.5 us.
+// 28 + 2 x 4 heads for each of four rows 18.4 -> 16.2 us.
 struct Turn {
 	double c[4], s[4];
 };
@@ -562,6 +565,8 @@ __device__ __forceinline__ void regrow(int8_t* at, int init, uint32_t levels) {
 
 // K or V of one KV head (z) in one page (x) of one row (y): the page's tokens land in LDS, their exponents run up the
 // page, then the codes are written; the waves of blocks past the last page take q's tokens, one each.
+// Bound by its instructions (a landing and a rotation are some 40 of doubles to a code) and, as one block takes a page's tokens, by that
+// block's length: 4 rows of 512 tokens, 28 + 2 x 4 heads of 128, 16.5 us, of which 16.5 MB are 3.5.
 constexpr int kStoreBlock = 512;
 template <int D>
 __global__ __launch_bounds__(kStoreBlock) void k_store_span(CacheStoreArgs a, int pages) {
@@ -670,7 +675,8 @@ __global__ __launch_bounds__(kStoreBlock) void k_store_span(CacheStoreArgs a, in
 }
 
 // Single tokens in one launch, a block per row: K's and V's octets, then q's.  The lanes of a head's octets find its
-// exponent; a page that grows is rounded by the whole block once all heads are known.
+// exponent; a page that grows is rounded by the whole block once all heads are known.  Its chain of loads bounds it: 8 rows 5.5 us, with
+// the span's two launches 9.7.
 template <int D>
 __global__ __launch_bounds__(kStoreBlock) void k_store_token(CacheStoreArgs a) {
 	__shared__ uint16_t s_grow[2 * 256];  // of each KV head's K and V: the exponents before and after
@@ -890,7 +896,8 @@ __device__ __forceinline__ bool cd_job(const CacheAttnArgs& a, const CaPlan& pl,
 	return j->p0 < j->p1;
 }
 
-// The scores of a plane, kept, and their maxima.  The first wave of a row's first plane also settles its constants.
+// The scores of a plane, kept, and their maxima: written once and read twice they cost less than two more products with K.  64 rows of
+// 28 heads / 4 KV x 128 by up to 8000 positions: 39 us, 149 MB of K at 3.8 TB/s; then k_cd_sum 15.5, k_cd_pv 47.  The first wave of a row's first plane also settles its constants.
 template <int D>
 __global__ __launch_bounds__(64 * kCaWaves) void k_cd_scores(CacheAttnArgs a, CaPlan pl, CaWork w) {
 	constexpr int NC = (D + 63) / 64;
@@ -1152,6 +1159,9 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cd_pv(Cache
 // The whole of a single token's row in one launch, a block per (row, KV head, tile of heads): its waves take 64 positions in
 // turn and keep their scores in LDS, or where these are too many (GS) in the workspace, from which i-exp and probabilities
 // run on full waves, four heads at a time; maxima, sums and contexts are joined in LDS.  k_ca_out finds one plane.
+// 12 heads / 2 KV x 128: 2 rows by 100 positions 10.8 us, the chain of one block's stages; 24 by 1500 19.9; 64 rows of 28 / 4 by up to
+// 8000 95.7 with the scores in the workspace, 298 MB at 3.1 TB/s: the longest rows' blocks end last, and i-exp and probabilities are
+// some 30 instructions of doubles to a score.
 template <int D>
 struct CrShape {
 	static constexpr int NW = D <= 128 ? 8 : 4, STEP = 64 * NW, LD = 68;  // LD: a head's 64 scores, moved apart by a few banks
@@ -1577,6 +1587,10 @@ __device__ __forceinline__ int64_t cc_sum(const CacheAttnArgs& a, const CaPlan& 
 	return bad ? -1 : sum;
 }
 
+// The maxima of 64 query rows over a plane: scores on the MFMAs from K tiles of 64 positions that the block's waves share through LDS.
+// The softmax rounds each probability by the whole row's sum, so a running maximum with rescaling would not be exact: maxima, sums
+// and P V are three passes that compute the scores again, less than keeping chunk x width of them would cost.  A chunk of 500 at 2000,
+// 12 heads / 2 KV x 128: 9.6 + 15.8 + 34.3 us.
 template <int D>
 __global__ __launch_bounds__(64 * kCaWaves) void k_cc_max(CacheAttnArgs a, CaPlan pl, CaWork w) {
 	constexpr int NC = (D + 63) / 64;
@@ -1609,6 +1623,7 @@ __global__ __launch_bounds__(64 * kCaWaves) void k_cc_max(CacheAttnArgs a, CaPla
 	if (g == 0 && l.t >= 0) w.pmax[((size_t)j.plane * a.tokens + l.t) * a.NH + l.h] = m;
 }
 
+// The sums of i-exp: the same scores again; bound by the doubles of i-exp, some 12 instructions to a score and lane.
 template <int D>
 __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 4 : 2) void k_cc_sum(CacheAttnArgs a, CaPlan pl, CaWork w) {
 	constexpr int NC = (D + 63) / 64;
@@ -1660,6 +1675,8 @@ __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 4 : 2) void k_cc_sum(Cach
 	if (g == 0 && live) w.psum[((size_t)j.plane * a.tokens + l.t) * a.NH + l.h] = bad ? -1 : sum;
 }
 
+// P V: the scores a third time, i-exp and the exact probability of each (some 20 instructions of doubles, which bound it), its 16 bits
+// and the page's exponent as three int8 operands, and three MFMAs for each 16 dims.
 template <int D>
 __global__ __launch_bounds__(64 * kCaWaves, D <= 128 ? 2 : 1) void k_cc_pv(CacheAttnArgs a, CaPlan pl, CaWork w) {
 	constexpr int NC = (D + 63) / 64, DT = D / 16;

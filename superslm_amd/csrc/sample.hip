@@ -55,7 +55,9 @@ __device__ __forceinline__ uint64_t weight(const Weight& w, uint32_t d) { return
 //   k_sample_gather  the exact sums of the weights before those buckets, and the elements in them
 //   k_sample_pick    the borders among these elements.  That each lies where it was expected is checked exactly, so an estimate
 //                    that misses (or a list that overflows) costs the radix search over the row, not the result.
-// Rows of one slice are searched in LDS by k_sample_pick alone.
+// Rows of one slice are searched in LDS by k_sample_pick alone.  At 151936 tokens 1 row takes 4.2 + 12.9 + 6.2 + 8.9 us, the chains of
+// four launches, and 128 rows 16.2 + 20.6 + 29 + 13.4: the first pass reads 79 MB at 4.9 TB/s, the second is bound by its doubles, plan and
+// pick are a block's chain of scans to a row.  The search over the row takes 870 us for 1 row and 1870 for 128.
 constexpr int kSampleBlock = 512;
 constexpr int kSampleSlice = 8192, kSampleLoads = kSampleSlice / kSampleBlock / 4;
 constexpr int kBuckets = 2048;

@@ -151,11 +151,8 @@ def compact(tables, lengths, p, pages, held=None):
     n = []
     for r in range(rows):
         m = int(lengths[r])
-        if not 0 <= m <= width * p:
-            return [INVALID, 0, 0, r], None, None, []
         n.append(-(-m // p))
-    for r in range(rows):
-        if not all(0 <= x < pages for x in tables[r, :n[r]]):
+        if not (0 <= m <= width * p and all(0 <= x < pages for x in tables[r, :n[r]])):
             return [INVALID, 0, 0, r], None, None, []
     live = sorted({int(x) for r in range(rows) for x in tables[r, :n[r]]})
     stay = set() if held is None else {x for x in range(pages) if held[x]}

@@ -10,7 +10,7 @@ import cache_ops_ref as ref
 from superslm_amd.batch_ops import BatchOps, Sampling, sampling_constants
 from superslm_amd.cache_ops import CacheOps
 from superslm_amd.device import Device
-from test_gpu_cache_ops import LEFT, SITE, Batch
+from test_gpu_cache_ops import LEFT, SITE, Batch, change_pages, scene
 
 pytestmark = pytest.mark.gpu
 
@@ -99,6 +99,55 @@ def test_pages_past_32_bits_change_hands(ops, dev):
             assert (pool.get(p * big, 4096, np.int8) == edge[was]).all() and (pool.get((p + 1) * big - 4096, 4096, np.int8) == edge[was][::-1]).all()
     finally:
         pool.free()
+
+
+def compacted(ops, dev, p, pages, tables, lengths, pool, held=None):
+    """(result, new tables, map, pool) after the call."""
+    b = [dev.upload(x) for x in (pool, tables, lengths, np.full_like(tables, LEFT), np.full(pages, LEFT, np.int32), np.full(4, LEFT, np.int32))]
+    h = dev.upload(held) if held is not None else None
+    n = ops.compact_workspace(len(tables), pages, tables.shape[1])
+    ws = dev.upload(np.full(n, 0xA5, np.uint8))
+    ops.compact(rows=len(tables), pages=pages, page_tokens=p, table_ld=tables.shape[1], pool=b[0].ptr, page_bytes=pool.shape[1], tables=b[1].ptr,
+                lengths=b[2].ptr, held=h.ptr if h else None, new_tables=b[3].ptr, map=b[4].ptr, result=b[5].ptr, workspace=ws.ptr, workspace_bytes=n)()
+    assert ops.lib.lib.sslm_hip_synchronize() == 0
+    return b[5].numpy().tolist(), b[3].numpy(), b[4].numpy(), b[0].numpy()
+
+
+@pytest.mark.parametrize("seed", range(3))
+def test_the_most_rows_and_pages(ops, dev, seed):
+    """Plans whose bitmaps fill LDS, rows that write into one another's open pages."""
+    rows, width, p, pages = 4096, 40, 16, 1 << 18
+    rng = np.random.default_rng(seed)
+    tables, lengths = scene(rng, rows, width, p, pages, width * p)
+    lengths = np.maximum(lengths - rng.integers(0, 2, rows), 0)
+    source = (rng.integers(0, rows, rows), rng.integers(0, rows, rows) // 64 * 64, np.arange(rows))[seed].astype(np.int32)
+    keep = lengths[source]
+    room = np.minimum(keep + rng.integers(0, 3, rows), width * p)
+    held = (rng.random(pages) < 0.1).astype(np.uint8) if seed else None
+    result, new, _ = change_pages(ops, dev, p, pages, tables, lengths, source, keep, room, held, page_bytes=16)
+    assert result[0] == 0 and (result[2] > 1000 or seed == 2)
+    pool = rng.integers(-127, 128, size=(pages, 16), dtype=np.int8)
+    want = ref.compact(new, room, p, pages, held)
+    got = compacted(ops, dev, p, pages, new, room, pool, held)
+    assert got[0] == want[0] and (got[1] == want[1]).all() and (got[2] == want[2]).all() and want[0][2] > 1000
+    for x, y in want[3]:
+        pool[y] = pool[x]
+    assert (got[3] == pool).all()
+
+
+def test_compaction_names_the_lowest_row_out_of_range(ops, dev):
+    """A page of row 3 that is none, a length of row 700 and pages of later rows, however the block's waves come to them."""
+    rng = np.random.default_rng(3)
+    for low, length in ((3, 700), (1100, 5), (900, None)):
+        tables, lengths = rng.integers(0, 50, (1200, 30)).astype(np.int32), np.full(1200, 480, np.int64)
+        tables[low, 29] = 50
+        tables[low + 40:, 0] = -1
+        if length is not None:
+            lengths[length] = -1
+        pool = np.zeros((50, 16), np.int8)
+        got = compacted(ops, dev, 16, 50, tables, lengths, pool)
+        assert got[0] == [ref.INVALID, 0, 0, min(low, length or low)] == ref.compact(tables, lengths, 16, 50)[0]
+        assert (got[1] == LEFT).all() and (got[2] == LEFT).all()
 
 
 @pytest.mark.parametrize("rows,heads,width", [(40, 16, 3_500_001), (1, 2, (1 << 24) - 5)])
