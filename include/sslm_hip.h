@@ -522,7 +522,7 @@ sslm_status sslm_hip_cache_compact(const sslm_hip_cache_compact_args* args, void
 
 /* New tokens of a ragged batch: q and k rotated, k and v landed in the rows' pages.  Row r has the tokens
  * [row_tokens[r], row_tokens[r + 1]), at positions row_start[r] on (row_tokens ascends within [0, tokens]; at most max_new each;
- * pages that rows write into are their own).  Codes
+ * pages that rows write into are their own; max_new and rope_rows are at most SSLM_HIP_CACHE_MAX_WIDTH).  Codes
  * are int8 with carried scales k_scale, v_scale (m, e) per token.  The reference's landing (forward_sites.cpp:513-653) with the
  * KV head's constants r_t, e_t gives units, clamped to +-127 2^8; pairs of the head's first rope_dim (a multiple of 8, 0:
  * none) dims, (2 i, 2 i + 1) or with rope_halves (i, i + rope_dim / 2), turn by the Q30 tables [rope_rows, rope_dim / 2] (src/intmath.cpp:782-792),
@@ -557,7 +557,8 @@ sslm_status sslm_hip_cache_store(const sslm_hip_cache_store_args* args, void* st
  * (single tokens: decode steps; several: a prompt's chunk, whose rows sslm_hip_cache_store has landed before).
  * score = (q . k) 2^s of k's page; the softmax, its constants (khead: the carried scale of one K unit over sqrt(head_dim)), the Q15
  * probabilities, fold and funnel are sslm_hip_shared_attention's; context = sum of p v 2^s of v's page.  max_width: at least
- * every row's positions.  Per token its codes, scale and status: 0, 9 (the row's lengths or a page of it out of range) or the
+ * every row's positions.  q is 16-byte aligned, max_new below 2^22; a workspace of 0 bytes: sizes outside the domain, or more blocks
+ * than a launch takes.  Per token its codes, scale and status: 0, 9 (the row's lengths or a page of it out of range) or the
  * reference's SslmForwardStatus value; tokens that no row has stay as they were. */
 typedef struct sslm_hip_cache_attention_args {
 	uint32_t struct_size;

@@ -1852,9 +1852,12 @@ size_t page_compact_workspace(int rows, int pages, int table_ld) {
 	return plan_work(rows, pages, table_ld, nullptr, &w);
 }
 
+// The most dynamic LDS that a launch here asks for; beside it the plans' 9 KB of their own.  A kernel's limit is always set to
+// this, so that calls of other sizes from other threads leave it where it is.
+constexpr int kMostLds = 150 * 1024;
 template <typename K>
 static void allow_lds(K kernel, size_t bytes) {
-	if (bytes > 32768 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess)
+	if (bytes > 32768 && (bytes > kMostLds || hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds) != hipSuccess))
 		throw LaunchRefused{"dynamic LDS"};
 }
 
@@ -1924,7 +1927,7 @@ constexpr int kCdTargetBlocks = 1536, kCcTargetBlocks = 768;
 template <int D>
 static int cr_form(int64_t units, int NH, int NKV, int64_t max_width) {
 	if (max_width * (210 - units) > 257000) return 0;
-	return CrShape<D>::lds(std::min(16, NH / NKV), max_width, false) <= 150 * 1024 ? 1 : 2;
+	return CrShape<D>::lds(std::min(16, NH / NKV), max_width, false) <= kMostLds ? 1 : 2;
 }
 static int cr_form(int64_t units, int NH, int NKV, int D, int64_t max_width) {
 	switch (D) {
@@ -1941,7 +1944,7 @@ static CaPlan ca_plan(int rows, int tokens, int max_new, int NH, int NKV, int D,
 	CaPlan p{};
 	const int G = NH / NKV, step = max_new == 1 ? kCdStep : 64;
 	p.ht = (G + 15) / 16;
-	p.groups = (int)((int64_t)tokens * G / 64 + rows);
+	p.groups = max_new == 1 ? 0 : (int)((int64_t)tokens * G / 64 + rows);
 	const int64_t units = max_new == 1 ? (int64_t)rows * NKV * p.ht : (int64_t)p.groups * NKV;
 	p.whole = max_new == 1 ? cr_form(units, NH, NKV, D, max_width) : 0;
 	const int64_t steps = (max_width + step - 1) / step;
@@ -1974,9 +1977,12 @@ static size_t ca_work(const CaPlan& p, int tokens, int max_new, int NH, int NKV,
 }
 
 size_t cache_attn_workspace(int rows, int tokens, int max_new, int NH, int NKV, int D, int64_t max_width) {
+	// a launch takes fewer than 2^32 threads along x
+	constexpr int64_t kMost = 1ll << 32;
+	if ((int64_t)max_new * 1024 >= kMost || (max_new > 1 && (int64_t)tokens * (NH / NKV) / 64 + rows >= kMost / 256)) return 0;
 	const CaPlan p = ca_plan(rows, tokens, max_new, NH, NKV, D, max_width);
-	// a launch's blocks
-	if ((int64_t)rows * NKV * p.ht * p.planes >= 1ll << 30 || ((int64_t)p.planes * NKV + 8) * p.groups >= 1ll << 30) return 0;
+	const int64_t blocks = max_new == 1 ? (int64_t)rows * NKV * p.ht * p.planes : (int64_t)((p.planes * NKV + 7) / 8 * 8) * p.groups;
+	if (blocks * (p.whole ? 512 : 64 * kCaWaves) >= kMost) return 0;
 	CaWork w;
 	return ca_work(p, tokens, max_new, NH, NKV, D, nullptr, &w);
 }
@@ -2106,7 +2112,7 @@ sslm_status sslm_hip_cache_compact(const sslm_hip_cache_compact_args* p, void* w
 sslm_status sslm_hip_cache_store(const sslm_hip_cache_store_args* p, void* stream) {
 	if (!p || p->struct_size != sizeof(*p)) return SSLM_INVALID_ARGUMENT;
 	const int lp = log2_page(p->page_tokens);
-	if (lp < 0 || p->rows < 1 || p->rows > kMaxRows || p->tokens < 1 || p->max_new < 1 || p->max_new > p->tokens || p->pages < 1 ||
+	if (lp < 0 || p->rows < 1 || p->rows > kMaxRows || p->tokens < 1 || p->max_new < 1 || p->max_new > p->tokens || p->max_new > SSLM_HIP_CACHE_MAX_WIDTH || p->pages < 1 ||
 	    p->table_ld < 1 || p->table_ld > SSLM_HIP_CACHE_MAX_WIDTH / 16 || !heads_ok(p->heads, p->kv_heads, p->head_dim) || p->rope_dim < 0 ||
 	    p->rope_dim % 8 || p->rope_dim > p->head_dim || !pool_ok(p->pool, p->page_bytes, p->pages) || !p->tables || !p->row_tokens ||
 	    !p->row_start || !p->k || !p->v || !p->k_scale || !p->v_scale || !p->r_t_k || !p->e_t_k || !p->r_t_v || !p->e_t_v || !p->clamped || !p->status)

@@ -103,6 +103,17 @@ def test_workspaces_of_sizes_outside_the_domain_are_zero(cache, batch):
     assert cache.attention_workspace(1, 1, 1, 4, 2, 64, 16, 1) > 0
 
 
+@pytest.mark.parametrize("rows,tokens,max_new,heads,kv_heads,dim,width,fits", [
+    (65535, 65535, 1, 256, 256, 32, 100, False), (32767, 32767, 1, 256, 256, 32, 100, True),  # a block of 512 threads per (row, KV head)
+    (65535, 65535, 1, 64, 64, 128, 100, True), (65535, 65535, 1, 256, 128, 32, 100, True),
+    (1, (1 << 31) - 1, 2, 256, 1, 32, 100, False), (1, (1 << 31) - 1, 1, 256, 1, 32, 100, True),  # 64 query rows to a block of 256
+    (1, 1 << 23, 2, 256, 1, 32, 100, False), (1, 1 << 21, 2, 256, 1, 32, 100, False), (1, 1 << 18, 2, 256, 1, 32, 100, True),
+    (1, 1 << 23, 1 << 22, 1, 1, 32, 100, False), (1, 1 << 23, (1 << 22) - 1, 1, 1, 32, 100, True)])
+def test_attention_that_no_launch_holds_has_no_workspace(cache, rows, tokens, max_new, heads, kv_heads, dim, width, fits):
+    n = cache.attention_workspace(rows, tokens, max_new, heads, kv_heads, dim, 16, width)
+    assert (n >= tokens * heads * dim * 4) if fits else n == 0
+
+
 def test_an_unknown_field_or_a_number_too_large_is_an_error(cache):
     with pytest.raises(TypeError):
         cache.compact(**PAGES, map=ANY, colour=1)
