@@ -55,8 +55,8 @@ __device__ __forceinline__ uint64_t weight(const Weight& w, uint32_t d) { return
 //   k_sample_gather  the exact sums of the weights before those buckets, and the elements in them
 //   k_sample_pick    the borders among these elements.  That each lies where it was expected is checked exactly, so an estimate
 //                    that misses (or a list that overflows) costs the radix search over the row, not the result.
-// Rows of one slice are searched in LDS by k_sample_pick alone.  At 151936 tokens 1 row takes 4.2 + 12.9 + 6.2 + 8.9 us, the chains of
-// four launches, and 128 rows 16.2 + 20.6 + 29 + 13.4: the first pass reads 79 MB at 4.9 TB/s, the second is bound by its doubles, plan and
+// Rows of one slice are searched in LDS by k_sample_pick alone.  At 151936 tokens 1 row takes 4.2 + 10.9 + 6.2 + 9.0 us, the chains of
+// four launches, and 128 rows 16.2 + 18.5 + 29 + 13.4: the first pass reads 79 MB at 4.9 TB/s, the second is bound by its doubles, plan and
 // pick are a block's chain of scans to a row.  The search over the row takes 870 us for 1 row and 1870 for 128.
 constexpr int kSampleBlock = 512;
 constexpr int kSampleSlice = 8192, kSampleLoads = kSampleSlice / kSampleBlock / 4;
@@ -182,6 +182,9 @@ struct Mass {
 __device__ __forceinline__ Mass operator+(const Mass& a, const Mass& b) { return Mass{a.c + b.c, a.e + b.e, a.k + b.k, a.v + b.v}; }
 
 constexpr int kPlanThreads = 512, kPlanBuckets = kBuckets / kPlanThreads;
+struct __attribute__((packed)) plan_counts {
+	uint64_t v;
+};
 
 // sums up to and with each thread's, in thread order, and the total
 __device__ __forceinline__ Mass mass_scan(Mass x, Mass* s, Mass* total) {
@@ -207,68 +210,64 @@ __device__ __forceinline__ Mass mass_scan(Mass x, Mass* s, Mass* total) {
 // it less f of all is nothing: with the errors of what is before and behind it apart, that has the variance (1 - f)^2 V_before +
 // f^2 V_behind, and the border is looked for within six deviations.
 __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, SampleWork w, int slices) {
-	__shared__ uint32_t s_hist[kBuckets];
+	__shared__ uint32_t s_off[SSLM_HIP_SAMPLE_MAX_VOCAB / kSampleSlice];
 	__shared__ Mass s_scan[kPlanThreads / 64];
-	__shared__ long long s_top;
 	__shared__ int s_a[3], s_b[3], s_n;
 	__shared__ uint32_t s_goal;
 	__shared__ double s_sum, s_kept, s_var, s_doubt, s_more;
 	__shared__ int s_few;
-	const int r = blockIdx.x, tid = threadIdx.x;
+	const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+	const int64_t* smax = w.smax + (size_t)r * slices;
+	int64_t best = smax[min(lane, slices - 1)];
 	const Sampling s = a.rules[r];
 	if (!sampling_ok(s, a.vocab)) return;
 	if (tid == 0) {
-		s_top = kNoLogit;
 		s_n = 0;
 		s_goal = 0;
 		s_doubt = 0.0;
 	}
 	if (tid < 3) s_a[tid] = s_b[tid] = kBuckets;
-	for (int i = tid; i < kBuckets; i += kPlanThreads) s_hist[i] = 0;
-	__syncthreads();
-	long long top = kNoLogit;
-	for (int i = tid; i < slices; i += kPlanThreads) top = max(top, (long long)w.smax[(size_t)r * slices + i]);
-	for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
-	if ((tid & 63) == 0) atomicMax(&s_top, top);
+	// every wave finds the row's largest logit
+	for (int i = lane + 64; i < slices; i += 64) best = i64max(best, smax[i]);
+	const bool some = __any(best != kNoLogit);
+	const int32_t top = (int32_t)(wave_max32(best == kNoLogit ? 0u : (uint32_t)(int32_t)best ^ 0x80000000u) ^ 0x80000000u);
+	const int sh = bucket_shift(s), rb = top >> sh;
+	for (int i = tid; i < slices; i += kPlanThreads) {
+		const int64_t m = smax[i];
+		s_off[i] = m == kNoLogit ? (uint32_t)kBuckets : min((uint32_t)rb - (uint32_t)((int32_t)m >> sh), (uint32_t)kBuckets);
+	}
 	__syncthreads();
 	SamplePlan p{};
 	p.state = -1;
-	if (s_top != kNoLogit) {
+	if (some) {
 		p.state = 0;
-		p.top = (int32_t)s_top;
-		p.sh = bucket_shift(s);
-		const int rb = p.top >> p.sh;
+		p.top = top;
+		p.sh = sh;
 		const uint32_t j0 = kPlanBuckets * tid;
-		// a wave to a slice, sixteen bytes of its counts to a lane, four slices on their way
-		constexpr int kWaves = kPlanThreads / 64, kAhead = 4;
-		for (int i0 = tid >> 6; i0 < slices; i0 += kAhead * kWaves) {
-			int64_t m[kAhead];
-			v4i x[kAhead][kBuckets / 512];
+		// The thread's four buckets of each slice, whose first one is the row's s_off, in eight bytes; 7 slices' counts stay below 2^16
+		// each, so that they are added as they stand.  1 and 128 rows of 151936: 10.9 and 18.5 us, 12.9 and 20.5 by atomics in LDS.
+		static_assert(kPlanBuckets == 4 && 7 * kSampleSlice < 1 << 16, "counts in 16 bits");
+		constexpr int kGroups = 3;
+		int c[kPlanBuckets] = {};
+		for (int i0 = 0; i0 < slices; i0 += 7 * kGroups) {
+			uint64_t x[7 * kGroups];
+			int first[7 * kGroups];
 #pragma unroll
-			for (int q = 0; q < kAhead; ++q) {
-				const size_t at = (size_t)r * slices + min(i0 + q * kWaves, slices - 1);
-				m[q] = w.smax[at];
-#pragma unroll
-				for (int k = 0; k < kBuckets / 512; ++k) x[q][k] = *(const v4i*)(w.hist + at * kBuckets + 8 * ((tid & 63) + 64 * k));
+			for (int q = 0; q < 7 * kGroups; ++q) {
+				const int i = min(i0 + q, slices - 1);
+				first[q] = i0 + q < slices ? (int)(j0 - s_off[i]) : -kBuckets;
+				x[q] = ((const plan_counts*)(w.hist + ((size_t)r * slices + i) * kBuckets + max(first[q], 0)))->v;
 			}
+			__builtin_amdgcn_sched_barrier(0);  // all of them before the first is waited for
 #pragma unroll
-			for (int q = 0; q < kAhead; ++q) {
-				if (m[q] == kNoLogit || i0 + q * kWaves >= slices) continue;
-				const uint32_t off = (uint32_t)rb - (uint32_t)((int32_t)m[q] >> p.sh);  // the slice's first bucket
-				if (off >= kBuckets) continue;
+			for (int g = 0; g < kGroups; ++g) {
+				uint64_t sum = 0;
 #pragma unroll
-				for (int k = 0; k < kBuckets / 512; ++k)
+				for (int q = 7 * g; q < 7 * g + 7; ++q) sum += first[q] >= 0 ? x[q] : (first[q] > -4 ? x[q] << 16 * -first[q] : 0);
 #pragma unroll
-					for (int e = 0; e < 8; ++e) {
-						const uint32_t j = 8 * ((tid & 63) + 64 * k) + e + off, n = (uint32_t)x[q][k][e / 2] >> 16 * (e & 1) & 0xffff;
-						if (n && j < kBuckets) atomicAdd(&s_hist[j], n);
-					}
+				for (int k = 0; k < kPlanBuckets; ++k) c[k] += (int)(sum >> 16 * k & 0xffff);
 			}
 		}
-		__syncthreads();
-		int c[kPlanBuckets];
-#pragma unroll
-		for (int k = 0; k < kPlanBuckets; ++k) c[k] = s_hist[j0 + k];
 		const Weight wt = weight_of(s);
 		const double least = (double)share_of((uint64_t)(s.q_b * s.q_b + s.q_c), s.min_p);
 		Mass one[kPlanBuckets], run[kPlanBuckets], all, mine{0, 0.0, 0.0, 0.0};
