@@ -478,7 +478,7 @@ sslm_status sslm_hip_sample_tokens(const sslm_hip_sample_args* args, void* works
  * inside the page and room past keep) gets a copy of it, but where every row that holds the page would write
  * into it the lowest of them keeps it.  Pages that no row and no `held` byte (optional) keeps are free and given out in
  * ascending order, row by row, a row's copy before its new pages.  new_tables (entries past a row's pages: -1) and
- * new_lengths (= room) may be tables and lengths themselves.  All or nothing: result[0] is 0, SSLM_INVALID_ARGUMENT
+ * new_lengths (= room) may be tables and lengths themselves, and keep or room (or both) may be that buffer too.  All or nothing: result[0] is 0, SSLM_INVALID_ARGUMENT
  * (result[3]: the first row whose source, keep, room, length or table is out of range) or SSLM_KV_POOL_EXHAUSTED, and then nothing
  * else is written; result[1]: pages free afterwards (negative: short by), result[2]: pages copied, result[3] else -1. */
 typedef struct sslm_hip_cache_update_args {
