@@ -214,7 +214,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, Samp
 	__shared__ Mass s_scan[kPlanThreads / 64];
 	__shared__ int s_a[3], s_b[3], s_n;
 	__shared__ uint32_t s_goal;
-	__shared__ double s_sum, s_kept, s_var, s_doubt, s_more;
+	__shared__ double s_sum, s_kept, s_var;
+	__shared__ unsigned long long s_doubt, s_kept_p, s_more;  // s_kept_p, s_more: bits of doubles that are not negative
 	__shared__ int s_few;
 	const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
 	const int64_t* smax = w.smax + (size_t)r * slices;
@@ -224,7 +225,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, Samp
 	if (tid == 0) {
 		s_n = 0;
 		s_goal = 0;
-		s_doubt = 0.0;
+		s_doubt = s_more = 0;
+		s_kept_p = ~0ull;
 	}
 	if (tid < 3) s_a[tid] = s_b[tid] = kBuckets;
 	// every wave finds the row's largest logit
@@ -282,7 +284,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, Samp
 			doubt += w0 >= least && w1 < least ? n * w0 : 0.0;
 			mine = mine + one[i];
 		}
-		if (s.min_p > 0 && doubt > 0.0) s_doubt = doubt;
+		// the i-exp rises a little where one of its segments ends, so that more than one bucket may be cut: a sum of integers below 2^62
+		if (s.min_p > 0 && doubt > 0.0) atomicAdd(&s_doubt, (unsigned long long)doubt);
 		Mass at = mass_scan(mine, s_scan, &all);
 #pragma unroll
 		for (int i = kPlanBuckets - 1; i >= 0; --i) {
@@ -294,7 +297,6 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, Samp
 			s_kept = all.k;
 			s_var = all.v;
 			s_few = all.c;
-			s_more = 0.0;
 		}
 		__syncthreads();
 		// top-k: exactly its bucket; the estimates up to its border
@@ -338,13 +340,16 @@ __global__ __launch_bounds__(kPlanThreads) void k_sample_plan(SampleArgs a, Samp
 #pragma unroll
 			for (int i = 0; i < kPlanBuckets; ++i)  // the kept weight up to there
 				if (run[i].e >= goal && run[i].e - one[i].e < goal) {
-					s_kept = fmin(kept_k, run[i].k - (1.0 - (goal - (run[i].e - one[i].e)) / one[i].e) * one[i].k);
-					s_more = 1.2 * one[i].e / (double)one[i].c;  // the run ends with a whole element
+					// apart from s_kept, which waves may still be reading; rounded sums can put the border into two neighbours: the lesser weight
+					// and the larger element, whichever thread comes first
+					const double k = run[i].k - (1.0 - (goal - (run[i].e - one[i].e)) / one[i].e) * one[i].k;
+					atomicMin(&s_kept_p, k > 0.0 ? (unsigned long long)__double_as_longlong(k) : 0ull);
+					atomicMax(&s_more, (unsigned long long)__double_as_longlong(1.2 * one[i].e / (double)one[i].c));  // the run ends with a whole element
 				}
 			__syncthreads();
-			kept = s_kept;
+			if (s_kept_p != ~0ull) kept = fmin(kept_k, __longlong_as_double((long long)s_kept_p));
 		}
-		range(2, true, kept * s.random * 0x1p-32, kept_k, s_doubt + s_more);
+		range(2, true, kept * s.random * 0x1p-32, kept_k, (double)s_doubt + __longlong_as_double((long long)s_more));
 		__syncthreads();
 		p.cut_k = cut_k;
 		p.goal_k = s_goal;
