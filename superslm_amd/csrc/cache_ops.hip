@@ -51,9 +51,9 @@ __device__ __forceinline__ T block_before(T v, T* total, T* s) {
 // What a plan leaves for the launch that carries it out.
 struct PlanWork {
 	int32_t* state;   // [0]: whether there is anything to do, [1]: pages to copy
-	int32_t* off;     // [rows] a row's first free page in `free`
-	int32_t* tail;    // [rows] the page it gets a copy of, or -1
-	int32_t *kept, *need;  // [rows] its pages that stay, and all of them: keep and room may be the buffer that new_lengths goes to
+	// [rows] a row's first free page in `free`, the page it gets a copy of or -1, its pages that stay, all of its pages: keep and room
+	// themselves may be the buffer that new_lengths goes to
+	v4i* row;
 	int32_t* free;    // [pages] free pages in the order they are given out (compaction: the holes)
 	int32_t *from, *to;  // pages to copy
 	int32_t* old;     // [rows, table_ld] the tables as they were, where the new ones take their place
@@ -168,13 +168,11 @@ __global__ __launch_bounds__(kPlanBlock) void k_update_plan(PageUpdateArgs a, co
 		int64_t all;  // pages below 2^40, copies above
 		const int64_t before = block_before<int64_t>(n + ((int64_t)(t >= 0) << 40), &all, s_scan), mine = (before >> 40) + copies;
 		if (r < a.rows) {
-			w.off[r] = (int)min((before & (((int64_t)1 << 40) - 1)) + wants, (int64_t)INT32_MAX);
-			w.tail[r] = t;
-			w.kept[r] = kept;
-			w.need[r] = need;
+			const int off = (int)min((before & (((int64_t)1 << 40) - 1)) + wants, (int64_t)INT32_MAX);
+			w.row[r] = v4i{off, t, kept, need};
 			if (t >= 0) {
 				w.from[mine] = t;
-				w.to[mine] = w.off[r];  // its place among the free pages
+				w.to[mine] = off;  // its place among the free pages
 			}
 		}
 		wants += all & (((int64_t)1 << 40) - 1);
@@ -231,8 +229,9 @@ __global__ __launch_bounds__(256) void k_update_apply(PageUpdateArgs a, const in
 	const int64_t cells = (int64_t)a.rows * a.table_ld;
 	for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < cells; c += (int64_t)gridDim.x * 256) {
 		const int r = (int)(c / a.table_ld), i = (int)(c - (int64_t)r * a.table_ld);
-		const int kept = w.kept[r], need = w.need[r], off = w.off[r];
-		const bool copied = w.tail[r] >= 0;
+		const v4i row = w.row[r];
+		const int off = row.x, kept = row.z, need = row.w;
+		const bool copied = row.y >= 0;
 		int p = -1;
 		if (i < kept) p = copied && i == kept - 1 ? w.free[off] : tables[(int64_t)a.source[r] * a.table_ld + i];
 		else if (i < need) p = w.free[off + copied + i - kept];
@@ -1839,10 +1838,7 @@ static size_t plan_work(int rows, int pages, int table_ld, char* base, PlanWork*
 		return p;
 	};
 	w->state = take(2);
-	w->off = take(rows);
-	w->tail = take(rows);
-	w->kept = take(rows);
-	w->need = take(rows);
+	w->row = (v4i*)take(4 * (size_t)rows);
 	w->free = take(pages);
 	w->from = take(std::max(rows, pages));
 	w->to = take(rows);
