@@ -557,8 +557,8 @@ sslm_status sslm_hip_cache_store(const sslm_hip_cache_store_args* args, void* st
  * (single tokens: decode steps; several: a prompt's chunk, whose rows sslm_hip_cache_store has landed before).
  * score = (q . k) 2^s of k's page; the softmax, its constants (khead: the carried scale of one K unit over sqrt(head_dim)), the Q15
  * probabilities, fold and funnel are sslm_hip_shared_attention's; context = sum of p v 2^s of v's page.  max_width: at least
- * every row's positions.  q is 16-byte aligned, max_new below 2^22; a workspace of 0 bytes: sizes outside the domain, or more blocks
- * than a launch takes.  Per token its codes, scale and status: 0, 9 (the row's lengths or a page of it out of range) or the
+ * every row's positions.  q is 16-byte aligned, max_new below 2^22; a workspace of 0 bytes: sizes outside the domain, more blocks
+ * than a launch takes, or 2^62 bytes and more.  Per token its codes, scale and status: 0, 9 (the row's lengths or a page of it out of range) or the
  * reference's SslmForwardStatus value; tokens that no row has stay as they were. */
 typedef struct sslm_hip_cache_attention_args {
 	uint32_t struct_size;

@@ -1986,6 +1986,8 @@ size_t cache_attn_workspace(int rows, int tokens, int max_new, int NH, int NKV, 
 	const CaPlan p = ca_plan(rows, tokens, max_new, NH, NKV, D, max_width);
 	const int64_t blocks = max_new == 1 ? (int64_t)rows * NKV * p.ht * p.planes : (int64_t)((p.planes * NKV + 7) / 8 * 8) * p.groups;
 	if (blocks * (p.whole ? 512 : 64 * kCaWaves) >= kMost) return 0;
+	// kept scores pass 64 bits of bytes at 2^38 (token, head)s by 2^24 positions; all the others stay below 2^58
+	if (max_new == 1 && (double)tokens * NH * (double)p.wpad * 4.0 >= 0x1p62) return 0;
 	CaWork w;
 	return ca_work(p, tokens, max_new, NH, NKV, D, nullptr, &w);
 }

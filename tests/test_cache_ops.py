@@ -114,6 +114,13 @@ def test_attention_that_no_launch_holds_has_no_workspace(cache, rows, tokens, ma
     assert (n >= tokens * heads * dim * 4) if fits else n == 0
 
 
+@pytest.mark.parametrize("tokens,heads,width,fits", [(1 << 30, 256, 1 << 24, False), ((1 << 31) - 1, 256, 1 << 24, False), ((1 << 31) - 1, 128, 1 << 24, False),
+                                                     (1 << 28, 256, 1 << 24, False), ((1 << 28) - 1, 256, 1 << 24, True), (1 << 30, 256, 3 << 20, True)])
+def test_attention_whose_scores_pass_64_bits_of_bytes_has_no_workspace(cache, tokens, heads, width, fits):
+    n = cache.attention_workspace(1, tokens, 1, heads, 1, 32, 16, width)
+    assert (n >= tokens * heads * width * 4) if fits else n == 0
+
+
 def test_an_unknown_field_or_a_number_too_large_is_an_error(cache):
     with pytest.raises(TypeError):
         cache.compact(**PAGES, map=ANY, colour=1)
