@@ -66,7 +66,7 @@ constexpr int kSampleList = 4096, kSliceList = 2048;  // elements gathered of a 
 // What the plan found: the borders' bucket ranges [a, b), 0 top-k, 1 top-p, 2 the draw (unused ones empty).
 struct SamplePlan {
 	int32_t top, sh;   // the row's largest logit
-	int32_t state;     // 0: to be drawn from the ranges, 1: by the search over the row, -1: no legal token
+	int32_t state;     // 0: to be drawn from the ranges, 1: by the search over the row, 2: by that, as the ranges missed, -1: no legal token
 	int32_t cut_k;     // whether top-k cuts, and how many of its first elements range 0 has
 	uint32_t goal_k;
 	uint32_t a[3], b[3];
@@ -660,6 +660,7 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_pick(SampleArgs a, Samp
 		if (tid == 0) {
 			s_top = INT32_MIN;
 			s_any = 0;
+			if (slices > 1 && p.state == 0) w.plan[r].state = 2;  // so that tests see which rows missed
 		}
 		__syncthreads();
 		auto legal = [&](int i) { return !s.mask || (global_ptr(s.mask)[i >> 3] >> (i & 7) & 1); };

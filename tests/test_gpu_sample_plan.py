@@ -60,3 +60,27 @@ def test_plans_of_equal_calls_are_equal(ops, dev, vocab):
     for p in others:
         for name in PLAN.names:
             assert (p[name] == first[name]).all(), name
+
+
+def normal(rng, rows, vocab):
+    return (rng.standard_normal((rows, vocab)) * 120000).astype(np.int32)
+
+
+@pytest.mark.parametrize("vocab", [8193, 20000, 151936])
+def test_ordinary_rows_are_drawn_without_the_search_over_the_row(ops, dev, vocab):
+    """Spreads of 2.2 to 4.4 natural units: a result that only the search made right would show here."""
+    rng = np.random.default_rng(vocab)
+    rules = [rule(45000.0 * float(rng.uniform(0.6, 1.2)), *((40, 60000, 0), (0, 55000, 0), (300, 60000, 2000), (0, 65536, 0), (0, 65536, 500), (50, 65536, 0))[r % 6],
+                  int(rng.integers(0, 1 << 32))) for r in range(36)]
+    assert (plans(ops, dev, normal(rng, 36, vocab), rules)[0]["state"] == 0).all()
+
+
+def test_rows_that_are_searched_whole(ops, dev):
+    """Too many elements around a border for the list; and, found while gathering, too many of them in one slice."""
+    rng = np.random.default_rng(7)
+    flat = [rule(45000.0 * 6, 0, 58982, 0, int(rng.integers(0, 1 << 32))) for _ in range(6)]
+    assert (plans(ops, dev, normal(rng, 6, 151936), flat)[0]["state"] == 1).all()
+    x = np.full((3, 30000), -100000000, np.int32)
+    x[:, 9000:11500] = 0
+    side = [rule(1000.0, random=int(u)) for u in (0, 1 << 31, (1 << 32) - 1)]
+    assert (plans(ops, dev, x, side)[0]["state"] == 2).all()
