@@ -559,7 +559,9 @@ sslm_status sslm_hip_cache_store(const sslm_hip_cache_store_args* args, void* st
  * probabilities, fold and funnel are sslm_hip_shared_attention's; context = sum of p v 2^s of v's page.  max_width: at least
  * every row's positions.  q is 16-byte aligned, max_new below 2^22; a workspace of 0 bytes: sizes outside the domain, more blocks
  * than a launch takes, or 2^62 bytes and more.  Per token its codes, scale and status: 0, 9 (the row's lengths or a page of it out of range) or the
- * reference's SslmForwardStatus value; tokens that no row has stay as they were. */
+ * reference's SslmForwardStatus value; tokens that no row has stay as they were.  A row whose row_tokens do not ascend within [0, tokens] has
+ * none, and there is nothing its status could stand beside without a place in another row's: a caller that cannot rule such rows out
+ * presets `status`, or looks at sslm_hip_cache_store's, which is per row. */
 typedef struct sslm_hip_cache_attention_args {
 	uint32_t struct_size;
 	int32_t rows, tokens, max_new, heads, kv_heads, head_dim, pages, page_tokens, table_ld, reserved;
