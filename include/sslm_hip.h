@@ -525,7 +525,8 @@ sslm_status sslm_hip_cache_compact(const sslm_hip_cache_compact_args* args, void
  * pages that rows write into are their own; max_new and rope_rows are at most SSLM_HIP_CACHE_MAX_WIDTH).  Codes
  * are int8 with carried scales k_scale, v_scale (m, e) per token.  The reference's landing (forward_sites.cpp:513-653) with the
  * KV head's constants r_t, e_t gives units, clamped to +-127 2^8; pairs of the head's first rope_dim (a multiple of 8, 0:
- * none) dims, (2 i, 2 i + 1) or with rope_halves (i, i + rope_dim / 2), turn by the Q30 tables [rope_rows, rope_dim / 2] (src/intmath.cpp:782-792),
+ * none) dims, (2 i, 2 i + 1) or with rope_halves (i, i + rope_dim / 2), turn by the Q30 tables [rope_rows, rope_dim / 2] (src/intmath.cpp:782-792;
+ * entries are read as 32 bits: a table scaled by its maker stays within [-2, 2)),
  * q's codes clamped to +-127, k's units to +-127 2^8.  A page's exponent for a KV head's K or V is 0 at its first slot and
  * grows to what a token needs, the least that keeps the token's codes within +-127; codes already there are then divided
  * by the power of two once more.  All roundings go to the nearest, ties away from zero.  Every split of a span into calls leaves
