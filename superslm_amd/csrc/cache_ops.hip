@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256) void k_table_copy(const int32_t* from, int32_t
 // One block: bitmaps of the pages that rows hold (seen), hold more than once (multi), and hold without writing
 // into them or keep from outside (fixed), in LDS; then who gets a copy, how many pages each row takes, and the free
 // pages in ascending order.  Bound by its chain of loads (a row's numbers, its source's length, the tables) and of block sums:
-// 6.2 us for 4 rows and 114 pages, 8.9 for 128 rows of 16 pages; a block per row would need its answers joined by further launches.
+// 6.2 us for 4 rows and 114 pages, 9.2 for 128 rows of 16 pages; a block per row would need its answers joined by further launches.
 constexpr int kLowSlots = 2048;
 constexpr int kWrites = 1 << 30;  // beside a row's number of kept pages: it writes into the last of them
 __global__ __launch_bounds__(kPlanBlock) void k_update_plan(PageUpdateArgs a, const int32_t* tables, PlanWork w) {
@@ -472,7 +472,7 @@ __device__ __forceinline__ void octet_store(const CacheStoreArgs& a, int8_t* hea
 	((unaligned8*)(head + 8 * g))->v = w;
 }
 // The angles of four pairs at `pos`, and the pairs turned by them (rope_pair), clamped to +-top; returns how many values were.
-// In doubles: a value of 16 bits times a table's 31, and the sum of two of these, are exact at the scale 2^-30, and so is half a
+// In doubles, the tables' entries taken as 32 bits: a value of 16 bits times an entry's 31, and the sum of two of these, are exact at the scale 2^-30, and so is half a
 // unit added away from zero before the conversion truncates.  Five instructions a value, the 64-bit form takes some thirty: 512 tokens of
 // 28 + 2 x 4 heads for each of four rows 18.4 -> 16.2 us.
 struct Turn {
@@ -570,7 +570,7 @@ __device__ __forceinline__ void regrow(int8_t* at, int init, uint32_t levels) {
 // K or V of one KV head (z) in one page (x) of one row (y): the page's tokens land in LDS, their exponents run up the
 // page, then the codes are written; the waves of blocks past the last page take q's tokens, one each.
 // Bound by its instructions (a landing and a rotation are some 40 of doubles to a code) and, as one block takes a page's tokens, by that
-// block's length: 4 rows of 512 tokens, 28 + 2 x 4 heads of 128, 16.5 us, of which 16.5 MB are 3.5.
+// block's length: 4 rows of 512 tokens, 28 + 2 x 4 heads of 128, 16 us, without queries 14.5; their 16.5 MB are 3.5.
 constexpr int kStoreBlock = 512;
 template <int D>
 __global__ __launch_bounds__(kStoreBlock) void k_store_span(CacheStoreArgs a, int pages) {
@@ -900,8 +900,9 @@ __device__ __forceinline__ bool cd_job(const CacheAttnArgs& a, const CaPlan& pl,
 	return j->p0 < j->p1;
 }
 
-// The scores of a plane, kept, and their maxima: written once and read twice they cost less than two more products with K.  64 rows of
-// 28 heads / 4 KV x 128 by up to 8000 positions: 39 us, 149 MB of K at 3.8 TB/s; then k_cd_sum 15.5, k_cd_pv 47.  The first wave of a row's first plane also settles its constants.
+// The scores of a plane, kept, and their maxima: written once and read twice they cost less than two more products with K.  8 rows of
+// 28 heads / 4 KV x 128 by 16000 positions: 18.8 us, 66 MB of K and 14 of scores at 4.2 TB/s; then k_cd_sum 7.7, k_cd_pv 21.6 and the join 7.9.
+// 2 rows of 12 / 2 by 8000, a chain of four launches: 5.9 + 4.2 + 8.6 + 4.3.  The first wave of a row's first plane also settles its constants.
 template <int D>
 __global__ __launch_bounds__(64 * kCaWaves) void k_cd_scores(CacheAttnArgs a, CaPlan pl, CaWork w) {
 	constexpr int NC = (D + 63) / 64;
@@ -1917,16 +1918,17 @@ void cache_store(const CacheStoreArgs& a, hipStream_t s) {
 	}
 }
 
-// Blocks that fill the chip: more cost their own start, fewer leave CUs idle.  64 rows of 28 heads / 4 KV x 128 with 1000 ..
-// 8000 positions, scores + P V: 81 us at 768 blocks, 86 at 1536, 102 at 2560, 116 at 4096; few rows want them all the same, so the
-// middle.  A chunk of 500 at 2000, its three launches: 62 at 384, 59 at 768, 73 at 1536.
+// Blocks that fill the chip: more cost their own start, fewer leave CUs idle.  A call at 768, 1536, 2560 and 4096 blocks: 64 rows of
+// 12 heads / 2 KV x 128 by 4000 positions 50, 48, 60 and 60 us, 2 rows by 8000 25, 23, 25 and 25, 8 rows of 28 / 4 by 16000 56 each.  A chunk of 500 at 2000, its three launches: 62 at 384, 59 at 768, 73 at 1536.
 constexpr int kCdTargetBlocks = 1536, kCcTargetBlocks = 768;
 
 // Rows of up to max_width by k_cr_row: 1 with their scores in LDS, 2 in the workspace, 0 by planes.  A block takes some 6.8 us for 1000
 // positions of 128 dims by itself; the planes' three launches take 8 us more to start and then share the chip, so that they are
 // the faster form the longer the rows and the fewer the (row, KV head)s.  Row kernel / planes, us: 2 x 2 KV heads 19.5 / 21.3 at 1000
 // positions, 26.6 / 20.6 at 2000; 16 x 4 28 / 27 at 2000, 45 / 40 at 4000; 64 x 2 46 / 47 at 4000, 78 / 72 at 8000; 64 x 4 59 / 78 at
-// 4000, 313 / 326 at 20000; 32 x 2 x 64 dims 18 / 20 at 1000, 24 / 23 at 2000; 24 x 2 x 256 25 / 25 at 1000, 38 / 35 at 2000.
+// 4000, 313 / 326 at 20000; 32 x 2 x 64 dims 18 / 20 at 1000, 24 / 23 at 2000; 24 x 2 x 256 25 / 25 at 1000, 38 / 35 at 2000.  These are rows
+// of one length.  From 210 blocks on every batch takes this form, also one whose longest row is far from the others, which then ends the
+// launch by itself: 110 rows of 100 positions and one of 100000, 2 KV heads, 745 / 197.
 template <int D>
 static int cr_form(int64_t units, int NH, int NKV, int64_t max_width) {
 	if (max_width * (210 - units) > 257000) return 0;

@@ -55,9 +55,11 @@ __device__ __forceinline__ uint64_t weight(const Weight& w, uint32_t d) { return
 //   k_sample_gather  the exact sums of the weights before those buckets, and the elements in them
 //   k_sample_pick    the borders among these elements.  That each lies where it was expected is checked exactly, so an estimate
 //                    that misses (or a list that overflows) costs the radix search over the row, not the result.
-// Rows of one slice are searched in LDS by k_sample_pick alone.  At 151936 tokens 1 row takes 4.2 + 10.9 + 6.2 + 9.0 us, the chains of
-// four launches, and 128 rows 16.2 + 18.5 + 29 + 13.4: the first pass reads 79 MB at 4.9 TB/s, the second is bound by its doubles, plan and
-// pick are a block's chain of scans to a row.  The search over the row takes 870 us for 1 row and 1870 for 128.
+// Rows of one slice are searched in LDS by k_sample_pick alone.  At 151936 tokens 1 row takes 4.2 + 11.0 + 6.1 + 9.2 us, the chains of
+// four launches, and 128 rows 16.3 + 18.4 + 29 + 13.5: the first pass reads 79 MB at 4.9 TB/s, the second is bound by its doubles, plan and
+// pick are a block's chain of scans to a row.  The search over the row takes 870 .. 980 us for 1 row and
+// some 1800 for 128: what a row costs whose borders' buckets hold more than kSampleList, a bell of 151936 logits of a spread below about 1.2
+// natural units.
 constexpr int kSampleBlock = 512;
 constexpr int kSampleSlice = 8192, kSampleLoads = kSampleSlice / kSampleBlock / 4;
 constexpr int kBuckets = 2048;
